@@ -339,12 +339,58 @@ int gdn2_gated_norm_bwd(const gdn2_norm_problem* p, const void* x, const void* z
                         float* dweight, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ---- gated linear recurrence ----------------------------------------------
+ * Per channel, over the rows [B][T] (or packed sequences, B = 1):
+ *   h_t = exp(g_t) h_{t-1} + w_t v_t,   y_t = h_t rounded to `dtype`
+ * v, w, y have `dtype`, g has `dtype` or fp32, states are fp32 [n_seqs][D].
+ * w NULL stands for ones, h0 NULL for zero; ht (or NULL) receives the states
+ * after the last tokens.  Row r = b*T + t of v, g, w, dy starts at element
+ * r * ld_*; y and the gradients are contiguous [B*T][D].  cu_seqlens (int32
+ * [n_seqs+1], device) starts at 0, ends at T and does not decrease; n_seqs = B
+ * without it.  A sequence without tokens passes its state on.
+ * Backward: dy of y and dht (or NULL) of ht give dv, dg, dw, dh0 (or NULL);
+ * `saved` (gdn2_scan_saved_bytes) is what the forward of the same inputs
+ * wrote; a forward with saved NULL keeps nothing.  The workspace
+ * (gdn2_scan_workspace_bytes, 16-byte aligned) is scratch of one call, forward
+ * or backward.  The order of all sums is fixed: equal inputs give equal bits. */
+typedef struct gdn2_scan_problem {
+    int32_t B;
+    int32_t D;
+    int64_t T;
+    int32_t dtype, g_dtype;
+    int32_t n_seqs;
+    const int32_t* cu_seqlens;
+    int64_t ld_v, ld_g, ld_w, ld_dy;  /* row strides in elements */
+} gdn2_scan_problem;
+
+size_t gdn2_scan_saved_bytes(const gdn2_scan_problem* p);
+size_t gdn2_scan_workspace_bytes(const gdn2_scan_problem* p);
+int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g,
+                  const void* w, const float* h0, void* y, float* ht,
+                  float* saved, void* workspace, size_t workspace_bytes,
+                  void* stream);
+int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g,
+                  const void* w, const float* h0, const float* saved,
+                  const void* dy, const float* dht, void* dv, void* dg,
+                  void* dw, float* dh0, void* workspace, size_t workspace_bytes,
+                  void* stream);
+/* One token for each of B sequences (T = 1) on a pool of states, updated in
+ * place: sequence b uses the row state_indices[b] (row b when NULL) of `state`
+ * (`pool` rows, `state_stride` elements apart).  An index outside [0, pool)
+ * marks padding: no state changes and its y is zero.  Two sequences must not
+ * name the same row. */
+int gdn2_scan_step(const gdn2_scan_problem* p, const void* v, const void* g,
+                   const void* w, float* state, int64_t state_stride,
+                   int32_t pool, const int32_t* state_indices, void* y,
+                   void* stream);
+
 /* Device-side fault bits.  Kernels that wait on asynchronous copies or on
  * tensor-core completion bound every wait in time (about one second); a wait
  * that runs out makes the kernel release its tensor memory, return without
  * finishing, and set a bit of a per-device fault word (bit 0: state passes,
  * bit 1: forward intra-chunk kernel, bit 2: decode, bit 3: backward
- * intra-chunk kernel).  gdn2_fault_status
+ * intra-chunk kernel, bit 4: gated linear recurrence, whose outputs after the
+ * wait are NaN).  gdn2_fault_status
  * synchronises `stream` (the default stream when NULL), returns the fault
  * word of the current device (0 = no fault) and resets it when `clear` is
  * nonzero; a negative return is a CUDA error.  No counterpart in the

@@ -1,0 +1,52 @@
+"""Float64 numpy oracle of the operators around the GDN-2 mixer: the gated
+linear recurrence, token log probabilities and the AdamW step, each written
+row by row from its definition."""
+
+from __future__ import annotations
+
+import numpy as np
+
+
+def _sequences(B, T, cu):
+    """(batch entry, first row, end row) of each sequence."""
+    if cu is None:
+        return [(b, 0, T) for b in range(B)]
+    return [(0, int(cu[n]), int(cu[n + 1])) for n in range(len(cu) - 1)]
+
+
+def scan_fwd(v, g, w=None, h0=None, cu=None):
+    """h_t = exp(g_t) h_{t-1} + w_t v_t over [B, T, D]; returns (h, ht)."""
+    B, T, D = v.shape
+    seqs = _sequences(B, T, cu)
+    y = np.zeros((B, T, D))
+    ht = np.zeros((len(seqs), D)) if h0 is None else np.array(h0, dtype=np.float64)
+    for n, (b, lo, hi) in enumerate(seqs):
+        h = ht[n].copy()
+        for t in range(lo, hi):
+            h = np.exp(g[b, t]) * h + (v[b, t] if w is None else w[b, t] * v[b, t])
+            y[b, t] = h
+        ht[n] = h
+    return y, ht
+
+
+def scan_bwd(v, g, w, h0, dy, dht=None, cu=None):
+    """Gradients (dv, dg, dw or None, dh0) of sum(y dy) + sum(ht dht)."""
+    B, T, D = v.shape
+    seqs = _sequences(B, T, cu)
+    y, _ = scan_fwd(v, g, w, h0, cu)
+    dv, dg = np.zeros_like(y), np.zeros_like(y)
+    dw = None if w is None else np.zeros_like(y)
+    dh0 = np.zeros((len(seqs), D))
+    for n, (b, lo, hi) in enumerate(seqs):
+        c = np.zeros(D) if dht is None else np.array(dht[n], dtype=np.float64)
+        for t in range(hi - 1, lo - 1, -1):
+            dh = dy[b, t] + c
+            prev = y[b, t - 1] if t > lo else (np.zeros(D) if h0 is None else h0[n])
+            a = np.exp(g[b, t])
+            dg[b, t] = a * prev * dh
+            dv[b, t] = dh if w is None else w[b, t] * dh
+            if w is not None:
+                dw[b, t] = v[b, t] * dh
+            c = a * dh
+        dh0[n] = c
+    return dv, dg, dw, dh0

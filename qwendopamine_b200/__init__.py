@@ -7,7 +7,8 @@ keep the reference kernel entry points.  All compute runs in
 """
 
 from .gdn2 import GDN2_BACKENDS, GatedDeltaNet2, RMSNormGated, ShortConvolution, resolve_gdn2_backend
-from .gdn2_ops import ChunkGDN2Function, chunk_gdn2, fused_recurrent_gdn2, fused_recurrent_gdn2_fwd
+from .gdn2_ops import (ChunkGDN2Function, chunk_gdn2, fused_recurrent_gdn2,
+                       fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step)
 from .registry import BLOCKS, build_block
 
 __all__ = [
@@ -21,5 +22,7 @@ __all__ = [
     "chunk_gdn2",
     "fused_recurrent_gdn2",
     "fused_recurrent_gdn2_fwd",
+    "gated_scan",
+    "gated_scan_step",
     "resolve_gdn2_backend",
 ]

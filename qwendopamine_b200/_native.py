@@ -48,6 +48,11 @@ EXPORTS = (
     "gdn2_gated_norm_fwd",
     "gdn2_gated_norm_bwd_workspace_bytes",
     "gdn2_gated_norm_bwd",
+    "gdn2_scan_saved_bytes",
+    "gdn2_scan_workspace_bytes",
+    "gdn2_scan_fwd",
+    "gdn2_scan_bwd",
+    "gdn2_scan_step",
     "gdn2_fault_status",
     "gdn2_test_fwd_state_wait_timeout",
 )
@@ -132,6 +137,22 @@ class NormProblem(ctypes.Structure):
     ]
 
 
+class ScanProblem(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32),
+        ("D", c_int32),
+        ("T", c_int64),
+        ("dtype", c_int32),
+        ("g_dtype", c_int32),
+        ("n_seqs", c_int32),
+        ("cu_seqlens", c_void_p),
+        ("ld_v", c_int64),
+        ("ld_g", c_int64),
+        ("ld_w", c_int64),
+        ("ld_dy", c_int64),
+    ]
+
+
 class GDN2Error(RuntimeError):
     """A libgdn2_b200 entry point returned an error status."""
 
@@ -150,6 +171,7 @@ def _declare(lib):
     rp = P(RecurrentProblem)
     vp = P(ConvProblem)
     np_ = P(NormProblem)
+    sp = P(ScanProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -182,6 +204,11 @@ def _declare(lib):
         "gdn2_gated_norm_fwd": ([np_, v, v, v, v, v], ctypes.c_int),
         "gdn2_gated_norm_bwd_workspace_bytes": ([np_], c_size_t),
         "gdn2_gated_norm_bwd": ([np_, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_scan_saved_bytes": ([sp], c_size_t),
+        "gdn2_scan_workspace_bytes": ([sp], c_size_t),
+        "gdn2_scan_fwd": ([sp, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_scan_step": ([sp, v, v, v, v, c_int64, c_int32, v, v, v], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -269,6 +296,13 @@ def phase(name: str, stream=None):
     finally:
         e.record(stream)
         rec.append((name, s, e))
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` current for a launch (a no-op when it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def ptr(t):

@@ -213,3 +213,42 @@ def test_negative_sm_budget_is_rejected(lib):
     assert lib.gdn2_chunk_fwd_intra(p, *([None] * 6), None, 0, None) == N.ERR_INVALID
     p.max_ctas = 116
     assert lib.gdn2_chunk_saved_bytes(p) > 0
+
+
+def test_scan_arguments_are_checked(lib):
+    """Gated linear recurrence: shapes, types, strides and buffer sizes are
+    validated before any CUDA call."""
+    def sp(**kw):
+        base = dict(B=2, D=70, T=200, dtype=1, g_dtype=0, n_seqs=2, cu_seqlens=None, ld_v=70,
+                    ld_g=70, ld_w=70, ld_dy=70)
+        base.update(kw)
+        return N.ScanProblem(**base)
+
+    f = ctypes.c_void_p(0x1000)
+    fwd = lambda p, ws=f, wb=1 << 30, v=f: lib.gdn2_scan_fwd(p, v, f, f, None, f, None, None, ws,
+                                                             wb, None)
+    # a state every 64 of the 400 rows
+    assert lib.gdn2_scan_saved_bytes(sp()) == 7 * 70 * 4
+    need = lib.gdn2_scan_workspace_bytes(sp())
+    assert need > 7 * 2 * 64 * 8
+    for bad, code in ((sp(D=0), N.ERR_INVALID), (sp(T=-1), N.ERR_INVALID),
+                      (sp(dtype=5), N.ERR_INVALID), (sp(g_dtype=2), N.ERR_UNSUPPORTED),
+                      (sp(n_seqs=3), N.ERR_INVALID), (sp(cu_seqlens=0x1000), N.ERR_INVALID),
+                      (sp(ld_v=69), N.ERR_INVALID), (sp(ld_w=3), N.ERR_INVALID),
+                      (sp(T=1 << 40, B=64, n_seqs=64), N.ERR_UNSUPPORTED)):
+        assert fwd(bad) == code, lib.gdn2_last_error()
+    assert fwd(sp(), v=None) == N.ERR_INVALID
+    assert fwd(sp(), ws=None) == N.ERR_WORKSPACE
+    assert fwd(sp(), wb=256) == N.ERR_WORKSPACE
+    assert fwd(sp(), ws=ctypes.c_void_p(0x1008)) == N.ERR_INVALID
+    bwd = lambda p, saved=f: lib.gdn2_scan_bwd(p, f, f, f, None, saved, f, None, f, f, f, None, f,
+                                               256, None)
+    assert bwd(sp(), saved=None) == N.ERR_INVALID
+    assert bwd(sp(ld_dy=2)) == N.ERR_INVALID
+    assert bwd(sp()) == N.ERR_WORKSPACE
+    step = lambda p, pool=9, stride=70: lib.gdn2_scan_step(p, f, f, f, f, stride, pool, None, f,
+                                                           None)
+    assert step(sp()) == N.ERR_INVALID and b"one token" in lib.gdn2_last_error()
+    assert step(sp(T=1), pool=1) == N.ERR_INVALID
+    assert step(sp(T=1), stride=69) == N.ERR_INVALID
+    assert lib.gdn2_scan_step(sp(T=1, B=0, n_seqs=0), *([None] * 4), 70, 0, None, None, None) == 0
