@@ -384,6 +384,41 @@ int gdn2_scan_step(const gdn2_scan_problem* p, const void* v, const void* g,
                    int32_t pool, const int32_t* state_indices, void* y,
                    void* stream);
 
+/* ---- log probabilities of given tokens ------------------------------------
+ * For each row x of logits [rows][vocab] (row r at element r * ld) and its
+ * token id, with z = x / temperature:
+ *   logprobs[r] = log_softmax(z)[id]
+ *   entropy[r]  = -sum p ln p                      (entropy NULL: not formed)
+ *   top_logprobs, top_ids [rows][top_k]: the top_k largest log probabilities
+ *   in falling order, equal ones by rising index (top_k = 0: not formed).
+ * Everything is formed and returned in fp32.  -inf logits have probability
+ * zero.  A row of only -inf has log probability -inf and entropy 0; one whose
+ * id is ignore_index gives 0, 0, -inf and index -1 and is not read; an id
+ * outside the vocabulary gives NaN.  NaN logits make the row's results NaN.
+ * `stats` (fp32 [rows][4], 16-byte aligned, or NULL) is what the backward
+ * needs of the forward.  Backward: dlogits [rows][vocab], contiguous, in the
+ * logits' dtype, from dlogprobs and dentropy (fp32 [rows], NULL for zero;
+ * dentropy only after a forward with entropy); zero for ignored rows and rows
+ * of only -inf.  top_k <= 128. */
+typedef struct gdn2_logprob_problem {
+    int64_t rows;
+    int64_t ld;
+    int64_t ignore_index;
+    int32_t vocab;
+    int32_t dtype;
+    int32_t top_k;
+    float temperature;
+} gdn2_logprob_problem;
+
+int gdn2_logprob_fwd(const gdn2_logprob_problem* p, const void* logits,
+                     const int64_t* token_ids, float* logprobs, float* entropy,
+                     float* top_logprobs, int64_t* top_ids, float* stats,
+                     void* stream);
+int gdn2_logprob_bwd(const gdn2_logprob_problem* p, const void* logits,
+                     const int64_t* token_ids, const float* stats,
+                     const float* dlogprobs, const float* dentropy,
+                     void* dlogits, void* stream);
+
 /* Device-side fault bits.  Kernels that wait on asynchronous copies or on
  * tensor-core completion bound every wait in time (about one second); a wait
  * that runs out makes the kernel release its tensor memory, return without

@@ -50,3 +50,42 @@ def scan_bwd(v, g, w, h0, dy, dht=None, cu=None):
             c = a * dh
         dh0[n] = c
     return dv, dg, dw, dh0
+
+
+def token_logprobs(x, ids, temperature=1.0, ignore=-100):
+    """Per row of x [R, V]: (log p of the id, entropy, log p of every token)."""
+    R, V = x.shape
+    logp, ent, table = np.zeros(R), np.zeros(R), np.full((R, V), -np.inf)
+    for r in range(R):
+        z = x[r] / temperature
+        m = z.max()
+        if m == -np.inf:
+            logp[r] = 0.0 if ids[r] == ignore else -np.inf
+            continue
+        table[r] = z - m - np.log(np.exp(z - m).sum())
+        if ids[r] == ignore:
+            continue
+        logp[r] = table[r, ids[r]]
+        p = np.exp(table[r])
+        ent[r] = -sum(p[j] * table[r, j] for j in range(V) if p[j] > 0)
+    return logp, ent, table
+
+
+def token_logprobs_bwd(x, ids, dlogp, dent=None, temperature=1.0, ignore=-100):
+    """Gradient of sum(logp dlogp) + sum(entropy dent) with respect to x."""
+    _, ent, table = token_logprobs(x, ids, temperature, ignore)
+    dx = np.zeros_like(x)
+    for r in range(x.shape[0]):
+        if ids[r] == ignore or not np.isfinite(table[r]).any():
+            continue
+        p = np.exp(table[r])
+        dx[r] = -dlogp[r] * p
+        dx[r, ids[r]] += dlogp[r]
+        if dent is not None:
+            dx[r] -= dent[r] * p * np.where(p > 0, np.where(p > 0, table[r], 0.0) + ent[r], 0.0)
+    return dx / temperature
+
+
+def top_tokens(x, k):
+    """Indices of the k largest of each row, equal values by rising index."""
+    return np.argsort(-x, axis=1, kind="stable")[:, :k]

@@ -8,7 +8,8 @@ keep the reference kernel entry points.  All compute runs in
 
 from .gdn2 import GDN2_BACKENDS, GatedDeltaNet2, RMSNormGated, ShortConvolution, resolve_gdn2_backend
 from .gdn2_ops import (ChunkGDN2Function, chunk_gdn2, fused_recurrent_gdn2,
-                       fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step)
+                       fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step, TokenLogprobs,
+                       token_logprobs)
 from .registry import BLOCKS, build_block
 
 __all__ = [
@@ -18,6 +19,7 @@ __all__ = [
     "GatedDeltaNet2",
     "RMSNormGated",
     "ShortConvolution",
+    "TokenLogprobs",
     "build_block",
     "chunk_gdn2",
     "fused_recurrent_gdn2",
@@ -25,4 +27,5 @@ __all__ = [
     "gated_scan",
     "gated_scan_step",
     "resolve_gdn2_backend",
+    "token_logprobs",
 ]

@@ -53,6 +53,8 @@ EXPORTS = (
     "gdn2_scan_fwd",
     "gdn2_scan_bwd",
     "gdn2_scan_step",
+    "gdn2_logprob_fwd",
+    "gdn2_logprob_bwd",
     "gdn2_fault_status",
     "gdn2_test_fwd_state_wait_timeout",
 )
@@ -153,6 +155,18 @@ class ScanProblem(ctypes.Structure):
     ]
 
 
+class LogprobProblem(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64),
+        ("ld", c_int64),
+        ("ignore_index", c_int64),
+        ("vocab", c_int32),
+        ("dtype", c_int32),
+        ("top_k", c_int32),
+        ("temperature", c_float),
+    ]
+
+
 class GDN2Error(RuntimeError):
     """A libgdn2_b200 entry point returned an error status."""
 
@@ -172,6 +186,7 @@ def _declare(lib):
     vp = P(ConvProblem)
     np_ = P(NormProblem)
     sp = P(ScanProblem)
+    lp = P(LogprobProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -208,6 +223,8 @@ def _declare(lib):
         "gdn2_scan_workspace_bytes": ([sp], c_size_t),
         "gdn2_scan_fwd": ([sp, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
         "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_scan_step": ([sp, v, v, v, v, c_int64, c_int32, v, v, v], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

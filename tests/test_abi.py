@@ -252,3 +252,28 @@ def test_scan_arguments_are_checked(lib):
     assert step(sp(T=1), pool=1) == N.ERR_INVALID
     assert step(sp(T=1), stride=69) == N.ERR_INVALID
     assert lib.gdn2_scan_step(sp(T=1, B=0, n_seqs=0), *([None] * 4), 70, 0, None, None, None) == 0
+
+
+def test_logprob_arguments_are_checked(lib):
+    """Token log probabilities: sizes, types and pointers are validated before
+    any CUDA call."""
+    def lp(**kw):
+        base = dict(rows=4, ld=1000, ignore_index=-100, vocab=1000, dtype=1, top_k=5,
+                    temperature=1.0)
+        base.update(kw)
+        return N.LogprobProblem(**base)
+
+    f = ctypes.c_void_p(0x1000)
+    fwd = lambda p, x=f, top=f, st=None: lib.gdn2_logprob_fwd(p, x, f, f, None, top, top, st, None)
+    for bad, code in ((lp(rows=-1), N.ERR_INVALID), (lp(vocab=0), N.ERR_INVALID),
+                      (lp(dtype=9), N.ERR_INVALID), (lp(ld=999), N.ERR_INVALID),
+                      (lp(temperature=0.0), N.ERR_INVALID),
+                      (lp(temperature=float("nan")), N.ERR_INVALID),
+                      (lp(top_k=-1), N.ERR_INVALID), (lp(top_k=1001), N.ERR_INVALID),
+                      (lp(top_k=129), N.ERR_UNSUPPORTED), (lp(rows=1 << 40), N.ERR_UNSUPPORTED)):
+        assert fwd(bad) == code, lib.gdn2_last_error()
+    assert fwd(lp(), x=None) == N.ERR_INVALID
+    assert fwd(lp(), top=None) == N.ERR_INVALID
+    assert fwd(lp(), st=ctypes.c_void_p(0x1004)) == N.ERR_INVALID
+    assert lib.gdn2_logprob_bwd(lp(), f, f, None, f, None, f, None) == N.ERR_INVALID
+    assert fwd(lp(rows=0), x=None) == N.OK

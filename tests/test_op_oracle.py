@@ -44,3 +44,18 @@ def test_scan_gradients_are_the_differences(gate, cu):
     for x, dx in zip((v, g, w, h0), grads):
         if x is not None:
             assert np.abs(differences(loss, x) - dx).max() < TOL
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.6])
+def test_logprob_gradients_are_the_differences(temperature):
+    rng = np.random.default_rng(4)
+    x = 2 * rng.standard_normal((4, 9))
+    ids = np.array([3, -100, 0, 8])
+    dlogp, dent = rng.standard_normal(4), rng.standard_normal(4)
+
+    def loss():
+        logp, ent, _ = O.token_logprobs(x, ids, temperature)
+        return (logp * dlogp).sum() + (ent * dent).sum()
+
+    dx = O.token_logprobs_bwd(x, ids, dlogp, dent, temperature)
+    assert np.abs(differences(loss, x) - dx).max() < TOL
