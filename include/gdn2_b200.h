@@ -419,6 +419,45 @@ int gdn2_logprob_bwd(const gdn2_logprob_problem* p, const void* logits,
                      const float* dlogprobs, const float* dentropy,
                      void* dlogits, void* stream);
 
+/* ---- AdamW over many tensors ----------------------------------------------
+ * One step (decoupled weight decay) for n tensors, 400 per launch, fp32
+ * arithmetic:
+ *   g = grad * grad_scale;  m = beta1 m + (1-beta1) g;  v = beta2 v + (1-beta2) g^2
+ *   p = p (1 - lr weight_decay)
+ *       - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * Parameters have `dtype`, gradients `dtype` or fp32, all contiguous.  With
+ * `master` (for all tensors or none) p is the fp32 master weight, and `param`
+ * its rounding; otherwise p is `param` itself, rounded to nearest after the
+ * step.  state_bits = 32: exp_avg and exp_avg_sq are fp32.  state_bits = 8:
+ * they are float8 e4m3 codes; blocks of 256 consecutive elements share a
+ * scale (fp32 [ceil(numel / 256)]), an element's m is code * exp_avg_scale and
+ * its v is (code * exp_avg_sq_scale)^2.  Blocks whose largest value is below
+ * 1e-30 are held as zeros.  All zeros is a valid start.  grad_scale and
+ * found_inf are device scalars or NULL: a nonzero found_inf leaves everything
+ * as it is.  The struct array is read before the call returns. */
+typedef struct gdn2_adamw_problem {
+    int32_t dtype, grad_dtype;
+    int32_t state_bits;
+    int64_t step;              /* of this step, from 1 */
+    double lr, beta1, beta2, eps, weight_decay;
+    const float* grad_scale;
+    const float* found_inf;
+} gdn2_adamw_problem;
+
+typedef struct gdn2_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    float* master;
+    int64_t numel;
+} gdn2_adamw_tensor;
+
+int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensors,
+                    int32_t n, void* stream);
+
 /* Device-side fault bits.  Kernels that wait on asynchronous copies or on
  * tensor-core completion bound every wait in time (about one second); a wait
  * that runs out makes the kernel release its tensor memory, return without

@@ -89,3 +89,33 @@ def token_logprobs_bwd(x, ids, dlogp, dent=None, temperature=1.0, ignore=-100):
 def top_tokens(x, k):
     """Indices of the k largest of each row, equal values by rising index."""
     return np.argsort(-x, axis=1, kind="stable")[:, :k]
+
+
+def e4m3(u):
+    """u rounded to the nearest e4m3 value (ties to even); |u| <= 448."""
+    step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(u), 2.0 ** -6))) - 3)
+    return np.round(u / step) * step
+
+
+def encode8(x, nonzero=False, block=256):
+    """(codes, scales) of a flat array: x ~ codes * scale of its block."""
+    codes, scales = np.zeros(x.size), np.zeros(-(-x.size // block))
+    for b in range(scales.size):
+        part = x[b * block:(b + 1) * block]
+        most = np.abs(part).max()
+        if most <= 1e-30:
+            continue
+        q = e4m3(part * (448.0 / most))
+        if nonzero:
+            q[(part > 0) & (q == 0)] = 2.0 ** -9
+        codes[b * block:(b + 1) * block] = q
+        scales[b] = most / 448.0
+    return codes, scales
+
+
+def adamw(p, g, m, v, step, lr, b1, b2, eps, wd):
+    """(p, m, v) after one step."""
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    mhat, vhat = m / (1 - b1 ** step), v / (1 - b2 ** step)
+    return p - lr * wd * p - lr * mhat / (np.sqrt(vhat) + eps), m, v

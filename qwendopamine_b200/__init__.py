@@ -7,12 +7,13 @@ keep the reference kernel entry points.  All compute runs in
 """
 
 from .gdn2 import GDN2_BACKENDS, GatedDeltaNet2, RMSNormGated, ShortConvolution, resolve_gdn2_backend
-from .gdn2_ops import (ChunkGDN2Function, chunk_gdn2, fused_recurrent_gdn2,
+from .gdn2_ops import (AdamW, ChunkGDN2Function, adamw_step, chunk_gdn2, fused_recurrent_gdn2,
                        fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step, TokenLogprobs,
                        token_logprobs)
 from .registry import BLOCKS, build_block
 
 __all__ = [
+    "AdamW",
     "BLOCKS",
     "ChunkGDN2Function",
     "GDN2_BACKENDS",
@@ -20,6 +21,7 @@ __all__ = [
     "RMSNormGated",
     "ShortConvolution",
     "TokenLogprobs",
+    "adamw_step",
     "build_block",
     "chunk_gdn2",
     "fused_recurrent_gdn2",

@@ -12,7 +12,7 @@ import contextlib
 import ctypes
 import os
 import threading
-from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -55,6 +55,7 @@ EXPORTS = (
     "gdn2_scan_step",
     "gdn2_logprob_fwd",
     "gdn2_logprob_bwd",
+    "gdn2_adamw_step",
     "gdn2_fault_status",
     "gdn2_test_fwd_state_wait_timeout",
 )
@@ -167,6 +168,27 @@ class LogprobProblem(ctypes.Structure):
     ]
 
 
+class AdamWProblem(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32),
+        ("grad_dtype", c_int32),
+        ("state_bits", c_int32),
+        ("step", c_int64),
+        ("lr", c_double),
+        ("beta1", c_double),
+        ("beta2", c_double),
+        ("eps", c_double),
+        ("weight_decay", c_double),
+        ("grad_scale", c_void_p),
+        ("found_inf", c_void_p),
+    ]
+
+
+# gdn2_adamw_tensor as 64-bit words: param, grad, exp_avg, exp_avg_sq,
+# exp_avg_scale, exp_avg_sq_scale, master, numel
+ADAMW_TENSOR_WORDS = 8
+
+
 class GDN2Error(RuntimeError):
     """A libgdn2_b200 entry point returned an error status."""
 
@@ -187,6 +209,7 @@ def _declare(lib):
     np_ = P(NormProblem)
     sp = P(ScanProblem)
     lp = P(LogprobProblem)
+    ap = P(AdamWProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -225,6 +248,7 @@ def _declare(lib):
         "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_adamw_step": ([ap, v, c_int32, v], ctypes.c_int),
         "gdn2_scan_step": ([sp, v, v, v, v, c_int64, c_int32, v, v, v], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

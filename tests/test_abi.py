@@ -277,3 +277,34 @@ def test_logprob_arguments_are_checked(lib):
     assert fwd(lp(), st=ctypes.c_void_p(0x1004)) == N.ERR_INVALID
     assert lib.gdn2_logprob_bwd(lp(), f, f, None, f, None, f, None) == N.ERR_INVALID
     assert fwd(lp(rows=0), x=None) == N.OK
+
+
+def test_adamw_arguments_are_checked(lib):
+    """AdamW: hyperparameters, types and pointers are validated before any
+    CUDA call; the struct array has the layout the binding fills."""
+    def ap(**kw):
+        base = dict(dtype=1, grad_dtype=1, state_bits=32, step=1, lr=1e-3, beta1=0.9, beta2=0.99,
+                    eps=1e-8, weight_decay=0.1, grad_scale=None, found_inf=None)
+        base.update(kw)
+        return N.AdamWProblem(**base)
+
+    def tensors(*rows):
+        flat = [w for r in rows for w in r]
+        return (ctypes.c_int64 * len(flat))(*flat)
+
+    a = 0x1000
+    good, empty = (a, a, a, a, 0, 0, 0, 10), (0, 0, 0, 0, 0, 0, 0, 0)
+    call = lambda p, *rows: lib.gdn2_adamw_step(p, tensors(*rows), len(rows), None)
+    for bad, code in ((ap(dtype=4), N.ERR_INVALID), (ap(grad_dtype=2), N.ERR_UNSUPPORTED),
+                      (ap(state_bits=16), N.ERR_INVALID), (ap(step=0), N.ERR_INVALID),
+                      (ap(beta1=1.0), N.ERR_INVALID), (ap(beta2=-0.1), N.ERR_INVALID),
+                      (ap(eps=float("nan")), N.ERR_INVALID), (ap(lr=float("inf")), N.ERR_INVALID)):
+        assert call(bad, empty) == code, lib.gdn2_last_error()
+    assert call(ap(), good[:7] + (-1,)) == N.ERR_INVALID
+    assert call(ap(), good[:7] + (1 << 44,)) == N.ERR_UNSUPPORTED
+    assert call(ap(), (0,) + good[1:]) == N.ERR_INVALID
+    assert call(ap(state_bits=8), good) == N.ERR_INVALID  # no scales
+    assert call(ap(), good[:6] + (a, 10), good) == N.ERR_INVALID  # master for one of two
+    assert call(ap(), empty, empty) == N.OK
+    assert lib.gdn2_adamw_step(ap(), None, 0, None) == N.OK
+    assert lib.gdn2_adamw_step(ap(), None, 1, None) == N.ERR_INVALID
