@@ -339,11 +339,24 @@ def phase(name: str, stream=None):
         rec.append((name, s, e))
 
 
-def on_device(device: torch.device):
-    """Makes ``device`` current for a launch (a no-op when it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_HERE = contextlib.nullcontext()
+
+
+def on_device(index: int):
+    """Makes the device of that index current for a launch (nothing to do when
+    it already is)."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def addr(t):
+    """Device address of a tensor as a plain integer (None -> NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of the device of that index, as ``stream_of`` gives
+    it, without building a stream object (small launches)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t):

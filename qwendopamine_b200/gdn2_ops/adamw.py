@@ -12,8 +12,8 @@ is the state before the first step.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from operator import attrgetter
 
 import torch
@@ -25,15 +25,12 @@ __all__ = ["AdamW", "adamw_step", "STATE_BLOCK"]
 STATE_BLOCK = 256  # elements that share a scale in the 8-bit states
 
 _ptr, _numel, _dense = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_dtype, _device = attrgetter("dtype"), attrgetter("device")
+_dtype, _device = attrgetter("dtype"), torch.Tensor.get_device
 
 
-def _uniform(name, tensors, dtype, device):
-    """Refuse tensors of a state list that are not what the kernel reads."""
-    if not all(map(_dense, tensors)):
-        raise ValueError(f"adamw_step: {name} must be contiguous")
-    if set(map(_dtype, tensors)) != {dtype} or set(map(_device, tensors)) != {device}:
-        raise ValueError(f"adamw_step: {name} must all be {dtype} on {device}")
+# places of the lists in a row of gdn2_adamw_tensor words
+_COLUMN = {"params": 0, "grads": 1, "exp_avgs": 2, "exp_avg_sqs": 3, "exp_avg_scales": 4,
+           "exp_avg_sq_scales": 5, "master_params": 6}
 
 
 def _scalar(name, t, device):
@@ -87,46 +84,43 @@ def adamw_step(
             raise ValueError(f"adamw_step: {name} has {len(x)} tensors, params {n}")
     if n == 0:
         return
-    device, dtype = params[0].device, params[0].dtype
+    device, dtype, gdtype = params[0].device, params[0].dtype, grads[0].dtype
     if device.type != "cuda":
         raise RuntimeError("adamw_step: tensors must be CUDA tensors -- the B200 build has no CPU "
                            "path")
     code = N.dtype_code(dtype)
-    gdtype = grads[0].dtype
     if gdtype != dtype and gdtype != torch.float32:
         raise NotImplementedError(f"adamw_step: gradients ({gdtype}) must be float32 or have the "
                                   f"parameters' dtype ({dtype})")
     sdtype = torch.float8_e4m3fn if eight else torch.float32
-    if not all(map(_dense, grads)):
-        grads = lists["grads"] = [g.contiguous() for g in grads]
-    for name, x, want in (("params", params, dtype), ("grads", grads, gdtype),
-                          ("exp_avgs", exp_avgs, sdtype), ("exp_avg_sqs", exp_avg_sqs, sdtype)):
-        _uniform(name, x, want, device)
+    want = {"params": dtype, "grads": gdtype, "exp_avgs": sdtype, "exp_avg_sqs": sdtype}
     sizes = list(map(_numel, params))
+    # one row of 64-bit words for each tensor, filled a column (a list) at a time
+    words = [0] * (n * N.ADAMW_TENSOR_WORDS)
+    words[N.ADAMW_TENSOR_WORDS - 1::N.ADAMW_TENSOR_WORDS] = sizes
     for name, x in lists.items():
-        if name in ("exp_avg_scales", "exp_avg_sq_scales"):
-            _uniform(name, x, torch.float32, device)
+        if set(map(_dtype, x)) != {want.get(name, torch.float32)} \
+                or set(map(_device, x)) != {device.index}:
+            raise ValueError(f"adamw_step: {name} must all be {want.get(name, torch.float32)} on "
+                             f"{device}")
+        if not all(map(_dense, x)):
+            if x is not grads:
+                raise ValueError(f"adamw_step: {name} must be contiguous")
+            x = grads = [g.contiguous() for g in grads]
+        if name.endswith("scales"):
             if list(map(_numel, x)) != [-(-s // STATE_BLOCK) for s in sizes]:
                 raise ValueError(f"adamw_step: {name} need one value for each {STATE_BLOCK} "
                                  "elements")
-        elif name != "params" and list(map(_numel, x)) != sizes:
+        elif x is not params and list(map(_numel, x)) != sizes:
             raise ValueError(f"adamw_step: {name} must have the parameters' sizes")
-    if master_params is not None:
-        _uniform("master_params", master_params, torch.float32, device)
-    none = [0] * n
-    words = [none] * N.ADAMW_TENSOR_WORDS
-    for i, x in enumerate((params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
-                           exp_avg_sq_scales, master_params)):
-        if x is not None:
-            words[i] = list(map(_ptr, x))
-    words[-1] = sizes
-    table = (ctypes.c_int64 * (n * N.ADAMW_TENSOR_WORDS))(*(w for row in zip(*words) for w in row))
+        words[_COLUMN[name]::N.ADAMW_TENSOR_WORDS] = list(map(_ptr, x))
     prob = N.AdamWProblem(code, N.dtype_code(gdtype), 8 if eight else 32, int(step), lr, betas[0],
                           betas[1], eps, weight_decay,
-                          N.ptr(_scalar("grad_scale", grad_scale, device)),
-                          N.ptr(_scalar("found_inf", found_inf, device)))
-    with N.on_device(device):
-        N.check(N.load().gdn2_adamw_step(prob, table, n, N.stream_of(device)), "gdn2_adamw_step")
+                          N.addr(_scalar("grad_scale", grad_scale, device)),
+                          N.addr(_scalar("found_inf", found_inf, device)))
+    with N.on_device(device.index):
+        N.check(N.load().gdn2_adamw_step(prob, struct.pack(f"{len(words)}q", *words), n,
+                                         N.raw_stream(device.index)), "gdn2_adamw_step")
 
 
 class AdamW(torch.optim.Optimizer):

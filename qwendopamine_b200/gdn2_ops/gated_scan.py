@@ -15,6 +15,8 @@ One launch of ``libgdn2_b200.so`` each (``gdn2_scan_fwd`` / ``gdn2_scan_bwd`` /
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -27,6 +29,8 @@ def _rows(x, B, T, D):
     """``x`` as rows ``[B*T, D]`` with one row stride, and that stride; copied
     only when its strides are not those of such a matrix (a slice of a fused
     projection is)."""
+    if x.is_contiguous():
+        return x, D
     x = x.reshape(B, T, D)
     sb, st, sd = x.stride()
     if T == 1:
@@ -43,7 +47,7 @@ class _Geometry:
 
     def __init__(self, v, g, w, cu):
         self.B, self.T = v.shape[0], v.shape[1]
-        self.D = v[0, 0].numel() if v.shape[0] and v.shape[1] else _width(v.shape[2:])
+        self.D = _width(v.shape[2:])
         self.n = self.B if cu is None else cu.numel() - 1
         self.v, self.ldv = _rows(v, self.B, self.T, self.D)
         self.g, self.ldg = _rows(g, self.B, self.T, self.D)
@@ -52,35 +56,31 @@ class _Geometry:
 
     def problem(self, ld_dy=None):
         return N.ScanProblem(self.B, self.D, self.T, N.dtype_code(self.v.dtype),
-                             N.dtype_code(self.g.dtype), self.n, N.ptr(self.cu), self.ldv,
+                             N.dtype_code(self.g.dtype), self.n, N.addr(self.cu), self.ldv,
                              self.ldg, self.ldw, self.D if ld_dy is None else ld_dy)
 
 
-def _width(shape):
-    n = 1
-    for s in shape:
-        n *= int(s)
-    return n
+_width = math.prod  # elements of a shape
 
 
 def _workspace(lib, prob, device):
     return torch.empty(lib.gdn2_scan_workspace_bytes(prob), dtype=torch.uint8, device=device)
 
 
-def _forward(geo, h0, want_final, keep):
+def _forward(geo, shape, h0, want_final, keep):
     lib = N.load()
     dev = geo.v.device
     prob = geo.problem()
-    y = torch.empty(geo.B, geo.T, geo.D, dtype=geo.v.dtype, device=dev)
+    y = torch.empty(shape, dtype=geo.v.dtype, device=dev)
     ht = torch.empty(geo.n, geo.D, dtype=torch.float32, device=dev) if want_final else None
     saved = None
     if keep:
         saved = torch.empty(lib.gdn2_scan_saved_bytes(prob) // 4, dtype=torch.float32, device=dev)
-    with N.on_device(dev):
+    with N.on_device(dev.index):
         ws = _workspace(lib, prob, dev)
-        N.check(lib.gdn2_scan_fwd(prob, N.ptr(geo.v), N.ptr(geo.g), N.ptr(geo.w), N.ptr(h0),
-                                  N.ptr(y), N.ptr(ht), N.ptr(saved), N.ptr(ws), ws.numel(),
-                                  N.stream_of(dev)), "gdn2_scan_fwd")
+        N.check(lib.gdn2_scan_fwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
+                                  N.addr(y), N.addr(ht), N.addr(saved), N.addr(ws), ws.numel(),
+                                  N.raw_stream(dev.index)), "gdn2_scan_fwd")
     return y, ht, saved
 
 
@@ -89,11 +89,10 @@ class GatedScanFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, v, g, w, h0, cu, want_final):
-        geo = _Geometry(v, g, w, cu)
-        y, ht, saved = _forward(geo, h0, want_final, keep=True)
+        y, ht, saved = _forward(_Geometry(v, g, w, cu), v.shape, h0, want_final, keep=True)
         ctx.save_for_backward(v, g, w, h0, cu, saved)
         ctx.set_materialize_grads(False)
-        return y.view(v.shape), ht
+        return y, ht
 
     @staticmethod
     @once_differentiable
@@ -112,12 +111,12 @@ class GatedScanFunction(torch.autograd.Function):
         dv, dg = new(v), new(g)
         dw = new(w) if w is not None else None
         dh0 = new(h0) if h0 is not None else None
-        with N.on_device(dev):
+        with N.on_device(dev.index):
             ws = _workspace(lib, prob, dev)
-            N.check(lib.gdn2_scan_bwd(prob, N.ptr(geo.v), N.ptr(geo.g), N.ptr(geo.w), N.ptr(h0),
-                                      N.ptr(saved), N.ptr(dy), N.ptr(dht), N.ptr(dv), N.ptr(dg),
-                                      N.ptr(dw), N.ptr(dh0), N.ptr(ws), ws.numel(),
-                                      N.stream_of(dev)), "gdn2_scan_bwd")
+            N.check(lib.gdn2_scan_bwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
+                                      N.addr(saved), N.addr(dy), N.addr(dht), N.addr(dv), N.addr(dg),
+                                      N.addr(dw), N.addr(dh0), N.addr(ws), ws.numel(),
+                                      N.raw_stream(dev.index)), "gdn2_scan_bwd")
         return dv, dg, dw, dh0, None, None
 
 
@@ -188,9 +187,9 @@ def gated_scan(
             t is not None and t.requires_grad for t in (v, g, w, h0)):
         y, ht = GatedScanFunction.apply(v, g, w, h0, cu, bool(output_final_state))
     else:
-        y, ht, _ = _forward(_Geometry(v, g, w, cu), h0, bool(output_final_state), keep=False)
-        y = y.view(v.shape)
-    return y, ht.view(n, *v.shape[2:]) if ht is not None else None
+        y, ht, _ = _forward(_Geometry(v, g, w, cu), v.shape, h0, bool(output_final_state),
+                            keep=False)
+    return y, ht.view(n, *v.shape[2:]) if ht is not None and v.ndim > 3 else ht
 
 
 def gated_scan_step(
@@ -216,7 +215,8 @@ def gated_scan_step(
     if state.device != v.device or state.shape[1:] != v.shape[1:]:
         raise ValueError(f"state must be [S, *{tuple(v.shape[1:])}] on {v.device}; got "
                          f"{tuple(state.shape)} on {state.device}")
-    if not state[:1].is_contiguous() or (state.shape[0] > 1 and state.stride(0) < D):
+    if not state.is_contiguous() and (not state[:1].is_contiguous() or (
+            state.shape[0] > 1 and state.stride(0) < D)):
         raise ValueError("state must hold each sequence's channels contiguously")
     idx = None
     if state_indices is not None:
@@ -231,13 +231,13 @@ def gated_scan_step(
         return y
     if state.shape[0] == 0:
         return y.zero_()
-    with torch.no_grad():
-        (v, ldv), (g, ldg) = _rows(v, n, 1, D), _rows(g, n, 1, D)
-        w, ldw = _rows(w, n, 1, D) if w is not None else (None, D)
-        prob = N.ScanProblem(n, D, 1, N.dtype_code(v.dtype), N.dtype_code(g.dtype), n, None, ldv,
-                             ldg, ldw, D)
-        with N.on_device(v.device):
-            N.check(N.load().gdn2_scan_step(
-                prob, N.ptr(v), N.ptr(g), N.ptr(w), N.ptr(state), max(state.stride(0), D),
-                state.shape[0], N.ptr(idx), N.ptr(y), N.stream_of(v.device)), "gdn2_scan_step")
+    (v, ldv), (g, ldg) = _rows(v, n, 1, D), _rows(g, n, 1, D)
+    w, ldw = _rows(w, n, 1, D) if w is not None else (None, D)
+    prob = N.ScanProblem(n, D, 1, N.dtype_code(v.dtype), N.dtype_code(g.dtype), n, None, ldv, ldg,
+                         ldw, D)
+    index = v.device.index
+    with N.on_device(index):
+        N.check(N.load().gdn2_scan_step(
+            prob, N.addr(v), N.addr(g), N.addr(w), N.addr(state), max(state.stride(0), D),
+            state.shape[0], N.addr(idx), N.addr(y), N.raw_stream(index)), "gdn2_scan_step")
     return y

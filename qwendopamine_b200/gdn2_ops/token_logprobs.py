@@ -33,6 +33,8 @@ class TokenLogprobs(NamedTuple):
 def _matrix(logits):
     """``logits`` as ``[rows, V]`` with one row stride, copied only if need be."""
     V = logits.shape[-1]
+    if logits.ndim == 2 and logits.is_contiguous():
+        return logits, V
     x = logits.reshape(-1, V)
     if (x.stride(1) != 1 and V > 1) or (x.shape[0] > 1 and x.stride(0) < V):
         x = x.contiguous()
@@ -52,10 +54,10 @@ def _forward(x, ld, ids, top_k, entropy, temperature, ignore_index, keep):
     top = f32(rows, top_k) if top_k else None
     top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
     stats = f32(rows, 4) if keep else None
-    with N.on_device(dev):
+    with N.on_device(dev.index):
         N.check(N.load().gdn2_logprob_fwd(
-            _problem(x, ld, top_k, temperature, ignore_index), N.ptr(x), N.ptr(ids), N.ptr(logp),
-            N.ptr(ent), N.ptr(top), N.ptr(top_ids), N.ptr(stats), N.stream_of(dev)),
+            _problem(x, ld, top_k, temperature, ignore_index), N.addr(x), N.addr(ids), N.addr(logp),
+            N.addr(ent), N.addr(top), N.addr(top_ids), N.addr(stats), N.raw_stream(dev.index)),
             "gdn2_logprob_fwd")
     return logp, ent, top, top_ids, stats
 
@@ -86,10 +88,10 @@ class TokenLogprobsFunction(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dlogp = dlogp.float().contiguous() if dlogp is not None else None
         dent = dent.float().contiguous() if dent is not None else None
-        with N.on_device(x.device):
+        with N.on_device(x.device.index):
             N.check(N.load().gdn2_logprob_bwd(
-                _problem(x, ld, 0, temperature, ignore_index), N.ptr(x), N.ptr(ids), N.ptr(stats),
-                N.ptr(dlogp), N.ptr(dent), N.ptr(dx), N.stream_of(x.device)), "gdn2_logprob_bwd")
+                _problem(x, ld, 0, temperature, ignore_index), N.addr(x), N.addr(ids), N.addr(stats),
+                N.addr(dlogp), N.addr(dent), N.addr(dx), N.raw_stream(x.device.index)), "gdn2_logprob_bwd")
         return dx.view(logits.shape), None, None, None, None, None
 
 
