@@ -420,7 +420,7 @@ int gdn2_logprob_bwd(const gdn2_logprob_problem* p, const void* logits,
                      void* dlogits, void* stream);
 
 /* ---- AdamW over many tensors ----------------------------------------------
- * One step (decoupled weight decay) for n tensors, 400 per launch, fp32
+ * One step (decoupled weight decay) for n tensors, 96 per launch, fp32
  * arithmetic:
  *   g = grad * grad_scale;  m = beta1 m + (1-beta1) g;  v = beta2 v + (1-beta2) g^2
  *   p = p (1 - lr weight_decay)

@@ -29,8 +29,11 @@
 // reads those of the tiles before it in its group of kGroup tiles, and the
 // state leaving the previous group, which that group's last tile publishes.
 // The order of the products is fixed by the positions alone: results do not
-// depend on timing.  Waits are bounded; one that runs out sets bit 4 of the
-// fault word and turns the tile's carry into NaN.
+// depend on timing.  A published pair is one 64-bit word that is all ones
+// before (no decay product is that NaN), so it needs no flag and no fence, and
+// a tile has all it reads in flight at once, eight words to a thread.  Waits
+// are bounded; one that runs out sets bit 4 of the fault word and turns the
+// tile's carry into NaN.
 #include "op_util.cuh"
 
 namespace gdn2 {
@@ -41,6 +44,7 @@ constexpr int kLanes = 16;        // threads across a tile's channels
 constexpr int kCpt = 4;           // channels of a thread
 constexpr int kSlots = 16;        // threads down a tile's rows
 constexpr int kScanThreads = kLanes * kSlots;
+constexpr int kWarps = kScanThreads / 32;
 constexpr int kFwdRows = 8;       // rows of a thread, forward
 constexpr int kBwdRows = 4;       // and backward (twice the tensors in registers)
 constexpr int kSaveRows = kSlots * kBwdRows;  // rows between states kept for the backward
@@ -58,13 +62,12 @@ struct ScanArgs {
   const float *h0, *dht;
   void *y, *dv, *dg, *dw;
   float *ht, *dh0, *saved;
-  unsigned *ticket, *flags, *gflags, *fault;
-  float2* agg;
-  float* gstate;
+  unsigned *ticket, *fault;
+  uint64_t *runs, *states;
 };
 
 struct ScanWorkspace {
-  size_t flags, gflags, zeroed, agg, gstate, total;
+  size_t runs, states, total;
 };
 
 ScanWorkspace scan_workspace(int64_t rows, int D, int tile) {
@@ -72,107 +75,149 @@ ScanWorkspace scan_workspace(int64_t rows, int D, int tile) {
   const size_t nslab = (size_t)(D + kSlab - 1) / kSlab;
   const size_t nt = (size_t)((rows + tile - 1) / tile), ng = (nt + kGroup - 1) / kGroup;
   size_t off = 256;  // the tile counter
-  w.flags = off; off += nt * nslab * 4;
-  w.gflags = off; off += ng * nslab * 4;
-  w.zeroed = off = align256(off);
-  w.agg = off; off = align256(off + nt * nslab * kSlab * sizeof(float2));
-  w.gstate = off; off = align256(off + ng * nslab * kSlab * sizeof(float));
+  w.runs = off; off += nt * nslab * kSlab * sizeof(uint64_t);
+  w.states = off; off += ng * nslab * kSlab * sizeof(uint64_t);
   w.total = off;
   return w;
 }
 
+// A run of rows: A in x (-1: it holds a reset), H in y.
 __device__ __forceinline__ float2 compose(float2 p, float2 q) {
   if (q.x < 0.f) return q;
   return make_float2(p.x < 0.f ? -1.f : p.x * q.x, fmaf(q.x, p.y, q.y));
 }
 
-// State after a run (A, H) that is entered with h.
+// State after a run that is entered with h.
 __device__ __forceinline__ float leave(float2 p, float h) {
   return p.x < 0.f ? p.y : fmaf(p.x, h, p.y);
 }
 
-__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+__device__ __forceinline__ uint64_t load_word(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void store_release(unsigned* p, unsigned v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ bool is_there(uint64_t v) { return (uint32_t)v != 0xffffffffu; }
+__device__ __forceinline__ float2 run_of(uint64_t v) {
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ void publish(uint64_t* p, float2 r) {
+  const uint32_t x = r.x != r.x ? 0x7fffffffu : __float_as_uint(r.x);
+  const uint64_t v = ((uint64_t)__float_as_uint(r.y) << 32) | x;
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-__device__ __forceinline__ void sync_pair() { asm volatile("bar.sync 1, 64;" ::: "memory"); }
 
-// Every lane with `want` waits for its flag; false if the time ran out.
-__device__ __forceinline__ bool wait_flags(const unsigned* p, bool want) {
-  bool there = !want || load_acquire(p) != 0u;
-  if (__all_sync(0xffffffffu, there)) return true;
+// Polls until the word is there; false if the time ran out.
+__device__ __forceinline__ bool wait_word(const uint64_t* p, uint64_t& v) {
+  if (is_there(v)) return true;
   const uint64_t t0 = now_ns();
   for (int round = 0; round < (1 << 24); ++round) {
-    there = there || load_acquire(p) != 0u;
-    if (__all_sync(0xffffffffu, there)) return true;
-    if (__any_sync(0xffffffffu, now_ns() - t0 > kScanWaitNs)) return false;
+    v = load_word(p);
+    if (is_there(v)) return true;
+    if (now_ns() - t0 > kScanWaitNs) return false;
   }
   return false;
 }
 
 struct ScanShared {
-  float2 part[kSlots][kSlab];
-  float carry[kSlab];
+  float2 part[kWarps][kSlab];   // runs of the warps' slot pairs, then the runs before them
+  float2 past[4][kSlab];        // runs of eight tiles of the group each
+  float carry[kSlab];           // state entering the tile
   unsigned item;
 };
 
-// Turns s.part[slot] into the run before each slot and s.carry into the state
-// that enters the tile; called by threads 0 .. 63, one per channel.  `pos` is
-// the tile's place in processing order; `up` walks the slots from the last.
+// A warp holds two slots of rows.  Puts their joint run into part[warp] and
+// returns the run of the warp's rows before this thread's.
+template <bool UP>
+__device__ __forceinline__ void join_pair(float2 (*part)[kSlab], const float (&A)[kCpt],
+                                          const float (&H)[kCpt], float2 (&before)[kCpt]) {
+  const int lane = threadIdx.x & 31, lc = (lane % kLanes) * kCpt;
+  const bool leads = (lane < kLanes) != UP;
+#pragma unroll
+  for (int j = 0; j < kCpt; ++j) {
+    const float2 mine = make_float2(A[j], H[j]);
+    const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, A[j], kLanes),
+                                     __shfl_xor_sync(0xffffffffu, H[j], kLanes));
+    before[j] = leads ? make_float2(1.f, 0.f) : other;
+    if (leads) part[threadIdx.x >> 5][lc + j] = compose(mine, other);
+  }
+}
+
+// Turns part[] into the runs before each warp; returns the tile's run.
+template <bool UP> __device__ __forceinline__ float2 fold_warps(float2 (*part)[kSlab], int ch) {
+  float2 p[kWarps], run = make_float2(1.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) p[k] = part[UP ? kWarps - 1 - k : k][ch];
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) {
+    part[UP ? kWarps - 1 - k : k][ch] = run;
+    run = compose(run, p[k]);
+  }
+  return run;
+}
+
+// Sets s.carry, the state that enters the tile, given s.part of join_pair;
+// `pos` is the tile's place in processing order.  Called by all threads after
+// a barrier; ends with one.
 template <bool UP>
 __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared& s, int64_t pos, int slab) {
-  const int ch = threadIdx.x, lane = threadIdx.x & 31;
-  float2 run = make_float2(1.f, 0.f);
-#pragma unroll
-  for (int k = 0; k < kSlots; ++k) {
-    const int slot = UP ? kSlots - 1 - k : k;
-    const float2 p = s.part[slot][ch];
-    s.part[slot][ch] = run;
-    run = compose(run, p);
+  const int ch = threadIdx.x % kSlab, q = threadIdx.x / kSlab;
+  const int64_t group = pos / kGroup, first = group * kGroup;
+  const int n = (int)(pos - first);
+  const int64_t stride = (int64_t)a.nslab * kSlab, at = (int64_t)slab * kSlab + ch;
+  float2 run;
+  uint64_t state = 0;
+  bool ok = true;
+  if (q == 0) {
+    run = fold_warps<UP>(s.part, ch);
+    if (a.chained) {
+      // the last tile's run is only needed in the group's state
+      if (n < kGroup - 1) publish(a.runs + pos * stride + at, run);
+      if (group > 0) state = load_word(a.states + (group - 1) * stride + at);
+    }
   }
-  float carry = 0.f;
   if (a.chained) {
-    const int64_t group = pos / kGroup, first = group * kGroup;
-    const int n = (int)(pos - first);
-    const int64_t at = pos * a.nslab + slab;
-    if (n < kGroup - 1) {  // the last tile's run is part of the group's state
-      a.agg[at * kSlab + ch] = run;
-      __threadfence();
-      sync_pair();
-      if (ch == 0) store_release(a.flags + at, 1u);
-    }
-    bool ok = wait_flags(a.flags + (first + lane) * a.nslab + slab, lane < n);
+    const uint64_t* p = a.runs + (first + q * (kGroup / 4)) * stride + at;
+    uint64_t v[kGroup / 4];
+#pragma unroll
+    for (int k = 0; k < kGroup / 4; ++k)
+      if (q * (kGroup / 4) + k < n) v[k] = load_word(p + k * stride);
     float2 acc = make_float2(1.f, 0.f);
-    for (int k = 0; k < n; ++k)
-      acc = compose(acc, __ldcg(a.agg + ((first + k) * a.nslab + slab) * kSlab + ch));
-    carry = acc.y;
-    if (group > 0 && !(acc.x < 0.f)) {
-      const int64_t before = (group - 1) * a.nslab + slab;
-      ok = wait_flags(a.gflags + before, lane == 0) && ok;
-      carry = leave(acc, __ldcg(a.gstate + before * kSlab + ch));
-    }
-    if (!ok) {
-      carry = __int_as_float(0x7fffffff);
-      if (lane == 0) atomicOr(a.fault, kScanFault);
-    }
-    if (n == kGroup - 1) {
-      const int64_t here = group * a.nslab + slab;
-      a.gstate[here * kSlab + ch] = leave(run, carry);
-      __threadfence();
-      sync_pair();
-      if (ch == 0) store_release(a.gflags + here, 1u);
-    }
+#pragma unroll
+    for (int k = 0; k < kGroup / 4; ++k)
+      if (q * (kGroup / 4) + k < n) {
+        ok = wait_word(p + k * stride, v[k]) && ok;
+        acc = compose(acc, run_of(v[k]));
+      }
+    s.past[q][ch] = acc;
+    ok = __syncthreads_and(ok);
   }
-  s.carry[ch] = carry;
+  if (q == 0) {
+    float carry = 0.f;
+    if (a.chained) {
+      float2 acc = s.past[0][ch];
+#pragma unroll
+      for (int k = 1; k < 4; ++k) acc = compose(acc, s.past[k][ch]);
+      carry = acc.y;
+      if (group > 0 && !(acc.x < 0.f)) {
+        ok = wait_word(a.states + (group - 1) * stride + at, state) && ok;
+        carry = leave(acc, run_of(state).y);
+      }
+      if (!ok) {
+        carry = __int_as_float(0x7fffffff);
+        atomicOr(a.fault, kScanFault);
+      }
+      if (n == kGroup - 1)
+        publish(a.states + group * stride + at, make_float2(0.f, leave(run, carry)));
+    }
+    s.carry[ch] = carry;
+  }
+  __syncthreads();
 }
 
 // The sequence that owns row r, and whether r is its first / last row.
@@ -211,7 +256,7 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, int slab, const fl
 
 __device__ __forceinline__ unsigned take_item(const ScanArgs& a, ScanShared& s) {
   if (!a.chained) return blockIdx.x;
-  if (threadIdx.x == 0) s.item = atomicAdd(a.ticket, 1u);
+  if (threadIdx.x == 0) s.item = atomicAdd(a.ticket, 1u) + 1u;  // starts at all ones
   __syncthreads();
   return s.item;
 }
@@ -281,14 +326,17 @@ __global__ void __launch_bounds__(kScanThreads, 2) k_scan_fwd(const ScanArgs a) 
     }
   }
 #pragma unroll
-  for (int j = 0; j < kCpt; ++j) s.part[slot][lc + j] = make_float2(seen ? -1.f : A[j], H[j]);
+  for (int j = 0; j < kCpt; ++j)
+    if (seen) A[j] = -1.f;
+  float2 lead[kCpt];
+  join_pair<false>(s.part, A, H, lead);
   __syncthreads();
-  if (threadIdx.x < kSlab) exchange<false>(a, s, pos, slab);
-  __syncthreads();
+  exchange<false>(a, s, pos, slab);
 
   float h[kCpt];
 #pragma unroll
-  for (int j = 0; j < kCpt; ++j) h[j] = leave(s.part[slot][lc + j], s.carry[lc + j]);
+  for (int j = 0; j < kCpt; ++j)
+    h[j] = leave(lead[j], leave(s.part[threadIdx.x >> 5][lc + j], s.carry[lc + j]));
   if (a.saved && (slot * R) % kSaveRows == 0 && r0 < a.rows) {
     float* keep = a.saved + r0 / kSaveRows * a.D + c;
 #pragma unroll
@@ -318,7 +366,8 @@ template <typename T, typename G, bool GATE, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 2) k_scan_bwd(const ScanArgs a) {
   constexpr int R = kBwdRows;
   __shared__ ScanShared s;
-  __shared__ float2 ahead[kSlots][kSlab];  // forward runs of the slots
+  __shared__ float2 ahead[kWarps][kSlab];  // the same for the recomputed states
+  __shared__ float enter[kSlab];
   __shared__ int first_s[kSlots * R], last_s[kSlots * R];
   const unsigned item = take_item(a, s);
   const int64_t pos = item / (unsigned)a.nslab;
@@ -366,6 +415,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) k_scan_bwd(const ScanArgs a) 
     return a.dht && j < nc ? __ldg(a.dht + (int64_t)seq * a.D + c + j) : 0.f;
   };
 
+  float2 lead[kCpt], trail[kCpt];  // runs of the pair's rows before / after these
   {
     float A[kCpt], H[kCpt], C[kCpt];
     bool began = false, ended = false;
@@ -396,33 +446,30 @@ __global__ void __launch_bounds__(kScanThreads, 2) k_scan_bwd(const ScanArgs a) 
 #pragma unroll
       for (int j = 0; j < kCpt; ++j) C[j] = d[i][j] * (raw_get(dy[i], j) + C[j]);
     }
+    float A2[kCpt];
 #pragma unroll
     for (int j = 0; j < kCpt; ++j) {
-      ahead[slot][lc + j] = make_float2(began ? -1.f : A[j], H[j]);
-      s.part[slot][lc + j] = make_float2(ended ? -1.f : A[j], C[j]);
+      A2[j] = ended ? -1.f : A[j];
+      if (began) A[j] = -1.f;
     }
+    join_pair<false>(ahead, A, H, lead);
+    join_pair<true>(s.part, A2, C, trail);
   }
   __syncthreads();
-  if (threadIdx.x < kSlab) {
-    exchange<true>(a, s, pos, slab);
-  } else if (threadIdx.x < 2 * kSlab) {
+  if (threadIdx.x / kSlab == 1) {
     const int ch = threadIdx.x - kSlab;
     const bool have = slab * kSlab + ch < a.D && tile * (kSlots * R) < a.rows;
-    float h = have ? a.saved[tile * a.D + slab * kSlab + ch] : 0.f;
-#pragma unroll
-    for (int k = 0; k < kSlots; ++k) {
-      const float2 p = ahead[k][ch];
-      ahead[k][ch].y = h;  // the state entering the slot
-      h = leave(p, h);
-    }
+    enter[ch] = have ? a.saved[tile * a.D + slab * kSlab + ch] : 0.f;
+    fold_warps<false>(ahead, ch);
   }
-  __syncthreads();
+  exchange<true>(a, s, pos, slab);
 
   float before[R][kCpt];  // a_t h_{t-1}
   {
     float h[kCpt];
 #pragma unroll
-    for (int j = 0; j < kCpt; ++j) h[j] = ahead[slot][lc + j].y;
+    for (int j = 0; j < kCpt; ++j)
+      h[j] = leave(lead[j], leave(ahead[threadIdx.x >> 5][lc + j], enter[lc + j]));
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int seq = first_s[slot * R + i];
@@ -439,7 +486,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) k_scan_bwd(const ScanArgs a) 
   }
   float cc[kCpt];
 #pragma unroll
-  for (int j = 0; j < kCpt; ++j) cc[j] = leave(s.part[slot][lc + j], s.carry[lc + j]);
+  for (int j = 0; j < kCpt; ++j)
+    cc[j] = leave(trail[j], leave(s.part[threadIdx.x >> 5][lc + j], s.carry[lc + j]));
 #pragma unroll
   for (int i = R - 1; i >= 0; --i) {
     const int64_t r = r0 + i;
@@ -557,8 +605,7 @@ ScanArgs scan_args(const gdn2_scan_problem* p, int tile) {
   return a;
 }
 
-int scan_chain(const gdn2_scan_problem* p, ScanArgs& a, int tile, void* ws, size_t bytes,
-               cudaStream_t st, const char* fn) {
+int scan_chain(ScanArgs& a, int tile, void* ws, size_t bytes, cudaStream_t st, const char* fn) {
   if (!a.chained) return GDN2_OK;
   const ScanWorkspace L = scan_workspace(a.rows, a.D, tile);
   if (!ws || bytes < L.total)
@@ -568,13 +615,10 @@ int scan_chain(const gdn2_scan_problem* p, ScanArgs& a, int tile, void* ws, size
     return fail(GDN2_ERR_INVALID, "%s: workspace must start on a 16-byte boundary", fn);
   char* b = static_cast<char*>(ws);
   a.ticket = reinterpret_cast<unsigned*>(b);
-  a.flags = reinterpret_cast<unsigned*>(b + L.flags);
-  a.gflags = reinterpret_cast<unsigned*>(b + L.gflags);
-  a.agg = reinterpret_cast<float2*>(b + L.agg);
-  a.gstate = reinterpret_cast<float*>(b + L.gstate);
+  a.runs = reinterpret_cast<uint64_t*>(b + L.runs);
+  a.states = reinterpret_cast<uint64_t*>(b + L.states);
   cudaError_t e = fault_word(&a.fault);
-  if (e == cudaSuccess) e = cudaMemsetAsync(ws, 0, L.zeroed, st);
-  (void)p;
+  if (e == cudaSuccess) e = cudaMemsetAsync(ws, 0xff, L.total, st);
   return cuda_status(e, fn);
 }
 
@@ -623,7 +667,7 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   if (w && p->ld_w < p->D) return fail(GDN2_ERR_INVALID, "%s: ld_w must be at least D", fn);
   if (a.n_seqs == 0 || (a.rows == 0 && !ht)) return GDN2_OK;
   const cudaStream_t st = (cudaStream_t)stream;
-  if ((rc = scan_chain(p, a, kSlots * kFwdRows, workspace, workspace_bytes, st, fn))) return rc;
+  if ((rc = scan_chain(a, kSlots * kFwdRows, workspace, workspace_bytes, st, fn))) return rc;
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.y = y; a.ht = ht; a.saved = saved;
   const size_t es = dtype_size(p->dtype);
   const bool vec = a.D % kCpt == 0 && group_ok(v, a.ldv, es) && group_ok(y, a.D, es) &&
@@ -653,7 +697,7 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     return fail(GDN2_ERR_INVALID, "%s: row strides must be at least D", fn);
   if (a.n_seqs == 0 || (a.rows == 0 && !dh0)) return GDN2_OK;
   const cudaStream_t st = (cudaStream_t)stream;
-  if ((rc = scan_chain(p, a, kSlots * kBwdRows, workspace, workspace_bytes, st, fn))) return rc;
+  if ((rc = scan_chain(a, kSlots * kBwdRows, workspace, workspace_bytes, st, fn))) return rc;
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.saved = const_cast<float*>(saved);
   a.dy = dy; a.dht = dht; a.dv = dv; a.dg = dg; a.dw = dw; a.dh0 = dh0;
   const size_t es = dtype_size(p->dtype), eg = dtype_size(p->g_dtype);
