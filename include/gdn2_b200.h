@@ -350,9 +350,8 @@ int gdn2_gated_norm_bwd(const gdn2_norm_problem* p, const void* x, const void* z
  * without it.  A sequence without tokens passes its state on.
  * Backward: dy of y and dht (or NULL) of ht give dv, dg, dw, dh0 (or NULL);
  * `saved` (gdn2_scan_saved_bytes) is what the forward of the same inputs
- * wrote; a forward with saved NULL keeps nothing.  The workspace
- * (gdn2_scan_workspace_bytes, 16-byte aligned) is scratch of one call, forward
- * or backward.  The order of all sums is fixed: equal inputs give equal bits. */
+ * wrote; a forward with saved NULL keeps nothing.  The order of all sums is
+ * fixed: equal inputs give equal bits. */
 typedef struct gdn2_scan_problem {
     int32_t B;
     int32_t D;
@@ -364,16 +363,13 @@ typedef struct gdn2_scan_problem {
 } gdn2_scan_problem;
 
 size_t gdn2_scan_saved_bytes(const gdn2_scan_problem* p);
-size_t gdn2_scan_workspace_bytes(const gdn2_scan_problem* p);
 int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g,
                   const void* w, const float* h0, void* y, float* ht,
-                  float* saved, void* workspace, size_t workspace_bytes,
-                  void* stream);
+                  float* saved, void* stream);
 int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g,
                   const void* w, const float* h0, const float* saved,
                   const void* dy, const float* dht, void* dv, void* dg,
-                  void* dw, float* dh0, void* workspace, size_t workspace_bytes,
-                  void* stream);
+                  void* dw, float* dh0, void* stream);
 /* One token for each of B sequences (T = 1) on a pool of states, updated in
  * place: sequence b uses the row state_indices[b] (row b when NULL) of `state`
  * (`pool` rows, `state_stride` elements apart).  An index outside [0, pool)
@@ -463,8 +459,7 @@ int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensor
  * that runs out makes the kernel release its tensor memory, return without
  * finishing, and set a bit of a per-device fault word (bit 0: state passes,
  * bit 1: forward intra-chunk kernel, bit 2: decode, bit 3: backward
- * intra-chunk kernel, bit 4: gated linear recurrence, whose outputs after the
- * wait are NaN).  gdn2_fault_status
+ * intra-chunk kernel).  gdn2_fault_status
  * synchronises `stream` (the default stream when NULL), returns the fault
  * word of the current device (0 = no fault) and resets it when `clear` is
  * nonzero; a negative return is a CUDA error.  No counterpart in the

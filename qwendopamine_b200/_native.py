@@ -49,7 +49,6 @@ EXPORTS = (
     "gdn2_gated_norm_bwd_workspace_bytes",
     "gdn2_gated_norm_bwd",
     "gdn2_scan_saved_bytes",
-    "gdn2_scan_workspace_bytes",
     "gdn2_scan_fwd",
     "gdn2_scan_bwd",
     "gdn2_scan_step",
@@ -243,9 +242,8 @@ def _declare(lib):
         "gdn2_gated_norm_bwd_workspace_bytes": ([np_], c_size_t),
         "gdn2_gated_norm_bwd": ([np_, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
         "gdn2_scan_saved_bytes": ([sp], c_size_t),
-        "gdn2_scan_workspace_bytes": ([sp], c_size_t),
-        "gdn2_scan_fwd": ([sp, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
-        "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_scan_fwd": ([sp, v, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_adamw_step": ([ap, v, c_int32, v], ctypes.c_int),

@@ -63,10 +63,6 @@ class _Geometry:
 _width = math.prod  # elements of a shape
 
 
-def _workspace(lib, prob, device):
-    return torch.empty(lib.gdn2_scan_workspace_bytes(prob), dtype=torch.uint8, device=device)
-
-
 def _forward(geo, shape, h0, want_final, keep):
     lib = N.load()
     dev = geo.v.device
@@ -77,10 +73,9 @@ def _forward(geo, shape, h0, want_final, keep):
     if keep:
         saved = torch.empty(lib.gdn2_scan_saved_bytes(prob) // 4, dtype=torch.float32, device=dev)
     with N.on_device(dev.index):
-        ws = _workspace(lib, prob, dev)
         N.check(lib.gdn2_scan_fwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
-                                  N.addr(y), N.addr(ht), N.addr(saved), N.addr(ws), ws.numel(),
-                                  N.raw_stream(dev.index)), "gdn2_scan_fwd")
+                                  N.addr(y), N.addr(ht), N.addr(saved), N.raw_stream(dev.index)),
+                "gdn2_scan_fwd")
     return y, ht, saved
 
 
@@ -112,11 +107,10 @@ class GatedScanFunction(torch.autograd.Function):
         dw = new(w) if w is not None else None
         dh0 = new(h0) if h0 is not None else None
         with N.on_device(dev.index):
-            ws = _workspace(lib, prob, dev)
-            N.check(lib.gdn2_scan_bwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
+                N.check(lib.gdn2_scan_bwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
                                       N.addr(saved), N.addr(dy), N.addr(dht), N.addr(dv), N.addr(dg),
-                                      N.addr(dw), N.addr(dh0), N.addr(ws), ws.numel(),
-                                      N.raw_stream(dev.index)), "gdn2_scan_bwd")
+                                      N.addr(dw), N.addr(dh0), N.raw_stream(dev.index)),
+                    "gdn2_scan_bwd")
         return dv, dg, dw, dh0, None, None
 
 

@@ -225,12 +225,9 @@ def test_scan_arguments_are_checked(lib):
         return N.ScanProblem(**base)
 
     f = ctypes.c_void_p(0x1000)
-    fwd = lambda p, ws=f, wb=1 << 30, v=f: lib.gdn2_scan_fwd(p, v, f, f, None, f, None, None, ws,
-                                                             wb, None)
-    # a state every 64 of the 400 rows
-    assert lib.gdn2_scan_saved_bytes(sp()) == 7 * 70 * 4
-    need = lib.gdn2_scan_workspace_bytes(sp())
-    assert need > 7 * 2 * 64 * 8
+    fwd = lambda p, v=f: lib.gdn2_scan_fwd(p, v, f, f, None, f, None, None, None)
+    # a state every 64 of the 400 rows, and one for each sequence's rest
+    assert lib.gdn2_scan_saved_bytes(sp()) == (6 + 2) * 70 * 4
     for bad, code in ((sp(D=0), N.ERR_INVALID), (sp(T=-1), N.ERR_INVALID),
                       (sp(dtype=5), N.ERR_INVALID), (sp(g_dtype=2), N.ERR_UNSUPPORTED),
                       (sp(n_seqs=3), N.ERR_INVALID), (sp(cu_seqlens=0x1000), N.ERR_INVALID),
@@ -238,14 +235,10 @@ def test_scan_arguments_are_checked(lib):
                       (sp(T=1 << 40, B=64, n_seqs=64), N.ERR_UNSUPPORTED)):
         assert fwd(bad) == code, lib.gdn2_last_error()
     assert fwd(sp(), v=None) == N.ERR_INVALID
-    assert fwd(sp(), ws=None) == N.ERR_WORKSPACE
-    assert fwd(sp(), wb=256) == N.ERR_WORKSPACE
-    assert fwd(sp(), ws=ctypes.c_void_p(0x1008)) == N.ERR_INVALID
-    bwd = lambda p, saved=f: lib.gdn2_scan_bwd(p, f, f, f, None, saved, f, None, f, f, f, None, f,
-                                               256, None)
+    bwd = lambda p, saved=f: lib.gdn2_scan_bwd(p, f, f, f, None, saved, f, None, f, f, f, None,
+                                               None)
     assert bwd(sp(), saved=None) == N.ERR_INVALID
     assert bwd(sp(ld_dy=2)) == N.ERR_INVALID
-    assert bwd(sp()) == N.ERR_WORKSPACE
     step = lambda p, pool=9, stride=70: lib.gdn2_scan_step(p, f, f, f, f, stride, pool, None, f,
                                                            None)
     assert step(sp()) == N.ERR_INVALID and b"one token" in lib.gdn2_last_error()
