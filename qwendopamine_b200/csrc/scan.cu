@@ -19,17 +19,20 @@
 // reading v again costs what reading a stored y would.
 //
 // Bound: HBM (a handful of flops per element).  Each tensor is read and
-// written once.  A cluster of CTAs walks a chain: kSlab channels of a stretch
-// of rows that starts with a sequence, one tile of rows per CTA and turn.  A
+// written once.  A cluster of CTAs walks a chain: W channels of a stretch of
+// rows that starts with a sequence, one tile of rows per CTA and turn.  A
 // thread holds its rows of the tile in registers across the exchange of runs
-// -- shuffles between a warp's two slots of rows, shared memory between warps,
-// distributed shared memory between the cluster's CTAs -- and walks them a
-// second time with the right entering state.  The next turn's rows come in by
+// (shared memory in a CTA, distributed shared memory in a cluster) and walks
+// them a second time from the state that enters them.  The next turn's rows come in by
 // cp.async meanwhile.  The state passes from turn to turn inside the cluster:
 // no CTA waits for another cluster, and the order of all products is fixed.
+// Two to four CTAs share an SM and cover one another's barriers, while a thread
+// still has enough rows to spread the cost of the exchange over.  A tile
+// without a sequence's edge takes a path without the checks for one.
 //
 // Chains: whole sequences are dealt to stretches while there are enough of
-// them to fill the GPU; clusters of 2 to 16 CTAs make up for too few.
+// them to fill the GPU; clusters of 2 to 16 CTAs and half-width slabs make up
+// for too few.
 #include <cooperative_groups.h>
 
 #include "mma16.cuh"
@@ -40,18 +43,28 @@ namespace cg = cooperative_groups;
 namespace gdn2 {
 namespace {
 
-constexpr int kSlab = 64;         // channels of a tile
-constexpr int kLanes = 16;        // threads across a tile's channels
 constexpr int kCpt = 4;           // channels of a thread
-constexpr int kSlots = 16;        // threads down a tile's rows
-constexpr int kScanThreads = kLanes * kSlots;
-constexpr int kWarps = kScanThreads / 32;
 constexpr int kKeep = 64;         // rows between the states kept for the backward
 constexpr int kMaxCluster = 16;
-constexpr int kCtas = 2;          // CTAs that share an SM
 
-// Rows of a thread: as many as its registers hold (16-bit tensors, forward).
-template <typename T, bool BWD> constexpr int rows_of() { return sizeof(T) == 2 && !BWD ? 8 : 4; }
+// A tile of W channels: `lanes` threads across and `slots` threads down, R rows
+// and kCpt channels each.
+template <int W, int R> struct Shape {
+  static constexpr int threads = 1024 / R;
+  static constexpr int lanes = W / kCpt, slots = threads / lanes, tile = slots * R;
+  static_assert(tile % kKeep == 0, "a kept state enters every tile");
+};
+
+// Rows of a thread, and CTAs that share an SM (what their registers allow).
+// Forward: four CTAs of 128 threads with eight rows each (B = 8, T = 4096,
+// D = 2048, bf16: 124 us; two of 256 with four rows 119 us, but 354 against
+// 267 us on one sequence of 131,072 x 1024).  Backward, with twice the tensors
+// in registers: two CTAs of 256 threads with four rows (215 us; three of 128
+// with eight rows 263 us).
+template <bool BWD> constexpr int rows_of() { return BWD ? 4 : 8; }
+template <typename T, bool BWD> constexpr int ctas_of() {
+  return BWD ? (sizeof(T) == 2 ? 2 : 1) : (sizeof(T) == 2 ? 4 : 3);
+}
 
 struct ScanArgs {
   int64_t rows, T;     // T: rows of a sequence, fixed length
@@ -77,90 +90,88 @@ __device__ __forceinline__ float leave(float2 p, float h) {
   return p.x < 0.f ? p.y : fmaf(p.x, h, p.y);
 }
 
-template <int TILE> struct ScanShared {
-  float2 part[kWarps][kSlab];   // runs of the warps' slot pairs, then the runs before them
-  float carry[kSlab];           // state entering the tile
-  // of this turn and, while it is finished, the next:
-  int seq[2][TILE];                      // the row's sequence
-  uint32_t first[2][TILE / 32], last[2][TILE / 32];  // whether it is its first / last row
-  float2 runs[2][kMaxCluster][kSlab];    // of the cluster's tiles, by turn
+template <int W, int R> struct ScanShared {
+  static constexpr int tile = Shape<W, R>::tile, slots = Shape<W, R>::slots;
+  // runs of the slots of rows, by turn's parity; then in H the states entering them
+  float A[2][slots][W], H[2][slots][W];
+  // of a turn with sequence edges in its tile
+  int seq[tile];                               // the row's sequence
+  uint32_t first[tile / 32], last[tile / 32];  // whether it is its first / last row
 };
 
-// A warp holds two slots of rows.  Puts their joint run into part[warp] and
-// returns the run of the warp's rows before this thread's.
-template <bool UP>
-__device__ __forceinline__ void join_pair(float2 (*part)[kSlab], const float2 (&A2)[2],
-                                          const float2 (&H2)[2], float2 (&before)[kCpt]) {
-  const float A[kCpt] = {A2[0].x, A2[0].y, A2[1].x, A2[1].y};
-  const float H[kCpt] = {H2[0].x, H2[0].y, H2[1].x, H2[1].y};
-  const int lane = threadIdx.x & 31, lc = (lane % kLanes) * kCpt;
-  const bool leads = (lane < kLanes) != UP;
-#pragma unroll
-  for (int j = 0; j < kCpt; ++j) {
-    const float2 mine = make_float2(A[j], H[j]);
-    const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, A[j], kLanes),
-                                     __shfl_xor_sync(0xffffffffu, H[j], kLanes));
-    before[j] = leads ? make_float2(1.f, 0.f) : other;
-    if (leads) part[threadIdx.x >> 5][lc + j] = compose(mine, other);
-  }
+__device__ __forceinline__ float4 quad(const float2 (&x)[2]) {
+  return make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+}
+__device__ __forceinline__ void unquad(float2 (&x)[2], const float4 f) {
+  x[0] = make_float2(f.x, f.y);
+  x[1] = make_float2(f.z, f.w);
 }
 
-// Turns part[] into the runs before each warp; returns the tile's run.
-template <bool UP> __device__ __forceinline__ float2 fold_warps(float2 (*part)[kSlab], int ch) {
-  float2 p[kWarps], run = make_float2(1.f, 0.f);
+// One channel's fold over the tile's slots of rows, in the order of the scan:
+// the tile's run, and the state entering each slot (put into H) and leaving the
+// last.  Slots are read again rather than held: registers are what is short.
+template <int W, int R, bool UP> struct Fold {
+  static constexpr int slots = Shape<W, R>::slots;
+  __device__ static __forceinline__ float2 run(const float (&A)[slots][W], const float (&H)[slots][W],
+                                               int ch) {
+    float2 all = make_float2(1.f, 0.f);
 #pragma unroll
-  for (int k = 0; k < kWarps; ++k) p[k] = part[UP ? kWarps - 1 - k : k][ch];
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) {
-    part[UP ? kWarps - 1 - k : k][ch] = run;
-    run = compose(run, p[k]);
+    for (int i = 0; i < slots; ++i) {
+      const int k = UP ? slots - 1 - i : i;
+      all = compose(all, make_float2(A[k][ch], H[k][ch]));
+    }
+    return all;
   }
-  return run;
-}
+  __device__ static __forceinline__ float enter(const float (&A)[slots][W], float (&H)[slots][W],
+                                                int ch, float state) {
+#pragma unroll
+    for (int i = 0; i < slots; ++i) {
+      const int k = UP ? slots - 1 - i : i;
+      const float2 r = make_float2(A[k][ch], H[k][ch]);
+      H[k][ch] = state;
+      state = leave(r, state);
+    }
+    return state;
+  }
+};
 
-// Sets s.carry, the state that enters this CTA's tile, from s.part of
-// join_pair, and moves `state` (threads 0 .. 63, one per channel) from the
-// state that enters the turn's first tile to the one that leaves its last.
-// Called by all threads after a barrier; ends with one.  The runs of turn i+2
-// overwrite those of turn i: every CTA has folded those before it arrived at
-// the cluster barrier of turn i+1.
-template <bool UP, int TILE>
-__device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<TILE>& s, int rank, int turn,
-                                         float& state) {
+// Puts the states that enter the slots of this CTA's tile into s.H and moves
+// `state` (threads 0 .. W-1, one per channel) from the state that enters the
+// turn's first tile to the one that leaves its last.  Called by all threads
+// after a barrier; ends with one.  `runs` holds the runs of the cluster's
+// tiles by turn's parity: those of turn i+2 overwrite those of turn i, which
+// every CTA has folded before it arrives at the cluster barrier of turn i+1.
+template <int W, int R, bool UP>
+__device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s, float2* runs, int rank,
+                                         int b, float& state) {
   const int ch = threadIdx.x;
   if (a.cluster == 1) {
-    if (ch < kSlab) {
-      const float2 run = fold_warps<UP>(s.part, ch);
-      s.carry[ch] = state;
-      state = leave(run, state);
-    }
+    if (ch < W) state = Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, state);
   } else {
     cg::cluster_group cluster = cg::this_cluster();
-    if (ch < kSlab) {
-      const float2 run = fold_warps<UP>(s.part, ch);
-      float2* const slot = &s.runs[turn][rank][ch];
-      for (int k = 0; k < a.cluster; ++k) *cluster.map_shared_rank(slot, k) = run;
+    runs += b * a.cluster * W;
+    if (ch < W) {
+      const float2 all = Fold<W, R, UP>::run(s.A[b], s.H[b], ch);
+      for (int k = 0; k < a.cluster; ++k) *cluster.map_shared_rank(runs + rank * W + ch, k) = all;
     }
     cluster.sync();
-    if (ch < kSlab) {
+    if (ch < W) {
       float carry = state;
 #pragma unroll 4
       for (int k = 0; k < a.cluster; ++k) {
         if (k == rank) carry = state;
-        state = leave(s.runs[turn][k][ch], state);
+        state = leave(runs[k * W + ch], state);
       }
-      s.carry[ch] = carry;
+      Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, carry);
     }
   }
   __syncthreads();
 }
 
-// Follows a row (one for each of the first TILE threads) from turn to turn:
-// its sequence, and where in it the row is.
-struct RowWalk {
-  int64_t at, len;  // place in the sequence, and the sequence's rows
+// The sequence that owns row r, and r's place in it.
+struct RowPlace {
+  int64_t at, len;
   int n;
-
   __device__ __forceinline__ void find(const ScanArgs& a, int64_t r) {
     if (!a.cu) {
       n = (int)(r / a.T);
@@ -168,7 +179,7 @@ struct RowWalk {
       len = a.T;
       return;
     }
-    int lo = 0, hi = a.n_seqs;  // the last n with cu[n] <= r owns the row
+    int lo = 0, hi = a.n_seqs;  // the last n with cu[n] <= r
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (__ldg(a.cu + mid) <= r) lo = mid; else hi = mid;
@@ -177,84 +188,91 @@ struct RowWalk {
     at = r - __ldg(a.cu + lo);
     len = (int64_t)__ldg(a.cu + lo + 1) - __ldg(a.cu + lo);
   }
-  // `r` is the row now, `by` (either sign) rows from the last one
-  __device__ __forceinline__ void move(const ScanArgs& a, int64_t r, int64_t by) {
+  // Moves to row r, `by` rows on (the same for the CTA); true if the tile of
+  // rows from there holds a sequence's first or last row or leaves [lo, hi).
+  __device__ __forceinline__ bool edges(const ScanArgs& a, int64_t r, int64_t by, int tile,
+                                        int64_t lo, int64_t hi) {
+    if (r < lo || r + tile > hi) {
+      len = 0;  // to be found again
+      return true;
+    }
     at += by;
-    if (at >= 0 && at < len) return;
-    if (a.cu || a.T < 4096) return find(a, r);  // a turn is at most 2048 rows
-    const int s = at < 0 ? -1 : 1;  // into the neighbour
-    at -= s * a.T;
-    n += s;
+    if (at < 0 || at >= len) find(a, r);
+    return at <= 0 || at + tile >= len;
   }
 };
 
-// Marks the rows of the tile that starts at row `tile` for a turn; rows outside
-// the chain have none.
-template <int TILE>
-__device__ __forceinline__ void mark_rows(const ScanArgs& a, ScanShared<TILE>& s, RowWalk& w,
-                                          int which, int64_t tile, int64_t by, int64_t lo,
-                                          int64_t hi) {
-  if (threadIdx.x >= TILE) return;
+// Marks the rows of the tile that starts at row `tile`; rows outside [lo, hi)
+// have no marks.
+template <int W, int R>
+__device__ __forceinline__ void mark_rows(const ScanArgs& a, ScanShared<W, R>& s, int64_t tile,
+                                          int64_t lo, int64_t hi) {
+  if (threadIdx.x >= Shape<W, R>::tile) return;
   const int64_t r = tile + threadIdx.x;
   const bool in = r >= lo && r < hi;
-  if (in) {
-    if (by == 0) w.find(a, r);
-    else w.move(a, r, by);
-  }
-  const uint32_t f = __ballot_sync(0xffffffffu, in && w.at == 0);
-  const uint32_t l = __ballot_sync(0xffffffffu, in && w.at == w.len - 1);
-  s.seq[which][threadIdx.x] = w.n;
+  RowPlace p{-1, 0, 0};
+  if (in) p.find(a, r);
+  const uint32_t f = __ballot_sync(0xffffffffu, in && p.at == 0);
+  const uint32_t l = __ballot_sync(0xffffffffu, in && p.at == p.len - 1);
+  s.seq[threadIdx.x] = p.n;
   if ((threadIdx.x & 31) == 0) {
-    s.first[which][threadIdx.x >> 5] = f;
-    s.last[which][threadIdx.x >> 5] = l;
+    s.first[threadIdx.x >> 5] = f;
+    s.last[threadIdx.x >> 5] = l;
   }
 }
 
 // Sequences without rows: their state passes through (`from` NULL: zero).
+template <int W, int THREADS>
 __device__ __forceinline__ void pass_empty(const ScanArgs& a, int slab, const float* from,
                                            float* to) {
   if (!to || (!a.cu && a.T > 0)) return;
-  const int c = slab * kSlab + (threadIdx.x & (kSlab - 1));
+  const int c = slab * W + (int)threadIdx.x % W;
   if (c >= a.D) return;
-  for (int n = threadIdx.x / kSlab; n < a.n_seqs; n += kScanThreads / kSlab)
+  for (int n = threadIdx.x / W; n < a.n_seqs; n += THREADS / W)
     if (!a.cu || __ldg(a.cu + n) == __ldg(a.cu + n + 1))
       to[(int64_t)n * a.D + c] = from ? from[(int64_t)n * a.D + c] : 0.f;
 }
 
 // A thread's own rows of a tile in shared memory, filled asynchronously by
-// the thread itself (no barrier) and read by it alone: group i of tensor k at
-// k's section, row i, thread.
+// the thread itself (no barrier) and read by it alone: group i of a tensor at
+// its section, row i, thread.
 template <typename T, int R> struct Stage {
   static constexpr int kGroupBytes = kCpt * (int)sizeof(T);
-  static constexpr int kBytes = R * kScanThreads * kGroupBytes;
   __device__ static __forceinline__ char* at(char* base, int i) {
-    return base + (i * kScanThreads + threadIdx.x) * kGroupBytes;
+    return base + (i * (1024 / R) + threadIdx.x) * kGroupBytes;
   }
-  __device__ static __forceinline__ void copy(char* base, int i, const T* src, int have) {
+  __device__ static __forceinline__ void copy(char* base, int i, const void* src, int have) {
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(base, i));
     if constexpr (kGroupBytes == 16)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
     else
       asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
   }
-  // rows r0 .. r0 + R - 1 of which those in [lo, hi) exist (`whole`: all, and
-  // all channels); what does not exist reads as zero
-  template <bool VEC>
-  __device__ static __forceinline__ void fill(char* base, const void* x, int64_t ld, int64_t r0,
-                                              int64_t lo, int64_t hi, int c, int nc, bool whole) {
-    const T* p = (const T*)x + r0 * ld + c;
-    if (VEC && whole) {
+  // The thread's rows of the tile at row `tile` (the same for the CTA), of
+  // which those in [lo, hi) exist, `nc` channels wide; what does not exist
+  // reads as zero, but a thread without channels reads nothing.
+  template <int W, bool VEC>
+  __device__ static __forceinline__ void fill(char* base, const void* x, int64_t ld, int64_t tile,
+                                              int64_t lo, int64_t hi, int slab, int nc) {
+    if (nc <= 0) return;
+    const int r0 = (int)threadIdx.x / Shape<W, R>::lanes * R;
+    const int lc = (int)threadIdx.x % Shape<W, R>::lanes * kCpt;
+    const char* p = (const char*)x + (tile * ld + slab * W) * (int64_t)sizeof(T);
+    if (VEC && tile >= lo && tile + Shape<W, R>::tile <= hi) {
+      const uint32_t off = (uint32_t)(r0 * (int)ld + lc) * (uint32_t)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < R; ++i, p += ld) copy(base, i, p, kGroupBytes);
+      for (int i = 0; i < R; ++i, p += ld * (int64_t)sizeof(T)) copy(base, i, p + off, kGroupBytes);
       return;
     }
+    const T* q = (const T*)p + r0 * ld + lc;
 #pragma unroll 1
-    for (int i = 0; i < R; ++i, p += ld) {
-      const int n = r0 + i >= lo && r0 + i < hi ? nc : 0;
+    for (int i = 0; i < R; ++i, q += ld) {
+      const int64_t r = tile + r0 + i;
+      const int n = r >= lo && r < hi ? nc : 0;
       if constexpr (VEC)
-        copy(base, i, n > 0 ? p : (const T*)x, n > 0 ? kGroupBytes : 0);
+        copy(base, i, n > 0 ? (const void*)q : x, n > 0 ? kGroupBytes : 0);
       else
-        *reinterpret_cast<Raw<T, kCpt>*>(at(base, i)) = load_group<T, kCpt, false>(p, n);
+        *reinterpret_cast<Raw<T, kCpt>*>(at(base, i)) = load_group<T, kCpt, false>(q, n);
     }
   }
   __device__ static __forceinline__ Raw<T, kCpt> get(char* base, int i) {
@@ -273,10 +291,11 @@ template <typename T, int R> struct Stage {
 __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Sections of a stage: g, v, w, dy.
-template <typename T, typename G, bool GATE, bool BWD, int R> struct StageLayout {
-  static constexpr int g = 0, v = Stage<G, R>::kBytes, w = v + Stage<T, R>::kBytes;
-  static constexpr int dy = w + (GATE ? Stage<T, R>::kBytes : 0);
-  static constexpr int bytes = dy + (BWD ? Stage<T, R>::kBytes : 0);
+template <typename T, typename G, bool GATE, bool BWD> struct StageLayout {
+  static constexpr int sg = 1024 * kCpt * (int)sizeof(G), st = 1024 * kCpt * (int)sizeof(T);
+  static constexpr int g = 0, v = sg, w = v + st;
+  static constexpr int dy = w + (GATE ? st : 0);
+  static constexpr int bytes = dy + (BWD ? st : 0);
 };
 
 // A CTA's chain and place in it.
@@ -285,7 +304,7 @@ struct Place {
   int64_t chain;    // which stretch
   int rank, slab, turns;
 };
-template <int TILE> __device__ __forceinline__ Place place_of(const ScanArgs& a) {
+template <int W, int R> __device__ __forceinline__ Place place_of(const ScanArgs& a) {
   Place p;
   const unsigned id = blockIdx.x / (unsigned)a.cluster;
   p.rank = (int)(blockIdx.x - id * a.cluster);
@@ -293,7 +312,7 @@ template <int TILE> __device__ __forceinline__ Place place_of(const ScanArgs& a)
   p.slab = (int)(id - p.chain * a.nslab);
   p.lo = p.chain * a.stretch;
   p.hi = min(p.lo + a.stretch, a.rows);
-  const int64_t step = (int64_t)a.cluster * TILE;
+  const int64_t step = (int64_t)a.cluster * Shape<W, R>::tile;
   p.turns = (int)((p.hi - p.lo + step - 1) / step);
   return p;
 }
@@ -305,11 +324,25 @@ template <typename T> __device__ __forceinline__ float2 pair_of(const Raw<T, kCp
   else
     return unpack2<T>(r.u[k]);
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_pairs(T* p, const float2 (&x)[2], int n) {
-  const float f[kCpt] = {x[0].x, x[0].y, x[1].x, x[1].y};
-  store_group<T, kCpt, VEC>(p, f, n);
-}
+
+// Where a thread's rows of a contiguous output go: the tile's first element
+// (the same for the CTA) and the thread's place from there.
+template <typename T, int W, int R> struct Target {
+  char* base;
+  uint32_t off;
+  int row_bytes;
+  __device__ __forceinline__ Target(void* x, int64_t tile, int slab, int D) {
+    base = (char*)x + (tile * D + slab * W) * (int64_t)sizeof(T);
+    const int r0 = (int)threadIdx.x / Shape<W, R>::lanes * R;
+    const int lc = (int)threadIdx.x % Shape<W, R>::lanes * kCpt;
+    off = (uint32_t)(r0 * D + lc) * (uint32_t)sizeof(T);
+    row_bytes = D * (int)sizeof(T);
+  }
+  template <bool VEC> __device__ __forceinline__ void put(int i, const float2 (&x)[2], int n) const {
+    const float f[kCpt] = {x[0].x, x[0].y, x[1].x, x[1].y};
+    store_group<T, kCpt, VEC>((T*)(base + (int64_t)i * row_bytes + off), f, n);
+  }
+};
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // exp of log-decays: 2^(g log2 e), the hardware's base-2 exponential.  Its
@@ -334,49 +367,39 @@ __device__ __forceinline__ void put_state(float* x, int64_t seq, int D, int c, i
     if (j < nc) x[seq * D + c + j] = f[j];
 }
 
-// What enters a thread's rows: through the runs of the pair's rows and of the
-// warps before them from the state entering the tile.
-__device__ __forceinline__ void entering(const float2 (&pair)[kCpt], const float2* warps,
-                                         const float* tile, float2 (&h)[2]) {
-  float f[kCpt];
-#pragma unroll
-  for (int j = 0; j < kCpt; ++j) f[j] = leave(pair[j], leave(warps[j], tile[j]));
-  h[0] = make_float2(f[0], f[1]);
-  h[1] = make_float2(f[2], f[3]);
-}
-
-template <typename T, typename G, bool GATE, bool VEC>
-__global__ void __launch_bounds__(kScanThreads, kCtas) k_scan_fwd(const ScanArgs a) {
-  constexpr int R = rows_of<T, false>(), TILE = R * kSlots;
-  using L = StageLayout<T, G, GATE, false, R>;
+template <typename T, typename G, bool GATE, int W, int R, bool VEC>
+__global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(const ScanArgs a) {
+  constexpr int TILE = Shape<W, R>::tile;
+  using L = StageLayout<T, G, GATE, false>;
   extern __shared__ __align__(16) char st[];
-  __shared__ ScanShared<TILE> s;
-  const Place p = place_of<TILE>(a);
-  const int slot = threadIdx.x / kLanes, warp = threadIdx.x >> 5;
-  const int lc = (threadIdx.x % kLanes) * kCpt, c = p.slab * kSlab + lc, nc = a.D - c;
+  __shared__ ScanShared<W, R> s;
+  const Place p = place_of<W, R>(a);
+  float2* const runs = reinterpret_cast<float2*>(st + L::bytes);
+  const int slot = threadIdx.x / Shape<W, R>::lanes, r0 = slot * R;
+  const int lc = (threadIdx.x % Shape<W, R>::lanes) * kCpt, c = p.slab * W + lc, nc = a.D - c;
   const int64_t step = (int64_t)a.cluster * TILE;
   int64_t tile = p.lo + (int64_t)p.rank * TILE;  // first row of this turn's tile
   auto fill = [&](int64_t row) {
-    const int64_t r0 = row + slot * R;
-    const bool whole = r0 + R <= p.hi && nc >= kCpt;
-    Stage<G, R>::template fill<VEC>(st + L::g, a.g, a.ldg, r0, p.lo, p.hi, c, nc, whole);
-    Stage<T, R>::template fill<VEC>(st + L::v, a.v, a.ldv, r0, p.lo, p.hi, c, nc, whole);
+    Stage<G, R>::template fill<W, VEC>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, VEC>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<VEC>(st + L::w, a.w, a.ldw, r0, p.lo, p.hi, c, nc, whole);
+      Stage<T, R>::template fill<W, VEC>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
   };
-  if (p.chain == 0 && p.rank == 0) pass_empty(a, p.slab, a.h0, a.ht);
+  if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.h0, a.ht);
   if (p.turns > 0) fill(tile);
   if (a.cluster > 1) cg::this_cluster().sync();  // all CTAs run before one writes to another
   float state = 0.f;
-  RowWalk walk{};
-  mark_rows(a, s, walk, 0, tile, 0, p.lo, p.hi);
+  RowPlace place{0, 0, 0};
 
   for (int turn = 0; turn < p.turns; ++turn, tile += step) {
     const int b = turn & 1;
+    const bool edges = place.edges(a, tile, step, TILE, p.lo, p.hi);
+    if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
     float2 d[R][2];
     // the inputs w v, packed as v where there is no gate
-    typename std::conditional<GATE, Raw<float, kCpt>, Raw<T, kCpt>>::type x[R];
+    using X = typename std::conditional<GATE, float, T>::type;
+    Raw<X, kCpt> x[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const Raw<G, kCpt> g = Stage<G, R>::get(st + L::g, i);
@@ -395,91 +418,95 @@ __global__ void __launch_bounds__(kScanThreads, kCtas) k_scan_fwd(const ScanArgs
       d[i][0] = decay_of(pair_of<G>(g, 0));
       d[i][1] = decay_of(pair_of<G>(g, 1));
     }
-    using X = typename std::conditional<GATE, float, T>::type;
     if (turn + 1 < p.turns) fill(tile + step);
-    __syncthreads();
-    const uint32_t first = (s.first[b][slot * R / 32] >> (slot * R % 32)) & ((1u << R) - 1);
-    const uint32_t last = (s.last[b][slot * R / 32] >> (slot * R % 32)) & ((1u << R) - 1);
-    const int* const seq = s.seq[b] + slot * R;
+    uint32_t first = 0, last = 0;
+    if (edges) {
+      __syncthreads();
+      first = (s.first[r0 / 32] >> (r0 % 32)) & ((1u << R) - 1);
+      last = (s.last[r0 / 32] >> (r0 % 32)) & ((1u << R) - 1);
+    }
 
-    float2 lead[kCpt];
-    {
-      float2 A[2] = {both(1.f), both(1.f)}, H[2] = {both(0.f), both(0.f)};
+    float2 A[2] = {both(1.f), both(1.f)}, h[2] = {both(0.f), both(0.f)};
+    auto walk = [&](auto edge, auto&& each) {
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        if (first >> i & 1) state_at(a.h0, seq[i], a.D, c, nc, H);
+        if constexpr (decltype(edge)::value)
+          if (first >> i & 1) state_at(a.h0, s.seq[r0 + i], a.D, c, nc, h);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          H[k] = fma2(d[i][k], H[k], pair_of<X>(x[i], k));
-          A[k] = mul2(A[k], d[i][k]);
-        }
+        for (int k = 0; k < 2; ++k) h[k] = fma2(d[i][k], h[k], pair_of<X>(x[i], k));
+        each(i);
       }
+    };
+    auto product = [&](int i) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) A[k] = mul2(A[k], d[i][k]);
+    };
+    if (edges) {
+      walk(std::true_type{}, product);
       if (first) A[0] = A[1] = both(-1.f);
-      join_pair<false>(s.part, A, H, lead);
+    } else {
+      walk(std::false_type{}, product);
     }
+    *reinterpret_cast<float4*>(&s.A[b][slot][lc]) = quad(A);
+    *reinterpret_cast<float4*>(&s.H[b][slot][lc]) = quad(h);
     __syncthreads();
-    if (turn + 1 < p.turns) mark_rows(a, s, walk, b ^ 1, tile + step, step, p.lo, p.hi);
-    exchange<false>(a, s, p.rank, b, state);
+    exchange<W, R, false>(a, s, runs, p.rank, b, state);
 
-    float2 h[2];
-    entering(lead, s.part[warp] + lc, s.carry + lc, h);
-    const int64_t r0 = tile + slot * R;
-    if (a.saved && (slot * R) % kKeep == 0 && r0 < p.hi)
-      put_state(a.saved, p.chain * a.keeps + (r0 - p.lo) / kKeep, a.D, c, nc, h);
-    const int here = (int)min((int64_t)R, p.hi - r0);  // rows that exist
-    T* y = (T*)a.y + r0 * a.D + c;
-#pragma unroll
-    for (int i = 0; i < R; ++i, y += a.D) {
-      if (first >> i & 1) state_at(a.h0, seq[i], a.D, c, nc, h);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) h[k] = fma2(d[i][k], h[k], pair_of<X>(x[i], k));
-      store_pairs<T, VEC>(y, h, i < here ? nc : 0);
-      if ((last >> i & 1) && a.ht) put_state(a.ht, seq[i], a.D, c, nc, h);
+    unquad(h, *reinterpret_cast<const float4*>(&s.H[b][slot][lc]));
+    const int64_t left = p.hi - tile - r0;  // rows that exist from here
+    if (a.saved && r0 % kKeep == 0 && left > 0)
+      put_state(a.saved, p.chain * a.keeps + (tile + r0 - p.lo) / kKeep, a.D, c, nc, h);
+    const Target<T, W, R> y(a.y, tile, p.slab, a.D);
+    if (edges) {
+      walk(std::true_type{}, [&](int i) {
+        y.template put<VEC>(i, h, i < left ? nc : 0);
+        if ((last >> i & 1) && a.ht) put_state(a.ht, s.seq[r0 + i], a.D, c, nc, h);
+      });
+      __syncthreads();  // the marks have been read
+    } else {
+      walk(std::false_type{}, [&](int i) { y.template put<VEC>(i, h, nc); });
     }
   }
 }
 
-template <typename T, typename G, bool GATE, bool VEC>
-__global__ void __launch_bounds__(kScanThreads, kCtas) k_scan_bwd(const ScanArgs a) {
-  constexpr int R = rows_of<T, true>(), TILE = R * kSlots;
-  static_assert(TILE == kKeep, "a kept state enters every tile of the backward");
-  using L = StageLayout<T, G, GATE, true, R>;
+template <typename T, typename G, bool GATE, int W, int R, bool VEC>
+__global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const ScanArgs a) {
+  constexpr int TILE = Shape<W, R>::tile;
+  using L = StageLayout<T, G, GATE, true>;
   extern __shared__ __align__(16) char st[];
-  __shared__ ScanShared<TILE> s;
-  __shared__ float2 ahead[kWarps][kSlab];  // s.part of the recomputed states
-  __shared__ float enter[kSlab];           // the state entering the tile
-  const Place p = place_of<TILE>(a);
-  const int slot = threadIdx.x / kLanes, warp = threadIdx.x >> 5;
-  const int lc = (threadIdx.x % kLanes) * kCpt, c = p.slab * kSlab + lc, nc = a.D - c;
+  __shared__ ScanShared<W, R> s;
+  __shared__ ScanShared<W, R> ahead;  // the same for the recomputed states (no marks)
+  const Place p = place_of<W, R>(a);
+  float2* const runs = reinterpret_cast<float2*>(st + L::bytes);
+  const int slot = threadIdx.x / Shape<W, R>::lanes, r0 = slot * R;
+  const int lc = (threadIdx.x % Shape<W, R>::lanes) * kCpt, c = p.slab * W + lc, nc = a.D - c;
   const int64_t step = (int64_t)a.cluster * TILE;
   // from the chain's last tile down; before the first there is nothing
   int64_t tile = p.lo + ((p.hi - p.lo + TILE - 1) / TILE - 1 - p.rank) * TILE;
   auto fill = [&](int64_t row) {
-    const int64_t r0 = row + slot * R;
-    const bool whole = r0 >= p.lo && r0 + R <= p.hi && nc >= kCpt;
-    Stage<G, R>::template fill<VEC>(st + L::g, a.g, a.ldg, r0, p.lo, p.hi, c, nc, whole);
-    Stage<T, R>::template fill<VEC>(st + L::v, a.v, a.ldv, r0, p.lo, p.hi, c, nc, whole);
-    Stage<T, R>::template fill<VEC>(st + L::dy, a.dy, a.lddy, r0, p.lo, p.hi, c, nc, whole);
+    Stage<G, R>::template fill<W, VEC>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, VEC>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, VEC>(st + L::dy, a.dy, a.lddy, row, p.lo, p.hi, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<VEC>(st + L::w, a.w, a.ldw, r0, p.lo, p.hi, c, nc, whole);
+      Stage<T, R>::template fill<W, VEC>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
   };
-  if (p.chain == 0 && p.rank == 0) pass_empty(a, p.slab, a.dht, a.dh0);
+  if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.dht, a.dh0);
   if (p.turns > 0) fill(tile);
   if (a.cluster > 1) cg::this_cluster().sync();  // all CTAs run before one writes to another
   float state = 0.f;
-  RowWalk walk{};
-  bool walking = tile + threadIdx.x < p.hi && tile >= p.lo;  // this thread's row was found
-  mark_rows(a, s, walk, 0, tile, 0, p.lo, p.hi);
+  RowPlace place{0, 0, 0};
 
   for (int turn = 0; turn < p.turns; ++turn, tile -= step) {
     const int b = turn & 1;
     const bool some = tile >= p.lo;
-    float kept = 0.f;
-    if (threadIdx.x / kSlab == 1) {
-      const int ch = p.slab * kSlab + threadIdx.x - kSlab;
+    const bool edges = place.edges(a, tile, -step, TILE, p.lo, p.hi);
+    float kept = 0.f;  // the state entering the tile
+    if (threadIdx.x / W == 1) {
+      const int ch = p.slab * W + threadIdx.x - W;
       if (some && ch < a.D)
         kept = __ldg(a.saved + (p.chain * a.keeps + (tile - p.lo) / kKeep) * a.D + ch);
     }
+    if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
     float2 d[R][2];
     Raw<T, kCpt> v[R], w[GATE ? R : 1], dy[R];
@@ -498,18 +525,20 @@ __global__ void __launch_bounds__(kScanThreads, kCtas) k_scan_bwd(const ScanArgs
       return x;
     };
     if (turn + 1 < p.turns) fill(tile - step);
-    __syncthreads();
-    const uint32_t first = (s.first[b][slot * R / 32] >> (slot * R % 32)) & ((1u << R) - 1);
-    const uint32_t last = (s.last[b][slot * R / 32] >> (slot * R % 32)) & ((1u << R) - 1);
-    const int* const seq = s.seq[b] + slot * R;
+    uint32_t first = 0, last = 0;
+    if (edges) {
+      __syncthreads();
+      first = (s.first[r0 / 32] >> (r0 % 32)) & ((1u << R) - 1);
+      last = (s.last[r0 / 32] >> (r0 % 32)) & ((1u << R) - 1);
+    }
 
-    float2 lead[kCpt], trail[kCpt];  // runs of the pair's rows before / after these
-    {
+    auto runs_of_rows = [&](auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
       float2 A[2] = {both(1.f), both(1.f)}, H[2] = {both(0.f), both(0.f)};
       float2 C[2] = {both(0.f), both(0.f)};
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        if (first >> i & 1) state_at(a.h0, seq[i], a.D, c, nc, H);
+        if (EDGE && (first >> i & 1)) state_at(a.h0, s.seq[r0 + i], a.D, c, nc, H);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           H[k] = fma2(d[i][k], H[k], input(i, k));
@@ -518,67 +547,70 @@ __global__ void __launch_bounds__(kScanThreads, kCtas) k_scan_bwd(const ScanArgs
       }
 #pragma unroll
       for (int i = R - 1; i >= 0; --i) {
-        if (last >> i & 1) state_at(a.dht, seq[i], a.D, c, nc, C);
+        if (EDGE && (last >> i & 1)) state_at(a.dht, s.seq[r0 + i], a.D, c, nc, C);
 #pragma unroll
         for (int k = 0; k < 2; ++k) C[k] = mul2(d[i][k], add2(pair_of<T>(dy[i], k), C[k]));
       }
-      const float2 Z[2] = {last ? both(-1.f) : A[0], last ? both(-1.f) : A[1]};
-      if (first) A[0] = A[1] = both(-1.f);
-      join_pair<false>(ahead, A, H, lead);
-      join_pair<true>(s.part, Z, C, trail);
-    }
+      const float4 reset = make_float4(-1.f, -1.f, -1.f, -1.f);
+      *reinterpret_cast<float4*>(&ahead.A[b][slot][lc]) = EDGE && first ? reset : quad(A);
+      *reinterpret_cast<float4*>(&ahead.H[b][slot][lc]) = quad(H);
+      *reinterpret_cast<float4*>(&s.A[b][slot][lc]) = EDGE && last ? reset : quad(A);
+      *reinterpret_cast<float4*>(&s.H[b][slot][lc]) = quad(C);
+    };
+    if (edges) runs_of_rows(std::true_type{});
+    else runs_of_rows(std::false_type{});
     __syncthreads();
-    if (threadIdx.x / kSlab == 1) {
-      enter[threadIdx.x - kSlab] = kept;
-      fold_warps<false>(ahead, threadIdx.x - kSlab);
-    }
-    if (turn + 1 < p.turns) {
-      mark_rows(a, s, walk, b ^ 1, tile - step, walking ? -step : 0, p.lo, p.hi);
-      walking = walking || tile - step + (int64_t)threadIdx.x < p.hi;
-    }
-    exchange<true>(a, s, p.rank, b, state);
+    if (threadIdx.x / W == 1)
+      Fold<W, R, false>::enter(ahead.A[b], ahead.H[b], threadIdx.x - W, kept);
+    exchange<W, R, true>(a, s, runs, p.rank, b, state);
 
-    float2 before[R][2];  // a_t h_{t-1}
-    {
-      float2 h[2];
-      entering(lead, ahead[warp] + lc, enter + lc, h);
+    const int64_t left = some ? p.hi - tile - r0 : 0;  // rows that exist from here
+    const Target<G, W, R> dg(a.dg, tile, p.slab, a.D);
+    const Target<T, W, R> dv(a.dv, tile, p.slab, a.D), dw(a.dw, tile, p.slab, a.D);
+    auto gradients = [&](auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
+      float2 before[R][2];  // a_t h_{t-1}
+      float2 h[2], cc[2];
+      unquad(h, *reinterpret_cast<const float4*>(&ahead.H[b][slot][lc]));
+      unquad(cc, *reinterpret_cast<const float4*>(&s.H[b][slot][lc]));
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        if (first >> i & 1) state_at(a.h0, seq[i], a.D, c, nc, h);
+        if (EDGE && (first >> i & 1)) state_at(a.h0, s.seq[r0 + i], a.D, c, nc, h);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           before[i][k] = mul2(d[i][k], h[k]);
           h[k] = add2(before[i][k], input(i, k));
         }
       }
-    }
-    float2 cc[2];
-    entering(trail, s.part[warp] + lc, s.carry + lc, cc);
-    const int64_t r0 = tile + slot * R, at = r0 * a.D + c;
-    const int here = some ? (int)min((int64_t)R, p.hi - r0) : 0;  // rows that exist
 #pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      const int n = i < here ? nc : 0;
-      const int64_t o = at + (int64_t)i * a.D;
-      if (last >> i & 1) state_at(a.dht, seq[i], a.D, c, nc, cc);
-      float2 dh[2], z[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        dh[k] = add2(pair_of<T>(dy[i], k), cc[k]);
-        cc[k] = mul2(d[i][k], dh[k]);
-        z[k] = mul2(before[i][k], dh[k]);
-      }
-      store_pairs<G, VEC>((G*)a.dg + o, z, n);
-      if constexpr (GATE) {
+      for (int i = R - 1; i >= 0; --i) {
+        const int n = !EDGE || i < left ? nc : 0;
+        if (EDGE && (last >> i & 1)) state_at(a.dht, s.seq[r0 + i], a.D, c, nc, cc);
+        float2 dh[2], z[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          z[k] = mul2(pair_of<T>(v[i], k), dh[k]);
-          dh[k] = mul2(dh[k], pair_of<T>(w[i], k));
+          dh[k] = add2(pair_of<T>(dy[i], k), cc[k]);
+          cc[k] = mul2(d[i][k], dh[k]);
+          z[k] = mul2(before[i][k], dh[k]);
         }
-        store_pairs<T, VEC>((T*)a.dw + o, z, n);
+        dg.template put<VEC>(i, z, n);
+        if constexpr (GATE) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            z[k] = mul2(pair_of<T>(v[i], k), dh[k]);
+            dh[k] = mul2(dh[k], pair_of<T>(w[i], k));
+          }
+          dw.template put<VEC>(i, z, n);
+        }
+        dv.template put<VEC>(i, dh, n);
+        if (EDGE && (first >> i & 1) && a.dh0) put_state(a.dh0, s.seq[r0 + i], a.D, c, nc, cc);
       }
-      store_pairs<T, VEC>((T*)a.dv + o, dh, n);
-      if ((first >> i & 1) && a.dh0) put_state(a.dh0, seq[i], a.D, c, nc, cc);
+    };
+    if (edges) {
+      gradients(std::true_type{});
+      __syncthreads();  // the marks have been read
+    } else {
+      gradients(std::false_type{});
     }
   }
 }
@@ -642,94 +674,109 @@ int check_scan(const gdn2_scan_problem* p, const char* fn) {
   if (p->ld_v < p->D || p->ld_g < p->D || p->ld_w < 0 || p->ld_dy < 0)
     return fail(GDN2_ERR_INVALID, "%s: row strides must be at least D", fn);
   const int64_t rows = (int64_t)p->B * p->T;
-  const int64_t nslab = (p->D + kSlab - 1) / kSlab;
+  const int64_t nslab = (p->D + 31) / 32;
   if ((p->T > 0 && rows / p->T != p->B) ||
       (rows / kKeep + p->B + kMaxCluster) > 2147483647LL / nslab)
     return fail(GDN2_ERR_UNSUPPORTED, "%s: too many rows x channels", fn);
   return GDN2_OK;
 }
 
-// How the rows are dealt out: `stretches` chains (each of whole sequences) and
-// `cluster` CTAs for a chain.
+// How the rows are dealt out.
 struct ScanPlan {
-  int64_t stretches;
-  int64_t rows;     // of a stretch
-  int cluster;
+  int64_t stretches;  // chains of a slab, each of whole sequences
+  int64_t rows;       // of a stretch
+  int slab, cluster;
 };
 
-// The largest number of CTAs that any SM slot works through, in tiles, is what
-// a plan costs; of equal ones the smaller cluster is taken (its exchange is
-// cheaper).  A GPC places clusters of 8 and 16 on all but a few of its SMs.
-ScanPlan scan_plan(const gdn2_scan_problem* p, int sms, int tile) {
-  const int64_t rows = (int64_t)p->B * p->T, nslab = (p->D + kSlab - 1) / kSlab;
-  ScanPlan best{1, rows, 1};
-  int64_t least = -1;
-  for (int c = 1; c <= kMaxCluster; c *= 2) {
-    const int64_t slots = (int64_t)sms * kCtas * (c >= 8 ? 86 : 100) / 100 / c;  // clusters at once
-    int64_t s = p->cu_seqlens ? 1 : slots / nslab;
-    if (s > p->B) s = p->B;
-    if (s < 1) s = 1;
-    const int64_t each = p->B > 0 ? (p->B + s - 1) / s : 0;  // sequences of a stretch
-    s = each > 0 ? (p->B + each - 1) / each : 1;
-    const int64_t r = p->cu_seqlens ? rows : each * p->T;
-    const int64_t waves = (s * nslab + slots - 1) / slots;
-    const int64_t cost = waves * ((r + (int64_t)c * tile - 1) / ((int64_t)c * tile));
-    if (least < 0 || cost < least) {
-      least = cost;
-      best = ScanPlan{s, r, c};
-    }
-  }
-  return best;
+// Stretches: as many as leave two or three CTAs for every SM.  They are the
+// same forward and backward, so that the kept states are found again.
+ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
+  ScanPlan l{1, (int64_t)p->B * p->T, 64, 1};
+  if (p->cu_seqlens || p->B == 0) return l;
+  int64_t s = (int64_t)sms * 3 / ((p->D + 63) / 64);
+  if (s > p->B) s = p->B;
+  if (s < 1) s = 1;
+  const int64_t each = (p->B + s - 1) / s;  // sequences of a stretch
+  l.stretches = (p->B + each - 1) / each;
+  l.rows = each * p->T;
+  return l;
 }
 
-int64_t scan_keeps(const ScanPlan& l) { return (l.rows + kKeep - 1) / kKeep; }
+// Slab and cluster: what takes the least time by a model of a turn, fitted to
+// runs of both directions over slabs and clusters (seven shapes from 9001 x 1000
+// to 131,072 x 1024; it chose within a tenth of the fastest in each).  Alone, a
+// CTA's turn takes as long as its SM needs for all its CTAs; a cluster adds the
+// latency of its barrier.  GPCs have 16 to 20 SMs, so large clusters leave some
+// of them out.
+void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan& l) {
+  static constexpr struct { int size; double reach; } kClusters[] = {
+      {1, 1.}, {2, 1.}, {4, .94}, {6, .9}, {8, .865}, {10, .83}, {12, .8}, {14, .77}, {16, .75}};
+  double least = -1.;
+  for (const auto& c : kClusters)
+    for (int w = 64; w >= 32; w /= 2) {
+      const int64_t slots = (int64_t)(sms * ctas * c.reach);
+      const int64_t need = l.stretches * ((p->D + w - 1) / w) * c.size;
+      const int64_t rows = (int64_t)c.size * (1024 * kCpt / w);
+      const double on_sm = (double)(need < slots ? need : slots) / sms;
+      const double alone = bwd ? 1.9 : 1.2, floor = bwd ? 2.2 : 1.2;  // microseconds
+      const double turn = c.size > 1 ? (bwd ? 2.9 : 2.) + .4 * on_sm + .05 * c.size
+                                     : (alone * on_sm > floor ? alone * on_sm : floor);
+      // single CTAs of a second wave start as others end, clusters hardly
+      double waves = (double)((need + slots - 1) / slots);
+      if (c.size == 1 && need > slots) waves = .5 * (waves + (double)need / slots);
+      const double cost = waves * (double)((l.rows + rows - 1) / rows + 2) * turn;
+      if (least < 0. || cost < least) {
+        least = cost;
+        l.slab = w;
+        l.cluster = c.size;
+      }
+    }
+}
 
-// The stretches are those of the backward's tiles in both directions, so that
-// the kept states are found again; the cluster follows the kernel's own tile.
-ScanArgs scan_args(const gdn2_scan_problem* p, int sms, int tile, int64_t* ctas) {
+ScanArgs scan_args(const gdn2_scan_problem* p, const ScanPlan& l) {
   ScanArgs a{};
   a.rows = (int64_t)p->B * p->T;
   a.T = p->T;
   a.D = p->D;
   a.n_seqs = p->n_seqs;
-  a.nslab = (p->D + kSlab - 1) / kSlab;
   a.cu = p->cu_seqlens;
   a.ldv = p->ld_v;
   a.ldg = p->ld_g;
   a.ldw = p->ld_w;
   a.lddy = p->ld_dy;
-  const ScanPlan l = scan_plan(p, sms, kKeep);
   a.stretch = l.rows;
-  a.keeps = scan_keeps(l);
+  a.keeps = (l.rows + kKeep - 1) / kKeep;
+  a.nslab = (p->D + l.slab - 1) / l.slab;
   a.cluster = l.cluster;
-  while (a.cluster > 1 && (int64_t)(a.cluster / 2) * tile >= l.rows) a.cluster /= 2;
-  *ctas = l.stretches * a.nslab * a.cluster;
   return a;
 }
 
 template <typename K>
-cudaError_t launch_scan(K kernel, const ScanArgs& a, int64_t ctas, int smem, cudaStream_t st) {
+cudaError_t launch_scan(K kernel, const ScanArgs& a, const ScanPlan& l, int threads, int stage,
+                        cudaStream_t st) {
+  const int smem = stage + (l.cluster > 1 ? 2 * l.cluster * l.slab * (int)sizeof(float2) : 0);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && a.cluster > 8)
+  if (e == cudaSuccess && l.cluster > 8)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kScanThreads);
+  cfg.gridDim = dim3((unsigned)(l.stretches * a.nslab * l.cluster));
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)a.cluster;
+  at.val.clusterDim.x = (unsigned)l.cluster;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  cfg.numAttrs = l.cluster > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 // Whether every group of kCpt channels of a row can be moved as one vector.
+// (and a tile's offsets held in 32 bits).
 bool group_ok(const void* p, int64_t ld, size_t es) {
-  return aligned_to(p, kCpt * es) && ld % kCpt == 0;
+  return aligned_to(p, kCpt * es) && ld % kCpt == 0 && ld <= (1 << 22);
 }
 
 // f(T, G, gate) over the element types and the presence of w.
@@ -771,10 +818,8 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   int sms = 0;
   const cudaError_t e = num_sms(&sms);
   if (e != cudaSuccess) return cuda_status(e, fn);
-  int64_t ctas = 0;
-  ScanArgs a = scan_args(p, sms, kSlots * (p->dtype == GDN2_DTYPE_F32 ? rows_of<float, false>()
-                                                                      : rows_of<__half, false>()),
-                         &ctas);
+  ScanPlan l = scan_stretches(p, sms);
+  ScanArgs a = scan_args(p, l);
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.y = y; a.ht = ht; a.saved = saved;
   const size_t es = dtype_size(p->dtype);
   const bool vec = a.D % kCpt == 0 && group_ok(v, a.ldv, es) && group_ok(y, a.D, es) &&
@@ -782,10 +827,20 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   return cuda_status(scan_dispatch(p, w != nullptr, [&](auto t, auto gt, auto gate) {
     using T = decltype(t);
     using G = decltype(gt);
-    constexpr bool W = decltype(gate)::value;
-    constexpr int smem = StageLayout<T, G, W, false, rows_of<T, false>()>::bytes;
-    return vec ? launch_scan(k_scan_fwd<T, G, W, true>, a, ctas, smem, st)
-               : launch_scan(k_scan_fwd<T, G, W, false>, a, ctas, smem, st);
+    constexpr bool GATE = decltype(gate)::value;
+    constexpr int stage = StageLayout<T, G, GATE, false>::bytes;
+    scan_fit(p, sms, ctas_of<T, false>(), false, l);
+    ScanArgs b = a;
+    b.nslab = (a.D + l.slab - 1) / l.slab;
+    b.cluster = l.cluster;
+    auto go = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      constexpr int R = rows_of<false>();
+      return vec ? launch_scan(k_scan_fwd<T, G, GATE, W, R, true>, b, l, 1024 / R, stage, st)
+                 : launch_scan(k_scan_fwd<T, G, GATE, W, R, false>, b, l, 1024 / R, stage, st);
+    };
+    return l.slab == 64 ? go(std::integral_constant<int, 64>{})
+                        : go(std::integral_constant<int, 32>{});
   }), fn);
 }
 
@@ -805,8 +860,8 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   int sms = 0;
   const cudaError_t e = num_sms(&sms);
   if (e != cudaSuccess) return cuda_status(e, fn);
-  int64_t ctas = 0;
-  ScanArgs a = scan_args(p, sms, kKeep, &ctas);
+  ScanPlan l = scan_stretches(p, sms);
+  ScanArgs a = scan_args(p, l);
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.saved = const_cast<float*>(saved);
   a.dy = dy; a.dht = dht; a.dv = dv; a.dg = dg; a.dw = dw; a.dh0 = dh0;
   const size_t es = dtype_size(p->dtype), eg = dtype_size(p->g_dtype);
@@ -816,10 +871,20 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   return cuda_status(scan_dispatch(p, w != nullptr, [&](auto t, auto gt, auto gate) {
     using T = decltype(t);
     using G = decltype(gt);
-    constexpr bool W = decltype(gate)::value;
-    constexpr int smem = StageLayout<T, G, W, true, rows_of<T, true>()>::bytes;
-    return vec ? launch_scan(k_scan_bwd<T, G, W, true>, a, ctas, smem, st)
-               : launch_scan(k_scan_bwd<T, G, W, false>, a, ctas, smem, st);
+    constexpr bool GATE = decltype(gate)::value;
+    constexpr int stage = StageLayout<T, G, GATE, true>::bytes;
+    scan_fit(p, sms, ctas_of<T, true>(), true, l);
+    ScanArgs b = a;
+    b.nslab = (a.D + l.slab - 1) / l.slab;
+    b.cluster = l.cluster;
+    auto go = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      constexpr int R = rows_of<true>();
+      return vec ? launch_scan(k_scan_bwd<T, G, GATE, W, R, true>, b, l, 1024 / R, stage, st)
+                 : launch_scan(k_scan_bwd<T, G, GATE, W, R, false>, b, l, 1024 / R, stage, st);
+    };
+    return l.slab == 64 ? go(std::integral_constant<int, 64>{})
+                        : go(std::integral_constant<int, 32>{});
   }), fn);
 }
 
