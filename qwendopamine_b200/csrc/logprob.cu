@@ -135,7 +135,14 @@ template <typename T> struct RowView {
   __device__ __forceinline__ bool whole(int j) const {
     return (j > 0 || off == 0) && (int64_t)(j + 1) * VE - off <= V;
   }
-  // absent elements read as -inf
+  // absent elements, and all of a vector that is not below `hi`, read as -inf
+  __device__ __forceinline__ Raw<T, VE> load(int j, int hi) const {
+    if (j < hi) return load(j);
+    float f[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = -INFINITY;
+    return raw_from<T, VE>(f);
+  }
   __device__ __forceinline__ Raw<T, VE> load(int j) const {
     if (whole(j)) return load_raw<T, VE>(base + (int64_t)j * VE);
     float f[VE];
@@ -149,7 +156,8 @@ template <typename T> struct RowView {
 };
 
 struct LogprobShared {
-  Soft warp[kLpWarps];
+  float warp_max[kLpWarps];
+  float2 warp_sum[kLpWarps];
   Soft total;
   uint32_t most[kLpThreads];
   int who[kLpThreads];
@@ -171,15 +179,11 @@ __device__ __forceinline__ void select_best(LogprobShared& s, int n, int k) {
   if (threadIdx.x == 0) s.n_best = n < k ? n : k;
 }
 
-// One warp's look through 32 vectors of the thread `s.who[u / segs]`.
+// Hands the elements of vector j that reach `least` to the CTA.
 template <typename T>
-__device__ __forceinline__ void collect(LogprobShared& s, const RowView<T>& row, int lo, int hi,
-                                        int u, int segs, uint64_t least) {
+__device__ __forceinline__ void collect(LogprobShared& s, const RowView<T>& row, int j,
+                                        uint64_t least) {
   constexpr int VE = RowView<T>::VE;
-  const int step = (u % segs) * 32 + (threadIdx.x & 31);
-  const int64_t jl = (int64_t)lo + s.who[u / segs] + (int64_t)step * kLpThreads;
-  if (jl >= hi) return;
-  const int j = (int)jl;
   const Raw<T, VE> r = row.load(j);
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
@@ -192,6 +196,50 @@ __device__ __forceinline__ void collect(LogprobShared& s, const RowView<T>& row,
   }
 }
 
+// The same for 32 vectors of the thread s.who[u / segs], one for each lane.
+template <typename T>
+__device__ __forceinline__ void collect_unit(LogprobShared& s, const RowView<T>& row, int lo, int hi,
+                                             int u, int segs, uint64_t least) {
+  const int step = (u % segs) * 32 + (threadIdx.x & 31);
+  const int64_t j = (int64_t)lo + s.who[u / segs] + (int64_t)step * kLpThreads;
+  if (j < hi) collect(s, row, (int)j, least);
+}
+
+// The k-th largest of the threads' values into s.bound (0 if fewer have one).
+// Up to 32 are found among the k largest of each warp, which a bitonic sort
+// puts in order; more by counting among all threads'.
+__device__ __forceinline__ void find_bound(LogprobShared& s, uint32_t mine, int k) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  int n = kLpThreads;
+  if (k <= 32) {
+    uint32_t x = mine;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int o = size / 2; o > 0; o /= 2) {
+        const uint32_t y = __shfl_xor_sync(0xffffffffu, x, o);
+        const bool falling = (lane & size) == 0, low = (lane & o) == 0;
+        x = low == falling ? max(x, y) : min(x, y);
+      }
+    n = kLpWarps * k;
+    if (lane < k) s.most[(tid >> 5) * k + lane] = x;
+  } else {
+    s.most[tid] = mine;
+  }
+  __syncthreads();
+  if (tid < n) {
+    const uint32_t x = s.most[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const uint32_t y = s.most[j];
+      rank += y > x || (y == x && j < tid);
+    }
+    if (rank == k - 1) s.bound = x;
+  }
+  __syncthreads();
+}
+
 // The CTA's k largest elements of vectors [lo, hi), given every thread's largest.
 template <typename T>
 __device__ void cta_top(LogprobShared& s, const RowView<T>& row, int lo, int hi, float most,
@@ -199,23 +247,29 @@ __device__ void cta_top(LogprobShared& s, const RowView<T>& row, int lo, int hi,
   const int tid = threadIdx.x, warp = tid >> 5;
   const bool any = lo + tid < hi;
   const uint32_t mine = any ? order_of(most) : 0u;
-  s.most[tid] = mine;
-  if (tid == 0) { s.n_who = 0; s.n_cand = 0; s.bound = 0u; }
-  __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int j = 0; j < kLpThreads; ++j)
-    rank += s.most[j] > mine || (s.most[j] == mine && j < tid);
-  if (rank == k - 1) s.bound = mine;
-  __syncthreads();
+  if (tid == 0) { s.n_who = 0; s.n_cand = 0; }
+  find_bound(s, mine, k);
   const uint32_t bound = s.bound;
-  if (any && mine >= bound) s.who[atomicAdd(&s.n_who, 1)] = tid;
-  __syncthreads();
   const int steps = (hi - lo + kLpThreads - 1) / kLpThreads, segs = (steps + 31) / 32;
-  const int units = s.n_who * segs;
-  for (int u = warp; u < units; u += kLpWarps)
-    collect(s, row, lo, hi, u, segs, (uint64_t)bound << 32);
+  const bool reach = any && mine >= bound;
+  if (steps <= 4) {  // few vectors: a thread looks through its own
+    if (reach)
+      for (int j = lo + tid; j < hi; j += kLpThreads) collect(s, row, j, (uint64_t)bound << 32);
+    __syncthreads();
+    if (s.n_cand <= kCandidates) {
+      select_best(s, s.n_cand, k);
+      __syncthreads();
+      return;
+    }
+  }
+  if (reach) s.who[atomicAdd(&s.n_who, 1)] = tid;
   __syncthreads();
+  const int units = s.n_who * segs;
+  if (steps > 4) {
+    for (int u = warp; u < units; u += kLpWarps)
+      collect_unit(s, row, lo, hi, u, segs, (uint64_t)bound << 32);
+    __syncthreads();
+  }
   const int n = s.n_cand;
   if (n <= kCandidates) {
     select_best(s, n, k);
@@ -229,7 +283,7 @@ __device__ void cta_top(LogprobShared& s, const RowView<T>& row, int lo, int hi,
   if (tid == 0) { s.n_cand = 0; s.least = (uint64_t)bound << 32; }
   __syncthreads();
   for (int u0 = 0; u0 < units; u0 += kLpWarps) {
-    if (u0 + warp < units) collect(s, row, lo, hi, u0 + warp, segs, s.least);
+    if (u0 + warp < units) collect_unit(s, row, lo, hi, u0 + warp, segs, s.least);
     __syncthreads();
     const int have = s.n_cand;
     const bool last = u0 + kLpWarps >= units;
@@ -248,25 +302,84 @@ __device__ void cta_top(LogprobShared& s, const RowView<T>& row, int lo, int hi,
   }
 }
 
+// Running maximum and sums of a thread's elements, four vectors at a time.
+template <typename T, bool ENT> struct Running {
+  static constexpr int VE = RowView<T>::VE;
+  float m = -FLT_MAX, most = -INFINITY;  // finite; the largest element itself
+  float2 s = make_float2(0.f, 0.f), w = make_float2(0.f, 0.f);
+
+  template <int N> __device__ __forceinline__ void add(const Raw<T, VE> (&v)[N], float c) {
+    float top = raw_max(v[0]);
+#pragma unroll
+    for (int u = 1; u < N; ++u) top = fmaxf(top, raw_max(v[u]));
+    most = fmaxf(most, top);
+    if (top > m) lift(top, c);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i) {
+        const float2 y = mul2(add2(raw_pair(v[u], i), f2(-m)), f2(c));
+        const float2 e = exp2_2(y);
+        s = add2(s, e);
+        if constexpr (ENT) w = fma2(e, make_float2(fmaxf(y.x, kLow), fmaxf(y.y, kLow)), w);
+      }
+  }
+  // the sums with respect to a larger maximum
+  __device__ __forceinline__ void lift(float top, float c) {
+    const float y = (m - top) * c, f = fast_exp2(y), g = fmaxf(y, kLow);
+    if constexpr (ENT) w = mul2(f2(f), fma2(s, f2(g), w));
+    s = mul2(s, f2(f));
+    m = top;
+  }
+};
+
+__device__ __forceinline__ float warp_most(float x) {  // NaN does not count
+  const uint32_t o = __reduce_max_sync(0xffffffffu, order_of(x));
+  return value_of(o);
+}
+
+// A row's results from its sums: log probability of x (NaN for a token outside
+// the vocabulary), entropy, and what the backward needs.
+struct RowEnd {
+  float lg, ent;
+  bool none;  // every logit is -inf
+  __device__ __forceinline__ RowEnd(const Soft& t) {
+    none = t.s == 0.f;
+    lg = log2f(t.s);
+    ent = none ? 0.f : kLn2 * (lg - t.w / t.s);
+  }
+  __device__ __forceinline__ float logp(const Soft& t, float x, float c) const {
+    return none ? -INFINITY : kLn2 * ((x - t.m) * c - lg);
+  }
+  __device__ __forceinline__ void write(const LogprobArgs& a, const Soft& t, int64_t r, int64_t id,
+                                        float x) const {
+    a.logp[r] = id >= 0 && id < a.V ? logp(t, x, a.c) : __uint_as_float(0x7fffffffu);
+    if (a.entropy) a.entropy[r] = ent;
+    if (a.stats) a.stats[r] = make_float4(t.m, none ? 0.f : 1.f / t.s, none ? 0.f : lg, ent);
+  }
+};
+
+__device__ __forceinline__ void write_ignored(const LogprobArgs& a, int64_t r, int thread, int threads) {
+  if (thread == 0) {
+    a.logp[r] = 0.f;
+    if (a.entropy) a.entropy[r] = 0.f;
+  }
+  for (int i = thread; i < a.k; i += threads) {
+    a.top_logp[r * a.k + i] = -INFINITY;
+    a.top_ids[r * a.k + i] = -1;
+  }
+}
+
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) k_logprob_fwd(const LogprobArgs a, const int parts) {
+__global__ void __launch_bounds__(kLpThreads, 5) k_logprob_fwd(const LogprobArgs a, const int parts) {
   constexpr int VE = RowView<T>::VE;
   __shared__ LogprobShared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / (unsigned)parts;
   const int part = (int)(blockIdx.x - r * parts);
   const int64_t id = a.ids[r];
   if (id == a.ignore) {  // the same for the whole cluster
-    if (part == 0) {
-      if (threadIdx.x == 0) {
-        a.logp[r] = 0.f;
-        if (a.entropy) a.entropy[r] = 0.f;
-      }
-      if constexpr (TOP)
-        for (int i = threadIdx.x; i < a.k; i += kLpThreads) {
-          a.top_logp[r * a.k + i] = -INFINITY;
-          a.top_ids[r * a.k + i] = -1;
-        }
-    }
+    if (part == 0) write_ignored(a, r, tid, kLpThreads);
     return;
   }
   const T* xr = (const T*)a.x + r * a.ld;
@@ -274,67 +387,47 @@ __global__ void __launch_bounds__(kLpThreads) k_logprob_fwd(const LogprobArgs a,
   const int per = (row.nvec + parts - 1) / parts;
   const int lo = min(part * per, row.nvec), hi = min(lo + per, row.nvec);
   const float c = a.c;
+  float given = 0.f;  // the token's logit, on its way early
+  if (tid == 0 && part == 0 && id >= 0 && id < a.V) given = to_f<T>(xr[id]);
 
-  float m = -FLT_MAX, most = -INFINITY;
-  float2 sum = make_float2(0.f, 0.f), wsum = make_float2(0.f, 0.f);
-  auto add = [&](const Raw<T, VE>* v, int n) {
-    float top = raw_max(v[0]);
-#pragma unroll
-    for (int u = 1; u < kLpUnroll; ++u)
-      if (u < n) top = fmaxf(top, raw_max(v[u]));
-    most = fmaxf(most, top);
-    if (top > m) {
-      const float y = (m - top) * c, f = fast_exp2(y), g = fmaxf(y, kLow);
-      if constexpr (ENT) {
-        wsum.x = f * fmaf(sum.x, g, wsum.x);
-        wsum.y = f * fmaf(sum.y, g, wsum.y);
-      }
-      sum.x *= f;
-      sum.y *= f;
-      m = top;
-    }
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u)
-      if (u < n) {
-#pragma unroll
-        for (int i = 0; i < VE / 2; ++i) {
-          const float2 y = mul2(add2(raw_pair(v[u], i), f2(-m)), f2(c));
-          const float2 e = exp2_2(y);
-          sum = add2(sum, e);
-          if constexpr (ENT)
-            wsum = fma2(e, make_float2(fmaxf(y.x, kLow), fmaxf(y.y, kLow)), wsum);
-        }
-      }
-  };
-  int j = lo + threadIdx.x;
+  Running<T, ENT> run;
+  Raw<T, VE> v[kLpUnroll];
+  int j = lo + tid;
   for (; j + (kLpUnroll - 1) * kLpThreads < hi; j += kLpUnroll * kLpThreads) {
-    Raw<T, VE> v[kLpUnroll];
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) v[u] = row.load(j + u * kLpThreads);
-    add(v, kLpUnroll);
+    run.add(v, c);
   }
-  for (; j < hi; j += kLpThreads) {
-    const Raw<T, VE> v = row.load(j);
-    add(&v, 1);
+  if (j < hi) {
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) v[u] = row.load(j + u * kLpThreads, hi);
+    run.add(v, c);
   }
 
-  Soft t{m, sum.x + sum.y, wsum.x + wsum.y};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Soft q{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o),
-                 __shfl_xor_sync(0xffffffffu, t.w, o)};
-    t = merge(t, q, c);
+  // the CTA's maximum, then its sums with respect to it
+  {
+    const float m = warp_most(run.m);
+    if (lane == 0) s.warp_max[warp] = m;
   }
-  if ((threadIdx.x & 31) == 0) s.warp[threadIdx.x >> 5] = t;
-  if constexpr (TOP) cta_top(s, row, lo, hi, most, a.k);
-  __syncthreads();
-  t = s.warp[0];
+  if constexpr (TOP) cta_top(s, row, lo, hi, run.most, a.k);
+  else __syncthreads();
+  float m = s.warp_max[0];
 #pragma unroll
-  for (int i = 1; i < kLpWarps; ++i) t = merge(t, s.warp[i], c);
+  for (int i = 1; i < kLpWarps; ++i) m = fmaxf(m, s.warp_max[i]);
+  run.lift(m, c);
+  const float ps = warp_sum(run.s.x + run.s.y), pw = ENT ? warp_sum(run.w.x + run.w.y) : 0.f;
+  if (lane == 0) s.warp_sum[warp] = make_float2(ps, pw);
+  __syncthreads();
+  Soft t{m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kLpWarps; ++i) {
+    t.s += s.warp_sum[i].x;
+    t.w += s.warp_sum[i].y;
+  }
 
   if (parts > 1) {
     cg::cluster_group cluster = cg::this_cluster();
-    if (threadIdx.x == 0) s.total = t;
+    if (tid == 0) s.total = t;
     cluster.sync();
     if (part == 0) {
       for (int q = 1; q < parts; ++q) t = merge(t, *cluster.map_shared_rank(&s.total, q), c);
@@ -343,7 +436,7 @@ __global__ void __launch_bounds__(kLpThreads) k_logprob_fwd(const LogprobArgs a,
         for (int q = 0; q < parts; ++q) {
           const LogprobShared* o = cluster.map_shared_rank(&s, q);
           const int have = o->n_best;
-          for (int i = threadIdx.x; i < have; i += kLpThreads) s.cand[n + i] = o->best[i];
+          for (int i = tid; i < have; i += kLpThreads) s.cand[n + i] = o->best[i];
           n += have;
         }
         __syncthreads();
@@ -355,24 +448,65 @@ __global__ void __launch_bounds__(kLpThreads) k_logprob_fwd(const LogprobArgs a,
     if (part != 0) return;
   }
 
-  const bool none = t.s == 0.f;  // every logit is -inf
-  const float lg = log2f(t.s);
-  const float ent = none ? 0.f : kLn2 * (lg - t.w / t.s);
-  if (threadIdx.x == 0) {
-    float lp = __uint_as_float(0x7fffffffu);  // a token outside the vocabulary
-    if (id >= 0 && id < a.V)
-      lp = none ? -INFINITY : kLn2 * ((to_f<T>(xr[id]) - t.m) * c - lg);
-    a.logp[r] = lp;
-    if constexpr (ENT)
-      if (a.entropy) a.entropy[r] = ent;
-    if (a.stats) a.stats[r] = make_float4(t.m, none ? 0.f : 1.f / t.s, none ? 0.f : lg, ent);
+  if (TOP || tid == 0) {
+    const RowEnd end(t);
+    if (tid == 0) end.write(a, t, r, id, given);
+    if constexpr (TOP)
+      for (int i = tid; i < a.k; i += kLpThreads) {
+        const uint64_t key = s.best[i];
+        a.top_logp[r * a.k + i] = end.logp(t, value_of((uint32_t)(key >> 32)), c);
+        a.top_ids[r * a.k + i] = (int64_t)(uint32_t)~(uint32_t)key;
+      }
   }
+}
+
+// Rows of up to 32 * kLpUnroll vectors: a warp each, the row in registers.  The
+// top k come out one by one: the lanes' best by two reductions (value, then the
+// lower index), and the lane that held it looks for its next.
+template <typename T, bool ENT, bool TOP>
+__global__ void __launch_bounds__(kLpThreads) k_logprob_small(const LogprobArgs a) {
+  constexpr int VE = RowView<T>::VE;
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kLpWarps + (threadIdx.x >> 5);
+  if (r >= a.rows) return;
+  const int64_t id = a.ids[r];
+  if (id == a.ignore) return write_ignored(a, r, lane, 32);
+  const T* xr = (const T*)a.x + r * a.ld;
+  const RowView<T> row(xr, a.V);
+  float given = 0.f;
+  if (lane == 0 && id >= 0 && id < a.V) given = to_f<T>(xr[id]);
+  Raw<T, VE> v[kLpUnroll];
+#pragma unroll
+  for (int u = 0; u < kLpUnroll; ++u) v[u] = row.load(lane + 32 * u, row.nvec);
+  Running<T, ENT> run;
+  run.add(v, a.c);
+  run.lift(warp_most(run.m), a.c);
+  const Soft t{run.m, warp_sum(run.s.x + run.s.y), ENT ? warp_sum(run.w.x + run.w.y) : 0.f};
+  const RowEnd end(t);
+  if (lane == 0) end.write(a, t, r, id, given);
   if constexpr (TOP) {
-    for (int i = threadIdx.x; i < a.k; i += kLpThreads) {
-      const uint64_t key = s.best[i];
-      const float x = value_of((uint32_t)(key >> 32));
-      a.top_logp[r * a.k + i] = none ? -INFINITY : kLn2 * ((x - t.m) * c - lg);
-      a.top_ids[r * a.k + i] = (int64_t)(uint32_t)~(uint32_t)key;
+    uint64_t last = ~0ull, best = 0;  // this lane's largest key below `last`
+    bool look = true;
+    for (int n = 0; n < a.k; ++n) {
+      if (look) {
+        best = 0;
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const int64_t i = (int64_t)(lane + 32 * u) * VE + e - row.off;
+            const uint64_t key = key_of(raw_get(v[u], e), (int)i);
+            if (i >= 0 && i < row.V && key < last && key > best) best = key;
+          }
+      }
+      const uint32_t hi = (uint32_t)(best >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+      const uint32_t lo = __reduce_max_sync(0xffffffffu, best && hi == top ? (uint32_t)best : 0u);
+      look = best && hi == top && (uint32_t)best == lo;
+      if (look) last = best;
+      if (lane == 0) {
+        a.top_logp[r * a.k + n] = end.logp(t, value_of(top), a.c);
+        a.top_ids[r * a.k + n] = (int64_t)(uint32_t)~lo;
+      }
     }
   }
 }
@@ -490,6 +624,12 @@ cudaError_t row_parts(int64_t rows, int64_t row_bytes, int* parts) {
 
 template <typename T, bool ENT, bool TOP>
 cudaError_t launch_logprob(const LogprobArgs& a, int parts, cudaStream_t st) {
+  // with one vector to spare for a row that starts inside one
+  if (a.V <= (32 * kLpUnroll - 1) * RowView<T>::VE) {
+    k_logprob_small<T, ENT, TOP>
+        <<<(unsigned)((a.rows + kLpWarps - 1) / kLpWarps), kLpThreads, 0, st>>>(a);
+    return cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * parts));
   cfg.blockDim = dim3(kLpThreads);
