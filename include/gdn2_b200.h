@@ -459,7 +459,8 @@ int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensor
  * that runs out makes the kernel release its tensor memory, return without
  * finishing, and set a bit of a per-device fault word (bit 0: state passes,
  * bit 1: forward intra-chunk kernel, bit 2: decode, bit 3: backward
- * intra-chunk kernel).  gdn2_fault_status
+ * intra-chunk kernel, bit 4: gated linear recurrence, which finishes with
+ * NaN).  gdn2_fault_status
  * synchronises `stream` (the default stream when NULL), returns the fault
  * word of the current device (0 = no fault) and resets it when `clear` is
  * nonzero; a negative return is a CUDA error.  No counterpart in the

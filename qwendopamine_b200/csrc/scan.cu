@@ -35,8 +35,8 @@
 // for too few.
 #include <cooperative_groups.h>
 
-#include "mma16.cuh"
 #include "op_util.cuh"
+#include "tc.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -46,6 +46,7 @@ namespace {
 constexpr int kCpt = 4;           // channels of a thread
 constexpr int kKeep = 64;         // rows between the states kept for the backward
 constexpr int kMaxCluster = 16;
+constexpr unsigned kScanFault = 16u;  // of the device's fault word
 
 // A tile of W channels: `lanes` threads across and `slots` threads down, R rows
 // and kCpt channels each.
@@ -57,10 +58,10 @@ template <int W, int R> struct Shape {
 
 // Rows of a thread, and CTAs that share an SM (what their registers allow).
 // Forward: four CTAs of 128 threads with eight rows each (B = 8, T = 4096,
-// D = 2048, bf16: 124 us; two of 256 with four rows 119 us, but 354 against
-// 267 us on one sequence of 131,072 x 1024).  Backward, with twice the tensors
-// in registers: two CTAs of 256 threads with four rows (215 us; three of 128
-// with eight rows 263 us).
+// D = 2048, bf16: 122 us, 85 % of the measured copy bandwidth; two of 256 with
+// four rows 119 us, but 354 against 267 us on one sequence of 131,072 x 1024).
+// Backward, with twice the tensors in registers: two CTAs of 256 threads with
+// four rows (214 us, 87 %; three of 128 with eight rows 263 us).
 template <bool BWD> constexpr int rows_of() { return BWD ? 4 : 8; }
 template <typename T, bool BWD> constexpr int ctas_of() {
   return BWD ? (sizeof(T) == 2 ? 2 : 1) : (sizeof(T) == 2 ? 4 : 3);
@@ -77,6 +78,7 @@ struct ScanArgs {
   const float *h0, *dht;
   void *y, *dv, *dg, *dw;
   float *ht, *dh0, *saved;
+  unsigned* fault;
 };
 
 // A run of rows: A in x (-1: it holds a reset), H in y.
@@ -94,6 +96,7 @@ template <int W, int R> struct ScanShared {
   static constexpr int tile = Shape<W, R>::tile, slots = Shape<W, R>::slots;
   // runs of the slots of rows, by turn's parity; then in H the states entering them
   float A[2][slots][W], H[2][slots][W];
+  uint64_t bar[2];  // the cluster's runs have come, by turn's parity
   // of a turn with sequence edges in its tile
   int seq[tile];                               // the row's sequence
   uint32_t first[tile / 32], last[tile / 32];  // whether it is its first / last row
@@ -135,27 +138,58 @@ template <int W, int R, bool UP> struct Fold {
   }
 };
 
+// A 64-bit store into another CTA's shared memory that counts on a barrier there.
+__device__ __forceinline__ void store_async(uint32_t to, uint32_t bar, float2 x) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to),
+               "l"(*reinterpret_cast<const uint64_t*>(&x)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t address_at(uint32_t a, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+
+// Before the first turn: the cluster's barriers, known to all its CTAs.
+template <int W, int R>
+__device__ __forceinline__ void open_exchange(const ScanArgs& a, ScanShared<W, R>& s) {
+  if (a.cluster == 1) return;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&s.bar[0], 1);
+    tc::mbar_init(&s.bar[1], 1);
+    tc::fence_mbar_init();
+  }
+  cg::this_cluster().sync();
+}
+
 // Puts the states that enter the slots of this CTA's tile into s.H and moves
 // `state` (threads 0 .. W-1, one per channel) from the state that enters the
 // turn's first tile to the one that leaves its last.  Called by all threads
-// after a barrier; ends with one.  `runs` holds the runs of the cluster's
-// tiles by turn's parity: those of turn i+2 overwrite those of turn i, which
-// every CTA has folded before it arrives at the cluster barrier of turn i+1.
+// after a barrier; ends with one.
+//
+// In a cluster every CTA sends its tile's run to all, into `runs` by turn's
+// parity, and waits for as many; a cluster-wide barrier would also wait for
+// the last turn's stores to reach memory.  A thread sends the run of turn i+1
+// after it has read those of turn i, and receives all of turn i+1 before it
+// sends turn i+2: the same places are free by then.  A wait that runs out sets
+// a fault bit and turns the states into NaN.
 template <int W, int R, bool UP>
 __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s, float2* runs, int rank,
-                                         int b, float& state) {
-  const int ch = threadIdx.x;
-  if (a.cluster == 1) {
-    if (ch < W) state = Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, state);
-  } else {
-    cg::cluster_group cluster = cg::this_cluster();
-    runs += b * a.cluster * W;
-    if (ch < W) {
+                                         int turn, float& state) {
+  const int ch = threadIdx.x, b = turn & 1;
+  if (ch < W) {
+    if (a.cluster == 1) {
+      state = Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, state);
+    } else {
+      runs += b * a.cluster * W;
       const float2 all = Fold<W, R, UP>::run(s.A[b], s.H[b], ch);
-      for (int k = 0; k < a.cluster; ++k) *cluster.map_shared_rank(runs + rank * W + ch, k) = all;
-    }
-    cluster.sync();
-    if (ch < W) {
+      if (ch == 0) tc::mbar_expect_tx(&s.bar[b], a.cluster * W * (int)sizeof(float2));
+      const uint32_t to = smem_u32(runs + rank * W + ch), bar = smem_u32(&s.bar[b]);
+      for (int k = 0; k < a.cluster; ++k) store_async(address_at(to, k), address_at(bar, k), all);
+      if (!tc::mbar_wait(&s.bar[b], (turn >> 1) & 1)) {
+        atomicOr(a.fault, kScanFault);
+        state = __int_as_float(0x7fffffff);
+      }
       float carry = state;
 #pragma unroll 4
       for (int k = 0; k < a.cluster; ++k) {
@@ -387,7 +421,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.h0, a.ht);
   if (p.turns > 0) fill(tile);
-  if (a.cluster > 1) cg::this_cluster().sync();  // all CTAs run before one writes to another
+  open_exchange(a, s);
   float state = 0.f;
   RowPlace place{0, 0, 0};
 
@@ -450,7 +484,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
     *reinterpret_cast<float4*>(&s.A[b][slot][lc]) = quad(A);
     *reinterpret_cast<float4*>(&s.H[b][slot][lc]) = quad(h);
     __syncthreads();
-    exchange<W, R, false>(a, s, runs, p.rank, b, state);
+    exchange<W, R, false>(a, s, runs, p.rank, turn, state);
 
     unquad(h, *reinterpret_cast<const float4*>(&s.H[b][slot][lc]));
     const int64_t left = p.hi - tile - r0;  // rows that exist from here
@@ -492,7 +526,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.dht, a.dh0);
   if (p.turns > 0) fill(tile);
-  if (a.cluster > 1) cg::this_cluster().sync();  // all CTAs run before one writes to another
+  open_exchange(a, s);
   float state = 0.f;
   RowPlace place{0, 0, 0};
 
@@ -562,7 +596,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
     __syncthreads();
     if (threadIdx.x / W == 1)
       Fold<W, R, false>::enter(ahead.A[b], ahead.H[b], threadIdx.x - W, kept);
-    exchange<W, R, true>(a, s, runs, p.rank, b, state);
+    exchange<W, R, true>(a, s, runs, p.rank, turn, state);
 
     const int64_t left = some ? p.hi - tile - r0 : 0;  // rows that exist from here
     const Target<G, W, R> dg(a.dg, tile, p.slab, a.D);
@@ -704,10 +738,9 @@ ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
 
 // Slab and cluster: what takes the least time by a model of a turn, fitted to
 // runs of both directions over slabs and clusters (seven shapes from 9001 x 1000
-// to 131,072 x 1024; it chose within a tenth of the fastest in each).  Alone, a
-// CTA's turn takes as long as its SM needs for all its CTAs; a cluster adds the
-// latency of its barrier.  GPCs have 16 to 20 SMs, so large clusters leave some
-// of them out.
+// to 131,072 x 1024).  A turn takes its latency, which grows with the cluster,
+// or what its SM needs for all its CTAs.  GPCs have 16 to 20 SMs, so large
+// clusters leave some of them out.
 void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan& l) {
   static constexpr struct { int size; double reach; } kClusters[] = {
       {1, 1.}, {2, 1.}, {4, .94}, {6, .9}, {8, .865}, {10, .83}, {12, .8}, {14, .77}, {16, .75}};
@@ -718,12 +751,13 @@ void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan&
       const int64_t need = l.stretches * ((p->D + w - 1) / w) * c.size;
       const int64_t rows = (int64_t)c.size * (1024 * kCpt / w);
       const double on_sm = (double)(need < slots ? need : slots) / sms;
-      const double alone = bwd ? 1.9 : 1.2, floor = bwd ? 2.2 : 1.2;  // microseconds
-      const double turn = c.size > 1 ? (bwd ? 2.9 : 2.) + .4 * on_sm + .05 * c.size
-                                     : (alone * on_sm > floor ? alone * on_sm : floor);
-      // single CTAs of a second wave start as others end, clusters hardly
-      double waves = (double)((need + slots - 1) / slots);
-      if (c.size == 1 && need > slots) waves = .5 * (waves + (double)need / slots);
+      // microseconds
+      const double latency = c.size > 1 ? (bwd ? 2.8 : 1.7) + .03 * c.size : (bwd ? 2.2 : 1.2);
+      const double work = on_sm * (bwd ? 1.93 : w == 64 ? 1.1 : 1.22);
+      const double turn = .25 + (latency > work ? latency : work);
+      // what a second wave holds starts as the first ends
+      const double waves = .5 * ((double)((need + slots - 1) / slots) +
+                                 (need > slots ? (double)need / slots : 1.));
       const double cost = waves * (double)((l.rows + rows - 1) / rows + 2) * turn;
       if (least < 0. || cost < least) {
         least = cost;
@@ -816,10 +850,11 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   if (p->n_seqs == 0 || (rows == 0 && !ht)) return GDN2_OK;
   const cudaStream_t st = (cudaStream_t)stream;
   int sms = 0;
-  const cudaError_t e = num_sms(&sms);
+  cudaError_t e = num_sms(&sms);
   if (e != cudaSuccess) return cuda_status(e, fn);
   ScanPlan l = scan_stretches(p, sms);
   ScanArgs a = scan_args(p, l);
+  if ((e = fault_word(&a.fault)) != cudaSuccess) return cuda_status(e, fn);
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.y = y; a.ht = ht; a.saved = saved;
   const size_t es = dtype_size(p->dtype);
   const bool vec = a.D % kCpt == 0 && group_ok(v, a.ldv, es) && group_ok(y, a.D, es) &&
@@ -858,10 +893,11 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   if (p->n_seqs == 0 || (rows == 0 && !dh0)) return GDN2_OK;
   const cudaStream_t st = (cudaStream_t)stream;
   int sms = 0;
-  const cudaError_t e = num_sms(&sms);
+  cudaError_t e = num_sms(&sms);
   if (e != cudaSuccess) return cuda_status(e, fn);
   ScanPlan l = scan_stretches(p, sms);
   ScanArgs a = scan_args(p, l);
+  if ((e = fault_word(&a.fault)) != cudaSuccess) return cuda_status(e, fn);
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.saved = const_cast<float*>(saved);
   a.dy = dy; a.dht = dht; a.dv = dv; a.dg = dg; a.dw = dw; a.dh0 = dh0;
   const size_t es = dtype_size(p->dtype), eg = dtype_size(p->g_dtype);
