@@ -275,38 +275,59 @@ template <typename T, int R> struct Stage {
   __device__ static __forceinline__ char* at(char* base, int i) {
     return base + (i * (1024 / R) + threadIdx.x) * kGroupBytes;
   }
-  __device__ static __forceinline__ void copy(char* base, int i, const void* src, int have) {
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(base, i));
-    if constexpr (kGroupBytes == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+  // `have` of the AL elements at src to a row's group, from element `e` on;
+  // what is missing is filled with zeros
+  template <int AL>
+  __device__ static __forceinline__ void copy(char* base, int i, int e, const void* src, int have) {
+    constexpr int bytes = AL * (int)sizeof(T);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(base, i)) + e * (int)sizeof(T);
+    const int n = have > 0 ? bytes : 0;
+    if constexpr (bytes == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
     else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(bytes) : "memory");
   }
   // The thread's rows of the tile at row `tile` (the same for the CTA), of
   // which those in [lo, hi) exist, `nc` channels wide; what does not exist
-  // reads as zero, but a thread without channels reads nothing.
-  template <int W, bool VEC>
+  // reads as zero, but a thread without channels reads nothing.  AL elements
+  // (4, 2 or 1) are aligned together; single 16-bit ones are too small to be
+  // copied asynchronously and go through registers.
+  template <int W, int AL>
   __device__ static __forceinline__ void fill(char* base, const void* x, int64_t ld, int64_t tile,
                                               int64_t lo, int64_t hi, int slab, int nc) {
     if (nc <= 0) return;
     const int r0 = (int)threadIdx.x / Shape<W, R>::lanes * R;
     const int lc = (int)threadIdx.x % Shape<W, R>::lanes * kCpt;
     const char* p = (const char*)x + (tile * ld + slab * W) * (int64_t)sizeof(T);
-    if (VEC && tile >= lo && tile + Shape<W, R>::tile <= hi) {
+    const bool inside = tile >= lo && tile + Shape<W, R>::tile <= hi && nc >= kCpt;
+    if (AL * sizeof(T) >= 4 && inside) {
       const uint32_t off = (uint32_t)(r0 * (int)ld + lc) * (uint32_t)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < R; ++i, p += ld * (int64_t)sizeof(T)) copy(base, i, p + off, kGroupBytes);
+      for (int i = 0; i < R; ++i, p += ld * (int64_t)sizeof(T))
+#pragma unroll
+        for (int e = 0; e < kCpt; e += AL)
+          copy<(AL * sizeof(T) >= 4 ? AL : 4)>(base, i, e, p + off + e * sizeof(T), AL);
       return;
     }
     const T* q = (const T*)p + r0 * ld + lc;
+    if constexpr (AL * sizeof(T) >= 4) {
 #pragma unroll 1
-    for (int i = 0; i < R; ++i, q += ld) {
-      const int64_t r = tile + r0 + i;
-      const int n = r >= lo && r < hi ? nc : 0;
-      if constexpr (VEC)
-        copy(base, i, n > 0 ? (const void*)q : x, n > 0 ? kGroupBytes : 0);
-      else
-        *reinterpret_cast<Raw<T, kCpt>*>(at(base, i)) = load_group<T, kCpt, false>(q, n);
+      for (int i = 0; i < R; ++i, q += ld) {
+        const int64_t r = tile + r0 + i;
+        const int n = r >= lo && r < hi ? nc : 0;
+#pragma unroll
+        for (int e = 0; e < kCpt; e += AL)
+          copy<AL>(base, i, e, n > e ? (const void*)(q + e) : x, n - e);
+      }
+    } else {
+      Raw<T, kCpt> rows[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i, q += ld) {
+        const int64_t r = tile + r0 + i;
+        rows[i] = load_group<T, kCpt, false>(q, inside ? kCpt : r >= lo && r < hi ? nc : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) *reinterpret_cast<Raw<T, kCpt>*>(at(base, i)) = rows[i];
     }
   }
   __device__ static __forceinline__ Raw<T, kCpt> get(char* base, int i) {
@@ -372,9 +393,16 @@ template <typename T, int W, int R> struct Target {
     off = (uint32_t)(r0 * D + lc) * (uint32_t)sizeof(T);
     row_bytes = D * (int)sizeof(T);
   }
-  template <bool VEC> __device__ __forceinline__ void put(int i, const float2 (&x)[2], int n) const {
-    const float f[kCpt] = {x[0].x, x[0].y, x[1].x, x[1].y};
-    store_group<T, kCpt, VEC>((T*)(base + (int64_t)i * row_bytes + off), f, n);
+  template <int AL> __device__ __forceinline__ void put(int i, const float2 (&x)[2], int n) const {
+    T* const p = (T*)(base + (int64_t)i * row_bytes + off);
+    if constexpr (AL == 2) {
+      const float f[2][2] = {{x[0].x, x[0].y}, {x[1].x, x[1].y}};
+      if (n > 0) store_raw<T, 2>(p, raw_from<T, 2>(f[0]));
+      if (n > 2) store_raw<T, 2>(p + 2, raw_from<T, 2>(f[1]));
+    } else {
+      const float f[kCpt] = {x[0].x, x[0].y, x[1].x, x[1].y};
+      store_group<T, kCpt, AL == 4>(p, f, n);
+    }
   }
 };
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
@@ -401,7 +429,7 @@ __device__ __forceinline__ void put_state(float* x, int64_t seq, int D, int c, i
     if (j < nc) x[seq * D + c + j] = f[j];
 }
 
-template <typename T, typename G, bool GATE, int W, int R, bool VEC>
+template <typename T, typename G, bool GATE, int W, int R, int AL>
 __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(const ScanArgs a) {
   constexpr int TILE = Shape<W, R>::tile;
   using L = StageLayout<T, G, GATE, false>;
@@ -414,10 +442,10 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
   const int64_t step = (int64_t)a.cluster * TILE;
   int64_t tile = p.lo + (int64_t)p.rank * TILE;  // first row of this turn's tile
   auto fill = [&](int64_t row) {
-    Stage<G, R>::template fill<W, VEC>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, VEC>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
+    Stage<G, R>::template fill<W, AL>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, AL>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<W, VEC>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
+      Stage<T, R>::template fill<W, AL>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.h0, a.ht);
   if (p.turns > 0) fill(tile);
@@ -493,17 +521,17 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
     const Target<T, W, R> y(a.y, tile, p.slab, a.D);
     if (edges) {
       walk(std::true_type{}, [&](int i) {
-        y.template put<VEC>(i, h, i < left ? nc : 0);
+        y.template put<AL>(i, h, i < left ? nc : 0);
         if ((last >> i & 1) && a.ht) put_state(a.ht, s.seq[r0 + i], a.D, c, nc, h);
       });
       __syncthreads();  // the marks have been read
     } else {
-      walk(std::false_type{}, [&](int i) { y.template put<VEC>(i, h, nc); });
+      walk(std::false_type{}, [&](int i) { y.template put<AL>(i, h, nc); });
     }
   }
 }
 
-template <typename T, typename G, bool GATE, int W, int R, bool VEC>
+template <typename T, typename G, bool GATE, int W, int R, int AL>
 __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const ScanArgs a) {
   constexpr int TILE = Shape<W, R>::tile;
   using L = StageLayout<T, G, GATE, true>;
@@ -518,11 +546,11 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   // from the chain's last tile down; before the first there is nothing
   int64_t tile = p.lo + ((p.hi - p.lo + TILE - 1) / TILE - 1 - p.rank) * TILE;
   auto fill = [&](int64_t row) {
-    Stage<G, R>::template fill<W, VEC>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, VEC>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, VEC>(st + L::dy, a.dy, a.lddy, row, p.lo, p.hi, p.slab, nc);
+    Stage<G, R>::template fill<W, AL>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, AL>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
+    Stage<T, R>::template fill<W, AL>(st + L::dy, a.dy, a.lddy, row, p.lo, p.hi, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<W, VEC>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
+      Stage<T, R>::template fill<W, AL>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.dht, a.dh0);
   if (p.turns > 0) fill(tile);
@@ -627,16 +655,16 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
           cc[k] = mul2(d[i][k], dh[k]);
           z[k] = mul2(before[i][k], dh[k]);
         }
-        dg.template put<VEC>(i, z, n);
+        dg.template put<AL>(i, z, n);
         if constexpr (GATE) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             z[k] = mul2(pair_of<T>(v[i], k), dh[k]);
             dh[k] = mul2(dh[k], pair_of<T>(w[i], k));
           }
-          dw.template put<VEC>(i, z, n);
+          dw.template put<AL>(i, z, n);
         }
-        dv.template put<VEC>(i, dh, n);
+        dv.template put<AL>(i, dh, n);
         if (EDGE && (first >> i & 1) && a.dh0) put_state(a.dh0, s.seq[r0 + i], a.D, c, nc, cc);
       }
     };
@@ -807,10 +835,10 @@ cudaError_t launch_scan(K kernel, const ScanArgs& a, const ScanPlan& l, int thre
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// Whether every group of kCpt channels of a row can be moved as one vector.
-// (and a tile's offsets held in 32 bits).
-bool group_ok(const void* p, int64_t ld, size_t es) {
-  return aligned_to(p, kCpt * es) && ld % kCpt == 0 && ld <= (1 << 22);
+// Whether every `n` channels of a row can be moved together (and a tile's
+// offsets held in 32 bits).
+bool group_ok(const void* p, int64_t ld, size_t es, int n = kCpt) {
+  return aligned_to(p, n * es) && ld % n == 0 && ld <= (1 << 22);
 }
 
 // f(T, G, gate) over the element types and the presence of w.
@@ -857,8 +885,11 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   if ((e = fault_word(&a.fault)) != cudaSuccess) return cuda_status(e, fn);
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.y = y; a.ht = ht; a.saved = saved;
   const size_t es = dtype_size(p->dtype);
-  const bool vec = a.D % kCpt == 0 && group_ok(v, a.ldv, es) && group_ok(y, a.D, es) &&
-                   group_ok(g, a.ldg, dtype_size(p->g_dtype)) && (!w || group_ok(w, a.ldw, es));
+  int al = kCpt;  // channels aligned together
+  for (; al > 1; al /= 2)
+    if (a.D % al == 0 && group_ok(v, a.ldv, es, al) && group_ok(y, a.D, es, al) &&
+        group_ok(g, a.ldg, dtype_size(p->g_dtype), al) && (!w || group_ok(w, a.ldw, es, al)))
+      break;
   return cuda_status(scan_dispatch(p, w != nullptr, [&](auto t, auto gt, auto gate) {
     using T = decltype(t);
     using G = decltype(gt);
@@ -871,8 +902,9 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<false>();
-      return vec ? launch_scan(k_scan_fwd<T, G, GATE, W, R, true>, b, l, 1024 / R, stage, st)
-                 : launch_scan(k_scan_fwd<T, G, GATE, W, R, false>, b, l, 1024 / R, stage, st);
+      if (al == 4) return launch_scan(k_scan_fwd<T, G, GATE, W, R, 4>, b, l, 1024 / R, stage, st);
+      if (al == 2) return launch_scan(k_scan_fwd<T, G, GATE, W, R, 2>, b, l, 1024 / R, stage, st);
+      return launch_scan(k_scan_fwd<T, G, GATE, W, R, 1>, b, l, 1024 / R, stage, st);
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
                         : go(std::integral_constant<int, 32>{});
@@ -901,9 +933,12 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   a.v = v; a.g = g; a.w = w; a.h0 = h0; a.saved = const_cast<float*>(saved);
   a.dy = dy; a.dht = dht; a.dv = dv; a.dg = dg; a.dw = dw; a.dh0 = dh0;
   const size_t es = dtype_size(p->dtype), eg = dtype_size(p->g_dtype);
-  const bool vec = a.D % kCpt == 0 && group_ok(v, a.ldv, es) && group_ok(dy, a.lddy, es) &&
-                   group_ok(g, a.ldg, eg) && group_ok(dv, a.D, es) && group_ok(dg, a.D, eg) &&
-                   (!w || (group_ok(w, a.ldw, es) && group_ok(dw, a.D, es)));
+  int al = kCpt;  // channels aligned together
+  for (; al > 1; al /= 2)
+    if (a.D % al == 0 && group_ok(v, a.ldv, es, al) && group_ok(dy, a.lddy, es, al) &&
+        group_ok(g, a.ldg, eg, al) && group_ok(dv, a.D, es, al) && group_ok(dg, a.D, eg, al) &&
+        (!w || (group_ok(w, a.ldw, es, al) && group_ok(dw, a.D, es, al))))
+      break;
   return cuda_status(scan_dispatch(p, w != nullptr, [&](auto t, auto gt, auto gate) {
     using T = decltype(t);
     using G = decltype(gt);
@@ -916,8 +951,9 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<true>();
-      return vec ? launch_scan(k_scan_bwd<T, G, GATE, W, R, true>, b, l, 1024 / R, stage, st)
-                 : launch_scan(k_scan_bwd<T, G, GATE, W, R, false>, b, l, 1024 / R, stage, st);
+      if (al == 4) return launch_scan(k_scan_bwd<T, G, GATE, W, R, 4>, b, l, 1024 / R, stage, st);
+      if (al == 2) return launch_scan(k_scan_bwd<T, G, GATE, W, R, 2>, b, l, 1024 / R, stage, st);
+      return launch_scan(k_scan_bwd<T, G, GATE, W, R, 1>, b, l, 1024 / R, stage, st);
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
                         : go(std::integral_constant<int, 32>{});
