@@ -11,6 +11,8 @@
  *                         (gdn2_ops/fused_recurrent_gdn2.py:344-555)
  *   - context-parallel pre-scan and merge (the FLA-CP algorithm of
  *                         gdn2_ops/chunk_kda.py:182-1299, applied to GDN-2)
+ * and offers what a decoder runs next to the mixer: a gated linear recurrence,
+ * log probabilities of given tokens and the AdamW step.
  *
  * Conventions
  *   - Every pointer is device memory unless stated otherwise; the caller owns
@@ -345,7 +347,7 @@ int gdn2_gated_norm_bwd(const gdn2_norm_problem* p, const void* x, const void* z
  * v, w, y have `dtype`, g has `dtype` or fp32, states are fp32 [n_seqs][D].
  * w NULL stands for ones, h0 NULL for zero; ht (or NULL) receives the states
  * after the last tokens.  Row r = b*T + t of v, g, w, dy starts at element
- * r * ld_*; y and the gradients are contiguous [B*T][D].  cu_seqlens (int32
+ * r * ld_* (up to 2^22); y and the gradients are contiguous [B*T][D].  cu_seqlens (int32
  * [n_seqs+1], device) starts at 0, ends at T and does not decrease; n_seqs = B
  * without it.  A sequence without tokens passes its state on.
  * Backward: dy of y and dht (or NULL) of ht give dv, dg, dw, dh0 (or NULL);

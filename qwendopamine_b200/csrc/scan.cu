@@ -45,6 +45,7 @@ namespace {
 
 constexpr int kCpt = 4;           // channels of a thread
 constexpr int kKeep = 64;         // rows between the states kept for the backward
+constexpr int kMaxStride = 1 << 22;  // a tile's offsets are held in 32 bits
 constexpr int kMaxCluster = 16;
 constexpr unsigned kScanFault = 16u;  // of the device's fault word
 
@@ -269,70 +270,84 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, int slab, const fl
 
 // A thread's own rows of a tile in shared memory, filled asynchronously by
 // the thread itself (no barrier) and read by it alone: group i of a tensor at
-// its section, row i, thread.
-template <typename T, int R> struct Stage {
-  static constexpr int kGroupBytes = kCpt * (int)sizeof(T);
+// its section, row i, thread.  AL elements (4, 2 or 1) of the tensor are
+// aligned together.  Single 16-bit elements are too small to be copied
+// asynchronously: such a group comes in as the three words that hold it and is
+// shifted into place when it is read.
+template <typename T, int R, int AL> struct Stage {
+  static constexpr bool kWords = AL * sizeof(T) < 4;
+  static constexpr int kGroupBytes = kWords ? 16 : kCpt * (int)sizeof(T);
+  static constexpr int kBytes = 1024 * kGroupBytes;
+  static constexpr int kPiece = kWords ? 4 : AL * (int)sizeof(T);  // bytes of a copy
+
   __device__ static __forceinline__ char* at(char* base, int i) {
     return base + (i * (1024 / R) + threadIdx.x) * kGroupBytes;
   }
-  // `have` of the AL elements at src to a row's group, from element `e` on;
-  // what is missing is filled with zeros
-  template <int AL>
-  __device__ static __forceinline__ void copy(char* base, int i, int e, const void* src, int have) {
-    constexpr int bytes = AL * (int)sizeof(T);
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(base, i)) + e * (int)sizeof(T);
-    const int n = have > 0 ? bytes : 0;
-    if constexpr (bytes == 16)
+  // a piece at byte `e` of a row's group; zeros where there is nothing
+  __device__ static __forceinline__ void copy(char* base, int i, int e, const void* src, bool there) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(at(base, i)) + e;
+    const int n = there ? kPiece : 0;
+    if constexpr (kPiece == 16)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
     else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(bytes) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(kPiece) : "memory");
   }
   // The thread's rows of the tile at row `tile` (the same for the CTA), of
   // which those in [lo, hi) exist, `nc` channels wide; what does not exist
-  // reads as zero, but a thread without channels reads nothing.  AL elements
-  // (4, 2 or 1) are aligned together; single 16-bit ones are too small to be
-  // copied asynchronously and go through registers.
-  template <int W, int AL>
+  // reads as zero, but a thread without channels reads nothing.
+  template <int W>
   __device__ static __forceinline__ void fill(char* base, const void* x, int64_t ld, int64_t tile,
-                                              int64_t lo, int64_t hi, int slab, int nc) {
+                                              int64_t lo, int64_t hi, int64_t rows, int slab, int nc) {
     if (nc <= 0) return;
     const int r0 = (int)threadIdx.x / Shape<W, R>::lanes * R;
     const int lc = (int)threadIdx.x % Shape<W, R>::lanes * kCpt;
+    const bool inside = tile >= lo && tile + Shape<W, R>::tile <= hi;
     const char* p = (const char*)x + (tile * ld + slab * W) * (int64_t)sizeof(T);
-    const bool inside = tile >= lo && tile + Shape<W, R>::tile <= hi && nc >= kCpt;
-    if (AL * sizeof(T) >= 4 && inside) {
+    if constexpr (kWords) {
+      // the three words may reach into the neighbouring rows, but not out of the
+      // tensor: its first and last elements come one by one
+      const T* q = (const T*)p + r0 * ld + lc;
+#pragma unroll
+      for (int i = 0; i < R; ++i, q += ld) {
+        const int64_t r = tile + r0 + i;
+        const uintptr_t a = reinterpret_cast<uintptr_t>(q) & ~(uintptr_t)3;
+        const bool row = inside || (r >= lo && r < hi);
+        const int odd = (int)(reinterpret_cast<uintptr_t>(q) >> 1) & 1;
+        if (row && r * ld + slab * W + lc > 0 && (rows - 1 - r) * ld + nc >= 6) {
+#pragma unroll
+          for (int e = 0; e < 12; e += 4) copy(base, i, e, (const void*)(a + e), e < 8 || odd);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kCpt; ++e)
+            *reinterpret_cast<T*>(at(base, i) + (e + odd) * 2) = row && e < nc ? q[e] : from_f<T>(0.f);
+        }
+      }
+    } else if (inside && nc >= kCpt) {
       const uint32_t off = (uint32_t)(r0 * (int)ld + lc) * (uint32_t)sizeof(T);
 #pragma unroll
       for (int i = 0; i < R; ++i, p += ld * (int64_t)sizeof(T))
 #pragma unroll
-        for (int e = 0; e < kCpt; e += AL)
-          copy<(AL * sizeof(T) >= 4 ? AL : 4)>(base, i, e, p + off + e * sizeof(T), AL);
-      return;
-    }
-    const T* q = (const T*)p + r0 * ld + lc;
-    if constexpr (AL * sizeof(T) >= 4) {
+        for (int e = 0; e < kGroupBytes; e += kPiece) copy(base, i, e, p + off + e, true);
+    } else {
+      const T* q = (const T*)p + r0 * ld + lc;
 #pragma unroll 1
       for (int i = 0; i < R; ++i, q += ld) {
         const int64_t r = tile + r0 + i;
         const int n = r >= lo && r < hi ? nc : 0;
 #pragma unroll
         for (int e = 0; e < kCpt; e += AL)
-          copy<AL>(base, i, e, n > e ? (const void*)(q + e) : x, n - e);
+          copy(base, i, e * (int)sizeof(T), n > e ? (const void*)(q + e) : x, n > e);
       }
-    } else {
-      Raw<T, kCpt> rows[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i, q += ld) {
-        const int64_t r = tile + r0 + i;
-        rows[i] = load_group<T, kCpt, false>(q, inside ? kCpt : r >= lo && r < hi ? nc : 0);
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) *reinterpret_cast<Raw<T, kCpt>*>(at(base, i)) = rows[i];
     }
   }
-  __device__ static __forceinline__ Raw<T, kCpt> get(char* base, int i) {
+  // `odd`: whether the row starts in the middle of a word
+  __device__ static __forceinline__ Raw<T, kCpt> get(char* base, int i, bool odd) {
     Raw<T, kCpt> r;
-    if constexpr (kGroupBytes == 16) {
+    if constexpr (kWords) {
+      const uint4 v = *reinterpret_cast<const uint4*>(at(base, i));
+      r.u[0] = odd ? __funnelshift_r(v.x, v.y, 16) : v.x;
+      r.u[1] = odd ? __funnelshift_r(v.y, v.z, 16) : v.y;
+    } else if constexpr (kGroupBytes == 16) {
       const uint4 v = *reinterpret_cast<const uint4*>(at(base, i));
       r.u[0] = v.x; r.u[1] = v.y; r.u[2] = v.z; r.u[3] = v.w;
     } else {
@@ -341,13 +356,18 @@ template <typename T, int R> struct Stage {
     }
     return r;
   }
+  // whether row r starts in the middle of a word (16-bit elements)
+  __device__ static __forceinline__ bool odd_row(const void* x, int64_t ld, int64_t r) {
+    if constexpr (!kWords) return false;
+    return ((reinterpret_cast<uintptr_t>(x) >> 1) + (uintptr_t)(r * ld)) & 1;
+  }
 };
 
 __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Sections of a stage: g, v, w, dy.
-template <typename T, typename G, bool GATE, bool BWD> struct StageLayout {
-  static constexpr int sg = 1024 * kCpt * (int)sizeof(G), st = 1024 * kCpt * (int)sizeof(T);
+template <typename T, typename G, bool GATE, bool BWD, int AL> struct StageLayout {
+  static constexpr int sg = Stage<G, 8, AL>::kBytes, st = Stage<T, 8, AL>::kBytes;
   static constexpr int g = 0, v = sg, w = v + st;
   static constexpr int dy = w + (GATE ? st : 0);
   static constexpr int bytes = dy + (BWD ? st : 0);
@@ -432,7 +452,7 @@ __device__ __forceinline__ void put_state(float* x, int64_t seq, int D, int c, i
 template <typename T, typename G, bool GATE, int W, int R, int AL>
 __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(const ScanArgs a) {
   constexpr int TILE = Shape<W, R>::tile;
-  using L = StageLayout<T, G, GATE, false>;
+  using L = StageLayout<T, G, GATE, false, AL>;
   extern __shared__ __align__(16) char st[];
   __shared__ ScanShared<W, R> s;
   const Place p = place_of<W, R>(a);
@@ -442,10 +462,10 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
   const int64_t step = (int64_t)a.cluster * TILE;
   int64_t tile = p.lo + (int64_t)p.rank * TILE;  // first row of this turn's tile
   auto fill = [&](int64_t row) {
-    Stage<G, R>::template fill<W, AL>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, AL>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
+    Stage<G, R, AL>::template fill<W>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, a.rows, p.slab, nc);
+    Stage<T, R, AL>::template fill<W>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, a.rows, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<W, AL>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
+      Stage<T, R, AL>::template fill<W>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, a.rows, p.slab, nc);
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.h0, a.ht);
   if (p.turns > 0) fill(tile);
@@ -458,16 +478,19 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
     const bool edges = place.edges(a, tile, step, TILE, p.lo, p.hi);
     if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
+    auto odd = [&](const void* x, int64_t ld, int i) {
+      return Stage<T, R, AL>::odd_row(x, ld, tile + r0 + i);
+    };
     float2 d[R][2];
     // the inputs w v, packed as v where there is no gate
     using X = typename std::conditional<GATE, float, T>::type;
     Raw<X, kCpt> x[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const Raw<G, kCpt> g = Stage<G, R>::get(st + L::g, i);
-      const Raw<T, kCpt> v = Stage<T, R>::get(st + L::v, i);
+      const Raw<G, kCpt> g = Stage<G, R, AL>::get(st + L::g, i, odd(a.g, a.ldg, i));
+      const Raw<T, kCpt> v = Stage<T, R, AL>::get(st + L::v, i, odd(a.v, a.ldv, i));
       if constexpr (GATE) {
-        const Raw<T, kCpt> w = Stage<T, R>::get(st + L::w, i);
+        const Raw<T, kCpt> w = Stage<T, R, AL>::get(st + L::w, i, odd(a.w, a.ldw, i));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float2 y = mul2(pair_of<T>(v, k), pair_of<T>(w, k));
@@ -534,7 +557,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
 template <typename T, typename G, bool GATE, int W, int R, int AL>
 __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const ScanArgs a) {
   constexpr int TILE = Shape<W, R>::tile;
-  using L = StageLayout<T, G, GATE, true>;
+  using L = StageLayout<T, G, GATE, true, AL>;
   extern __shared__ __align__(16) char st[];
   __shared__ ScanShared<W, R> s;
   __shared__ ScanShared<W, R> ahead;  // the same for the recomputed states (no marks)
@@ -546,11 +569,11 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   // from the chain's last tile down; before the first there is nothing
   int64_t tile = p.lo + ((p.hi - p.lo + TILE - 1) / TILE - 1 - p.rank) * TILE;
   auto fill = [&](int64_t row) {
-    Stage<G, R>::template fill<W, AL>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, AL>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, p.slab, nc);
-    Stage<T, R>::template fill<W, AL>(st + L::dy, a.dy, a.lddy, row, p.lo, p.hi, p.slab, nc);
+    Stage<G, R, AL>::template fill<W>(st + L::g, a.g, a.ldg, row, p.lo, p.hi, a.rows, p.slab, nc);
+    Stage<T, R, AL>::template fill<W>(st + L::v, a.v, a.ldv, row, p.lo, p.hi, a.rows, p.slab, nc);
+    Stage<T, R, AL>::template fill<W>(st + L::dy, a.dy, a.lddy, row, p.lo, p.hi, a.rows, p.slab, nc);
     if constexpr (GATE)
-      Stage<T, R>::template fill<W, AL>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, p.slab, nc);
+      Stage<T, R, AL>::template fill<W>(st + L::w, a.w, a.ldw, row, p.lo, p.hi, a.rows, p.slab, nc);
   };
   if (p.chain == 0 && p.rank == 0) pass_empty<W, Shape<W, R>::threads>(a, p.slab, a.dht, a.dh0);
   if (p.turns > 0) fill(tile);
@@ -570,14 +593,17 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
     }
     if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
+    auto odd = [&](const void* x, int64_t ld, int i) {
+      return Stage<T, R, AL>::odd_row(x, ld, tile + r0 + i);
+    };
     float2 d[R][2];
     Raw<T, kCpt> v[R], w[GATE ? R : 1], dy[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const Raw<G, kCpt> g = Stage<G, R>::get(st + L::g, i);
-      v[i] = Stage<T, R>::get(st + L::v, i);
-      dy[i] = Stage<T, R>::get(st + L::dy, i);
-      if constexpr (GATE) w[i] = Stage<T, R>::get(st + L::w, i);
+      const Raw<G, kCpt> g = Stage<G, R, AL>::get(st + L::g, i, odd(a.g, a.ldg, i));
+      v[i] = Stage<T, R, AL>::get(st + L::v, i, odd(a.v, a.ldv, i));
+      dy[i] = Stage<T, R, AL>::get(st + L::dy, i, odd(a.dy, a.lddy, i));
+      if constexpr (GATE) w[i] = Stage<T, R, AL>::get(st + L::w, i, odd(a.w, a.ldw, i));
       d[i][0] = decay_of(pair_of<G>(g, 0));
       d[i][1] = decay_of(pair_of<G>(g, 1));
     }
@@ -735,6 +761,8 @@ int check_scan(const gdn2_scan_problem* p, const char* fn) {
                 "%s: packed sequences need B = 1 (T < 2^31), others n_seqs = B", fn);
   if (p->ld_v < p->D || p->ld_g < p->D || p->ld_w < 0 || p->ld_dy < 0)
     return fail(GDN2_ERR_INVALID, "%s: row strides must be at least D", fn);
+  if (p->ld_v > kMaxStride || p->ld_g > kMaxStride || p->ld_w > kMaxStride || p->ld_dy > kMaxStride)
+    return fail(GDN2_ERR_UNSUPPORTED, "%s: D and row strides up to %d are supported", fn, kMaxStride);
   const int64_t rows = (int64_t)p->B * p->T;
   const int64_t nslab = (p->D + 31) / 32;
   if ((p->T > 0 && rows / p->T != p->B) ||
@@ -835,10 +863,9 @@ cudaError_t launch_scan(K kernel, const ScanArgs& a, const ScanPlan& l, int thre
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// Whether every `n` channels of a row can be moved together (and a tile's
-// offsets held in 32 bits).
+// Whether every `n` channels of a row can be moved together.
 bool group_ok(const void* p, int64_t ld, size_t es, int n = kCpt) {
-  return aligned_to(p, n * es) && ld % n == 0 && ld <= (1 << 22);
+  return aligned_to(p, n * es) && ld % n == 0;
 }
 
 // f(T, G, gate) over the element types and the presence of w.
@@ -894,7 +921,6 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     using T = decltype(t);
     using G = decltype(gt);
     constexpr bool GATE = decltype(gate)::value;
-    constexpr int stage = StageLayout<T, G, GATE, false>::bytes;
     scan_fit(p, sms, ctas_of<T, false>(), false, l);
     ScanArgs b = a;
     b.nslab = (a.D + l.slab - 1) / l.slab;
@@ -902,9 +928,13 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<false>();
-      if (al == 4) return launch_scan(k_scan_fwd<T, G, GATE, W, R, 4>, b, l, 1024 / R, stage, st);
-      if (al == 2) return launch_scan(k_scan_fwd<T, G, GATE, W, R, 2>, b, l, 1024 / R, stage, st);
-      return launch_scan(k_scan_fwd<T, G, GATE, W, R, 1>, b, l, 1024 / R, stage, st);
+      auto run = [&](auto k, auto aligned) {
+        constexpr int stage = StageLayout<T, G, GATE, false, decltype(aligned)::value>::bytes;
+        return launch_scan(k, b, l, 1024 / R, stage, st);
+      };
+      if (al == 4) return run(k_scan_fwd<T, G, GATE, W, R, 4>, std::integral_constant<int, 4>{});
+      if (al == 2) return run(k_scan_fwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
+      return run(k_scan_fwd<T, G, GATE, W, R, 1>, std::integral_constant<int, 1>{});
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
                         : go(std::integral_constant<int, 32>{});
@@ -943,7 +973,6 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     using T = decltype(t);
     using G = decltype(gt);
     constexpr bool GATE = decltype(gate)::value;
-    constexpr int stage = StageLayout<T, G, GATE, true>::bytes;
     scan_fit(p, sms, ctas_of<T, true>(), true, l);
     ScanArgs b = a;
     b.nslab = (a.D + l.slab - 1) / l.slab;
@@ -951,9 +980,13 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<true>();
-      if (al == 4) return launch_scan(k_scan_bwd<T, G, GATE, W, R, 4>, b, l, 1024 / R, stage, st);
-      if (al == 2) return launch_scan(k_scan_bwd<T, G, GATE, W, R, 2>, b, l, 1024 / R, stage, st);
-      return launch_scan(k_scan_bwd<T, G, GATE, W, R, 1>, b, l, 1024 / R, stage, st);
+      auto run = [&](auto k, auto aligned) {
+        constexpr int stage = StageLayout<T, G, GATE, true, decltype(aligned)::value>::bytes;
+        return launch_scan(k, b, l, 1024 / R, stage, st);
+      };
+      if (al == 4) return run(k_scan_bwd<T, G, GATE, W, R, 4>, std::integral_constant<int, 4>{});
+      if (al == 2) return run(k_scan_bwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
+      return run(k_scan_bwd<T, G, GATE, W, R, 1>, std::integral_constant<int, 1>{});
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
                         : go(std::integral_constant<int, 32>{});

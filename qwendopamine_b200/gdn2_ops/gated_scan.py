@@ -24,6 +24,8 @@ from .. import _native as N
 
 __all__ = ["GatedScanFunction", "gated_scan", "gated_scan_step"]
 
+MAX_STRIDE = 1 << 22  # of rows, in elements (the C entries refuse more)
+
 
 def _rows(x, B, T, D):
     """``x`` as rows ``[B*T, D]`` with one row stride, and that stride; copied
@@ -37,7 +39,7 @@ def _rows(x, B, T, D):
         st = sb
     elif B > 1 and sb != T * st:
         st = -1
-    if (sd != 1 and D > 1) or (B * T > 1 and st < D):
+    if (sd != 1 and D > 1) or (B * T > 1 and st < D) or st > MAX_STRIDE:
         return x.contiguous(), D
     return x, max(st, D)
 

@@ -232,6 +232,7 @@ def test_scan_arguments_are_checked(lib):
                       (sp(dtype=5), N.ERR_INVALID), (sp(g_dtype=2), N.ERR_UNSUPPORTED),
                       (sp(n_seqs=3), N.ERR_INVALID), (sp(cu_seqlens=0x1000), N.ERR_INVALID),
                       (sp(ld_v=69), N.ERR_INVALID), (sp(ld_w=3), N.ERR_INVALID),
+                      (sp(ld_g=(1 << 22) + 1), N.ERR_UNSUPPORTED),
                       (sp(T=1 << 40, B=64, n_seqs=64), N.ERR_UNSUPPORTED)):
         assert fwd(bad) == code, lib.gdn2_last_error()
     assert fwd(sp(), v=None) == N.ERR_INVALID

@@ -107,11 +107,11 @@ def test_gradient_of_the_end_state_alone(cuda_device):
         close(a, b)
 
 
-@pytest.mark.parametrize("decay", ["strong", "none", "reset", "growth"])
+@pytest.mark.parametrize("decay", ["strong", "none", "reset", "growth", "slow"])
 def test_extreme_decays(cuda_device, decay):
     f = {"strong": lambda z: -40 - z.abs(), "none": lambda z: z * 0,
          "reset": lambda z: torch.where(z > 1, -torch.inf, -0.1 * z.abs()),
-         "growth": lambda z: 0.01 * z.abs()}[decay]
+         "growth": lambda z: 0.01 * z.abs(), "slow": lambda z: -0.01 * z.abs()}[decay]
     check(inputs(cuda_device, 2, 260, 48, F32, F32, True, 2, seed=5, decay=f))
 
 
@@ -179,6 +179,35 @@ def test_strided_rows_and_views(cuda_device):
     heads = torch.randn(2, 9, 3, 5, generator=gen).to(cuda_device)
     y, ht = gated_scan(heads, -heads.abs(), output_final_state=True)
     assert y.shape == heads.shape and ht.shape == (2, 3, 5)
+
+
+def test_rows_far_apart(cuda_device):
+    """A row stride beyond what a tile's 32-bit offsets hold."""
+    far = torch.zeros(3, (1 << 22) + 8, device=cuda_device)
+    x = inputs(cuda_device, 1, 3, 40, F32, F32, False, 1, seed=13)
+    far[:, 3:43] = x["v"][0]
+    y, _ = gated_scan(far[None, :, 3:43], x["g"])
+    assert torch.equal(y, gated_scan(x["v"], x["g"])[0])
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """More than 2^31 values: the last sequence is as good as the first."""
+    B, T, D = 70, 16384, 1900
+    v = torch.zeros(B, T, D, dtype=BF, device=cuda_device)
+    g = torch.full((1, 1, 1), -0.01, dtype=BF, device=cuda_device).expand(B, T, D).contiguous()
+    v[-1] = torch.randn(T, D, device=cuda_device).to(BF)
+    v.requires_grad_()
+    y, ht = gated_scan(v, g, output_final_state=True)
+    ry, rh = O.scan_fwd(np64(v[-1:, :, :40]), np64(g[-1:, :, :40]))
+    close(y[-1:, :, :40], ry)
+    close(ht[-1:, :40], rh)
+    assert not y[-2].any()
+    dy = torch.zeros_like(v)
+    dy[-1] = v[-1].detach()
+    d, = torch.autograd.grad(y, v, dy)
+    want = O.scan_bwd(np64(v[-1:, :, :40]), np64(g[-1:, :, :40]), None, None, np64(dy[-1:, :, :40]))
+    close(d[-1:, :, :40], want[0])
+    assert not d[-2].any()
 
 
 def test_gradient_of_a_broadcast_decay(cuda_device):
