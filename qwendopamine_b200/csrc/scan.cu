@@ -775,13 +775,14 @@ int check_scan(const gdn2_scan_problem* p, const char* fn) {
 struct ScanPlan {
   int64_t stretches;  // chains of a slab, each of whole sequences
   int64_t rows;       // of a stretch
+  int64_t sequences;  // and its sequences
   int slab, cluster;
 };
 
 // Stretches: as many as leave two or three CTAs for every SM.  They are the
 // same forward and backward, so that the kept states are found again.
 ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
-  ScanPlan l{1, (int64_t)p->B * p->T, 64, 1};
+  ScanPlan l{1, (int64_t)p->B * p->T, p->n_seqs, 64, 1};
   if (p->cu_seqlens || p->B == 0) return l;
   int64_t s = (int64_t)sms * 3 / ((p->D + 63) / 64);
   if (s > p->B) s = p->B;
@@ -789,13 +790,14 @@ ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
   const int64_t each = (p->B + s - 1) / s;  // sequences of a stretch
   l.stretches = (p->B + each - 1) / each;
   l.rows = each * p->T;
+  l.sequences = each;
   return l;
 }
 
 // Slab and cluster: what takes the least time by a model of a turn, fitted to
 // runs of both directions over slabs and clusters (seven shapes from 9001 x 1000
-// to 131,072 x 1024).  A turn takes its latency, which grows with the cluster,
-// or what its SM needs for all its CTAs.  GPCs have 16 to 20 SMs, so large
+// to 131,072 x 1024).  A turn takes its latency, which grows with the cluster
+// and with a sequence's edge in it, or what its SM needs for all its CTAs.  GPCs have 16 to 20 SMs, so large
 // clusters leave some of them out.
 void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan& l) {
   static constexpr struct { int size; double reach; } kClusters[] = {
@@ -808,13 +810,16 @@ void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan&
       const int64_t rows = (int64_t)c.size * (1024 * kCpt / w);
       const double on_sm = (double)(need < slots ? need : slots) / sms;
       // microseconds
-      const double latency = c.size > 1 ? (bwd ? 2.8 : 1.7) + .03 * c.size : (bwd ? 2.2 : 1.2);
+      const int64_t turns = (l.rows + rows - 1) / rows;
+      const double edge = turns > l.sequences ? (double)l.sequences / turns : 1.;
+      const double latency =
+          1.2 * edge + (c.size > 1 ? (bwd ? 2.8 : 1.7) + .03 * c.size : (bwd ? 2.2 : 1.2));
       const double work = on_sm * (bwd ? 1.93 : w == 64 ? 1.1 : 1.22);
       const double turn = .25 + (latency > work ? latency : work);
       // what a second wave holds starts as the first ends
       const double waves = .5 * ((double)((need + slots - 1) / slots) +
                                  (need > slots ? (double)need / slots : 1.));
-      const double cost = waves * (double)((l.rows + rows - 1) / rows + 2) * turn;
+      const double cost = waves * (double)(turns + 2) * turn;
       if (least < 0. || cost < least) {
         least = cost;
         l.slab = w;
