@@ -2,7 +2,10 @@
 
 Drop-in for ``qwendopamine.models.gdn2``: :class:`GatedDeltaNet2` keeps the
 reference module's API; :func:`chunk_gdn2` and :func:`fused_recurrent_gdn2`
-keep the reference kernel entry points.  All compute runs in
+keep the reference kernel entry points.  Next to them stand a gated linear
+recurrence (:func:`gated_scan`, :func:`gated_scan_step`), log probabilities of
+given tokens (:func:`token_logprobs`) and the optimizer (:class:`AdamW`,
+:func:`adamw_step`).  All compute runs in
 ``libgdn2_b200.so`` (hand-written CUDA for sm_100a) through a C ABI.
 """
 

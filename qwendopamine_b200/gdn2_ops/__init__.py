@@ -1,4 +1,5 @@
-"""B200 kernels behind the GDN-2 token mixer (chunkwise and recurrent)."""
+"""B200 kernels behind the GDN-2 token mixer (chunkwise and recurrent), and the
+operators that a decoder runs next to it."""
 
 from .adamw import AdamW, adamw_step
 from .chunk_gdn2 import ChunkGDN2Function, chunk_gdn2
