@@ -93,10 +93,23 @@ __device__ __forceinline__ float leave(float2 p, float h) {
   return p.x < 0.f ? p.y : fmaf(p.x, h, p.y);
 }
 
+// Runs of a tile's rows on their way, in groups of `own` slots: with own = 1 the
+// slots themselves, else a warp's, which it folds itself before and after the
+// tile's barriers, so that fewer are left between them.  That pays forward
+// (131,072 x 128: 176 -> 139 us), not with the backward's two folds (B = 8,
+// T = 4096, D = 2048: 214 -> 228 us).
+template <int W, int R> struct Runs {
+  using S = Shape<W, R>;
+  static constexpr int own = R == rows_of<false>() ? 32 / S::lanes : 1, groups = S::slots / own;
+  float A[groups][W], H[groups][W];
+  float enter[groups][W];  // the states entering the groups
+  // a warp's slots (own > 1); in sH later the states entering them
+  float sA[own > 1 ? S::slots : 1][W], sH[own > 1 ? S::slots : 1][W];
+};
+
 template <int W, int R> struct ScanShared {
-  static constexpr int tile = Shape<W, R>::tile, slots = Shape<W, R>::slots;
-  // runs of the slots of rows, by turn's parity; then in H the states entering them
-  float A[2][slots][W], H[2][slots][W];
+  static constexpr int tile = Shape<W, R>::tile;
+  Runs<W, R> runs;
   uint64_t bar[2];  // the cluster's runs have come, by turn's parity
   // of a turn with sequence edges in its tile
   int seq[tile];                               // the row's sequence
@@ -111,31 +124,71 @@ __device__ __forceinline__ void unquad(float2 (&x)[2], const float4 f) {
   x[1] = make_float2(f.z, f.w);
 }
 
-// One channel's fold over the tile's slots of rows, in the order of the scan:
-// the tile's run, and the state entering each slot (put into H) and leaving the
-// last.  Slots are read again rather than held: registers are what is short.
+// The fold of a tile's runs, in the order of the scan.
 template <int W, int R, bool UP> struct Fold {
-  static constexpr int slots = Shape<W, R>::slots;
-  __device__ static __forceinline__ float2 run(const float (&A)[slots][W], const float (&H)[slots][W],
-                                               int ch) {
+  using S = Runs<W, R>;
+  // a thread's run, and its group's
+  __device__ static __forceinline__ void put(S& s, int slot, int lc, const float4& A, const float4& H) {
+    float (&a)[W] = S::own > 1 ? s.sA[slot] : s.A[slot];
+    float (&h)[W] = S::own > 1 ? s.sH[slot] : s.H[slot];
+    *reinterpret_cast<float4*>(a + lc) = A;
+    *reinterpret_cast<float4*>(h + lc) = H;
+    if constexpr (S::own > 1) {
+      __syncwarp();
+      const int w = threadIdx.x >> 5;
+#pragma unroll
+      for (int ch = threadIdx.x & 31; ch < W; ch += 32) {
+        float2 all = make_float2(1.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < S::own; ++i) {
+          const int k = w * S::own + (UP ? S::own - 1 - i : i);
+          all = compose(all, make_float2(s.sA[k][ch], s.sH[k][ch]));
+        }
+        s.A[w][ch] = all.x;
+        s.H[w][ch] = all.y;
+      }
+    }
+  }
+  // one channel of the groups' runs: the tile's
+  __device__ static __forceinline__ float2 run(const S& s, int ch) {
     float2 all = make_float2(1.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < slots; ++i) {
-      const int k = UP ? slots - 1 - i : i;
-      all = compose(all, make_float2(A[k][ch], H[k][ch]));
+    for (int i = 0; i < S::groups; ++i) {
+      const int k = UP ? S::groups - 1 - i : i;
+      all = compose(all, make_float2(s.A[k][ch], s.H[k][ch]));
     }
     return all;
   }
-  __device__ static __forceinline__ float enter(const float (&A)[slots][W], float (&H)[slots][W],
-                                                int ch, float state) {
+  // one channel of the states entering the groups; returns the one that leaves
+  __device__ static __forceinline__ float enter(S& s, int ch, float state) {
 #pragma unroll
-    for (int i = 0; i < slots; ++i) {
-      const int k = UP ? slots - 1 - i : i;
-      const float2 r = make_float2(A[k][ch], H[k][ch]);
-      H[k][ch] = state;
-      state = leave(r, state);
+    for (int i = 0; i < S::groups; ++i) {
+      const int k = UP ? S::groups - 1 - i : i;
+      s.enter[k][ch] = state;
+      state = leave(make_float2(s.A[k][ch], s.H[k][ch]), state);
     }
     return state;
+  }
+  // the state entering a thread's rows
+  __device__ static __forceinline__ float4 get(S& s, int slot, int lc) {
+    if constexpr (S::own == 1) {
+      return *reinterpret_cast<const float4*>(&s.enter[slot][lc]);
+    } else {
+      const int w = threadIdx.x >> 5;
+#pragma unroll
+      for (int ch = threadIdx.x & 31; ch < W; ch += 32) {
+        float state = s.enter[w][ch];
+#pragma unroll
+        for (int i = 0; i < S::own; ++i) {
+          const int k = w * S::own + (UP ? S::own - 1 - i : i);
+          const float2 r = make_float2(s.sA[k][ch], s.sH[k][ch]);
+          s.sH[k][ch] = state;
+          state = leave(r, state);
+        }
+      }
+      __syncwarp();
+      return *reinterpret_cast<const float4*>(&s.sH[slot][lc]);
+    }
   }
 };
 
@@ -163,10 +216,10 @@ __device__ __forceinline__ void open_exchange(const ScanArgs& a, ScanShared<W, R
   cg::this_cluster().sync();
 }
 
-// Puts the states that enter the slots of this CTA's tile into s.H and moves
-// `state` (threads 0 .. W-1, one per channel) from the state that enters the
-// turn's first tile to the one that leaves its last.  Called by all threads
-// after a barrier; ends with one.
+// Finds the states that enter the groups of this CTA's tile and moves `state`
+// (threads 0 .. W-1, one per channel) from the state that enters the turn's
+// first tile to the one that leaves its last.  Called by all threads after a
+// barrier; ends with one.
 //
 // In a cluster every CTA sends its tile's run to all, into `runs` by turn's
 // parity, and waits for as many; a cluster-wide barrier would also wait for
@@ -180,10 +233,10 @@ __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s,
   const int ch = threadIdx.x, b = turn & 1;
   if (ch < W) {
     if (a.cluster == 1) {
-      state = Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, state);
+      state = Fold<W, R, UP>::enter(s.runs, ch, state);
     } else {
       runs += b * a.cluster * W;
-      const float2 all = Fold<W, R, UP>::run(s.A[b], s.H[b], ch);
+      const float2 all = Fold<W, R, UP>::run(s.runs, ch);
       if (ch == 0) tc::mbar_expect_tx(&s.bar[b], a.cluster * W * (int)sizeof(float2));
       const uint32_t to = smem_u32(runs + rank * W + ch), bar = smem_u32(&s.bar[b]);
       for (int k = 0; k < a.cluster; ++k) store_async(address_at(to, k), address_at(bar, k), all);
@@ -197,7 +250,7 @@ __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s,
         if (k == rank) carry = state;
         state = leave(runs[k * W + ch], state);
       }
-      Fold<W, R, UP>::enter(s.A[b], s.H[b], ch, carry);
+      Fold<W, R, UP>::enter(s.runs, ch, carry);
     }
   }
   __syncthreads();
@@ -474,7 +527,6 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
   RowPlace place{0, 0, 0};
 
   for (int turn = 0; turn < p.turns; ++turn, tile += step) {
-    const int b = turn & 1;
     const bool edges = place.edges(a, tile, step, TILE, p.lo, p.hi);
     if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
@@ -532,12 +584,11 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
     } else {
       walk(std::false_type{}, product);
     }
-    *reinterpret_cast<float4*>(&s.A[b][slot][lc]) = quad(A);
-    *reinterpret_cast<float4*>(&s.H[b][slot][lc]) = quad(h);
+    Fold<W, R, false>::put(s.runs, slot, lc, quad(A), quad(h));
     __syncthreads();
     exchange<W, R, false>(a, s, runs, p.rank, turn, state);
 
-    unquad(h, *reinterpret_cast<const float4*>(&s.H[b][slot][lc]));
+    unquad(h, Fold<W, R, false>::get(s.runs, slot, lc));
     const int64_t left = p.hi - tile - r0;  // rows that exist from here
     if (a.saved && r0 % kKeep == 0 && left > 0)
       put_state(a.saved, p.chain * a.keeps + (tile + r0 - p.lo) / kKeep, a.D, c, nc, h);
@@ -560,7 +611,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   using L = StageLayout<T, G, GATE, true, AL>;
   extern __shared__ __align__(16) char st[];
   __shared__ ScanShared<W, R> s;
-  __shared__ ScanShared<W, R> ahead;  // the same for the recomputed states (no marks)
+  __shared__ Runs<W, R> ahead;  // of the recomputed states
   const Place p = place_of<W, R>(a);
   float2* const runs = reinterpret_cast<float2*>(st + L::bytes);
   const int slot = threadIdx.x / Shape<W, R>::lanes, r0 = slot * R;
@@ -582,7 +633,6 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   RowPlace place{0, 0, 0};
 
   for (int turn = 0; turn < p.turns; ++turn, tile -= step) {
-    const int b = turn & 1;
     const bool some = tile >= p.lo;
     const bool edges = place.edges(a, tile, -step, TILE, p.lo, p.hi);
     float kept = 0.f;  // the state entering the tile
@@ -640,16 +690,14 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
         for (int k = 0; k < 2; ++k) C[k] = mul2(d[i][k], add2(pair_of<T>(dy[i], k), C[k]));
       }
       const float4 reset = make_float4(-1.f, -1.f, -1.f, -1.f);
-      *reinterpret_cast<float4*>(&ahead.A[b][slot][lc]) = EDGE && first ? reset : quad(A);
-      *reinterpret_cast<float4*>(&ahead.H[b][slot][lc]) = quad(H);
-      *reinterpret_cast<float4*>(&s.A[b][slot][lc]) = EDGE && last ? reset : quad(A);
-      *reinterpret_cast<float4*>(&s.H[b][slot][lc]) = quad(C);
+      Fold<W, R, false>::put(ahead, slot, lc, EDGE && first ? reset : quad(A), quad(H));
+      Fold<W, R, true>::put(s.runs, slot, lc, EDGE && last ? reset : quad(A), quad(C));
     };
     if (edges) runs_of_rows(std::true_type{});
     else runs_of_rows(std::false_type{});
     __syncthreads();
     if (threadIdx.x / W == 1)
-      Fold<W, R, false>::enter(ahead.A[b], ahead.H[b], threadIdx.x - W, kept);
+      Fold<W, R, false>::enter(ahead, threadIdx.x - W, kept);
     exchange<W, R, true>(a, s, runs, p.rank, turn, state);
 
     const int64_t left = some ? p.hi - tile - r0 : 0;  // rows that exist from here
@@ -659,8 +707,8 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
       constexpr bool EDGE = decltype(edge)::value;
       float2 before[R][2];  // a_t h_{t-1}
       float2 h[2], cc[2];
-      unquad(h, *reinterpret_cast<const float4*>(&ahead.H[b][slot][lc]));
-      unquad(cc, *reinterpret_cast<const float4*>(&s.H[b][slot][lc]));
+      unquad(h, Fold<W, R, false>::get(ahead, slot, lc));
+      unquad(cc, Fold<W, R, true>::get(s.runs, slot, lc));
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         if (EDGE && (first >> i & 1)) state_at(a.h0, s.seq[r0 + i], a.D, c, nc, h);
