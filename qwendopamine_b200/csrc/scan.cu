@@ -65,7 +65,7 @@ template <int W, int R> struct Shape {
 // four rows (214 us, 87 %; three of 128 with eight rows 263 us).
 template <bool BWD> constexpr int rows_of() { return BWD ? 4 : 8; }
 template <typename T, bool BWD> constexpr int ctas_of() {
-  return BWD ? (sizeof(T) == 2 ? 2 : 1) : (sizeof(T) == 2 ? 4 : 3);
+  return BWD ? 2 : (sizeof(T) == 2 ? 4 : 3);
 }
 
 struct ScanArgs {
@@ -986,7 +986,8 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
         return launch_scan(k, b, l, 1024 / R, stage, st);
       };
       if (al == 4) return run(k_scan_fwd<T, G, GATE, W, R, 4>, std::integral_constant<int, 4>{});
-      if (al == 2) return run(k_scan_fwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
+      if constexpr (sizeof(T) == 2)  // two fp32 channels gain nothing over one
+        if (al == 2) return run(k_scan_fwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
       return run(k_scan_fwd<T, G, GATE, W, R, 1>, std::integral_constant<int, 1>{});
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
@@ -1038,7 +1039,8 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
         return launch_scan(k, b, l, 1024 / R, stage, st);
       };
       if (al == 4) return run(k_scan_bwd<T, G, GATE, W, R, 4>, std::integral_constant<int, 4>{});
-      if (al == 2) return run(k_scan_bwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
+      if constexpr (sizeof(T) == 2)  // two fp32 channels gain nothing over one
+        if (al == 2) return run(k_scan_bwd<T, G, GATE, W, R, 2>, std::integral_constant<int, 2>{});
       return run(k_scan_bwd<T, G, GATE, W, R, 1>, std::integral_constant<int, 1>{});
     };
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
