@@ -149,8 +149,9 @@ def gated_scan(
     r"""``h_t = exp(g_t) h_{t-1} + w_t v_t`` over the second dimension.
 
     v: ``[B, T, ...]`` (float32, bfloat16 or float16); g, the log-decay, of
-    v's shape in float32 or v's dtype; w of v's shape and dtype, or None for
-    ones.  ``initial_state`` and the returned final state (None unless
+    v's shape in float32 or v's dtype (-inf cuts the past off; positive values
+    grow the state, as long as the product of the decays over a few thousand
+    rows stays finite in float32); w of v's shape and dtype, or None for ones.  ``initial_state`` and the returned final state (None unless
     ``output_final_state``) are float32 ``[N, ...]``.  With ``cu_seqlens``
     (``[N+1]``, from 0 to T, not decreasing; not checked on the device) B must
     be 1 and the N packed sequences, empty ones included, each start from
