@@ -345,8 +345,8 @@ int gdn2_gated_norm_bwd(const gdn2_norm_problem* p, const void* x, const void* z
  * Per channel, over the rows [B][T] (or packed sequences, B = 1):
  *   h_t = exp(g_t) h_{t-1} + w_t v_t,   y_t = h_t rounded to `dtype`
  * v, w, y have `dtype`, g has `dtype` or fp32, states are fp32 [n_seqs][D].
- * Runs of up to 2048 rows are composed: with g > 0 the product of a run's
- * decays has to stay finite in fp32.
+ * Runs of up to 128 rows are composed: with g > 0 the product of a run's decays
+ * has to stay finite in fp32.
  * w NULL stands for ones, h0 NULL for zero; ht (or NULL) receives the states
  * after the last tokens.  Row r = b*T + t of v, g, w, dy starts at element
  * r * ld_* (up to 2^22); y and the gradients are contiguous [B*T][D].  cu_seqlens (int32

@@ -845,8 +845,8 @@ ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
 // Slab and cluster: what takes the least time by a model of a turn, fitted to
 // runs of both directions over slabs and clusters (seven shapes from 9001 x 1000
 // to 131,072 x 1024).  A turn takes its latency, which grows with the cluster
-// and with a sequence's edge in it, or what its SM needs for all its CTAs.  GPCs have 16 to 20 SMs, so large
-// clusters leave some of them out.
+// and with a sequence's edge in it, or what its SM needs for all its CTAs.
+// GPCs have 16 to 20 SMs, so large clusters leave some of them out.
 void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan& l) {
   static constexpr struct { int size; double reach; } kClusters[] = {
       {1, 1.}, {2, 1.}, {4, .94}, {6, .9}, {8, .865}, {10, .83}, {12, .8}, {14, .77}, {16, .75}};

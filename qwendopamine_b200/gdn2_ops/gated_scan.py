@@ -109,10 +109,10 @@ class GatedScanFunction(torch.autograd.Function):
         dw = new(w) if w is not None else None
         dh0 = new(h0) if h0 is not None else None
         with N.on_device(dev.index):
-                N.check(lib.gdn2_scan_bwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
-                                      N.addr(saved), N.addr(dy), N.addr(dht), N.addr(dv), N.addr(dg),
-                                      N.addr(dw), N.addr(dh0), N.raw_stream(dev.index)),
-                    "gdn2_scan_bwd")
+            N.check(lib.gdn2_scan_bwd(prob, N.addr(geo.v), N.addr(geo.g), N.addr(geo.w), N.addr(h0),
+                                      N.addr(saved), N.addr(dy), N.addr(dht), N.addr(dv),
+                                      N.addr(dg), N.addr(dw), N.addr(dh0),
+                                      N.raw_stream(dev.index)), "gdn2_scan_bwd")
         return dv, dg, dw, dh0, None, None
 
 
@@ -150,8 +150,9 @@ def gated_scan(
 
     v: ``[B, T, ...]`` (float32, bfloat16 or float16); g, the log-decay, of
     v's shape in float32 or v's dtype (-inf cuts the past off; positive values
-    grow the state, as long as the product of the decays over a few thousand
-    rows stays finite in float32); w of v's shape and dtype, or None for ones.  ``initial_state`` and the returned final state (None unless
+    grow the state, as long as the product of the decays of 128 rows stays
+    finite in float32); w of v's shape and dtype, or None for ones.
+    ``initial_state`` and the returned final state (None unless
     ``output_final_state``) are float32 ``[N, ...]``.  With ``cu_seqlens``
     (``[N+1]``, from 0 to T, not decreasing; not checked on the device) B must
     be 1 and the N packed sequences, empty ones included, each start from

@@ -91,7 +91,8 @@ class TokenLogprobsFunction(torch.autograd.Function):
         with N.on_device(x.device.index):
             N.check(N.load().gdn2_logprob_bwd(
                 _problem(x, ld, 0, temperature, ignore_index), N.addr(x), N.addr(ids), N.addr(stats),
-                N.addr(dlogp), N.addr(dent), N.addr(dx), N.raw_stream(x.device.index)), "gdn2_logprob_bwd")
+                N.addr(dlogp), N.addr(dent), N.addr(dx), N.raw_stream(x.device.index)),
+                "gdn2_logprob_bwd")
         return dx.view(logits.shape), None, None, None, None, None
 
 
