@@ -180,6 +180,21 @@ def test_8bit_codes_at_their_limits(cuda_device):
     assert x["p"][0].isfinite().all() and x["p"][0].abs().max() < 1
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_whose_squares_overflow(cuda_device, bits):
+    """A gradient of 1e30 moves its parameter by a step's size at most and
+    leaves its neighbours alone; a NaN stays where it is."""
+    x = make(cuda_device, F32, F32, bits, False, sizes=[256, 512], seed=10)
+    x["g"][0][7] = 1e30
+    x["g"][1][300] = float("nan")
+    before = [p.clone() for p in x["p"]]
+    call(x, bits, False, step=1, weight_decay=0.0)
+    assert x["p"][0].isfinite().all()
+    assert (x["p"][0] - before[0])[7].abs() <= 2 * H["lr"] / (1 - H["betas"][0])
+    bad = x["p"][1].isnan()
+    assert bad[300] and int(bad.sum()) == 1
+
+
 def test_many_steps_with_8bit_states_follow_32bit(cuda_device):
     """A least-squares problem: both reach the same loss."""
     gen = torch.Generator().manual_seed(5)
