@@ -394,7 +394,8 @@ int gdn2_scan_step(const gdn2_scan_problem* p, const void* v, const void* g,
  * Everything is formed and returned in fp32.  -inf logits have probability
  * zero.  A row of only -inf has log probability -inf and entropy 0; one whose
  * id is ignore_index gives 0, 0, -inf and index -1 and is not read; an id
- * outside the vocabulary gives NaN.  NaN logits make the row's results NaN.
+ * outside the vocabulary gives NaN.  NaN logits make the row's results NaN;
+ * as alternatives they come after all numbers, by rising index.
  * `stats` (fp32 [rows][4], 16-byte aligned, or NULL) is what the backward
  * needs of the forward.  Backward: dlogits [rows][vocab], contiguous, in the
  * logits' dtype, from dlogprobs and dentropy (fp32 [rows], NULL for zero;

@@ -13,8 +13,9 @@
 // seen.  The k-th largest of those is a bound that at least k elements reach,
 // so only the threads whose maximum reaches it (k of them, more with ties)
 // look through their elements again, from L2, and hand those that reach the
-// bound to the CTA.  Candidates are ordered as 64-bit keys, value first and
-// then the lower index, so the result does not depend on any order of arrival.
+// bound to the CTA.  Candidates are ordered as 64-bit keys, value first (NaN
+// last) and then the lower index, so the result does not depend on any order of
+// arrival.
 //
 // Bound: HBM for many rows (forward: one read of the logits; backward: one
 // read and one write).  4096 x 151936 bf16 with entropy: forward 209 us (5.96
@@ -253,7 +254,9 @@ __device__ void cta_top(LogprobShared& s, const RowView<T>& row, int lo, int hi,
   const uint32_t mine = any ? order_of(most) : 0u;
   if (tid == 0) { s.n_who = 0; s.n_cand = 0; }
   find_bound(s, mine, k);
-  const uint32_t bound = s.bound;
+  // -inf is also what a thread reports that has read NaN alone, so it bounds
+  // nothing: below it come the NaN, which fill up the places that are left
+  const uint32_t bound = s.bound == order_of(-INFINITY) ? 0u : s.bound;
   const int steps = (hi - lo + kLpThreads - 1) / kLpThreads, segs = (steps + 31) / 32;
   const bool reach = any && mine >= bound;
   if (steps <= 4) {  // few vectors: a thread looks through its own

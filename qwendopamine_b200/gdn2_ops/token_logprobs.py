@@ -117,7 +117,8 @@ def token_logprobs(
     -inf logits (a mask) have probability zero; a row of only -inf has log
     probability -inf, entropy 0 and no gradient.  Rows whose id is
     ``ignore_index`` give 0 and 0 (-inf and id -1 as alternatives), no
-    gradient, and are not read; an id outside the vocabulary gives NaN.
+    gradient, and are not read; an id outside the vocabulary gives NaN.  NaN
+    logits make the row's results NaN and come last among the alternatives.
     Differentiable (once) in ``logits`` through ``logprobs`` and ``entropy``.
     """
     if not logits.is_cuda:

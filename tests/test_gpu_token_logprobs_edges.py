@@ -1,0 +1,57 @@
+"""Token log probabilities of rows that hold NaN: the alternatives' ids, and
+rows whose numbers are fewer than the alternatives asked for."""
+
+import numpy as np
+import pytest
+import torch
+
+from qwendopamine_b200 import token_logprobs
+
+pytestmark = pytest.mark.gpu
+
+F32, BF, FH = torch.float32, torch.bfloat16, torch.float16
+NAN, NINF = float("nan"), float("-inf")
+
+
+def ranked(x, k):
+    """The k best of each row by falling value, equal ones by rising index, NaN last."""
+    x = x.double().cpu().numpy()
+    out = []
+    for row in x:
+        nan = np.isnan(row)
+        order = np.lexsort((np.arange(row.size), np.where(nan, 0.0, -row), nan))
+        out.append(order[:k])
+    return np.stack(out)
+
+
+# a warp a row; a CTA a row (many rows); a row split over a cluster (few rows)
+@pytest.mark.parametrize("rows,V", [(9, 250), (200, 2049), (9, 70001), (9, 151936)])
+@pytest.mark.parametrize("dtype", [F32, BF, FH])
+@pytest.mark.parametrize("k", [1, 5, 32, 33, 128])
+def test_ids_of_rows_with_nan(cuda_device, rows, V, dtype, k):
+    gen = torch.Generator().manual_seed(V + k)
+    x = (torch.randn(rows, V, generator=gen) * 3).to(dtype)
+    x[0] = NAN
+    x[1] = NAN  # fewer numbers than alternatives
+    x[1, V - k + 1:] = torch.arange(k - 1, 0, -1).to(dtype)
+    x[2] = NAN  # as many
+    at = torch.randperm(V, generator=gen)[:k]
+    x[2, at] = torch.randn(k, generator=gen).to(dtype)
+    x[3] = NAN  # one number
+    x[3, V // 2] = 1.0
+    x[4, ::2] = NAN  # numbers, -inf and NaN
+    x[4, 1::2] = NINF
+    x[4, 1] = 0.5
+    x[5] = NAN  # fewer -inf than alternatives, and nothing else
+    x[5, 3:3 + (k + 1) // 2] = NINF
+    x[6, V // 3] = NAN
+    x[7] = NAN  # neighbours, read by one thread
+    x[7, 16:24] = torch.arange(8).to(dtype)
+    want = ranked(x, k)
+    x = x.to(cuda_device)
+    ids = torch.zeros(rows, dtype=torch.int64, device=cuda_device)
+    r = token_logprobs(x, ids, top_k=k, entropy=True)
+    assert (r.top_ids.cpu().numpy() == want).all()
+    assert r.top_logprobs[:8].isnan().all() and r.logprobs[:8].isnan().all()
+    assert r.entropy[:8].isnan().all()
+    assert r.top_logprobs[8:].isfinite().all()
