@@ -897,8 +897,12 @@ ScanArgs scan_args(const gdn2_scan_problem* p, const ScanPlan& l) {
 template <typename K>
 cudaError_t launch_scan(K kernel, const ScanArgs& a, const ScanPlan& l, int threads, int stage,
                         cudaStream_t st) {
-  const int smem = stage + (l.cluster > 1 ? 2 * l.cluster * l.slab * (int)sizeof(float2) : 0);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int run = 2 * l.slab * (int)sizeof(float2);  // of a CTA of the cluster, both parities
+  const int smem = stage + (l.cluster > 1 ? l.cluster * run : 0);
+  // The limit belongs to the kernel, and other host threads launch it with other
+  // clusters: always what the largest needs.
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       stage + kMaxCluster * run);
   if (e == cudaSuccess && l.cluster > 8)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;

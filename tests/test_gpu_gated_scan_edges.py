@@ -1,0 +1,56 @@
+"""Gated linear recurrence on the GPU: calls at the edges of what the entry
+points take."""
+
+import threading
+
+import pytest
+import torch
+
+from qwendopamine_b200 import _native as N
+from qwendopamine_b200 import gated_scan
+
+pytestmark = pytest.mark.gpu
+
+F32, BF = torch.float32, torch.bfloat16
+
+
+def inputs(dev, B, T, D, dtype, gdtype, gate, n, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    return dict(v=rn(B, T, D).to(dev, dtype),
+                g=torch.nn.functional.logsigmoid(rn(B, T, D) + 3).to(dev, gdtype),
+                w=torch.sigmoid(rn(B, T, D)).to(dev, dtype) if gate else None,
+                h0=rn(n, D).to(dev))
+
+
+def test_shapes_of_several_host_threads(cuda_device):
+    """One kernel serves a long sequence (a cluster of CTAs, more shared memory)
+    and short ones (single CTAs) from several host threads at once."""
+    lib, D = N.load(), 40
+    calls, errors, start = [], [], threading.Barrier(4)
+    for i, T in enumerate((2000, 300, 2000, 300)):
+        x = inputs(cuda_device, 1, T, D, F32, F32, True, 1, seed=20 + i)
+        want, _ = gated_scan(x["v"], x["g"], x["w"])
+        calls.append((x, want, torch.empty_like(want), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def work(x, want, y, stream):
+        T = want.shape[1]
+        prob = N.ScanProblem(1, D, T, N.dtype_code(F32), N.dtype_code(F32), 1, None, D, D, D, D)
+        args = (prob, *(x[k].data_ptr() for k in ("v", "g", "w")), None, y.data_ptr(), None, None,
+                stream.cuda_stream)
+        start.wait()
+        try:
+            for _ in range(20000):
+                N.check(lib.gdn2_scan_fwd(*args), "gdn2_scan_fwd")
+            stream.synchronize()
+            assert torch.equal(y, want)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
