@@ -14,9 +14,11 @@ from __future__ import annotations
 
 import math
 import struct
+from itertools import chain
 from operator import attrgetter
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -68,7 +70,7 @@ def adamw_step(
     16-bit parameters are rounded to nearest after the step.  ``step`` counts
     from 1.  ``grad_scale`` (a float32 device scalar) multiplies the gradients,
     and a nonzero ``found_inf`` leaves everything as it is; neither is read on
-    the host.
+    the host.  What is written counts as changed in place for autograd.
     """
     n = len(params)
     lists = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs}
@@ -121,6 +123,10 @@ def adamw_step(
     with N.on_device(device.index):
         N.check(N.load().gdn2_adamw_step(prob, struct.pack(f"{len(words)}q", *words), n,
                                          N.raw_stream(device.index)), "gdn2_adamw_step")
+    del lists["grads"]
+    # autograd does not see the kernel's writes: a graph that saved one of these
+    # tensors has to fail instead of differentiating with the new values
+    increment_version(chain.from_iterable(lists.values()))
 
 
 class AdamW(torch.optim.Optimizer):

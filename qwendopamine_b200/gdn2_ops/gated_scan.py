@@ -19,6 +19,7 @@ import math
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -238,4 +239,5 @@ def gated_scan_step(
         N.check(N.load().gdn2_scan_step(
             prob, N.addr(v), N.addr(g), N.addr(w), N.addr(state), max(state.stride(0), D),
             state.shape[0], N.addr(idx), N.addr(y), N.raw_stream(index)), "gdn2_scan_step")
+    increment_version(state)  # autograd does not see the kernel's writes
     return y

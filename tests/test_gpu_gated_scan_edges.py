@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from qwendopamine_b200 import _native as N
-from qwendopamine_b200 import gated_scan
+from qwendopamine_b200 import gated_scan, gated_scan_step
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,20 @@ def test_shapes_of_several_host_threads(cuda_device):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def test_step_marks_the_pool_as_changed(cuda_device):
+    """A graph that saved the states cannot be differentiated after a step on them."""
+    x = inputs(cuda_device, 3, 1, 16, F32, F32, False, 3, seed=22)
+    pool = x["h0"].clone()
+    leaf = torch.ones(3, 16, device=cuda_device, requires_grad=True)
+    loss = (leaf * pool).sum()
+    version = pool._version
+    gated_scan_step(x["v"][:, 0], x["g"][:, 0], state=pool)
+    assert pool._version > version
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # tensors without a version
+        own = torch.zeros(3, 16, device=cuda_device)
+        y = gated_scan_step(x["v"][:, 0], x["g"][:, 0], state=own)
+        assert torch.equal(y, own)
