@@ -15,6 +15,7 @@ import threading
 from ctypes import c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgdn2_b200.so")
 
@@ -344,6 +345,16 @@ def on_device(index: int):
     """Makes the device of that index current for a launch (nothing to do when
     it already is)."""
     return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def traced(*tensors):
+    """Whether a call on these tensors (or None) has to go through autograd: a
+    gradient is asked for, or one of them carries a forward-mode tangent, which
+    the Functions here refuse."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return fwAD._current_level >= 0 and any(
+        t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def addr(t):

@@ -159,8 +159,8 @@ def gated_scan(
     be 1 and the N packed sequences, empty ones included, each start from
     their own state; N = B otherwise.  Returns ``(y, final_state)``, y in v's
     dtype; states and sums are float32.  Differentiable (once) in v, g, w and
-    ``initial_state``; the gradients need no forward value but a state every
-    64 tokens.  Rows may be strided (slices of a fused projection).
+    ``initial_state``, in reverse mode; the gradients need no forward value but
+    a state every 64 tokens.  Rows may be strided (slices of a fused projection).
     """
     _check("gated_scan", v, g, w, 2)
     n = v.shape[0]
@@ -182,8 +182,7 @@ def gated_scan(
             raise ValueError(f"initial_state must be [{n}, *{tuple(v.shape[2:])}] on {v.device}; "
                              f"got {tuple(h0.shape)} on {h0.device}")
         h0 = h0.contiguous()
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (v, g, w, h0)):
+    if N.traced(v, g, w, h0):
         y, ht = GatedScanFunction.apply(v, g, w, h0, cu, bool(output_final_state))
     else:
         y, ht, _ = _forward(_Geometry(v, g, w, cu), v.shape, h0, bool(output_final_state),

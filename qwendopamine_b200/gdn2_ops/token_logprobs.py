@@ -119,7 +119,8 @@ def token_logprobs(
     ``ignore_index`` give 0 and 0 (-inf and id -1 as alternatives), no
     gradient, and are not read; an id outside the vocabulary gives NaN.  NaN
     logits make the row's results NaN and come last among the alternatives.
-    Differentiable (once) in ``logits`` through ``logprobs`` and ``entropy``.
+    Differentiable (once, in reverse mode) in ``logits`` through ``logprobs``
+    and ``entropy``.
     """
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs: logits must be a CUDA tensor -- the B200 build has no "
@@ -136,7 +137,7 @@ def token_logprobs(
     lead = logits.shape[:-1]
     ids = token_ids.to(device=logits.device, dtype=torch.int64).reshape(-1).contiguous()
     args = (int(top_k), bool(entropy), float(temperature), int(ignore_index))
-    if logits.requires_grad and torch.is_grad_enabled():
+    if N.traced(logits):
         logp, ent, top, top_ids = TokenLogprobsFunction.apply(logits, ids, *args)
     else:
         logp, ent, top, top_ids, _ = _forward(*_matrix(logits), ids, *args, keep=False)

@@ -5,6 +5,7 @@ import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from qwendopamine_b200 import _native as N
 from qwendopamine_b200 import gated_scan, gated_scan_step
@@ -71,3 +72,19 @@ def test_step_marks_the_pool_as_changed(cuda_device):
         own = torch.zeros(3, 16, device=cuda_device)
         y = gated_scan_step(x["v"][:, 0], x["g"][:, 0], state=own)
         assert torch.equal(y, own)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(cuda_device, grad):
+    """No tangent is lost without a word, also where nothing requires a gradient."""
+    x = inputs(cuda_device, 1, 6, 8, F32, F32, True, 1, seed=23)
+    names = ("v", "g", "w", "h0")
+    plain, _ = gated_scan(x["v"], x["g"], x["w"], x["h0"])
+    for name in names:
+        with fwAD.dual_level(), torch.set_grad_enabled(grad):
+            d = dict(x)
+            d[name] = fwAD.make_dual(x[name], torch.ones_like(x[name]))
+            with pytest.raises(RuntimeError, match="forward"):
+                gated_scan(*(d[k] for k in names))
+            y, _ = gated_scan(*(x[k] for k in names))  # no tangents: as ever
+            assert torch.equal(y, plain)

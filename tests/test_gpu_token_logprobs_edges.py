@@ -4,6 +4,7 @@ rows whose numbers are fewer than the alternatives asked for."""
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from qwendopamine_b200 import token_logprobs
 
@@ -55,3 +56,15 @@ def test_ids_of_rows_with_nan(cuda_device, rows, V, dtype, k):
     assert r.top_logprobs[:8].isnan().all() and r.logprobs[:8].isnan().all()
     assert r.entropy[:8].isnan().all()
     assert r.top_logprobs[8:].isfinite().all()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(cuda_device, grad):
+    """No tangent is lost without a word, also where nothing requires a gradient."""
+    x = torch.randn(3, 40, device=cuda_device)
+    ids = torch.zeros(3, dtype=torch.int64, device=cuda_device)
+    plain = token_logprobs(x, ids).logprobs
+    with fwAD.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(RuntimeError, match="forward"):
+            token_logprobs(fwAD.make_dual(x, torch.ones_like(x)), ids)
+        assert torch.equal(token_logprobs(x, ids).logprobs, plain)
