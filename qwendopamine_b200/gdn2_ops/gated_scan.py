@@ -221,7 +221,10 @@ def gated_scan_step(
         if state_indices.shape != (n,) or state_indices.is_floating_point():
             raise ValueError(f"state_indices must be {n} integers; got "
                              f"{tuple(state_indices.shape)} {state_indices.dtype}")
-        idx = state_indices.to(device=v.device, dtype=torch.int32).contiguous()
+        idx = state_indices
+        if idx.dtype.itemsize > 4:  # outside the pool stays outside in 32 bits
+            idx = idx.to(torch.int64).clamp(-1, state.shape[0])
+        idx = idx.to(device=v.device, dtype=torch.int32).contiguous()
     elif state.shape[0] < n:
         raise ValueError(f"{n} sequences need as many states; got {state.shape[0]}")
     y = torch.empty(v.shape, dtype=v.dtype, device=v.device)

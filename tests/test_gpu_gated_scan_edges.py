@@ -88,3 +88,24 @@ def test_forward_mode_is_refused(cuda_device, grad):
                 gated_scan(*(d[k] for k in names))
             y, _ = gated_scan(*(x[k] for k in names))  # no tangents: as ever
             assert torch.equal(y, plain)
+
+
+@pytest.mark.parametrize("itype", [torch.int64, torch.int32])
+def test_wide_indices_outside_the_pool_are_padding(cuda_device, itype):
+    """Sentinels that do not fit 32 bits mark padding like any other index
+    outside the pool."""
+    far = [torch.iinfo(itype).min, torch.iinfo(itype).max, -1, 4]
+    if itype == torch.int64:
+        far += [1 << 32, (1 << 32) + 1, -(1 << 32), (1 << 31) + 1]
+    n, D = len(far) + 1, 40
+    x = inputs(cuda_device, n, 1, D, F32, F32, False, n, seed=21)
+    v, g = x["v"][:, 0], x["g"][:, 0]
+    pool = torch.randn(4, D, device=cuda_device)
+    before = pool.clone()
+    idx = torch.tensor(far + [3], dtype=itype, device=cuda_device)
+    y = gated_scan_step(v, g, state=pool, state_indices=idx)
+    assert torch.equal(pool[:3], before[:3]) and not torch.equal(pool[3], before[3])
+    assert not y[:-1].any() and torch.equal(y[-1], pool[3])
+    # indices on the host give the same
+    y2 = gated_scan_step(v[-1:], g[-1:], state=before, state_indices=idx[-1:].cpu())
+    assert torch.equal(y2, y[-1:]) and torch.equal(before, pool)
