@@ -807,6 +807,9 @@ int check_scan(const gdn2_scan_problem* p, const char* fn) {
   if (p->cu_seqlens ? p->B != 1 || p->T > 2147483647LL : p->n_seqs != p->B)
     return fail(GDN2_ERR_INVALID,
                 "%s: packed sequences need B = 1 (T < 2^31), others n_seqs = B", fn);
+  if (p->cu_seqlens && p->n_seqs == 0 && p->T > 0)
+    return fail(GDN2_ERR_INVALID, "%s: cu_seqlens without a sequence cannot end at T = %lld", fn,
+                (long long)p->T);
   if (p->ld_v < p->D || p->ld_g < p->D || p->ld_w < 0 || p->ld_dy < 0)
     return fail(GDN2_ERR_INVALID, "%s: row strides must be at least D", fn);
   if (p->ld_v > kMaxStride || p->ld_g > kMaxStride || p->ld_w > kMaxStride || p->ld_dy > kMaxStride)

@@ -109,3 +109,13 @@ def test_wide_indices_outside_the_pool_are_padding(cuda_device, itype):
     # indices on the host give the same
     y2 = gated_scan_step(v[-1:], g[-1:], state=before, state_indices=idx[-1:].cpu())
     assert torch.equal(y2, y[-1:]) and torch.equal(before, pool)
+
+
+def test_rows_without_a_sequence_are_refused(cuda_device):
+    """Offsets without a sequence cannot end at the last of some rows."""
+    v = torch.ones(1, 5, 8, device=cuda_device)
+    cu = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        gated_scan(v, -v, cu_seqlens=cu)
+    y, ht = gated_scan(v[:, :0], v[:, :0], cu_seqlens=cu, output_final_state=True)
+    assert y.shape == (1, 0, 8) and ht.shape == (0, 8)
