@@ -97,8 +97,8 @@ __device__ __forceinline__ float leave(float2 p, float h) {
 // slots themselves, else a warp's, which it folds itself before and after the
 // tile's barriers, so that fewer are left between them.  That pays forward
 // (131,072 x 128: 176 -> 139 us), not with the backward's two folds (B = 8,
-// T = 4096, D = 2048: 214 -> 228 us).
-template <int W, int R> struct Runs {
+// T = 4096, D = 2048: 214 -> 228 us).  Read and written four channels at a time.
+template <int W, int R> struct alignas(16) Runs {
   using S = Shape<W, R>;
   static constexpr int own = R == rows_of<false>() ? 32 / S::lanes : 1, groups = S::slots / own;
   float A[groups][W], H[groups][W];
