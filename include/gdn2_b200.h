@@ -464,8 +464,8 @@ int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensor
  * that runs out makes the kernel release its tensor memory, return without
  * finishing, and set a bit of a per-device fault word (bit 0: state passes,
  * bit 1: forward intra-chunk kernel, bit 2: decode, bit 3: backward
- * intra-chunk kernel, bit 4: gated linear recurrence, which finishes with
- * NaN).  gdn2_fault_status
+ * intra-chunk kernel, bit 4: gated linear recurrence, which finishes with NaN
+ * in the rows that were left).  gdn2_fault_status
  * synchronises `stream` (the default stream when NULL), returns the fault
  * word of the current device (0 = no fault) and resets it when `clear` is
  * nonzero; a negative return is a CUDA error.  No counterpart in the
@@ -486,6 +486,15 @@ int gdn2_fault_status(void* stream, int32_t clear);
 int gdn2_test_fwd_state_wait_timeout(const gdn2_chunk_problem* p, void* o, void* saved,
                                      size_t saved_bytes, int32_t skip_chunk, uint64_t wait_ns,
                                      void* stream);
+/* The same for the gated linear recurrence: the forward (dy NULL; without a
+ * gate or states, `saved` as in gdn2_scan_fwd) or the backward pass with every
+ * CTA of a cluster waiting for more runs than come, `wait_ns` at most.  The first
+ * waits run out, all results are NaN, bit 4 of the fault word is set and the
+ * launch itself succeeds.  Problems that single CTAs serve are refused before a
+ * launch. */
+int gdn2_test_scan_wait_timeout(const gdn2_scan_problem* p, const void* v, const void* g, void* y,
+                                float* saved, const void* dy, void* dv, void* dg,
+                                uint64_t wait_ns, void* stream);
 
 #ifdef __cplusplus
 }

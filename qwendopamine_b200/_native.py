@@ -58,6 +58,7 @@ EXPORTS = (
     "gdn2_adamw_step",
     "gdn2_fault_status",
     "gdn2_test_fwd_state_wait_timeout",
+    "gdn2_test_scan_wait_timeout",
 )
 
 
@@ -248,6 +249,8 @@ def _declare(lib):
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_adamw_step": ([ap, v, c_int32, v], ctypes.c_int),
+        "gdn2_test_scan_wait_timeout": ([sp, v, v, v, v, v, v, v, ctypes.c_uint64, v],
+                                        ctypes.c_int),
         "gdn2_scan_step": ([sp, v, v, v, v, c_int64, c_int32, v, v, v], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

@@ -80,6 +80,8 @@ struct ScanArgs {
   void *y, *dv, *dg, *dw;
   float *ht, *dh0, *saved;
   unsigned* fault;
+  uint64_t wait_ns;  // limit of a wait for the cluster's runs
+  int expect;        // bytes of them that come in a turn
 };
 
 // A run of rows: A in x (-1: it holds a reset), H in y.
@@ -107,10 +109,13 @@ template <int W, int R> struct alignas(16) Runs {
   float sA[own > 1 ? S::slots : 1][W], sH[own > 1 ? S::slots : 1][W];
 };
 
-template <int W, int R> struct ScanShared {
+// Whole lines, so that the stages behind it start on one (16 bytes more of it alone
+// cost B = 8, T = 4096, D = 2048 forward 123 -> 127 us).
+template <int W, int R> struct alignas(128) ScanShared {
   static constexpr int tile = Shape<W, R>::tile;
   Runs<W, R> runs;
   uint64_t bar[2];  // the cluster's runs have come, by turn's parity
+  int lost;         // a wait for them has run out
   // of a turn with sequence edges in its tile
   int seq[tile];                               // the row's sequence
   uint32_t first[tile / 32], last[tile / 32];  // whether it is its first / last row
@@ -212,8 +217,16 @@ __device__ __forceinline__ void open_exchange(const ScanArgs& a, ScanShared<W, R
     tc::mbar_init(&s.bar[0], 1);
     tc::mbar_init(&s.bar[1], 1);
     tc::fence_mbar_init();
+    s.lost = 0;
   }
   cg::this_cluster().sync();
+}
+
+// After the last turn.  A CTA that has received all runs of its last turn could
+// leave, since nothing more is sent to it; after a wait that ran out that is not
+// known, so all stay until all have sent what they send.
+__device__ __forceinline__ void close_exchange(const ScanArgs& a) {
+  if (a.cluster > 1) cg::this_cluster().sync();
 }
 
 // Finds the states that enter the groups of this CTA's tile and moves `state`
@@ -225,8 +238,11 @@ __device__ __forceinline__ void open_exchange(const ScanArgs& a, ScanShared<W, R
 // parity, and waits for as many; a cluster-wide barrier would also wait for
 // the last turn's stores to reach memory.  A thread sends the run of turn i+1
 // after it has read those of turn i, and receives all of turn i+1 before it
-// sends turn i+2: the same places are free by then.  A wait that runs out sets
-// a fault bit and turns the states into NaN.
+// sends turn i+2: the same places are free by then.
+//
+// A wait that runs out sets a fault bit and `lost`.  The CTA then gives up: what
+// lies in `runs` is of no turn, and its barrier, whose phase is still open, cannot
+// be used again.  It sends nothing more, so the others' waits run out as well.
 template <int W, int R, bool UP>
 __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s, float2* runs, int rank,
                                          int turn, float& state) {
@@ -237,12 +253,12 @@ __device__ __forceinline__ void exchange(const ScanArgs& a, ScanShared<W, R>& s,
     } else {
       runs += b * a.cluster * W;
       const float2 all = Fold<W, R, UP>::run(s.runs, ch);
-      if (ch == 0) tc::mbar_expect_tx(&s.bar[b], a.cluster * W * (int)sizeof(float2));
+      if (ch == 0) tc::mbar_expect_tx(&s.bar[b], a.expect);
       const uint32_t to = smem_u32(runs + rank * W + ch), bar = smem_u32(&s.bar[b]);
       for (int k = 0; k < a.cluster; ++k) store_async(address_at(to, k), address_at(bar, k), all);
-      if (!tc::mbar_wait(&s.bar[b], (turn >> 1) & 1)) {
+      if (!tc::mbar_wait(&s.bar[b], (turn >> 1) & 1, a.wait_ns)) {
         atomicOr(a.fault, kScanFault);
-        state = __int_as_float(0x7fffffff);
+        s.lost = 1;
       }
       float carry = state;
 #pragma unroll 4
@@ -445,6 +461,20 @@ template <int W, int R> __device__ __forceinline__ Place place_of(const ScanArgs
   return p;
 }
 
+// each(r, c) for the rows of the CTA's tiles from the one at row `tile` on, and
+// their channels (after it has given up).
+template <int W, int R, typename F>
+__device__ __forceinline__ void for_rest(const ScanArgs& a, const Place& p, int64_t tile, int64_t step,
+                                         int turns, F&& each) {
+  const int c = p.slab * W + (int)threadIdx.x % W;
+  if (c >= a.D) return;
+  for (; turns > 0; --turns, tile += step) {
+    const int64_t end = min(tile + Shape<W, R>::tile, p.hi);
+    for (int64_t r = tile + threadIdx.x / W; r < end; r += Shape<W, R>::threads / W)
+      if (r >= p.lo) each(r, c);
+  }
+}
+
 // Groups of four channels as two packed pairs.
 template <typename T> __device__ __forceinline__ float2 pair_of(const Raw<T, kCpt>& r, int k) {
   if constexpr (sizeof(T) == 4)
@@ -526,7 +556,8 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
   float state = 0.f;
   RowPlace place{0, 0, 0};
 
-  for (int turn = 0; turn < p.turns; ++turn, tile += step) {
+  int turn = 0;
+  for (; turn < p.turns; ++turn, tile += step) {
     const bool edges = place.edges(a, tile, step, TILE, p.lo, p.hi);
     if (edges) mark_rows(a, s, tile, p.lo, p.hi);
     stage_wait();
@@ -587,6 +618,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
     Fold<W, R, false>::put(s.runs, slot, lc, quad(A), quad(h));
     __syncthreads();
     exchange<W, R, false>(a, s, runs, p.rank, turn, state);
+    if (a.cluster > 1 && s.lost) break;
 
     unquad(h, Fold<W, R, false>::get(s.runs, slot, lc));
     const int64_t left = p.hi - tile - r0;  // rows that exist from here
@@ -603,6 +635,18 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, false>()) k_scan_fwd(cons
       walk(std::false_type{}, [&](int i) { y.template put<AL>(i, h, nc); });
     }
   }
+  if (turn < p.turns) {
+    const float nan = __int_as_float(0x7fffffff);
+    stage_wait();  // the next turn's rows
+    for_rest<W, R>(a, p, tile, step, p.turns - turn, [&](int64_t r, int c) {
+      ((T*)a.y)[r * a.D + c] = from_f<T>(nan);
+      if (a.saved && (r - p.lo) % kKeep == 0)
+        a.saved[(p.chain * a.keeps + (r - p.lo) / kKeep) * a.D + c] = nan;
+      place.find(a, r);
+      if (a.ht && place.at == place.len - 1) a.ht[(int64_t)place.n * a.D + c] = nan;
+    });
+  }
+  close_exchange(a);
 }
 
 template <typename T, typename G, bool GATE, int W, int R, int AL>
@@ -632,7 +676,8 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
   float state = 0.f;
   RowPlace place{0, 0, 0};
 
-  for (int turn = 0; turn < p.turns; ++turn, tile -= step) {
+  int turn = 0;
+  for (; turn < p.turns; ++turn, tile -= step) {
     const bool some = tile >= p.lo;
     const bool edges = place.edges(a, tile, -step, TILE, p.lo, p.hi);
     float kept = 0.f;  // the state entering the tile
@@ -699,6 +744,7 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
     if (threadIdx.x / W == 1)
       Fold<W, R, false>::enter(ahead, threadIdx.x - W, kept);
     exchange<W, R, true>(a, s, runs, p.rank, turn, state);
+    if (a.cluster > 1 && s.lost) break;
 
     const int64_t left = some ? p.hi - tile - r0 : 0;  // rows that exist from here
     const Target<G, W, R> dg(a.dg, tile, p.slab, a.D);
@@ -749,6 +795,18 @@ __global__ void __launch_bounds__(1024 / R, ctas_of<T, true>()) k_scan_bwd(const
       gradients(std::false_type{});
     }
   }
+  if (turn < p.turns) {
+    const float nan = __int_as_float(0x7fffffff);
+    stage_wait();  // the next turn's rows
+    for_rest<W, R>(a, p, tile, -step, p.turns - turn, [&](int64_t r, int c) {
+      ((T*)a.dv)[r * a.D + c] = from_f<T>(nan);
+      ((G*)a.dg)[r * a.D + c] = from_f<G>(nan);
+      if constexpr (GATE) ((T*)a.dw)[r * a.D + c] = from_f<T>(nan);
+      place.find(a, r);
+      if (a.dh0 && place.at == 0) a.dh0[(int64_t)place.n * a.D + c] = nan;
+    });
+  }
+  close_exchange(a);
 }
 
 // One token for each of n sequences: the state pool's slot is read, updated
@@ -939,24 +997,16 @@ template <typename F> cudaError_t scan_dispatch(const gdn2_scan_problem* p, bool
   });
 }
 
-}  // namespace
-}  // namespace gdn2
+// How long a wait for the cluster's runs may take, and whether it waits for more
+// than comes (a test).
+struct Wait {
+  uint64_t ns = tc::kWaitLimitNs;
+  bool in_vain = false;
+};
 
-using namespace gdn2;
-
-extern "C" {
-
-size_t gdn2_scan_saved_bytes(const gdn2_scan_problem* p) {
-  if (check_scan(p, "gdn2_scan_saved_bytes") != GDN2_OK) return 0;
-  // whatever the stretches are: a state for every 64 rows and one for the rest
-  // of each stretch, of which there are at most B
-  const size_t rows = (size_t)p->B * p->T;
-  return (rows / kKeep + p->B) * p->D * sizeof(float);
-}
-
-int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, const void* w,
-                  const float* h0, void* y, float* ht, float* saved, void* stream) {
-  const char* fn = "gdn2_scan_fwd";
+int scan_fwd(const char* fn, const gdn2_scan_problem* p, const void* v, const void* g,
+             const void* w, const float* h0, void* y, float* ht, float* saved, void* stream,
+             const Wait& wait) {
   int rc = check_scan(p, fn);
   if (rc) return rc;
   const int64_t rows = (int64_t)p->B * p->T;
@@ -985,6 +1035,9 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     ScanArgs b = a;
     b.nslab = (a.D + l.slab - 1) / l.slab;
     b.cluster = l.cluster;
+    if (wait.in_vain && l.cluster == 1) return cudaErrorNotSupported;
+    b.wait_ns = wait.ns;
+    b.expect = (l.cluster * l.slab + wait.in_vain) * (int)sizeof(float2);
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<false>();
@@ -1002,10 +1055,9 @@ int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
   }), fn);
 }
 
-int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, const void* w,
-                  const float* h0, const float* saved, const void* dy, const float* dht,
-                  void* dv, void* dg, void* dw, float* dh0, void* stream) {
-  const char* fn = "gdn2_scan_bwd";
+int scan_bwd(const char* fn, const gdn2_scan_problem* p, const void* v, const void* g,
+             const void* w, const float* h0, const float* saved, const void* dy, const float* dht,
+             void* dv, void* dg, void* dw, float* dh0, void* stream, const Wait& wait) {
   int rc = check_scan(p, fn);
   if (rc) return rc;
   const int64_t rows = (int64_t)p->B * p->T;
@@ -1038,6 +1090,9 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     ScanArgs b = a;
     b.nslab = (a.D + l.slab - 1) / l.slab;
     b.cluster = l.cluster;
+    if (wait.in_vain && l.cluster == 1) return cudaErrorNotSupported;
+    b.wait_ns = wait.ns;
+    b.expect = (l.cluster * l.slab + wait.in_vain) * (int)sizeof(float2);
     auto go = [&](auto w) {
       constexpr int W = decltype(w)::value;
       constexpr int R = rows_of<true>();
@@ -1053,6 +1108,46 @@ int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, cons
     return l.slab == 64 ? go(std::integral_constant<int, 64>{})
                         : go(std::integral_constant<int, 32>{});
   }), fn);
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+size_t gdn2_scan_saved_bytes(const gdn2_scan_problem* p) {
+  if (check_scan(p, "gdn2_scan_saved_bytes") != GDN2_OK) return 0;
+  // whatever the stretches are: a state for every 64 rows and one for the rest
+  // of each stretch, of which there are at most B
+  const size_t rows = (size_t)p->B * p->T;
+  return (rows / kKeep + p->B) * p->D * sizeof(float);
+}
+
+int gdn2_scan_fwd(const gdn2_scan_problem* p, const void* v, const void* g, const void* w,
+                  const float* h0, void* y, float* ht, float* saved, void* stream) {
+  return scan_fwd("gdn2_scan_fwd", p, v, g, w, h0, y, ht, saved, stream, Wait{});
+}
+
+int gdn2_scan_bwd(const gdn2_scan_problem* p, const void* v, const void* g, const void* w,
+                  const float* h0, const float* saved, const void* dy, const float* dht,
+                  void* dv, void* dg, void* dw, float* dh0, void* stream) {
+  return scan_bwd("gdn2_scan_bwd", p, v, g, w, h0, saved, dy, dht, dv, dg, dw, dh0, stream, Wait{});
+}
+
+int gdn2_test_scan_wait_timeout(const gdn2_scan_problem* p, const void* v, const void* g, void* y,
+                                float* saved, const void* dy, void* dv, void* dg,
+                                uint64_t wait_ns, void* stream) {
+  const char* fn = "gdn2_test_scan_wait_timeout";
+  if (wait_ns == 0 || wait_ns > tc::kWaitLimitNs)
+    return fail(GDN2_ERR_INVALID, "%s: wait_ns must be in 1 .. 1e9 (got %llu)", fn,
+                (unsigned long long)wait_ns);
+  const Wait wait{wait_ns, true};
+  if (dy)
+    return scan_bwd(fn, p, v, g, nullptr, nullptr, saved, dy, nullptr, dv, dg, nullptr, nullptr,
+                    stream, wait);
+  return scan_fwd(fn, p, v, g, nullptr, nullptr, y, nullptr, saved, stream, wait);
 }
 
 int gdn2_scan_step(const gdn2_scan_problem* p, const void* v, const void* g, const void* w,

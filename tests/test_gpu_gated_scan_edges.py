@@ -119,3 +119,60 @@ def test_rows_without_a_sequence_are_refused(cuda_device):
         gated_scan(v, -v, cu_seqlens=cu)
     y, ht = gated_scan(v[:, :0], v[:, :0], cu_seqlens=cu, output_final_state=True)
     assert y.shape == (1, 0, 8) and ht.shape == (0, 8)
+
+
+def fault_word():
+    return N.load().gdn2_fault_status(None, 1)
+
+
+@pytest.mark.parametrize("dtype,gdtype", [(F32, F32), (BF, F32)])
+@pytest.mark.parametrize("T,D", [(40000, 64), (700, 20), (9001, 1000)])
+def test_bounded_wait_runs_out_cleanly(cuda_device, T, D, dtype, gdtype):
+    """The failure path of the exchange between a cluster's CTAs, made to happen
+    without a fault: every CTA waits for more than comes, 50 us at most.  The
+    launch succeeds, bit 4 of the fault word is set, all results are NaN, and the
+    next call on the same context is as good as ever."""
+    lib = N.load()
+    fault_word()
+    x = inputs(cuda_device, 1, T, D, dtype, gdtype, False, 1, seed=30)
+    v, g = x["v"], x["g"]
+    prob = N.ScanProblem(1, D, T, N.dtype_code(dtype), N.dtype_code(gdtype), 1, None, D, D, D, D)
+    saved, lost = (torch.zeros(lib.gdn2_scan_saved_bytes(prob) // 4, device=cuda_device)
+                   for _ in range(2))
+    y, y2, dy, dv, dv2 = (torch.zeros_like(v) for _ in range(5))
+    dg, dg2 = torch.zeros_like(g), torch.zeros_like(g)
+    dy.copy_(torch.randn(v.shape, generator=torch.Generator().manual_seed(31)))
+    a, st = (lambda t: t.data_ptr()), N.raw_stream(0)
+
+    def normal():
+        N.check(lib.gdn2_scan_fwd(prob, a(v), a(g), None, None, a(y), None, a(saved), st), "fwd")
+        N.check(lib.gdn2_scan_bwd(prob, a(v), a(g), None, None, a(saved), a(dy), None, a(dv), a(dg),
+                                  None, None, st), "bwd")
+
+    normal()
+    want = [t.clone() for t in (y, saved, dv, dg)]
+    N.check(lib.gdn2_test_scan_wait_timeout(prob, a(v), a(g), a(y2), a(lost), None, None, None,
+                                            50_000, st), "fwd")
+    assert fault_word() == 16
+    used = -(-T // 64) * D  # a state for every 64 rows
+    assert y2.isnan().all() and lost[:used].isnan().all() and not lost[used:].any()
+    N.check(lib.gdn2_test_scan_wait_timeout(prob, a(v), a(g), None, a(saved), a(dy), a(dv2), a(dg2),
+                                            50_000, st), "bwd")
+    assert fault_word() == 16
+    assert dv2.isnan().all() and dg2.isnan().all()
+    for t in (y, dv, dg):
+        t.zero_()
+    normal()
+    assert fault_word() == 0
+    assert all(torch.equal(t, w) for t, w in zip((y, saved, dv, dg), want))
+
+
+def test_wait_hook_argument_checks(cuda_device):
+    lib, buf = N.load(), torch.zeros(4, 20, device=cuda_device)
+    one = N.ScanProblem(1, 20, 4, 0, 0, 1, None, 20, 20, 20, 20)
+    a = buf.data_ptr()
+    call = lambda p, ns: lib.gdn2_test_scan_wait_timeout(p, a, a, a, None, None, None, None, ns, None)
+    for ns in (0, 2_000_000_000):
+        assert call(one, ns) == N.ERR_INVALID
+    assert call(one, 1000) == N.ERR_CUDA and b"not supported" in lib.gdn2_last_error()
+    assert lib.gdn2_fault_status(None, 1) == 0
