@@ -1,5 +1,6 @@
 """AdamW on the GPU: calls at the edges of what the entry points take."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -7,7 +8,7 @@ from qwendopamine_b200 import AdamW, adamw_step
 
 pytestmark = pytest.mark.gpu
 
-BF = torch.bfloat16
+BF, F8 = torch.bfloat16, torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -33,3 +34,55 @@ def test_step_on_tensors_without_a_version(cuda_device):
         p, g, m, v = (torch.full((40,), x, device=cuda_device) for x in (1.0, 1.0, 0.0, 0.0))
         adamw_step([p], [g], [m], [v], step=1, lr=0.5, weight_decay=0.0)
         assert (p - 0.5).abs().max() < 1e-6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_roots_of_second_moments(cuda_device, bits):
+    """Second moments from the smallest fp32 value up, with an eps below their
+    roots: the update divides by the root, and the codes hold it.
+
+    With no first-moment and second-moment gradient (g = 0, beta2 = 1/2) v' = v / 2
+    is exact above 2^-148, so the change of a parameter is lr m' / (root' + eps):
+    one rounding each of a few operations, and 2^-22 of the root and of the
+    reciprocal: 2e-6 in all, and the root of v' (subnormal ones exact in fp32)
+    enters as it is."""
+    e = np.arange(-147, 120).astype(np.float64)
+    more = np.random.default_rng(0).uniform(1, 2, (6, e.size))
+    v = np.concatenate([m * 2.0 ** e for m in (1.0, 1.9999, *more)]).astype(np.float32)
+    # beta2 v with beta2 = 1/2, rounded as fp32 has it
+    half = (v * np.float32(0.5)).astype(np.float64)
+    want_root = np.sqrt(half)
+    n = v.size
+    dev = cuda_device
+    if bits == 32:
+        # m' = m / 2 such that the step is lr * m' / root = about lr
+        m = (want_root * 2).astype(np.float32)
+        args = [torch.from_numpy(m).to(dev)], [torch.from_numpy(v).to(dev)]
+        p = [torch.zeros(n, device=dev)]
+        adamw_step(p, [torch.zeros(n, device=dev)], *args, step=400, lr=1e-3, betas=(0.5, 0.5),
+                   eps=1e-30, weight_decay=0.0)
+        mm = m.astype(np.float64) / 2
+        want = -1e-3 * mm / (want_root + 1e-30)
+        got = p[0].double().cpu().numpy()
+        assert (np.abs(got - want) <= 2e-6 * np.abs(want)).all()
+        return
+    # 8 bits: a gradient alone in its block, v' = g^2 / 2; its root is the block's
+    # largest value, so its scale is root / 448, and the step is lr m' / root
+    g = np.zeros((n, 256), dtype=np.float32)
+    g[:, 3] = np.sqrt(v.astype(np.float64)).astype(np.float32)
+    sq = (g[:, 3] * g[:, 3] * np.float32(0.5)).astype(np.float64)  # rounded step by step
+    keep = sq > 0
+    want_root = np.sqrt(sq)
+    p = torch.zeros(n * 256, device=dev)
+    codes = [torch.zeros(n * 256, dtype=torch.uint8, device=dev).view(F8) for _ in range(2)]
+    sm, sv = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+    adamw_step([p], [torch.from_numpy(g).to(dev).view(-1)], [codes[0]], [codes[1]], step=400,
+               lr=1e-3, betas=(0.5, 0.5), eps=1e-32, weight_decay=0.0, exp_avg_scales=[sm],
+               exp_avg_sq_scales=[sv])
+    got = sv.double().cpu().numpy() * 448
+    # the root's rounding (twice that in rare cases), 1 / 448's and the product's, each
+    # at most 2^-24
+    assert (np.abs(got - want_root)[keep] <= 5 * 2.0 ** -24 * want_root[keep]).all()
+    step = -1e-3 * (g[:, 3].astype(np.float64) / 2) / (want_root + 1e-32)
+    got = p.view(n, 256)[:, 3].double().cpu().numpy()
+    assert (np.abs(got - step)[keep] <= 2e-6 * np.abs(step)[keep]).all()
