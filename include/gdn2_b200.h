@@ -433,7 +433,8 @@ int gdn2_logprob_bwd(const gdn2_logprob_problem* p, const void* logits,
  * they are float8 e4m3 codes; blocks of 256 consecutive elements share a
  * scale (fp32 [ceil(numel / 256)]), an element's m is code * exp_avg_scale and
  * its v is (code * exp_avg_sq_scale)^2.  Blocks whose largest value is below
- * 1e-30 are held as zeros.  All zeros is a valid start.  grad_scale and
+ * 1e-30 are held as zeros.  All zeros is a valid start.  An eps in (0, 2^-126)
+ * counts as 2^-126.  grad_scale and
  * found_inf are device scalars or NULL: a nonzero found_inf leaves everything
  * as it is.  The struct array is read before the call returns. */
 typedef struct gdn2_adamw_problem {

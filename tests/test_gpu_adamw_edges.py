@@ -86,3 +86,16 @@ def test_roots_of_second_moments(cuda_device, bits):
     step = -1e-3 * (g[:, 3].astype(np.float64) / 2) / (want_root + 1e-32)
     got = p.view(n, 256)[:, 3].double().cpu().numpy()
     assert (np.abs(got - step)[keep] <= 2e-6 * np.abs(step)[keep]).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-38, 1e-39, 2.0 ** -149])
+def test_an_eps_below_the_normal_range(cuda_device, bits, eps):
+    """Parameters without a gradient so far stay where they are: 0 / eps is 0."""
+    p = torch.ones(300, device=cuda_device)
+    z = lambda n: torch.zeros(n, device=cuda_device)
+    st = [z(300), z(300)] if bits == 32 else [
+        torch.zeros(300, dtype=torch.uint8, device=cuda_device).view(F8) for _ in range(2)]
+    kw = {} if bits == 32 else dict(exp_avg_scales=[z(2)], exp_avg_sq_scales=[z(2)])
+    adamw_step([p], [z(300)], [st[0]], [st[1]], step=1, lr=1e-3, eps=eps, weight_decay=0.0, **kw)
+    assert p.eq(1).all()
