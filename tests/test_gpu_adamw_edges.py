@@ -99,3 +99,21 @@ def test_an_eps_below_the_normal_range(cuda_device, bits, eps):
     kw = {} if bits == 32 else dict(exp_avg_scales=[z(2)], exp_avg_sq_scales=[z(2)])
     adamw_step([p], [z(300)], [st[0]], [st[1]], step=1, lr=1e-3, eps=eps, weight_decay=0.0, **kw)
     assert p.eq(1).all()
+
+
+def test_codes_of_the_largest_first_moments(cuda_device):
+    """Blocks whose largest value is near fp32's keep their codes: m' = g / 2, held to
+    half a step of e4m3, at most 2^-4 of a normal code or 2^-10 of 448 of the rest."""
+    g = torch.zeros(4, 256)
+    for i, most in enumerate((3e38, 1.7e38, 9e37, 5e37)):
+        g[i] = torch.linspace(-1, 1, 256) * most
+    p, z8 = torch.zeros(1024, device=cuda_device), []
+    for _ in range(2):
+        z8.append(torch.zeros(1024, dtype=torch.uint8, device=cuda_device).view(F8))
+    ms, vs = torch.zeros(4, device=cuda_device), torch.zeros(4, device=cuda_device)
+    adamw_step([p], [g.view(-1).to(cuda_device)], [z8[0]], [z8[1]], step=1, lr=1e-3,
+               betas=(0.5, 0.5), exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+    m = (z8[0].double() * ms.double().repeat_interleave(256)).view(4, 256).cpu()
+    want = g.double() / 2
+    most = want.abs().amax(1, keepdim=True)
+    assert ((m - want).abs() <= 1.0001 * torch.maximum(want.abs() / 16, most * 2.0 ** -10 / 448)).all()
