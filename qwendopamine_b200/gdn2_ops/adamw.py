@@ -180,26 +180,34 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            batches: dict = {}
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW (B200 build) does not take sparse gradients")
-                s = self._state_of(p, group)
-                s["step"] += 1
-                key = (p.device, p.dtype, p.grad.dtype, s["step"], "master" in s,
-                       "exp_avg_scale" in s)
-                batches.setdefault(key, []).append((p, s))
-            for (_, _, _, step, master, eight), items in batches.items():
-                of = lambda k: [s[k] for _, s in items]
-                adamw_step([p for p, _ in items], [p.grad for p, _ in items], of("exp_avg"),
-                           of("exp_avg_sq"), step=step, lr=group["lr"], betas=group["betas"],
-                           eps=group["eps"], weight_decay=group["weight_decay"],
-                           exp_avg_scales=of("exp_avg_scale") if eight else None,
-                           exp_avg_sq_scales=of("exp_avg_sq_scale") if eight else None,
-                           master_params=of("master") if master else None,
-                           grad_scale=grad_scale, found_inf=found_inf)
+            batches: dict = {}  # what is counted and not yet taken
+            try:
+                for p in group["params"]:
+                    if p.grad is None:
+                        continue
+                    if p.grad.is_sparse:
+                        raise RuntimeError("AdamW (B200 build) does not take sparse gradients")
+                    s = self._state_of(p, group)
+                    s["step"] += 1
+                    key = (p.device, p.dtype, p.grad.dtype, s["step"], "master" in s,
+                           "exp_avg_scale" in s)
+                    batches.setdefault(key, []).append((p, s))
+                for key, items in list(batches.items()):
+                    _, _, _, step, master, eight = key
+                    of = lambda k: [s[k] for _, s in items]
+                    adamw_step([p for p, _ in items], [p.grad for p, _ in items], of("exp_avg"),
+                               of("exp_avg_sq"), step=step, lr=group["lr"], betas=group["betas"],
+                               eps=group["eps"], weight_decay=group["weight_decay"],
+                               exp_avg_scales=of("exp_avg_scale") if eight else None,
+                               exp_avg_sq_scales=of("exp_avg_sq_scale") if eight else None,
+                               master_params=of("master") if master else None,
+                               grad_scale=grad_scale, found_inf=found_inf)
+                    del batches[key]
+            except BaseException:
+                for items in batches.values():
+                    for _, s in items:
+                        s["step"] -= 1
+                raise
         return loss
 
     def load_state_dict(self, state_dict):

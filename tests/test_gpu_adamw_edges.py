@@ -117,3 +117,34 @@ def test_codes_of_the_largest_first_moments(cuda_device):
     want = g.double() / 2
     most = want.abs().amax(1, keepdim=True)
     assert ((m - want).abs() <= 1.0001 * torch.maximum(want.abs() / 16, most * 2.0 ** -10 / 448)).all()
+
+
+def test_a_refused_step_is_not_counted(cuda_device):
+    good = torch.nn.Parameter(torch.ones(8, 4, device=cuda_device))
+    strided = torch.nn.Parameter(torch.ones(4, 8, device=cuda_device).t())
+    half = torch.nn.Parameter(torch.ones(5, device=cuda_device, dtype=BF))
+    opt = AdamW([half, good, strided], lr=1e-2)
+    for p in (good, strided, half):
+        p.grad = torch.ones_like(p)
+    for n in range(3):
+        with pytest.raises(ValueError, match="contiguous"):
+            opt.step()
+        # one launch for each type: the first was taken, the refused one was not
+        assert opt.state[half]["step"] == n + 1
+        assert opt.state[good]["step"] == opt.state[strided]["step"] == 0
+    strided.grad = None
+    opt.step()
+    # the first step's bias correction: 1e-2 whatever the gradient
+    assert (good - (1 - 1e-2 * 1e-2) + 1e-2).abs().max() < 1e-6
+    assert opt.state[good]["step"] == 1 and opt.state[half]["step"] == 4
+
+
+def test_a_sparse_gradient_counts_no_step(cuda_device):
+    dense = torch.nn.Parameter(torch.ones(4, 2, device=cuda_device))
+    table = torch.nn.Parameter(torch.ones(4, 2, device=cuda_device))
+    opt = AdamW([dense, table])
+    dense.grad = torch.ones_like(dense)
+    table.grad = torch.sparse_coo_tensor([[1]], torch.ones(1, 2), (4, 2)).to(cuda_device)
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert opt.state[dense]["step"] == 0 and dense.eq(1).all()
