@@ -400,7 +400,7 @@ int gdn2_scan_step(const gdn2_scan_problem* p, const void* v, const void* g,
  * needs of the forward.  Backward: dlogits [rows][vocab], contiguous, in the
  * logits' dtype, from dlogprobs and dentropy (fp32 [rows], NULL for zero;
  * dentropy only after a forward with entropy); zero for ignored rows and rows
- * of only -inf.  top_k <= 128. */
+ * of only -inf.  top_k <= 128, temperature >= 4.3e-39. */
 typedef struct gdn2_logprob_problem {
     int64_t rows;
     int64_t ld;

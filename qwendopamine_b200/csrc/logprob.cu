@@ -594,8 +594,10 @@ int check_logprob(const gdn2_logprob_problem* p, const char* fn) {
   if (!dtype_valid(p->dtype)) return fail(GDN2_ERR_INVALID, "%s: unknown dtype %d", fn, p->dtype);
   if (p->ld < p->vocab)
     return fail(GDN2_ERR_INVALID, "%s: the row stride must be at least vocab", fn);
-  if (!(p->temperature > 0.f) || p->temperature > FLT_MAX)
-    return fail(GDN2_ERR_INVALID, "%s: temperature must be positive and finite", fn);
+  // log2(e) / temperature overflows below 4.3e-39
+  if (!(p->temperature > 0.f) || p->temperature > FLT_MAX || kLog2e / p->temperature > FLT_MAX)
+    return fail(GDN2_ERR_INVALID, "%s: temperature must be positive and finite, and so its inverse",
+                fn);
   if (p->top_k < 0 || p->top_k > p->vocab)
     return fail(GDN2_ERR_INVALID, "%s: top_k must be in 0 .. vocab (got %d)", fn, p->top_k);
   if (p->top_k > kMaxTop)

@@ -27,3 +27,14 @@ def test_scan_of_rows_without_a_sequence(lib):
         assert call(scan(n_seqs=0)) == N.ERR_INVALID and b"cu_seqlens" in lib.gdn2_last_error()
         assert call(scan(n_seqs=0, T=0)) == N.OK
     assert lib.gdn2_scan_saved_bytes(scan(n_seqs=0)) == 0
+
+
+def test_logprob_temperature_without_an_inverse(lib):
+    f = ctypes.c_void_p(0x1000)
+    for t in (4e-39, 2.0 ** -149):
+        p = N.LogprobProblem(4, 1000, -100, 1000, 1, 5, t)
+        assert lib.gdn2_logprob_fwd(p, f, f, f, None, f, f, None, None) == N.ERR_INVALID
+        assert b"temperature" in lib.gdn2_last_error()
+        assert lib.gdn2_logprob_bwd(p, f, f, f, f, None, f, None) == N.ERR_INVALID
+    none = N.LogprobProblem(0, 1000, -100, 1000, 1, 5, 1e-38)
+    assert lib.gdn2_logprob_fwd(none, None, None, None, None, None, None, None, None) == N.OK

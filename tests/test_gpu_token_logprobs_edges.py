@@ -68,3 +68,18 @@ def test_forward_mode_is_refused(cuda_device, grad):
         with pytest.raises(RuntimeError, match="forward"):
             token_logprobs(fwAD.make_dual(x, torch.ones_like(x)), ids)
         assert torch.equal(token_logprobs(x, ids).logprobs, plain)
+
+
+def test_a_temperature_without_an_inverse_is_refused(cuda_device):
+    """Below about 4e-39 log2(e) / temperature is not finite in fp32."""
+    x = torch.randn(3, 40, device=cuda_device)
+    ids = x.argmax(1)
+    for t in (4e-39, 1e-39, 2.0 ** -149):
+        with pytest.raises(ValueError, match="temperature"):
+            token_logprobs(x, ids, temperature=t)
+    r = token_logprobs(x, ids, top_k=2, entropy=True, temperature=1e-38)
+    assert not r.logprobs.any() and not r.entropy.any()
+    best = x.double().topk(2).values  # the second's is its distance over the temperature
+    want = (best[:, 1] - best[:, 0]) / 1e-38
+    assert (r.top_ids[:, 0] == ids).all()
+    assert ((r.top_logprobs[:, 1] - want).abs() <= 1e-6 * want.abs()).all()
