@@ -185,6 +185,10 @@ class AdamWProblem(ctypes.Structure):
     ]
 
 
+# Sizes of sequences, states and tokens are 32-bit fields, to which ctypes cuts
+# larger numbers down without a word.
+INT32_MAX = 0x7FFFFFFF
+
 # gdn2_adamw_tensor as 64-bit words: param, grad, exp_avg, exp_avg_sq,
 # exp_avg_scale, exp_avg_sq_scale, master, numel
 ADAMW_TENSOR_WORDS = 8

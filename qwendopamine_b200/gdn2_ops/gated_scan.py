@@ -173,6 +173,9 @@ def gated_scan(
         if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
             raise ValueError("cu_seqlens must be a 1-D tensor of offsets")
         n = cu_seqlens.numel() - 1
+    if n > N.INT32_MAX:
+        raise ValueError(f"gated_scan: up to 2^31 - 1 sequences are supported; got {n}")
+    if cu_seqlens is not None:
         cu = cu_seqlens.to(device=v.device, dtype=torch.int32).contiguous()
     h0 = initial_state
     if h0 is not None:
@@ -213,6 +216,9 @@ def gated_scan_step(
     if state.device != v.device or state.shape[1:] != v.shape[1:]:
         raise ValueError(f"state must be [S, *{tuple(v.shape[1:])}] on {v.device}; got "
                          f"{tuple(state.shape)} on {state.device}")
+    if n > N.INT32_MAX or state.shape[0] > N.INT32_MAX:
+        raise ValueError(f"gated_scan_step: up to 2^31 - 1 sequences and states are supported; got "
+                         f"{n} and {state.shape[0]}")
     if not state.is_contiguous() and (not state[:1].is_contiguous() or (
             state.shape[0] > 1 and state.stride(0) < D)):
         raise ValueError("state must hold each sequence's channels contiguously")
@@ -222,9 +228,9 @@ def gated_scan_step(
             raise ValueError(f"state_indices must be {n} integers; got "
                              f"{tuple(state_indices.shape)} {state_indices.dtype}")
         idx = state_indices
-        if idx.dtype.itemsize > 4:  # outside the pool stays outside in 32 bits
-            idx = idx.to(torch.int64).clamp(-1, state.shape[0])
-        idx = idx.to(device=v.device, dtype=torch.int32).contiguous()
+        if idx.dtype is not torch.int32:  # outside the pool stays outside in 32 bits
+            idx = idx.to(torch.int64).clamp(-1, state.shape[0]).to(torch.int32)
+        idx = idx.to(v.device).contiguous()
     elif state.shape[0] < n:
         raise ValueError(f"{n} sequences need as many states; got {state.shape[0]}")
     y = torch.empty(v.shape, dtype=v.dtype, device=v.device)

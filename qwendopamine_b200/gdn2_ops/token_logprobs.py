@@ -125,8 +125,9 @@ def token_logprobs(
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs: logits must be a CUDA tensor -- the B200 build has no "
                            "CPU path")
-    if logits.ndim < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"token_logprobs: logits need a vocabulary; got {tuple(logits.shape)}")
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] <= N.INT32_MAX:
+        raise ValueError(f"token_logprobs: logits need a vocabulary of up to 2^31 - 1 tokens; got "
+                         f"{tuple(logits.shape)}")
     if token_ids.shape != logits.shape[:-1] or token_ids.is_floating_point() \
             or token_ids.dtype == torch.bool:
         raise ValueError(f"token_logprobs: token_ids must be {tuple(logits.shape[:-1])} integers; "

@@ -176,3 +176,17 @@ def test_wait_hook_argument_checks(cuda_device):
         assert call(one, ns) == N.ERR_INVALID
     assert call(one, 1000) == N.ERR_CUDA and b"not supported" in lib.gdn2_last_error()
     assert lib.gdn2_fault_status(None, 1) == 0
+
+
+def test_sizes_beyond_32_bits_are_refused(cuda_device):
+    """The library holds these sizes in 32 bits; the rows are one row, expanded."""
+    many = (1 << 32) + 1
+    one = torch.zeros(1, 1, 1, device=cuda_device)
+    with pytest.raises(ValueError, match="2.31 - 1 sequences"):
+        gated_scan(one.expand(many, 1, 1), one.expand(many, 1, 1))
+    with pytest.raises(ValueError, match="2.31 - 1 sequences"):
+        gated_scan(one, one, cu_seqlens=torch.zeros(1, device=cuda_device).int().expand(many + 1))
+    with pytest.raises(ValueError, match="2.31 - 1 sequences"):
+        gated_scan_step(one[0].expand(many, 1), one[0].expand(many, 1), state=one[0])
+    with pytest.raises(ValueError, match="2.31 - 1 sequences and states"):
+        gated_scan_step(one[0], one[0], state=one[0].expand(many, 1))

@@ -83,3 +83,9 @@ def test_a_temperature_without_an_inverse_is_refused(cuda_device):
     want = (best[:, 1] - best[:, 0]) / 1e-38
     assert (r.top_ids[:, 0] == ids).all()
     assert ((r.top_logprobs[:, 1] - want).abs() <= 1e-6 * want.abs()).all()
+
+
+def test_a_vocabulary_beyond_32_bits_is_refused(cuda_device):
+    x = torch.zeros(1, 1, device=cuda_device).expand(1, (1 << 32) + 5)
+    with pytest.raises(ValueError, match="2.31 - 1 tokens"):
+        token_logprobs(x, torch.zeros(1, dtype=torch.int64, device=cuda_device))
