@@ -354,12 +354,9 @@ def on_device(index: int):
     return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def traced(*tensors):
-    """Whether a call on these tensors (or None) has to go through autograd: a
-    gradient is asked for, or one of them carries a forward-mode tangent, which
-    the Functions here refuse."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
+def forward_mode(*tensors) -> bool:
+    """Whether one of the tensors (or None) carries a forward-mode tangent: the
+    call then has to go through autograd, where the Functions here refuse it."""
     return fwAD._current_level >= 0 and any(
         t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)
 

@@ -185,7 +185,8 @@ def gated_scan(
             raise ValueError(f"initial_state must be [{n}, *{tuple(v.shape[2:])}] on {v.device}; "
                              f"got {tuple(h0.shape)} on {h0.device}")
         h0 = h0.contiguous()
-    if N.traced(v, g, w, h0):
+    if N.forward_mode(v, g, w, h0) or torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (v, g, w, h0)):
         y, ht = GatedScanFunction.apply(v, g, w, h0, cu, bool(output_final_state))
     else:
         y, ht, _ = _forward(_Geometry(v, g, w, cu), v.shape, h0, bool(output_final_state),

@@ -138,7 +138,7 @@ def token_logprobs(
     lead = logits.shape[:-1]
     ids = token_ids.to(device=logits.device, dtype=torch.int64).reshape(-1).contiguous()
     args = (int(top_k), bool(entropy), float(temperature), int(ignore_index))
-    if N.traced(logits):
+    if logits.requires_grad and torch.is_grad_enabled() or N.forward_mode(logits):
         logp, ent, top, top_ids = TokenLogprobsFunction.apply(logits, ids, *args)
     else:
         logp, ent, top, top_ids, _ = _forward(*_matrix(logits), ids, *args, keep=False)
