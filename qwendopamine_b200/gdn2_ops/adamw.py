@@ -70,7 +70,7 @@ def adamw_step(
     16-bit parameters are rounded to nearest after the step.  ``step`` counts
     from 1.  ``grad_scale`` (a float32 device scalar) multiplies the gradients,
     and a nonzero ``found_inf`` leaves everything as it is; neither is read on
-    the host.  What is written counts as changed in place for autograd.
+    the host.  A captured call keeps ``step`` and ``lr``.  What is written counts as changed in place for autograd.
     """
     n = len(params)
     lists = {"params": params, "grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs}

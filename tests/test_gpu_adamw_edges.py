@@ -148,3 +148,35 @@ def test_a_sparse_gradient_counts_no_step(cuda_device):
     with pytest.raises(RuntimeError, match="sparse"):
         opt.step()
     assert opt.state[dense]["step"] == 0 and dense.eq(1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_capture_of_one_step(cuda_device, bits):
+    """A captured step replays with the step count and learning rate it was
+    captured with, on the gradients that then lie in the buffers."""
+    new = lambda: torch.randn(700, generator=torch.Generator().manual_seed(3)).to(cuda_device)
+    z = lambda n: torch.zeros(n, device=cuda_device)
+    z8 = lambda n: torch.zeros(n, dtype=torch.uint8, device=cuda_device).view(F8)
+    scale = torch.full((), 0.5, device=cuda_device)
+
+    def fresh():
+        st = [z(700), z(700)] if bits == 32 else [z8(700), z8(700)]
+        sc = {} if bits == 32 else dict(exp_avg_scales=[z(3)], exp_avg_sq_scales=[z(3)])
+        return new(), z(700), st, sc
+
+    def step(p, g, st, sc):
+        adamw_step([p], [g], [st[0]], [st[1]], step=3, lr=1e-2, grad_scale=scale, **sc)
+
+    a, b = fresh(), fresh()
+    step(*fresh())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*a)
+    for seed in (1, 2):
+        g = torch.randn(700, generator=torch.Generator().manual_seed(seed)).to(cuda_device)
+        a[1].copy_(g)
+        b[1].copy_(g)
+        graph.replay()
+        step(*b)
+        assert torch.equal(a[0], b[0])

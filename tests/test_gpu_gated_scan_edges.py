@@ -190,3 +190,39 @@ def test_sizes_beyond_32_bits_are_refused(cuda_device):
         gated_scan_step(one[0].expand(many, 1), one[0].expand(many, 1), state=one[0])
     with pytest.raises(ValueError, match="2.31 - 1 sequences and states"):
         gated_scan_step(one[0], one[0], state=one[0].expand(many, 1))
+
+
+def test_capture_in_a_graph(cuda_device):
+    """Forward, backward and step replayed on new inputs in the captured buffers."""
+    x = inputs(cuda_device, 2, 300, 40, BF, F32, True, 2, seed=24)
+    leaves = [x[k].requires_grad_() for k in ("v", "g", "w", "h0")]
+    dy, dht = torch.randn_like(x["v"]), torch.randn_like(x["h0"])
+    pool = torch.randn(2, 40, device=cuda_device)
+    slots = torch.tensor([1, 0], device=cuda_device)
+
+    def go():
+        y, ht = gated_scan(*leaves[:3], initial_state=leaves[3], output_final_state=True)
+        grads = torch.autograd.grad((y, ht), leaves, (dy, dht))
+        with torch.no_grad():
+            one = gated_scan_step(*(t[:, 0] for t in leaves[:3]), state=pool, state_indices=slots)
+        return (y, ht, *grads, one)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        go()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = go()
+    other = inputs(cuda_device, 2, 300, 40, BF, F32, True, 2, seed=25)
+    with torch.no_grad():
+        for leaf, k in zip(leaves, ("v", "g", "w", "h0")):
+            leaf.copy_(other[k])
+    before = pool.clone()
+    graph.replay()
+    got, moved = [t.clone() for t in out], pool.clone()
+    pool.copy_(before)
+    for a, b in zip(got, go()):
+        assert torch.equal(a, b)
+    assert torch.equal(moved, pool)

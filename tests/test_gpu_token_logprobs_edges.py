@@ -89,3 +89,29 @@ def test_a_vocabulary_beyond_32_bits_is_refused(cuda_device):
     x = torch.zeros(1, 1, device=cuda_device).expand(1, (1 << 32) + 5)
     with pytest.raises(ValueError, match="2.31 - 1 tokens"):
         token_logprobs(x, torch.zeros(1, dtype=torch.int64, device=cuda_device))
+
+
+def test_capture_in_a_graph(cuda_device):
+    for rows, V in ((3, 400), (5, 70001), (300, 5000)):
+        x = torch.randn(rows, V, device=cuda_device).to(BF).requires_grad_()
+        ids = torch.zeros(rows, dtype=torch.int64, device=cuda_device)
+        dl = torch.randn(rows, device=cuda_device)
+
+        def go():
+            r = token_logprobs(x, ids, top_k=5, entropy=True)
+            return (*r, *torch.autograd.grad((r.logprobs, r.entropy), x, (dl, dl)))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            go()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = go()
+        with torch.no_grad():
+            x.copy_(torch.randn(rows, V, device=cuda_device))
+            ids.copy_(torch.arange(rows))
+        graph.replay()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, go()))
