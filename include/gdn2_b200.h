@@ -346,7 +346,7 @@ int gdn2_gated_norm_bwd(const gdn2_norm_problem* p, const void* x, const void* z
  *   h_t = exp(g_t) h_{t-1} + w_t v_t,   y_t = h_t rounded to `dtype`
  * v, w, y have `dtype`, g has `dtype` or fp32, states are fp32 [n_seqs][D].
  * Runs of up to 128 rows are composed: with g > 0 the product of a run's decays
- * has to stay finite in fp32.
+ * has to stay finite in fp32, also where the state is zero.
  * w NULL stands for ones, h0 NULL for zero; ht (or NULL) receives the states
  * after the last tokens.  Row r = b*T + t of v, g, w, dy starts at element
  * r * ld_* (up to 2^22); y and the gradients are contiguous [B*T][D].  cu_seqlens (int32
@@ -434,9 +434,9 @@ int gdn2_logprob_bwd(const gdn2_logprob_problem* p, const void* logits,
  * scale (fp32 [ceil(numel / 256)]), an element's m is code * exp_avg_scale and
  * its v is (code * exp_avg_sq_scale)^2.  Blocks whose largest value is below
  * 1e-30 are held as zeros.  All zeros is a valid start.  An eps in (0, 2^-126)
- * counts as 2^-126.  grad_scale and
- * found_inf are device scalars or NULL: a nonzero found_inf leaves everything
- * as it is.  The struct array is read before the call returns. */
+ * counts as 2^-126.  grad_scale and found_inf are device scalars or NULL: a
+ * nonzero found_inf leaves everything as it is.  The struct array is read before
+ * the call returns; step, lr and the rest travel with the launch. */
 typedef struct gdn2_adamw_problem {
     int32_t dtype, grad_dtype;
     int32_t state_bits;

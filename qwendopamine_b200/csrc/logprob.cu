@@ -20,7 +20,7 @@
 // Bound: HBM for many rows (forward: one read of the logits; backward: one
 // read and one write).  4096 x 151936 bf16 with entropy: forward 209 us (5.96
 // TB/s), backward 363 us (6.87 TB/s, the logits' last rows still in L2);
-// 2048 rows with top 1: 118 us (5.28 TB/s).  Few rows are split over the CTAs
+// 2048 rows with top 1: 118 us (5.28 TB/s; ncu, each).  Few rows are split over the CTAs
 // of a cluster, which join their partial sums and candidates through
 // distributed shared memory (32 rows with top 5: 13.7 us); small vocabularies
 // take a warp a row.
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kLpThreads, 5) k_logprob_fwd(const LogprobArgs
 }
 
 // Rows of up to 32 * kLpUnroll vectors: a warp each, the row in registers
-// (8192 x 500 bf16 with top 1: 29 us a call, 56 us with a CTA each).  The
+// (8192 x 500 bf16 with top 1: 25 us a call, 51 us with a CTA each).  The
 // top k come out one by one: the lanes' best by two reductions (value, then the
 // lower index), and the lane that held it looks for its next.
 template <typename T, bool ENT, bool TOP>
@@ -622,8 +622,9 @@ LogprobArgs logprob_args(const gdn2_logprob_problem* p) {
 }
 
 // CTAs of a row: one when the rows alone fill the GPU, else as many (2, 4, 8)
-// as keep the grid within two CTAs per SM and 16 KB for each (2048 rows of
-// 151936: one 110 us, two 133 us; 32 rows: one 24.4 us a call, eight 21.6 us).
+// as keep the grid within two CTAs per SM and 16 KB for each (bf16, between
+// events: 2048 rows of 151936 with top 1 one 115 us, two 132 us; 32 rows with top
+// 5 one 21.2 us, two 15.1, eight 13.0 us).
 cudaError_t row_parts(int64_t rows, int64_t row_bytes, int* parts) {
   int sms = 0;
   const cudaError_t e = num_sms(&sms);

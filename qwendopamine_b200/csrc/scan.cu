@@ -59,10 +59,11 @@ template <int W, int R> struct Shape {
 
 // Rows of a thread, and CTAs that share an SM (what their registers allow).
 // Forward: four CTAs of 128 threads with eight rows each (B = 8, T = 4096,
-// D = 2048, bf16: 122 us, 85 % of the measured copy bandwidth; two of 256 with
-// four rows 119 us, but 354 against 267 us on one sequence of 131,072 x 1024).
+// D = 2048, bf16 with a gate: 123 us between events, 84 % of the measured copy
+// bandwidth; two of 256 with four rows 119 us, but 254 against 213 us on one
+// sequence of 131,072 x 1024 and 98 against 78 us on 512 of 64 x 1024).
 // Backward, with twice the tensors in registers: two CTAs of 256 threads with
-// four rows (214 us, 87 %; three of 128 with eight rows 263 us).
+// four rows (211 us, 89 %; three of 128 with eight rows 242 us).
 template <bool BWD> constexpr int rows_of() { return BWD ? 4 : 8; }
 template <typename T, bool BWD> constexpr int ctas_of() {
   return BWD ? 2 : (sizeof(T) == 2 ? 4 : 3);
@@ -98,8 +99,8 @@ __device__ __forceinline__ float leave(float2 p, float h) {
 // Runs of a tile's rows on their way, in groups of `own` slots: with own = 1 the
 // slots themselves, else a warp's, which it folds itself before and after the
 // tile's barriers, so that fewer are left between them.  That pays forward
-// (131,072 x 128: 176 -> 139 us), not with the backward's two folds (B = 8,
-// T = 4096, D = 2048: 214 -> 228 us).  Read and written four channels at a time.
+// (131,072 x 128: 137 -> 133 us, 60,000 x 1001: 305 -> 293 us), not with the
+// backward's two folds (B = 8, T = 4096, D = 2048: 211 -> 219 us).  Read and written four channels at a time.
 template <int W, int R> struct alignas(16) Runs {
   using S = Shape<W, R>;
   static constexpr int own = R == rows_of<false>() ? 32 / S::lanes : 1, groups = S::slots / own;
@@ -906,7 +907,8 @@ ScanPlan scan_stretches(const gdn2_scan_problem* p, int sms) {
 // Slab and cluster: what takes the least time by a model of a turn, fitted to
 // runs of both directions over slabs and clusters (seven shapes from 9001 x 1000
 // to 131,072 x 1024).  A turn takes its latency, which grows with the cluster
-// and with a sequence's edge in it, or what its SM needs for all its CTAs.
+// and with a sequence's edge in it, or what its SM needs for all its CTAs.  Scans
+// of a few hundred channels and packed training were not among the shapes.
 // GPCs have 16 to 20 SMs, so large clusters leave some of them out.
 void scan_fit(const gdn2_scan_problem* p, int sms, int ctas, bool bwd, ScanPlan& l) {
   static constexpr struct { int size; double reach; } kClusters[] = {

@@ -152,7 +152,7 @@ def gated_scan(
     v: ``[B, T, ...]`` (float32, bfloat16 or float16); g, the log-decay, of
     v's shape in float32 or v's dtype (-inf cuts the past off; positive values
     grow the state, as long as the product of the decays of 128 rows stays
-    finite in float32); w of v's shape and dtype, or None for ones.
+    finite in float32, also where the state is zero); w of v's shape and dtype, or None for ones.
     ``initial_state`` and the returned final state (None unless
     ``output_final_state``) are float32 ``[N, ...]``.  With ``cu_seqlens``
     (``[N+1]``, from 0 to T, not decreasing; not checked on the device) B must
