@@ -460,6 +460,37 @@ typedef struct gdn2_adamw_tensor {
 int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensors,
                     int32_t n, void* stream);
 
+/* ---- norm of many gradients, and its clipping ------------------------------
+ * The norm of n tensors taken as one vector, 256 tensors per launch and one
+ * launch more:
+ *   norm = sqrt(sum g^2) (norm_type 2) or max |g| (norm_type 0)
+ *   coef = min(1, max_norm / (norm + 1e-6))
+ * out (fp32 [3], device): norm; coef, 1 for max_norm < 0 (none) and where norm is
+ * not finite; 1 where norm is not finite, else 0.  Tensors are contiguous, their
+ * dtypes may differ, a tensor may be listed twice and counts twice.  Sums are
+ * fp64 and their order is fixed: equal inputs give equal bits.  The workspace
+ * (gdn2_grad_norm_workspace_bytes, 8-byte aligned) belongs to one call at a time.
+ * gdn2_grad_scale multiplies the tensors in place by a device scalar, rounded
+ * once; a coefficient of 1 writes nothing.  Tensors that share memory are refused.
+ * The struct array is read before a call returns. */
+typedef struct gdn2_grad_problem {
+    int32_t norm_type;
+    double max_norm;
+} gdn2_grad_problem;
+
+typedef struct gdn2_grad_tensor {
+    void* data;
+    int64_t numel;
+    int64_t dtype;
+} gdn2_grad_tensor;
+
+size_t gdn2_grad_norm_workspace_bytes(int32_t n);
+int gdn2_grad_norm(const gdn2_grad_problem* p, const gdn2_grad_tensor* tensors,
+                   int32_t n, float* out, void* workspace, size_t workspace_bytes,
+                   void* stream);
+int gdn2_grad_scale(const gdn2_grad_tensor* tensors, int32_t n, const float* coef,
+                    void* stream);
+
 /* Device-side fault bits.  Kernels that wait on asynchronous copies or on
  * tensor-core completion bound every wait in time (about one second); a wait
  * that runs out makes the kernel release its tensor memory, return without

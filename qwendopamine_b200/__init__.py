@@ -10,9 +10,9 @@ given tokens (:func:`token_logprobs`) and the optimizer (:class:`AdamW`,
 """
 
 from .gdn2 import GDN2_BACKENDS, GatedDeltaNet2, RMSNormGated, ShortConvolution, resolve_gdn2_backend
-from .gdn2_ops import (AdamW, ChunkGDN2Function, adamw_step, chunk_gdn2, fused_recurrent_gdn2,
-                       fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step, TokenLogprobs,
-                       token_logprobs)
+from .gdn2_ops import (AdamW, ChunkGDN2Function, GradNorm, adamw_step, chunk_gdn2, clip_grad_norm_,
+                       fused_recurrent_gdn2, fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step,
+                       grad_norm, TokenLogprobs, token_logprobs)
 from .registry import BLOCKS, build_block
 
 __all__ = [
@@ -21,16 +21,19 @@ __all__ = [
     "ChunkGDN2Function",
     "GDN2_BACKENDS",
     "GatedDeltaNet2",
+    "GradNorm",
     "RMSNormGated",
     "ShortConvolution",
     "TokenLogprobs",
     "adamw_step",
     "build_block",
     "chunk_gdn2",
+    "clip_grad_norm_",
     "fused_recurrent_gdn2",
     "fused_recurrent_gdn2_fwd",
     "gated_scan",
     "gated_scan_step",
+    "grad_norm",
     "resolve_gdn2_backend",
     "token_logprobs",
 ]

@@ -56,6 +56,9 @@ EXPORTS = (
     "gdn2_logprob_fwd",
     "gdn2_logprob_bwd",
     "gdn2_adamw_step",
+    "gdn2_grad_norm_workspace_bytes",
+    "gdn2_grad_norm",
+    "gdn2_grad_scale",
     "gdn2_fault_status",
     "gdn2_test_fwd_state_wait_timeout",
     "gdn2_test_scan_wait_timeout",
@@ -185,6 +188,13 @@ class AdamWProblem(ctypes.Structure):
     ]
 
 
+class GradProblem(ctypes.Structure):
+    _fields_ = [
+        ("norm_type", c_int32),
+        ("max_norm", c_double),
+    ]
+
+
 # Sizes of sequences, states and tokens are 32-bit fields, to which ctypes cuts
 # larger numbers down without a word.
 INT32_MAX = 0x7FFFFFFF
@@ -215,6 +225,7 @@ def _declare(lib):
     sp = P(ScanProblem)
     lp = P(LogprobProblem)
     ap = P(AdamWProblem)
+    gp = P(GradProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -252,6 +263,9 @@ def _declare(lib):
         "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_grad_norm_workspace_bytes": ([c_int32], c_size_t),
+        "gdn2_grad_norm": ([gp, v, c_int32, v, v, c_size_t, v], ctypes.c_int),
+        "gdn2_grad_scale": ([v, c_int32, v, v], ctypes.c_int),
         "gdn2_adamw_step": ([ap, v, c_int32, v], ctypes.c_int),
         "gdn2_test_scan_wait_timeout": ([sp, v, v, v, v, v, v, v, ctypes.c_uint64, v],
                                         ctypes.c_int),

@@ -1,5 +1,5 @@
 // op_util.cuh -- helpers shared by the operators around the GDN-2 mixer
-// (scan.cu, logprob.cu, adamw.cu): error reporting at the C entries, element
+// (scan.cu, logprob.cu, adamw.cu, gradnorm.cu): error reporting at the C entries, element
 // groups of a row with or without vector access, and dtype dispatch.
 #pragma once
 
