@@ -460,6 +460,35 @@ typedef struct gdn2_adamw_tensor {
 int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensors,
                     int32_t n, void* stream);
 
+/* ---- a token from logits and a random number -------------------------------
+ * For each row x of logits [rows][vocab] (row r at element r * ld) one index,
+ * with w = exp((x - max x) / temperature):
+ *   1. min_p keeps w >= min_p (the maximum in any case);
+ *   2. top_k keeps the k largest of those (0: all);
+ *   3. top_p keeps of those, in falling order, up to the first whose running sum
+ *      reaches top_p of their sum; equal logits rank by rising index;
+ *   4. token_ids[r] is the lowest index whose running sum of kept weights, by
+ *      rising index, exceeds uniform[r] * (their sum).
+ * Weights and sums are fp64, equal inputs give equal tokens.  temperature,
+ * top_k, top_p, min_p: device arrays [rows] (fp32, int32), or NULL for the
+ * problem's value.  Temperature or top_p <= 0, or top_k = 1, take the first
+ * maximum; top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.  -inf logits are
+ * never taken; uniform counts as 0 below 0 and as 1 above 1, where the last kept
+ * index is taken.  -1 where there is no distribution: NaN or +inf among the
+ * logits, all of them -inf, or a NaN among uniform and the options. */
+typedef struct gdn2_sample_problem {
+    int64_t rows;
+    int64_t ld;
+    int32_t vocab;
+    int32_t dtype;
+    int64_t top_k;
+    double temperature, top_p, min_p;
+} gdn2_sample_problem;
+
+int gdn2_sample(const gdn2_sample_problem* p, const void* logits, const float* uniform,
+                const float* temperature, const int32_t* top_k, const float* top_p,
+                const float* min_p, int64_t* token_ids, void* stream);
+
 /* ---- norm of many gradients, and its clipping ------------------------------
  * The norm of n tensors taken as one vector, 256 tensors per launch and one
  * launch more:

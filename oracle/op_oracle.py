@@ -119,3 +119,28 @@ def adamw(p, g, m, v, step, lr, b1, b2, eps, wd):
     v = b2 * v + (1 - b2) * g * g
     mhat, vhat = m / (1 - b1 ** step), v / (1 - b2 ** step)
     return p - lr * wd * p - lr * mhat / (np.sqrt(vhat) + eps), m, v
+
+
+def sample_token(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Index taken from one row of logits by the uniform number u; -1 without a
+    distribution."""
+    x = np.asarray(x, dtype=np.float64)
+    if np.isnan(x).any() or x.max() in (np.inf, -np.inf):
+        return -1
+    order, top_k = np.argsort(-x, kind="stable"), int(top_k)
+    if temperature <= 0 or top_p <= 0 or top_k == 1:
+        return int(order[0])
+    w = np.exp((x - x.max()) / temperature)
+    n = int(np.isfinite(x).sum())
+    if min_p > 0:
+        n = max(1, int((w >= min(min_p, 1.0)).sum()))
+    if top_k > 0:
+        n = min(n, top_k)
+    if top_p < 1:
+        mass = np.concatenate([[0.0], np.cumsum(w[order[:n]])])
+        n = max(1, int((mass[:-1] < top_p * mass[-1]).sum()))
+    kept = np.zeros_like(w)
+    kept[order[:n]] = w[order[:n]]
+    run = np.cumsum(kept)
+    above = np.nonzero(run > min(max(u, 0.0), 1.0) * run[-1])[0]
+    return int(above[0]) if above.size else int(np.nonzero(kept)[0][-1])

@@ -56,6 +56,7 @@ EXPORTS = (
     "gdn2_logprob_fwd",
     "gdn2_logprob_bwd",
     "gdn2_adamw_step",
+    "gdn2_sample",
     "gdn2_grad_norm_workspace_bytes",
     "gdn2_grad_norm",
     "gdn2_grad_scale",
@@ -188,6 +189,19 @@ class AdamWProblem(ctypes.Structure):
     ]
 
 
+class SampleProblem(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int64),
+        ("ld", c_int64),
+        ("vocab", c_int32),
+        ("dtype", c_int32),
+        ("top_k", c_int64),
+        ("temperature", c_double),
+        ("top_p", c_double),
+        ("min_p", c_double),
+    ]
+
+
 class GradProblem(ctypes.Structure):
     _fields_ = [
         ("norm_type", c_int32),
@@ -226,6 +240,7 @@ def _declare(lib):
     lp = P(LogprobProblem)
     ap = P(AdamWProblem)
     gp = P(GradProblem)
+    tp = P(SampleProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -263,6 +278,7 @@ def _declare(lib):
         "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_sample": ([tp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_grad_norm_workspace_bytes": ([c_int32], c_size_t),
         "gdn2_grad_norm": ([gp, v, c_int32, v, v, c_size_t, v], ctypes.c_int),
         "gdn2_grad_scale": ([v, c_int32, v, v], ctypes.c_int),

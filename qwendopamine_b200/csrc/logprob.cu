@@ -82,83 +82,12 @@ __device__ __forceinline__ Soft merge(Soft a, Soft b, float c) {
   return Soft{m, a.s + b.s, a.w + b.w};
 }
 
-// Largest of the packed elements; a NaN does not count.
-template <typename T, int N> __device__ __forceinline__ float raw_max(const Raw<T, N>& r) {
-  if constexpr (sizeof(T) == 4) {
-    float m = __uint_as_float(r.u[0]);
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, __uint_as_float(r.u[i]));
-    return m;
-  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&r.u[0]);
-#pragma unroll
-    for (int i = 1; i < N / 2; ++i)
-      m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&r.u[i]));
-    const float2 f = __bfloat1622float2(m);
-    return fmaxf(f.x, f.y);
-  } else {
-    __half2 m = *reinterpret_cast<const __half2*>(&r.u[0]);
-#pragma unroll
-    for (int i = 1; i < N / 2; ++i) m = __hmax2(m, *reinterpret_cast<const __half2*>(&r.u[i]));
-    const float2 f = __half22float2(m);
-    return fmaxf(f.x, f.y);
-  }
-}
-
 template <typename T, int N> __device__ __forceinline__ float2 raw_pair(const Raw<T, N>& r, int i) {
   if constexpr (sizeof(T) == 4)
     return make_float2(__uint_as_float(r.u[2 * i]), __uint_as_float(r.u[2 * i + 1]));
   else
     return unpack2<T>(r.u[i]);
 }
-
-// Order-preserving map of a float to 32 bits; -0 counts as 0, NaN as least.
-__device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0u;
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float value_of(uint32_t o) {
-  if (o == 0u) return __uint_as_float(0x7fffffffu);
-  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
-}
-__device__ __forceinline__ uint64_t key_of(float x, int idx) {
-  return ((uint64_t)order_of(x) << 32) | (uint32_t)~(uint32_t)idx;
-}
-
-// A row as aligned 16-byte vectors: vector j holds the elements j*VE - off
-// .. j*VE - off + VE - 1 of which those in [0, V) exist.
-template <typename T> struct RowView {
-  static constexpr int VE = 16 / (int)sizeof(T);
-  const T* base;  // element -off
-  int off, V, nvec;
-  __device__ __forceinline__ RowView(const T* row, int v) : V(v) {
-    off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    base = row - off;
-    nvec = (int)(((int64_t)V + off + VE - 1) / VE);
-  }
-  __device__ __forceinline__ bool whole(int j) const {
-    return (j > 0 || off == 0) && (int64_t)(j + 1) * VE - off <= V;
-  }
-  // absent elements, and all of a vector that is not below `hi`, read as -inf
-  __device__ __forceinline__ Raw<T, VE> load(int j, int hi) const {
-    if (j < hi) return load(j);
-    float f[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) f[e] = -INFINITY;
-    return raw_from<T, VE>(f);
-  }
-  __device__ __forceinline__ Raw<T, VE> load(int j) const {
-    if (whole(j)) return load_raw<T, VE>(base + (int64_t)j * VE);
-    float f[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const int64_t i = (int64_t)j * VE + e - off;
-      f[e] = i >= 0 && i < V ? to_f<T>(base[(int64_t)j * VE + e]) : -INFINITY;
-    }
-    return raw_from<T, VE>(f);
-  }
-};
 
 struct LogprobShared {
   float warp_max[kLpWarps];

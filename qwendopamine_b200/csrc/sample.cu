@@ -1,0 +1,708 @@
+// sample.cu -- one token for each row of logits from one given random number.
+//
+// Mathematics, with m = max x and w_i = exp((x_i - m) / temperature) = 2^y_i:
+//   kept by min-p:  w_i >= min_p;   by top-k: the k largest of those;
+//   by top-p: of what is left, in falling order, up to the first running sum
+//   that reaches top_p of the sum;  equal logits rank by rising index
+//   token = the lowest index whose running sum of kept weights, in the order of
+//   the vocabulary, exceeds uniform * (their sum).
+//
+// A token far down the vocabulary may hold a millionth of the sum, so whether
+// the running sum has passed the target is decided by digits that fp32 does not
+// have: weights and sums are fp64 (2^y from a table of 16 roots and the Taylor
+// polynomial of 2^f, |f| <= 1/32, to f^5: 2e-13 relative).  Sums are formed in a
+// fixed order or as whole numbers: equal inputs give equal tokens.
+//
+// Top-k and top-p need no sort of the row.  A histogram over bins of equal width
+// in x (counts, and weights as whole numbers of 2^-44) gives the bin in which the
+// bound lies; what is in the bin, or all down to it where that is a short list,
+// is sorted in shared memory.  A bin with more values than the list holds is cut
+// by the digits of the values' ordered bits, 11 at a time, and among equal values
+// the lower indices are counted out.
+//
+// Bound: by temperature alone the row is read once and the time is that of the
+// fp64 pipe, 11 operations for a value; with a bound the row is read again from
+// L2 for the histogram, the list and the sums.  Few rows are split over the CTAs
+// of a cluster, which exchange through distributed shared memory.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "mma16.cuh"
+#include "op_util.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace gdn2 {
+namespace {
+
+constexpr int kSmThreads = 512;
+constexpr int kSmWarps = kSmThreads / 32;
+constexpr int kSmUnroll = 4;                   // vectors of a lane in flight
+constexpr int kBins = 2048;
+constexpr int kBinsPer = kBins / kSmThreads;   // bins of a thread
+constexpr int kList = 2048;                    // longest list that is sorted
+constexpr float kBinsPerUnit = 46.f;           // bins of a logit: 44 units below the maximum
+
+struct SampleArgs {
+  int64_t rows, ld;
+  int V;
+  double weight_unit;  // 2^(52 - s), with weights counted in 2^-s
+  const void* x;
+  const float *uniform, *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  double temperature1, top_p1, min_p1;  // for all rows, where there is no pointer
+  int64_t top_k1;
+  int64_t* ids;
+};
+
+// What the cluster agrees on; the leader's copy counts.
+struct Decision {
+  uint64_t bound;    // keys of at least this are kept
+  int bin;           // of the histogram that holds the bound, -1 where none does
+  uint32_t above, in;          // values above the bin and in it
+  uint64_t mass_above, mass;   // weights above the bin, and in all
+  int64_t at;        // index found
+};
+
+struct SampleShared {
+  double root[16];               // 2^(i/16)
+  double warp_sum[kSmWarps];
+  double total;                  // of this CTA
+  uint32_t warp_max[kSmWarps], warp_bad[kSmWarps];
+  uint32_t most, bad;            // of this CTA: the maximum's key, whether there is a NaN
+  uint32_t warp_count[kSmWarps];
+  uint64_t warp_mass[kSmWarps];
+  Decision d;
+  int n_list;
+  uint32_t count[kBins];
+  uint64_t mass[kBins];
+  uint64_t list[kList];
+};
+
+// 2^y for y <= 0 as fp64; 0 below 2^-1022, and for -inf
+__device__ __forceinline__ double pow2_of(const double* root, double y) {
+  constexpr double magic = 6755399441055744.;  // 1.5 * 2^52: rounds to whole numbers
+  constexpr double c1 = 0.69314718055994531, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
+                   c5 = c4 * c1 / 5;
+  const double t = fma(y, 16., magic);
+  const int k = __double2loint(t);
+  const double f = fma(t - magic, -.0625, y);
+  double p = fma(fma(fma(fma(fma(c5, f, c4), f, c3), f, c2), f, c1), f, 1.);
+  p *= root[k & 15];
+  const double w = __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
+  return y >= -1022. ? w : 0.;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(uint32_t w, float) { return w & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t abs_bits(uint32_t w, __nv_bfloat16) { return w & 0x7fff7fffu; }
+__device__ __forceinline__ uint32_t abs_bits(uint32_t w, __half) { return w & 0x7fff7fffu; }
+
+// Largest magnitude's bits, NaN above infinity (two 16-bit halves, or one word).
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest_bits(const Raw<T, N>& r, uint32_t most) {
+#pragma unroll
+  for (int i = 0; i < Raw<T, N>::kWords; ++i) {
+    const uint32_t b = abs_bits(r.u[i], T{});
+    if constexpr (sizeof(T) == 4) most = max(most, b);
+    else most = __vmaxu2(most, b);
+  }
+  return most;
+}
+template <typename T> __device__ __forceinline__ bool bits_are_nan(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m > 0x7f800000u;
+  else {
+    constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return (m & 0xffffu) > inf || (m >> 16) > inf;
+  }
+}
+
+// Row r of a CTA of a cluster: the vectors [lo, hi) of its warp, in the order of
+// the row (parts, then warps).
+template <typename T> struct RowShare {
+  RowView<T> row;
+  int lo, hi, part, parts;
+  static constexpr int VE = RowView<T>::VE;
+  __device__ __forceinline__ RowShare(const T* p, int V, int part_, int parts_)
+      : row(p, V), part(part_), parts(parts_) {
+    const int per = (row.nvec + parts - 1) / parts;
+    const int plo = min(part * per, row.nvec), phi = min(plo + per, row.nvec);
+    const int wper = (phi - plo + kSmWarps - 1) / kSmWarps;
+    lo = min(plo + (int)(threadIdx.x >> 5) * wper, phi);
+    hi = min(lo + wper, phi);
+  }
+  __device__ __forceinline__ int64_t index(int j, int e) const { return (int64_t)j * VE + e - row.off; }
+  // f(vector, its place) for the lane's vectors of the warp's
+  template <typename F> __device__ __forceinline__ void sweep(F&& f) const {
+    const int lane = threadIdx.x & 31;
+    int j = lo + lane;
+    for (; j + (kSmUnroll - 1) * 32 < hi; j += kSmUnroll * 32) {
+      Raw<T, VE> v[kSmUnroll];
+#pragma unroll
+      for (int u = 0; u < kSmUnroll; ++u) v[u] = row.load(j + u * 32);
+#pragma unroll
+      for (int u = 0; u < kSmUnroll; ++u) f(v[u], j + u * 32);
+    }
+    for (; j < hi; j += 32) f(row.load(j), j);
+  }
+};
+
+__device__ __forceinline__ double warp_total(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// The parameters of one row, and which values they keep.
+struct RowRule {
+  float m;
+  double c, min_y;   // weights 2^((x - m) c); kept from y = min_y
+  uint64_t bound;    // and from this key
+  float tau;         // the bound's value
+  bool all_y, all_keys;
+  const double* root;
+  __device__ __forceinline__ double weight(float x) const { return pow2_of(root, ((double)x - m) * c); }
+  __device__ __forceinline__ bool keeps(float x, int64_t i) const {
+    if (x == -INFINITY) return false;
+    if (!all_keys && !(x > tau) && (x < tau || key_of(x, (int)i) < bound)) return false;
+    return all_y || ((double)x - m) * c >= min_y;
+  }
+};
+
+// The index at which the running sum of f(x, index) >= 0 over the row, in fp64,
+// exceeds target(sum); where rounding leaves none, the last with f > 0.  The
+// result is in the leader's d.at.  The warps' sums are given in s.warp_sum if
+// `have`.  Called by all threads of the cluster.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void locate(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
+                                       bool have, F&& f, G&& target) {
+  constexpr int VE = RowView<T>::VE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!have) {
+    double mine = 0.;
+    sh.sweep([&](const Raw<T, VE>& v, int j) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mine += f(raw_get(v, e), sh.index(j, e));
+    });
+    mine = warp_total(mine);
+    if (lane == 0) s.warp_sum[warp] = mine;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    double t = 0.;
+    for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
+    s.total = t;
+    s.d.at = -1;
+  }
+  cluster.sync();
+  double before = 0., sum = 0.;
+  int owner = -1, last = 0;  // the part with the target, the last that has a weight
+  for (int q = 0; q < sh.parts; ++q) sum += *cluster.map_shared_rank(&s.total, q);
+  const double goal = target(sum);
+  double run = 0.;
+  for (int q = 0; q < sh.parts; ++q) {
+    const double t = *cluster.map_shared_rank(&s.total, q);
+    if (t > 0.) last = q;
+    if (owner < 0 && run + t > goal && t > 0.) { owner = q; before = run; }
+    run += t;
+  }
+  bool none = owner < 0;
+  if (none) owner = last;
+  if (owner == sh.part) {
+    // the warp with the target, by the same sums in the same order
+    int who = -1, some = 0;
+    double at = before;
+    if (!none) {
+      double r = before;
+      for (int i = 0; i < kSmWarps; ++i) {
+        const double t = s.warp_sum[i];
+        if (who < 0 && t > 0. && r + t > goal) { who = i; at = r; }
+        r += t;
+      }
+    }
+    for (int i = 0; i < kSmWarps; ++i)
+      if (s.warp_sum[i] > 0.) some = i;
+    if (who < 0) {
+      who = some;
+      none = true;
+    }
+    if (warp == who) {
+      int64_t found = -1, tail = -1;  // tail: the last index with a weight
+      for (int j0 = sh.lo; j0 < sh.hi && found < 0; j0 += 32) {
+        const int j = j0 + lane;
+        Raw<T, VE> v;
+        double mine = 0.;
+        int64_t mytail = -1;
+        if (j < sh.hi) {
+          v = sh.row.load(j);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const double w = f(raw_get(v, e), sh.index(j, e));
+            if (w > 0.) mytail = sh.index(j, e);
+            mine += w;
+          }
+        }
+        double incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const double y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, !none && mine > 0. && at + incl > goal);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          int64_t mineat = -1;
+          if (lane == l) {
+            double r = at + (incl - mine);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const double w = f(raw_get(v, e), sh.index(j, e));
+              r += w;
+              if (mineat < 0 && w > 0. && r > goal) mineat = sh.index(j, e);
+            }
+            if (mineat < 0) mineat = mytail;
+          }
+          found = __shfl_sync(0xffffffffu, mineat, l);
+        }
+        const unsigned has = __ballot_sync(0xffffffffu, mytail >= 0);
+        if (has) tail = __shfl_sync(0xffffffffu, mytail, 31 - __clz(has));
+        at += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) cluster.map_shared_rank(&s.d, 0)->at = found >= 0 ? found : tail;
+    }
+  }
+  cluster.sync();
+}
+
+// Adds the parts' histograms into the leader's and finds the first bin at which
+// the running count reaches k (MASS false) or the running weight share * (all).
+template <bool MASS>
+__device__ __forceinline__ void find_bin(cg::cluster_group& cluster, SampleShared& s, int part, int parts,
+                                         uint32_t k, double share, uint32_t above0, uint64_t mass0,
+                                         uint64_t mass_all) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster.sync();  // histograms complete
+  if (part == 0) {
+    uint32_t c[kBinsPer], cs = 0u;
+    uint64_t w[kBinsPer], ws = 0u;
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) {
+      const int b = tid * kBinsPer + i;
+      c[i] = s.count[b];
+      w[i] = s.mass[b];
+    }
+    for (int q = 1; q < parts; ++q) {
+      const SampleShared* o = cluster.map_shared_rank(&s, q);
+#pragma unroll
+      for (int i = 0; i < kBinsPer; ++i) {
+        c[i] += o->count[tid * kBinsPer + i];
+        w[i] += o->mass[tid * kBinsPer + i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) {
+      cs += c[i];
+      ws += w[i];
+    }
+    uint32_t ci = cs;
+    uint64_t wi = ws;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t a = __shfl_up_sync(0xffffffffu, ci, o);
+      const uint64_t b = __shfl_up_sync(0xffffffffu, wi, o);
+      if (lane >= o) { ci += a; wi += b; }
+    }
+    if (lane == 31) { s.warp_count[warp] = ci; s.warp_mass[warp] = wi; }
+    if (tid == 0) s.d.bin = -1;
+    __syncthreads();
+    uint32_t cb = above0, call = above0;
+    uint64_t wb = mass0, wall = mass0;
+    for (int i = 0; i < kSmWarps; ++i) {
+      if (i < warp) { cb += s.warp_count[i]; wb += s.warp_mass[i]; }
+      call += s.warp_count[i];
+      wall += s.warp_mass[i];
+    }
+    cb += ci - cs;
+    wb += wi - ws;
+    // whole numbers up to 2^62 as fp64: the bound moves by 2^-53 of itself at most
+    const uint64_t all = mass_all ? mass_all : wall;
+    const double goal = share * (double)all;
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) {
+      const bool here = MASS ? (double)wb < goal && (double)(wb + w[i]) >= goal
+                             : cb < k && cb + c[i] >= k;
+      if (here) {  // one bin of all
+        s.d.bin = tid * kBinsPer + i;
+        s.d.above = cb;
+        s.d.mass_above = wb;
+        s.d.in = c[i];
+      }
+      cb += c[i];
+      wb += w[i];
+    }
+    if (tid == 0) s.d.mass = all;
+  }
+  cluster.sync();
+}
+
+// Sorts s.list[0 .. n) in falling order (bitonic).
+__device__ __forceinline__ void sort_list(SampleShared& s, int n) {
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = threadIdx.x + n; i < size; i += kSmThreads) s.list[i] = 0u;
+  for (int k = 2; k <= size; k *= 2)
+    for (int o = k / 2; o > 0; o /= 2) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += kSmThreads) {
+        const int a = 2 * i - (i & (o - 1)), b = a + o;
+        const uint64_t x = s.list[a], y = s.list[b];
+        if ((x < y) == ((a & k) == 0)) { s.list[a] = y; s.list[b] = x; }
+      }
+    }
+  __syncthreads();
+}
+
+// A weight as a whole number of 2^-s (unit = 2^(52 - s)).
+__device__ __forceinline__ uint64_t whole_weight(double w, double unit) {
+  return (uint64_t)__double_as_longlong(w + unit) & 0xfffffffffffffull;
+}
+
+// Of the first n of the sorted list, how many are kept while the weights before
+// them, on top of `above`, are below share * all (all = 0: the list's own weight);
+// at least one.  Called by all threads of the leader.
+__device__ __forceinline__ int count_by_mass(SampleShared& s, int n, uint64_t above, double share,
+                                             uint64_t all, const RowRule& rule, double unit) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int per = kList / kSmThreads;
+  uint64_t w[per], ws = 0u;
+#pragma unroll
+  for (int i = 0; i < per; ++i) {
+    const int at = tid * per + i;
+    w[i] = at < n ? whole_weight(rule.weight(value_of((uint32_t)(s.list[at] >> 32))), unit) : 0u;
+    ws += w[i];
+  }
+  uint64_t before = ws;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const uint64_t b = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += b;
+  }
+  if (lane == 31) s.warp_mass[warp] = before;
+  __syncthreads();
+  before += above - ws;
+  uint64_t own = 0u;
+  for (int i = 0; i < kSmWarps; ++i) {
+    if (i < warp) before += s.warp_mass[i];
+    own += s.warp_mass[i];
+  }
+  const double goal = share * (double)(all ? all : own);
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < per; ++i) {
+    kept += tid * per + i < n && (tid * per + i == 0 || (double)before < goal);
+    before += w[i];
+  }
+  kept = __reduce_add_sync(0xffffffffu, kept);
+  if (lane == 0) s.warp_count[warp] = (uint32_t)kept;
+  __syncthreads();
+  kept = 0;
+  for (int i = 0; i < kSmWarps; ++i) kept += (int)s.warp_count[i];
+  return kept;
+}
+
+// Narrows rule.bound to the k largest kept values (MASS false), or to those whose
+// weight before them is below share * (all).  With then_share < 1 the second
+// follows the first, if a list serves both; returns whether it did.
+template <typename T, bool MASS>
+__device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
+                                       const SampleArgs& a, RowRule& rule, int64_t k, double share,
+                                       double then_share) {
+  constexpr int VE = RowView<T>::VE;
+  const int tid = threadIdx.x;
+  SampleShared* lead = cluster.map_shared_rank(&s, 0);
+  // falling values have rising bins; the same function wherever a bin is asked for
+  auto bin_of = [&](float x) { return min((int)(__fmul_rn(__fsub_rn(rule.m, x), kBinsPerUnit)), kBins - 1); };
+  int bin = -1, shift = 32;   // the bin that was cut, the bits of `prefix` are those above shift
+  uint32_t prefix = 0u, above = 0u;
+  uint64_t mass_above = 0u, mass_all = 0u;
+  for (int round = 0;; ++round) {
+    // round 0: bins of equal width; then digits of the ordered bits, in the bin
+    const int width = round == 3 ? 10 : 11;
+    if (round > 0) shift -= width;
+    for (int i = tid; i < kBins; i += kSmThreads) { s.count[i] = 0u; s.mass[i] = 0u; }
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    sh.sweep([&](const Raw<T, VE>& v, int j) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float x = raw_get(v, e);
+        if (!rule.keeps(x, sh.index(j, e))) continue;
+        int b = bin_of(x);
+        if (round > 0) {
+          if (b != bin) continue;
+          const uint32_t o = order_of(x);
+          if (round > 1 && (o >> (shift + width)) != prefix) continue;
+          b = (1 << width) - 1 - (int)((o >> shift) & ((1u << width) - 1u));
+        }
+        atomicAdd(&s.count[b], 1u);
+        if constexpr (MASS)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]),
+                    (unsigned long long)whole_weight(rule.weight(x), a.weight_unit));
+      }
+    });
+    __syncthreads();
+    find_bin<MASS>(cluster, s, sh.part, sh.parts, (uint32_t)min(k, (int64_t)0x7fffffff), share, above,
+                   mass_above, mass_all);
+    const int b = lead->d.bin;
+    if (b < 0) {  // fewer values than k: all are kept
+      cluster.sync();
+      return false;
+    }
+    above = lead->d.above;
+    mass_above = lead->d.mass_above;
+    mass_all = lead->d.mass;
+    const uint32_t in = lead->d.in;
+    const bool whole = round == 0 && above + in <= kList;  // all down to the bin as one list
+    if (whole || in <= kList) {
+      sh.sweep([&](const Raw<T, VE>& v, int j) {
+        const float most = raw_max(v);
+        if (most == -INFINITY || (round == 0 ? bin_of(most) > b : bin_of(most) > bin)) return;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float x = raw_get(v, e);
+          if (!rule.keeps(x, sh.index(j, e))) continue;
+          const int c = bin_of(x);
+          if (round == 0) {
+            if (c > b || (!whole && c < b)) continue;
+          } else {
+            if (c != bin) continue;
+            const uint32_t o = order_of(x);
+            if (round > 1 && (o >> (shift + width)) != prefix) continue;
+            if ((1 << width) - 1 - (int)((o >> shift) & ((1u << width) - 1u)) != b) continue;
+          }
+          const int at = atomicAdd(&lead->n_list, 1);  // as many as were counted
+          if (at < kList) lead->list[at] = key_of(x, (int)sh.index(j, e));
+        }
+      });
+      cluster.sync();
+      if (sh.part == 0) {
+        const int n = min(s.n_list, kList);
+        sort_list(s, n);
+        if (whole) above = 0u;
+        int kept;
+        if constexpr (MASS) {
+          kept = count_by_mass(s, n, whole ? 0u : mass_above, share, mass_all, rule, a.weight_unit);
+        } else {
+          kept = (int)min(k - above, (int64_t)n);
+          if (whole && then_share < 1.)
+            kept = count_by_mass(s, kept, 0u, then_share, 0u, rule, a.weight_unit);
+        }
+        if (tid == 0) s.d.bound = s.list[kept - 1];
+      }
+      cluster.sync();
+      rule.bound = lead->d.bound;
+      rule.tau = value_of((uint32_t)(rule.bound >> 32));
+      rule.all_keys = false;
+      cluster.sync();
+      return whole;
+    }
+    if (round == 0) {
+      bin = b;
+    } else {
+      prefix = (round == 1 ? 0u : prefix << width) | (uint32_t)((1 << width) - 1 - b);
+    }
+    cluster.sync();  // the decision has been read
+    if (round == 3) {
+      // `in` values are equal: the first of them by index are kept
+      const float x0 = value_of(prefix);
+      int64_t need;
+      if constexpr (MASS) {
+        const double w = (double)whole_weight(rule.weight(x0), a.weight_unit);
+        const double left = share * (double)mass_all - (double)mass_above;
+        need = w > 0. ? (int64_t)fmin(ceil(left / w), (double)in) : (int64_t)in;
+      } else {
+        need = k - above;
+      }
+      if (need < 1) need = 1;
+      locate<T>(cluster, s, sh, false,
+                [&](float x, int64_t i) { return x == x0 && rule.keeps(x, i) ? 1. : 0.; },
+                [&](double) { return (double)need - .5; });
+      rule.bound = key_of(x0, (int)lead->d.at);
+      rule.tau = x0;
+      rule.all_keys = false;
+      cluster.sync();
+      return false;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, const int parts) {
+  constexpr int VE = RowView<T>::VE;
+  __shared__ SampleShared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - r * parts);
+  const RowShare<T> sh((const T*)a.x + r * a.ld, a.V, part, parts);
+  const double temperature = a.temperature ? (double)a.temperature[r] : a.temperature1;
+  const double top_p = a.top_p ? (double)a.top_p[r] : a.top_p1;
+  const double min_p = a.min_p ? (double)a.min_p[r] : a.min_p1;
+  const int64_t top_k = a.top_k ? (int64_t)a.top_k[r] : a.top_k1;
+  const float uniform = a.uniform[r];
+  const bool greedy = temperature <= 0. || top_k == 1 || top_p <= 0.;
+  const bool by_k = !greedy && top_k > 1 && top_k < a.V, by_p = !greedy && top_p < 1.;
+  const bool by_min = !greedy && min_p > 0.;
+  if (tid < 16) s.root[tid] = exp2(tid / 16.);
+  __syncthreads();
+
+  // The row's maximum; where nothing is cut off, the weights' sums with it, each
+  // lane's in units of its own running maximum.
+  // (a factor of at most 1e300 keeps the maximum's weight at 2^0)
+  RowRule rule{0.f, fmin(1.4426950408889634 / temperature, 1e300), 0., 0u, -INFINITY, true, true, s.root};
+  const bool at_once = !greedy && !by_k && !by_p && !by_min;
+  float mine = -INFINITY;
+  double sum = 0.;
+  uint32_t bits = 0u;
+  sh.sweep([&](const Raw<T, VE>& v, int) {
+    bits = largest_bits(v, bits);
+    const float top = raw_max(v);
+    if (at_once) {
+      if (top > mine) {
+        if (sum > 0.) sum *= pow2_of(s.root, ((double)mine - top) * rule.c);
+        mine = top;
+      }
+      if (mine != -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) sum += pow2_of(s.root, ((double)raw_get(v, e) - mine) * rule.c);
+      }
+    } else {
+      mine = fmaxf(mine, top);
+    }
+  });
+  // absent elements read as -inf, whose bits are those of infinity
+  const bool nan = bits_are_nan<T>(bits);
+  {
+    const uint32_t o = __reduce_max_sync(0xffffffffu, order_of(mine));
+    const unsigned bad = __ballot_sync(0xffffffffu, nan);
+    if (lane == 0) { s.warp_max[warp] = o; s.warp_bad[warp] = bad; }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t o = 0u, bad = 0u;
+    for (int i = 0; i < kSmWarps; ++i) { o = max(o, s.warp_max[i]); bad |= s.warp_bad[i]; }
+    s.most = o;
+    s.bad = bad;
+  }
+  cluster.sync();
+  uint32_t most = 0u, bad = 0u;
+  for (int q = 0; q < parts; ++q) {
+    most = max(most, *cluster.map_shared_rank(&s.most, q));
+    bad |= *cluster.map_shared_rank(&s.bad, q);
+  }
+  cluster.sync();
+  rule.m = value_of(most);
+  // no distribution: NaN, +inf, nothing but -inf, or options that are NaN
+  if (bad || rule.m == INFINITY || rule.m == -INFINITY || temperature != temperature || top_p != top_p ||
+      min_p != min_p || uniform != uniform) {
+    if (part == 0 && tid == 0) a.ids[r] = -1;
+    return;
+  }
+
+  if (greedy) {  // the first index of the maximum
+    locate<T>(cluster, s, sh, false, [&](float x, int64_t) { return x == rule.m ? 1. : 0.; },
+              [](double) { return 0.; });
+  } else {
+    if (by_min) {
+      rule.all_y = false;
+      rule.min_y = min_p < 1. ? log2(min_p) : 0.;
+    }
+    bool done = false;
+    if (by_k) done = narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1.);
+    if (by_p && !done) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
+    if (at_once) {
+      const double f = mine == -INFINITY ? 0. : pow2_of(s.root, ((double)mine - rule.m) * rule.c);
+      sum = warp_total(sum * f);
+      if (lane == 0) s.warp_sum[warp] = sum;
+    }
+    const double u = fmin(fmax((double)uniform, 0.), 1.);
+    locate<T>(cluster, s, sh, at_once,
+              [&](float x, int64_t i) { return rule.keeps(x, i) ? rule.weight(x) : 0.; },
+              [&](double w) { return u * w; });
+  }
+  if (part == 0 && tid == 0) a.ids[r] = s.d.at;
+}
+
+// ---------------------------------------------------------------------------
+// entry point
+// ---------------------------------------------------------------------------
+template <typename T> cudaError_t launch_sample(const SampleArgs& a, int parts, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(a.rows * parts));
+  cfg.blockDim = dim3(kSmThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)parts;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_sample<T>, a, parts);
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+int gdn2_sample(const gdn2_sample_problem* p, const void* logits, const float* uniform,
+                const float* temperature, const int32_t* top_k, const float* top_p,
+                const float* min_p, int64_t* token_ids, void* stream) {
+  const char* fn = "gdn2_sample";
+  if (!p) return fail(GDN2_ERR_INVALID, "%s: null problem", fn);
+  if (p->rows < 0 || p->vocab <= 0)
+    return fail(GDN2_ERR_INVALID, "%s: needs rows >= 0 and vocab > 0 (got %lld, %d)", fn,
+                (long long)p->rows, p->vocab);
+  if (!dtype_valid(p->dtype)) return fail(GDN2_ERR_INVALID, "%s: unknown dtype %d", fn, p->dtype);
+  if (p->ld < p->vocab)
+    return fail(GDN2_ERR_INVALID, "%s: the row stride must be at least vocab", fn);
+  if (!(temperature || (p->temperature >= 0. && std::isfinite(p->temperature))) ||
+      !(top_k || p->top_k >= 0) || !(top_p || (p->top_p >= 0. && p->top_p <= 1.)) ||
+      !(min_p || (p->min_p >= 0. && p->min_p <= 1.)))
+    return fail(GDN2_ERR_INVALID,
+                "%s: needs a finite temperature >= 0, top_k >= 0, top_p and min_p in [0, 1]", fn);
+  // CTAs of a row: one where the rows fill the GPU, else as many (2, 4, 8) as keep
+  // the grid within two CTAs per SM and 16 KB for each
+  int sms = 0, parts = 1;
+  if (p->rows > 2147483647LL / 8) return fail(GDN2_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  if (p->rows == 0) return GDN2_OK;
+  if (!logits || !uniform || !token_ids) return fail(GDN2_ERR_INVALID, "%s: null pointer", fn);
+  if (!aligned_to(logits, dtype_size(p->dtype)))
+    return fail(GDN2_ERR_INVALID, "%s: logits are not aligned to their elements", fn);
+  const cudaError_t e = num_sms(&sms);
+  if (e != cudaSuccess) return cuda_status(e, fn);
+  const int64_t row_bytes = (int64_t)p->vocab * (int64_t)dtype_size(p->dtype);
+  while (parts < 8 && p->rows * parts * 2 <= 2 * sms && row_bytes / (parts * 2) >= 16384) parts *= 2;
+  SampleArgs a{};
+  a.rows = p->rows;
+  a.ld = p->ld;
+  a.V = p->vocab;
+  // sums of vocab weights of at most 2^s stay below 2^63
+  int bits = 1;
+  while (bits < 31 && (1LL << bits) <= p->vocab) ++bits;
+  a.weight_unit = std::ldexp(1., 52 - std::min(44, 62 - bits));
+  a.x = logits; a.uniform = uniform; a.temperature = temperature; a.top_k = top_k;
+  a.top_p = top_p; a.min_p = min_p;
+  a.temperature1 = p->temperature; a.top_k1 = p->top_k; a.top_p1 = p->top_p; a.min_p1 = p->min_p;
+  a.ids = token_ids;
+  const cudaStream_t st = (cudaStream_t)stream;
+  return cuda_status(with_dtype(p->dtype, [&](auto t) {
+    return launch_sample<decltype(t)>(a, parts, st);
+  }), fn);
+}
+
+}  // extern "C"
