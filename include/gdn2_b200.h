@@ -460,6 +460,63 @@ typedef struct gdn2_adamw_tensor {
 int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensors,
                     int32_t n, void* stream);
 
+/* ---- selective state space scan ----------------------------------------------
+ * N states for each channel, over the rows [B][T] (or packed sequences, B = 1),
+ * with d = dt + dt_bias, and its softplus where dt_softplus is set:
+ *   h_t[n] = exp(d_t A[n]) h_{t-1}[n] + d_t x_t B_t[n]
+ *   y_t = (sum_n h_t[n] C_t[n] + D x_t) silu(z_t)      rounded to `dtype`
+ * x, z, y, B, C have `dtype`, dt has `dt_dtype` (`dtype` or fp32); A [D][N], D and
+ * dt_bias [D] (or NULL) and states [n_seqs][D][N] are fp32; z NULL stands for no
+ * gate, h0 NULL for zero, ht (or NULL) receives the states after the last tokens.
+ * The channels are G groups of D / G neighbours, and each group has its own N
+ * values in a row [G][N] of B and C.  N <= 64.  Row r = b*T + t of a tensor starts at
+ * element r * ld_* (up to 2^22); y and the gradients are contiguous.  cu_seqlens
+ * (int32 [n_seqs+1], device) starts at 0, ends at T and does not decrease; n_seqs =
+ * B without it.  A sequence without tokens passes its state on.
+ * Where the time axis is cut (few channels and sequences), a chunk's decays are
+ * composed before they are applied: with d A > 0 their product over a chunk has
+ * to stay finite in fp32.
+ * Backward: dy of y and dht (or NULL) of ht give the gradients; dD, ddt_bias and
+ * dh0 may be NULL, dz where there is no z; dA, dD, ddt_bias, dh0 are fp32, the
+ * others have their tensor's dtype.  `saved` (gdn2_selective_saved_bytes, 16-byte
+ * aligned) is what the forward of the same inputs wrote, one state in front of
+ * every 16 rows; a forward with saved NULL keeps nothing.  The workspace
+ * (gdn2_selective_workspace_bytes, 16-byte aligned) belongs to one call at a time.
+ * The order of all sums is fixed: equal inputs give equal bits. */
+typedef struct gdn2_selective_problem {
+    int32_t B, D, G, N;
+    int64_t T;
+    int32_t dtype, dt_dtype;
+    int32_t dt_softplus;
+    int32_t n_seqs;
+    const int32_t* cu_seqlens;
+    int64_t ld_x, ld_dt, ld_z, ld_b, ld_c, ld_dy;  /* row strides in elements */
+} gdn2_selective_problem;
+
+size_t gdn2_selective_saved_bytes(const gdn2_selective_problem* p);
+size_t gdn2_selective_workspace_bytes(const gdn2_selective_problem* p, int32_t backward);
+int gdn2_selective_fwd(const gdn2_selective_problem* p, const void* x, const void* dt,
+                       const float* A, const void* B, const void* C, const float* D,
+                       const void* z, const float* dt_bias, const float* h0, void* y,
+                       float* ht, float* saved, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int gdn2_selective_bwd(const gdn2_selective_problem* p, const void* x, const void* dt,
+                       const float* A, const void* B, const void* C, const float* D,
+                       const void* z, const float* dt_bias, const float* h0,
+                       const float* saved, const void* dy, const float* dht, void* dx,
+                       void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
+                       float* ddt_bias, float* dh0, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* One token for each of B sequences (T = 1) on a pool of states [pool][D][N],
+ * `state_stride` elements apart, updated in place: sequence b uses the row
+ * state_indices[b] (row b when NULL).  An index outside [0, pool) marks padding: no
+ * state changes and its y is zero.  Two sequences must not name the same row. */
+int gdn2_selective_step(const gdn2_selective_problem* p, const void* x, const void* dt,
+                        const float* A, const void* B, const void* C, const float* D,
+                        const void* z, const float* dt_bias, float* state,
+                        int64_t state_stride, int32_t pool,
+                        const int32_t* state_indices, void* y, void* stream);
+
 /* ---- a token from logits and a random number -------------------------------
  * For each row x of logits [rows][vocab] (row r at element r * ld) one index,
  * with w = exp((x - max x) / temperature):

@@ -144,3 +144,65 @@ def sample_token(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     run = np.cumsum(kept)
     above = np.nonzero(run > min(max(u, 0.0), 1.0) * run[-1])[0]
     return int(above[0]) if above.size else int(np.nonzero(kept)[0][-1])
+
+
+def softplus(v):
+    return np.maximum(v, 0) + np.log1p(np.exp(-np.abs(v)))
+
+
+def _selective(x, dt, A, B, C, D, z, bias, plus, h0, cu):
+    """Inputs of the selective scan with its defaults filled in, B and C for each
+    channel [B, T, D, N]."""
+    nb, T, d = x.shape
+    pre = dt if bias is None else dt + bias
+    delta = softplus(pre) if plus else pre
+    if B.ndim == 3:
+        B, C = B[:, :, None], C[:, :, None]
+    wide = lambda v: np.repeat(v, d // v.shape[2], axis=2)
+    seqs = _sequences(nb, T, cu)
+    h0 = np.zeros((len(seqs), d, A.shape[1])) if h0 is None else np.array(h0, dtype=np.float64)
+    skip = np.zeros(d) if D is None else D
+    return pre, delta, wide(B), wide(C), skip, seqs, h0
+
+
+def selective_fwd(x, dt, A, B, C, D=None, z=None, bias=None, plus=False, h0=None, cu=None):
+    """(y, states after every token, final states) of the selective state space scan."""
+    _, delta, Bw, Cw, skip, seqs, ht = _selective(x, dt, A, B, C, D, z, bias, plus, h0, cu)
+    H = np.zeros((*x.shape, A.shape[1]))
+    for n, (b, lo, hi) in enumerate(seqs):
+        h = ht[n].copy()
+        for t in range(lo, hi):
+            h = np.exp(delta[b, t][:, None] * A) * h + (delta[b, t] * x[b, t])[:, None] * Bw[b, t]
+            H[b, t] = h
+        ht[n] = h
+    y = (H * Cw).sum(-1) + skip * x
+    return (y if z is None else y * z / (1 + np.exp(-z))), H, ht
+
+
+def selective_bwd(x, dt, A, B, C, D, z, bias, plus, h0, dy, dht=None, cu=None):
+    """Gradients of sum(y dy) + sum(ht dht): a dict by the names of the inputs."""
+    pre, delta, Bw, Cw, skip, seqs, start = _selective(x, dt, A, B, C, D, z, bias, plus, h0, cu)
+    _, H, _ = selective_fwd(x, dt, A, B, C, D, z, bias, plus, h0, cu)
+    sig = np.ones_like(x) if z is None else 1 / (1 + np.exp(-z))
+    out = dy if z is None else dy * z * sig
+    E, P = np.zeros_like(H), np.zeros_like(H)  # gradients of the states; decayed states
+    dh0 = np.zeros_like(start) if dht is None else np.array(dht, dtype=np.float64)
+    for n, (b, lo, hi) in enumerate(seqs):
+        c = dh0[n].copy()
+        for t in range(hi - 1, lo - 1, -1):
+            a = np.exp(delta[b, t][:, None] * A)
+            E[b, t] = out[b, t][:, None] * Cw[b, t] + c
+            P[b, t] = a * (H[b, t - 1] if t > lo else start[n])
+            c = a * E[b, t]
+        dh0[n] = c
+    sb = (E * Bw).sum(-1)
+    ddelta = (E * P * A).sum(-1) + x * sb
+    dpre = ddelta / (1 + np.exp(-pre)) if plus else ddelta
+    groups = 1 if B.ndim == 3 else B.shape[2]
+    fold = lambda v: v.reshape(*x.shape[:2], groups, -1, A.shape[1]).sum(3).reshape(B.shape)
+    g = dict(x=delta * sb + skip * out, dt=dpre, A=(E * P * delta[..., None]).sum((0, 1)),
+             B=fold(E * (delta * x)[..., None]), C=fold(H * out[..., None]), D=(out * x).sum((0, 1)),
+             dt_bias=dpre.sum((0, 1)), h0=dh0)
+    if z is not None:
+        g["z"] = dy * ((H * Cw).sum(-1) + skip * x) * sig * (1 + z * (1 - sig))
+    return g

@@ -12,7 +12,8 @@ given tokens (:func:`token_logprobs`) and the optimizer (:class:`AdamW`,
 from .gdn2 import GDN2_BACKENDS, GatedDeltaNet2, RMSNormGated, ShortConvolution, resolve_gdn2_backend
 from .gdn2_ops import (AdamW, ChunkGDN2Function, GradNorm, adamw_step, chunk_gdn2, clip_grad_norm_,
                        fused_recurrent_gdn2, fused_recurrent_gdn2_fwd, gated_scan, gated_scan_step,
-                       grad_norm, sample_tokens, TokenLogprobs, token_logprobs)
+                       grad_norm, sample_tokens, selective_scan, selective_scan_step,
+                       TokenLogprobs, token_logprobs)
 from .registry import BLOCKS, build_block
 
 __all__ = [
@@ -36,5 +37,7 @@ __all__ = [
     "grad_norm",
     "resolve_gdn2_backend",
     "sample_tokens",
+    "selective_scan",
+    "selective_scan_step",
     "token_logprobs",
 ]

@@ -56,6 +56,11 @@ EXPORTS = (
     "gdn2_logprob_fwd",
     "gdn2_logprob_bwd",
     "gdn2_adamw_step",
+    "gdn2_selective_saved_bytes",
+    "gdn2_selective_workspace_bytes",
+    "gdn2_selective_fwd",
+    "gdn2_selective_bwd",
+    "gdn2_selective_step",
     "gdn2_sample",
     "gdn2_grad_norm_workspace_bytes",
     "gdn2_grad_norm",
@@ -189,6 +194,27 @@ class AdamWProblem(ctypes.Structure):
     ]
 
 
+class SelectiveProblem(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32),
+        ("D", c_int32),
+        ("G", c_int32),
+        ("N", c_int32),
+        ("T", c_int64),
+        ("dtype", c_int32),
+        ("dt_dtype", c_int32),
+        ("dt_softplus", c_int32),
+        ("n_seqs", c_int32),
+        ("cu_seqlens", c_void_p),
+        ("ld_x", c_int64),
+        ("ld_dt", c_int64),
+        ("ld_z", c_int64),
+        ("ld_b", c_int64),
+        ("ld_c", c_int64),
+        ("ld_dy", c_int64),
+    ]
+
+
 class SampleProblem(ctypes.Structure):
     _fields_ = [
         ("rows", c_int64),
@@ -241,6 +267,7 @@ def _declare(lib):
     ap = P(AdamWProblem)
     gp = P(GradProblem)
     tp = P(SampleProblem)
+    ep = P(SelectiveProblem)
     v = c_void_p
     sig = {
         "gdn2_version": ([], ctypes.c_char_p),
@@ -278,6 +305,11 @@ def _declare(lib):
         "gdn2_scan_bwd": ([sp, v, v, v, v, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_fwd": ([lp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_logprob_bwd": ([lp, v, v, v, v, v, v, v], ctypes.c_int),
+        "gdn2_selective_saved_bytes": ([ep], c_size_t),
+        "gdn2_selective_workspace_bytes": ([ep, c_int32], c_size_t),
+        "gdn2_selective_fwd": ([ep] + [v] * 13 + [c_size_t, v], ctypes.c_int),
+        "gdn2_selective_bwd": ([ep] + [v] * 22 + [c_size_t, v], ctypes.c_int),
+        "gdn2_selective_step": ([ep] + [v] * 9 + [c_int64, c_int32, v, v, v], ctypes.c_int),
         "gdn2_sample": ([tp, v, v, v, v, v, v, v, v], ctypes.c_int),
         "gdn2_grad_norm_workspace_bytes": ([c_int32], c_size_t),
         "gdn2_grad_norm": ([gp, v, c_int32, v, v, c_size_t, v], ctypes.c_int),

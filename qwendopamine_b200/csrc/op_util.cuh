@@ -1,5 +1,5 @@
 // op_util.cuh -- helpers shared by the operators around the GDN-2 mixer
-// (scan.cu, logprob.cu, adamw.cu, sample.cu, gradnorm.cu): error
+// (scan.cu, selective.cu, logprob.cu, sample.cu, adamw.cu, gradnorm.cu): error
 // reporting at the C entries, element groups of a row with or without vector
 // access, rows as aligned vectors, ordered keys of values, and dtype dispatch.
 #pragma once
