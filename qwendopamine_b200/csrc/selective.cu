@@ -35,15 +35,25 @@ namespace {
 constexpr int kSelThreads = 128;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSub = 16;   // rows of a block: one kept state for each
-constexpr int kHalf = 8;   // rows whose states the backward holds at a time
+constexpr int kHeld = 4;   // rows whose states the backward holds at a time
+constexpr int kHalf = 8;   // rows whose sums it hands on at a time
+constexpr int kMostChunks = 640;  // of the time axis
 constexpr float kSelLn2 = 0.6931471805599453f;
+
+struct SelSource {  // a token tensor's rows
+  const void* p;
+  int64_t ld;
+};
 
 struct SelArgs {
   int B, D, G, N, NP, n_seqs;   // NP: N rounded up to 4
   int64_t T;
   const int32_t* cu;
-  const void *x, *dt, *z, *Bv, *Cv;
-  int64_t ldx, lddt, ldz, ldb, ldc;
+  SelSource tok[4];   // x, dy (backward only), z, dt where it has their type
+  SelSource dt32;     // dt where it is fp32
+  SelSource vec[2];   // B, C
+  const void *x, *dt, *z, *Bv, *Cv;  // of one token
+  int64_t ldx, lddt, ldz, ldb, ldc, lddy;
   const float *A, *Dk, *bias, *h0;
   bool dt_f32, softplus;
   void* y;
@@ -54,8 +64,6 @@ struct SelArgs {
   float* carry;       // [B][chunks][D][NP]
   float* decay;       // [B][chunks][D]: sums of dt
   // backward
-  const void* dy;
-  int64_t lddy;
   const float* dht;
   void *dx, *ddt, *dz;
   float* dh0;
@@ -67,21 +75,42 @@ struct SelArgs {
 // ---------------------------------------------------------------------------
 // elementary functions of a token's values
 // ---------------------------------------------------------------------------
-// ln(1 + e^v) without loss for very negative v
-__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
-
-// 1 / (1 + e^-v): exact functions where results are fp32, the hardware's where
-// they are rounded to 16 bits (its errors are about 2^-21)
-template <typename T> __device__ __forceinline__ float sigmoid_of(float v) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-v));
-  else return __fdividef(1.f, 1.f + __expf(-v));
+__device__ __forceinline__ float rcp_fast(float x) {  // relative error 2^-23
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+
+__device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_fast(x.x), rcp_fast(x.y)); }
+
+// ln(1 + e^v) = max(v, 0) + ln(1 + t), t = e^-|v|, without loss for very negative
+// v: with s = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh s = 2 (s + s^3/3 + s^5/5 ...),
+// whose terms from s^17 on are below 1e-9 of it.  Errors of about 2^-22.
+__device__ __forceinline__ float2 softplus2(float2 v) {
+  const float2 t = exp2_2(mul2(make_float2(fabsf(v.x), fabsf(v.y)), f2(-kLog2e)));
+  const float2 s = mul2(t, rcp2(add2(t, f2(2.f)))), q = mul2(s, s);
+  float2 p = fma2(q, f2(1.f / 15.f), f2(1.f / 13.f));
+  p = fma2(q, p, f2(1.f / 11.f));
+  p = fma2(q, p, f2(1.f / 9.f));
+  p = fma2(q, p, f2(1.f / 7.f));
+  p = fma2(q, p, f2(1.f / 5.f));
+  p = fma2(q, p, f2(1.f / 3.f));
+  return fma2(f2(2.f), fma2(mul2(s, q), p, s), make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+}
+__device__ __forceinline__ float softplus_f(float v) { return softplus2(f2(v)).x; }
+
+// 1 / (1 + e^-v), errors of about 2^-21 (the exponent's rounding)
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  return rcp2(add2(exp2_2(mul2(v, f2(-kLog2e))), f2(1.f)));
+}
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_fast(1.f + fast_exp2(-v * kLog2e)); }
 
 // ---------------------------------------------------------------------------
 // geometry
 // ---------------------------------------------------------------------------
-struct SelSpan {  // rows of a chunk, and the sequences they belong to
-  int64_t lo, hi;
+struct SelSpan {  // rows of a chunk
+  int64_t lo;
+  int rows;
   int b, c;
 };
 
@@ -89,9 +118,9 @@ __device__ __forceinline__ SelSpan sel_span(const SelArgs& a, int bc) {
   SelSpan s;
   s.b = bc / a.chunks;
   s.c = bc - s.b * a.chunks;
-  const int64_t first = (int64_t)s.b * a.T;
-  s.lo = first + s.c * a.chunk;
-  s.hi = min(s.lo + a.chunk, first + a.T);
+  const int64_t at = s.c * a.chunk;
+  s.lo = (int64_t)s.b * a.T + at;
+  s.rows = (int)min(a.chunk, a.T - at);
   return s;
 }
 
@@ -111,6 +140,17 @@ __device__ __forceinline__ SelSeq seq_of(const SelArgs& a, int b, int64_t r) {
   return SelSeq{a.cu[lo], a.cu[lo + 1], lo};
 }
 
+// The rows of a chunk at which the sequence of its row r begins and behind which it
+// ends.
+struct SelSides {
+  int lo, hi;
+  __device__ __forceinline__ SelSides(const SelArgs& a, const SelSpan& sp, int r) {
+    const SelSeq s = seq_of(a, sp.b, sp.lo + r);
+    lo = (int)max(s.lo - sp.lo, (int64_t)-1);
+    hi = (int)min(s.hi - sp.lo, (int64_t)0x7fffffff);
+  }
+};
+
 // Sequences that begin and end at rows r0 .. r0 + 15 (-1: none), by 16 threads.
 struct SelEdges {
   int begin[kSub], end[kSub];
@@ -129,235 +169,416 @@ __device__ __forceinline__ void mark_edges(const SelArgs& a, SelEdges& m, int b,
   }
 }
 
-// Four states of a channel in an [..][D][N] array.
-__device__ __forceinline__ void load_states(const float* p, int N, int n0, bool on, float2 (&h)[2]) {
-  float f[4];
+// M neighbouring states of a channel, from n0 on, in an [..][D][N] array.
+template <int M>
+__device__ __forceinline__ void load_states(const float* p, int N, int n0, bool on, float2 (&h)[M / 2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = p && on && n0 + i < N ? p[n0 + i] : 0.f;
-  h[0] = make_float2(f[0], f[1]);
-  h[1] = make_float2(f[2], f[3]);
+  for (int i = 0; i < M / 2; ++i) {
+    h[i].x = p && on && n0 + 2 * i < N ? p[n0 + 2 * i] : 0.f;
+    h[i].y = p && on && n0 + 2 * i + 1 < N ? p[n0 + 2 * i + 1] : 0.f;
+  }
 }
-__device__ __forceinline__ void store_states(float* p, int N, int n0, bool on, const float2 (&h)[2]) {
-  const float f[4] = {h[0].x, h[0].y, h[1].x, h[1].y};
+template <int M>
+__device__ __forceinline__ void store_states(float* p, int N, int n0, bool on, const float2 (&h)[M / 2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (on && n0 + i < N) p[n0 + i] = f[i];
+  for (int i = 0; i < M / 2; ++i) {
+    if (on && n0 + 2 * i < N) p[n0 + 2 * i] = h[i].x;
+    if (on && n0 + 2 * i + 1 < N) p[n0 + 2 * i + 1] = h[i].y;
+  }
 }
-// The same in an [..][D][NP] array of this file: one vector.
-__device__ __forceinline__ void load_states4(const float* p, int NP, int n0, bool on, float2 (&h)[2]) {
+// The same in an [..][D][NP] array of this file, as one vector.
+__device__ __forceinline__ void load_packed(const float* p, int NP, int n0, bool on, float2 (&h)[2]) {
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (on && n0 < NP) v = *reinterpret_cast<const float4*>(p + n0);
   h[0] = make_float2(v.x, v.y);
   h[1] = make_float2(v.z, v.w);
 }
-__device__ __forceinline__ void store_states4(float* p, int NP, int n0, bool on, const float2 (&h)[2]) {
+__device__ __forceinline__ void store_packed(float* p, int NP, int n0, bool on, const float2 (&h)[2]) {
   if (on && n0 < NP) *reinterpret_cast<float4*>(p + n0) = make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
 }
 
-// R values of each of L lanes (neighbours) summed over the lanes: lane l gets
-// the sum of value l % R.
-template <int L, int R> __device__ __forceinline__ float sum_transposed(float (&v)[R], int l) {
-#pragma unroll
-  for (int o = R / 2; o > 0; o /= 2)
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const bool up = l & o;
-      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-    }
-#pragma unroll
-  for (int o = R; o < L; o *= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-  return v[0];
-}
-
-__device__ __forceinline__ float2 decay2(float dt, float2 A2) {
-  const float2 y = mul2(f2(dt), A2);
-  return make_float2(fast_exp2(y.x), fast_exp2(y.y));
-}
-
-// A running sum that keeps what rounding takes away.
-struct LongSum {
-  float hi = 0.f, lo = 0.f;
-  __device__ __forceinline__ void add(float x) {
-    const float s = hi + x, b = s - hi;
-    lo += (hi - (s - b)) + (x - b);
-    hi = s;
+// A thread's running sums of blocks of rows, four in its place of shared memory.
+struct BlockSums {
+  float4 v[kSelThreads];
+  __device__ __forceinline__ void clear() { v[threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void add(float2 x, float2 y) {
+    const float4 a = v[threadIdx.x];
+    v[threadIdx.x] = make_float4(a.x + x.x, a.y + x.y, a.z + y.x, a.w + y.y);
   }
-  __device__ __forceinline__ float get() const { return hi + lo; }
 };
 
-template <typename T, int L> struct SelTile {
-  static constexpr int CH = kSelThreads / L;  // channels of a CTA
+// Two neighbouring values in shared memory.
+template <typename E> __device__ __forceinline__ float2 pair_at(const E* p) { return ld2<E>(p); }
+
+// 16 rows of W columns of each of K tensors (those that are there) on their way into
+// shared memory, one tensor after the other.  The 16-byte pieces are dealt out to
+// the threads; a thread keeps its pieces' addresses, which move from block to block
+// of 16 rows, in its place of shared memory.  What does not exist becomes zero.
+template <typename E, int W, int K> struct RowCursor {
+  static constexpr int VE = 16 / (int)sizeof(E), CPR = W / VE, PIECES = kSub * CPR;
+  static constexpr int NS = (K * PIECES + kSelThreads - 1) / kSelThreads;
+  static_assert(W % VE == 0 && (kSelThreads % PIECES == 0 || PIECES % kSelThreads == 0), "whole pieces");
+  struct alignas(16) Piece {
+    const char* p;
+    int step;   // bytes from block to block
+    int bytes;  // of the piece; -1: no tensor
+  };
+  Piece of[NS][kSelThreads];
+
+  static __device__ __forceinline__ int row_of(int i) {
+    return (threadIdx.x % PIECES) / CPR + (i * kSelThreads % PIECES) / CPR;
+  }
+  // Blocks from row r0 on, forward (way 1) or backward (-1).  Returns whether all
+  // rows start on 16-byte boundaries, as asynchronous copies need.
+  __device__ __forceinline__ bool start(const SelSource* src, int64_t r0, int64_t col, int ncols, int way) {
+    bool vec = true;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      vec = vec && (!src[k].p || ((reinterpret_cast<uintptr_t>((const E*)src[k].p + col) |
+                                   (uint64_t)(src[k].ld * sizeof(E))) & 15) == 0);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int k = (threadIdx.x + i * kSelThreads) / PIECES;
+      Piece x{nullptr, 0, -1};
+      if ((K * PIECES % kSelThreads == 0 || k < K) && src[k].p) {
+        const int c = threadIdx.x % CPR * VE, n = max(0, min(ncols - c, VE));
+        // a piece without a value reads nothing, from an address that exists
+        x.p = (const char*)((const E*)src[k].p + (n ? (r0 + row_of(i)) * src[k].ld + col + c : 0));
+        x.step = n ? (int)(way * kSub * src[k].ld * (int)sizeof(E)) : 0;
+        x.bytes = n * (int)sizeof(E);
+      }
+      of[i][threadIdx.x] = x;
+    }
+    return vec;
+  }
+  // the next block, of which `rows` rows exist
+  __device__ __forceinline__ void request(E* to, int rows, bool vec) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const Piece x = of[i][threadIdx.x];
+      if (x.bytes < 0) continue;
+      E* dst = to + (threadIdx.x + i * kSelThreads) * VE;
+      if (rows >= kSub && vec) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(x.p), "r"(x.bytes)
+                     : "memory");
+      } else {
+        const int n = row_of(i) < rows ? x.bytes / (int)sizeof(E) : 0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) dst[e] = e < n ? ((const E*)x.p)[e] : from_f<E>(0.f);
+      }
+      of[i][threadIdx.x].p = x.p + x.step;
+    }
+  }
+};
+
+// The channels of a CTA (L lanes of four states for each in the forward, 2 L of
+// two in the backward), and what a thread stages of them.
+template <int L> struct SelTile {
+  static constexpr int CH = kSelThreads / L;  // channels
   static constexpr int NL = 4 * L;            // states, padded
-  static constexpr int PER = kSub / L;        // rows of a thread when it stages
-  static constexpr int PAD = CH + 32 / L;     // row stride of what lanes write by row
-  static constexpr int VPT = kSub * NL / kSelThreads;  // B (or C) values a thread stages
+  static constexpr int PAIRS = CH / 2;        // pairs of channels: a thread stages one, in
+  static constexpr int STEP = 2 * L;          // every STEP-th row
+  static constexpr int BC_STEP = kSelThreads / (2 * NL), BC_ROWS = kHalf / BC_STEP < 1 ? 1 : kHalf / BC_STEP;
+  static constexpr int PER = STEP < kSub ? kSub / STEP : 1, PER_HALF = STEP < kHalf ? kHalf / STEP : 1;
   int d0, nch, g, tile;
-  int l, mc, d;       // as a lane: which of the channel's, which channel
-  bool on;
-  int sc, sr;         // when staging: channel, first row
+  int pc, pr;         // the pair's first channel, the first row
   __device__ __forceinline__ SelTile(const SelArgs& a, int tile_) : tile(tile_) {
     g = tile / a.tiles_per_group;
     const int dg = a.D / a.G, at = (tile - g * a.tiles_per_group) * CH;
     d0 = g * dg + at;
     nch = min(CH, dg - at);
-    l = threadIdx.x % L;
-    mc = threadIdx.x / L;
-    on = mc < nch;
-    d = d0 + mc;
-    sc = threadIdx.x % CH;
-    sr = threadIdx.x / CH;
+    pc = 2 * (threadIdx.x % PAIRS);
+    pr = threadIdx.x / PAIRS;
   }
-  __device__ __forceinline__ void load_rates(const SelArgs& a, float2 (&A2)[2]) const {
-    load_states(a.A + (int64_t)d * a.N, a.N, 4 * l, on, A2);
-    A2[0] = mul2(A2[0], f2(kLog2e));
-    A2[1] = mul2(A2[1], f2(kLog2e));
+  // a parameter's values of the staged pair (zero without it)
+  __device__ __forceinline__ float2 pair_of(const float* p) const {
+    return make_float2(p && pc < nch ? p[d0 + pc] : 0.f, p && pc + 1 < nch ? p[d0 + pc + 1] : 0.f);
   }
-  // B or C of 16 rows, zero where there is no state or row
-  __device__ __forceinline__ void load_vectors(const SelArgs& a, const void* p, int64_t ld, int64_t r0,
-                                               int64_t hi, float (&v)[VPT]) const {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int idx = threadIdx.x + i * kSelThreads, n = idx % NL;
-      const int64_t r = r0 + idx / NL;
-      v[i] = n < a.N && r < hi ? to_f<T>(((const T*)p)[r * ld + g * a.N + n]) : 0.f;
-    }
+  // whether a staged pair can be stored as one word in contiguous [rows][D] results
+  template <typename E> __device__ __forceinline__ bool whole(const void* p, int D) const {
+    return pc + 1 < nch && (D & 1) == 0 && ((reinterpret_cast<uintptr_t>((const E*)p + d0 + pc)) & (2 * sizeof(E) - 1)) == 0;
   }
-  __device__ __forceinline__ void put_vectors(float* s, const float (&v)[VPT]) const {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) s[threadIdx.x + i * kSelThreads] = v[i];
-  }
-  // a token tensor's values of this thread's channel and rows
-  __device__ __forceinline__ void load_tokens(const void* p, bool f32, int64_t ld, int64_t r0, int64_t hi,
-                                              float (&v)[PER]) const {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int64_t r = r0 + sr + L * i;
-      const int64_t at = r * ld + d0 + sc;
-      v[i] = 0.f;
-      if (r < hi && sc < nch) v[i] = f32 ? ((const float*)p)[at] : to_f<T>(((const T*)p)[at]);
+  template <typename E> __device__ __forceinline__ void store_pair(E* to, bool whole, float2 v) const {
+    if (whole) {
+      if constexpr (sizeof(E) == 4) *reinterpret_cast<float2*>(to) = v;
+      else *reinterpret_cast<uint32_t*>(to) = pack2<E>(v.x, v.y);
+    } else {
+      if (pc < nch) to[0] = from_f<E>(v.x);
+      if (pc + 1 < nch) to[1] = from_f<E>(v.y);
     }
   }
 };
+
+__device__ __forceinline__ int64_t block_states(const SelArgs& a, int b, int64_t r0) {
+  return ((int64_t)b * a.subs + (r0 - (int64_t)b * a.T) / kSub) * a.D * a.NP;
+}
+
+// Values of 16 rows as they come from memory: x, dy (backward), z, and dt where it
+// has their type.
+template <typename T, int L, bool BWD> struct SelRaw {
+  using S = SelTile<L>;
+  static constexpr int V = kSub * S::CH, K = BWD ? 4 : 3;
+  alignas(16) T tok[K * V];
+  alignas(16) T vec[2 * kSub * S::NL];  // B, C
+  __device__ __forceinline__ float2 x(int i) const { return pair_at(tok + i); }
+  __device__ __forceinline__ float2 dy(int i) const { return pair_at(tok + V + i); }
+  __device__ __forceinline__ float2 z(int i) const { return pair_at(tok + (K - 2) * V + i); }
+  __device__ __forceinline__ float2 dt(int i) const { return pair_at(tok + (K - 1) * V + i); }
+};
+
+// Their copies.
+template <typename T, int L, bool BWD> struct SelCopies {
+  using S = SelTile<L>;
+  using R = SelRaw<T, L, BWD>;
+  RowCursor<T, S::CH, R::K> tok;
+  RowCursor<T, S::NL, 2> vec;
+};
+template <typename T, int L, bool BWD, typename Shared>
+__device__ __forceinline__ bool start_copies(const SelArgs& a, const SelTile<L>& t, Shared& s, int64_t r0) {
+  constexpr int way = BWD ? -1 : 1;
+  bool vec = s.copies.tok.start(a.tok, r0, t.d0, t.nch, way);
+  vec &= s.copies.vec.start(a.vec, r0, (int64_t)t.g * a.N, a.N, way);
+  if (a.dt_f32) vec &= s.dt32.cursor.start(&a.dt32, r0, t.d0, t.nch, way);
+  return vec;
+}
+template <typename Shared>
+__device__ __forceinline__ void request_copies(const SelArgs& a, Shared& s, int at, int rows, bool vec) {
+  s.copies.tok.request(s.raw[at].tok, rows, vec);
+  s.copies.vec.request(s.raw[at].vec, rows, vec);
+  if (a.dt_f32) s.dt32.cursor.request(s.dt32.v[at], rows, vec);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// dt as fp32, of both blocks: the end of shared memory, left out where dt is not.
+template <int L> struct SelDt32 {
+  RowCursor<float, SelTile<L>::CH, 1> cursor;
+  alignas(16) float v[2][kSub * SelTile<L>::CH];
+};
+
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// B or C of 16 rows as fp32.
+template <typename T, int L> __device__ __forceinline__ void widen(float* to, const T* from) {
+#pragma unroll
+  for (int i = 0; i < (kSub * 2 * L + kSelThreads - 1) / kSelThreads; ++i) {
+    const int at = 2 * (threadIdx.x + i * kSelThreads);
+    if (kSub * 4 * L % (2 * kSelThreads) == 0 || at < kSub * 4 * L)
+      *reinterpret_cast<float2*>(to + at) = pair_at(from + at);
+  }
+}
+
+// Two fp32 values in a 64-bit register, as packed arithmetic takes them: pairs that
+// come from shared memory as 64-bit words need no moves.
+typedef unsigned long long pair64;
+__device__ __forceinline__ pair64 pmul(pair64 a, pair64 b) {
+  pair64 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ pair64 pfma(pair64 a, pair64 b, pair64 c) {
+  pair64 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ pair64 pexp2(pair64 a) {  // as fast_exp2
+  pair64 d;
+  asm("{\n\t.reg .f32 x, y;\n\tmov.b64 {x, y}, %1;\n\tex2.approx.ftz.f32 x, x;\n\t"
+      "ex2.approx.ftz.f32 y, y;\n\tmov.b64 %0, {x, y};\n\t}"
+      : "=l"(d)
+      : "l"(a));
+  return d;
+}
+__device__ __forceinline__ pair64 to_pair(float2 v) {
+  pair64 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(v.x), "f"(v.y));
+  return d;
+}
+__device__ __forceinline__ float2 of_pair(pair64 v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ ulonglong2 two_pairs(const void* p) { return *reinterpret_cast<const ulonglong2*>(p); }
+
+// The factor of a channel goes to both of its states: scalar operations, which need
+// no second copy of it, where packed ones would.
+__device__ __forceinline__ float2 scale2(float a, float2 x) { return make_float2(a * x.x, a * x.y); }
+__device__ __forceinline__ float2 scale_add2(float a, float2 x, float2 y) {
+  return make_float2(fmaf(a, x.x, y.x), fmaf(a, x.y, y.y));
+}
+
+__device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
 template <typename T, int L> struct SelFwdShared {
-  using S = SelTile<T, L>;
+  using S = SelTile<L>;
+  SelRaw<T, L, false> raw[2];
   alignas(16) float b[kSub * S::NL];
   alignas(16) float c[kSub * S::NL];
-  float2 dd[kSub][S::CH];       // dt, dt x
-  float y[kSub][S::PAD];
+  alignas(16) float2 dd[kSub][S::CH];       // dt, dt x
+  alignas(16) float y[kSub][kSelThreads];   // each lane's share of its channel's sum
   SelEdges edges;
+  SelCopies<T, L, false> copies;
+  SelDt32<L> dt32;
+  static constexpr int without_dt32() { return (int)(sizeof(SelFwdShared) - sizeof(SelDt32<L>)); }
+};
+
+struct FwdLane {
+  int l, mc, d;  // which of the channel's lanes, which channel
+  bool on;
 };
 
 // 16 rows of one lane's states; LOCAL: only the states.
-template <typename T, int L, bool LOCAL, bool EDGE>
-__device__ __forceinline__ void fwd_rows(const SelArgs& a, SelFwdShared<T, L>& s, const SelTile<T, L>& t,
-                                         const float2 (&A2)[2], float2 (&h)[2], float& dsum) {
-  using S = SelTile<T, L>;
-#pragma unroll 1
-  for (int q = 0; q < kSub; q += L) {
-    float v[L];
+template <bool LOCAL, bool EDGE, typename T, int L>
+__device__ __forceinline__ void fwd_rows(const SelArgs& a, SelFwdShared<T, L>& s, const FwdLane& t,
+                                         const pair64 (&A2)[2], pair64 (&h)[2], float& dsum) {
+  using S = SelTile<L>;
+  constexpr int U = 4;  // rows whose decays and inputs are formed together
+#pragma unroll 2
+  for (int q = 0; q < kSub; q += U) {
+    pair64 da[U][2], in[U][2];
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
+    for (int j = 0; j < U; ++j) {
+      const float2 dd = s.dd[q + j][t.mc];
+      const float4 B = *reinterpret_cast<const float4*>(s.b + (q + j) * S::NL + 4 * t.l);
+      da[j][0] = to_pair(exp2_2(scale2(dd.x, of_pair(A2[0]))));
+      da[j][1] = to_pair(exp2_2(scale2(dd.x, of_pair(A2[1]))));
+      in[j][0] = to_pair(scale2(dd.y, lo2(B)));
+      in[j][1] = to_pair(scale2(dd.y, hi2(B)));
+      if constexpr (LOCAL) dsum += dd.x;
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
       const int r = q + j;
-      const float2 dd = s.dd[r][t.mc];
-      const float4 B = *reinterpret_cast<const float4*>(s.b + r * S::NL + 4 * t.l);
       if constexpr (EDGE) {
         const int n = s.edges.begin[r];
         if (n >= 0) {
-          load_states(a.h0 ? a.h0 + ((int64_t)n * a.D + t.d) * a.N : nullptr, a.N, 4 * t.l, t.on, h);
+          float2 v[2];
+          load_states<4>(a.h0 ? a.h0 + ((int64_t)n * a.D + t.d) * a.N : nullptr, a.N, 4 * t.l, t.on, v);
+          h[0] = to_pair(v[0]);
+          h[1] = to_pair(v[1]);
         }
       }
-      h[0] = fma2(decay2(dd.x, A2[0]), h[0], mul2(f2(dd.y), make_float2(B.x, B.y)));
-      h[1] = fma2(decay2(dd.x, A2[1]), h[1], mul2(f2(dd.y), make_float2(B.z, B.w)));
-      if constexpr (LOCAL) {
-        dsum += dd.x;
-      } else {
-        const float4 C = *reinterpret_cast<const float4*>(s.c + r * S::NL + 4 * t.l);
-        const float2 o = fma2(h[0], make_float2(C.x, C.y), mul2(h[1], make_float2(C.z, C.w)));
-        v[j] = o.x + o.y;
+      h[0] = pfma(da[j][0], h[0], in[j][0]);
+      h[1] = pfma(da[j][1], h[1], in[j][1]);
+      if constexpr (!LOCAL) {
+        const ulonglong2 C = two_pairs(s.c + r * S::NL + 4 * t.l);
+        const float2 o = of_pair(pfma(h[1], C.y, pmul(h[0], C.x)));
+        s.y[r][threadIdx.x] = o.x + o.y;
         if constexpr (EDGE) {
           const int n = s.edges.end[r];
-          if (n >= 0 && a.ht) store_states(a.ht + ((int64_t)n * a.D + t.d) * a.N, a.N, 4 * t.l, t.on, h);
+          const float2 v[2] = {of_pair(h[0]), of_pair(h[1])};
+          if (n >= 0 && a.ht) store_states<4>(a.ht + ((int64_t)n * a.D + t.d) * a.N, a.N, 4 * t.l, t.on, v);
         }
       }
     }
-    if constexpr (!LOCAL) s.y[q + t.l][t.mc] = sum_transposed<L, L>(v, t.l);
+  }
+}
+
+// The sum of a channel's L shares.
+template <int L> __device__ __forceinline__ float sum_shares(const float* p) {
+  if constexpr (L == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    return v.x + v.y;
+  } else {
+    float f = 0.f;
+#pragma unroll
+    for (int i = 0; i < L / 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(p)[i];
+      f += (v.x + v.y) + (v.z + v.w);
+    }
+    return f;
   }
 }
 
 template <typename T, int L, bool LOCAL>
 __global__ void __launch_bounds__(kSelThreads) k_sel_fwd(const SelArgs a) {
-  using S = SelTile<T, L>;
-  __shared__ SelFwdShared<T, L> s;
+  using S = SelTile<L>;
+  extern __shared__ __align__(16) char raw_shared[];
+  SelFwdShared<T, L>& s = *reinterpret_cast<SelFwdShared<T, L>*>(raw_shared);
   const int bc = blockIdx.x / a.tiles;
   const S t(a, blockIdx.x - bc * a.tiles);
   const SelSpan sp = sel_span(a, bc);
   if (LOCAL && sp.c + 1 == a.chunks) return;  // nothing follows the last
-  float2 A2[2], h[2];
-  t.load_rates(a, A2);
+  const bool vec = start_copies<T, L, false>(a, t, s, sp.lo);
+  request_copies(a, s, 0, sp.rows, vec);
+  const int mc = threadIdx.x / L;
+  const FwdLane lane{(int)threadIdx.x % L, mc, t.d0 + mc, mc < t.nch};
+  float2 rate[2], start[2] = {f2(0.f), f2(0.f)};
+  load_states<4>(a.A + (int64_t)lane.d * a.N, a.N, 4 * lane.l, lane.on, rate);
+  const pair64 A2[2] = {to_pair(mul2(rate[0], f2(kLog2e))), to_pair(mul2(rate[1], f2(kLog2e)))};
   float dsum = 0.f;
-  if (LOCAL || sp.c == 0) h[0] = h[1] = f2(0.f);
-  else load_states4(a.carry + ((int64_t)bc * a.D + t.d) * a.NP, a.NP, 4 * t.l, t.on, h);
-  const float bias = a.bias && t.sc < t.nch ? a.bias[t.d0 + t.sc] : 0.f;
-  const float skip = a.Dk && t.sc < t.nch ? a.Dk[t.d0 + t.sc] : 0.f;
-  SelSeq seq = seq_of(a, sp.b, sp.lo);
-
-  float x[S::PER], dt[S::PER], z[S::PER], vb[S::VPT], vc[S::VPT];
-  auto load = [&](int64_t r0) {
-    t.load_tokens(a.x, false, a.ldx, r0, sp.hi, x);
-    t.load_tokens(a.dt, a.dt_f32, a.lddt, r0, sp.hi, dt);
-    t.load_vectors(a, a.Bv, a.ldb, r0, sp.hi, vb);
-    if constexpr (!LOCAL) {
-      if (a.z) t.load_tokens(a.z, false, a.ldz, r0, sp.hi, z);
-      t.load_vectors(a, a.Cv, a.ldc, r0, sp.hi, vc);
-    }
+  const int64_t mine = (int64_t)lane.d * a.NP;
+  if (!LOCAL && sp.c > 0)
+    load_packed(a.carry + (int64_t)bc * a.D * a.NP + mine, a.NP, 4 * lane.l, lane.on, start);
+  pair64 h[2] = {to_pair(start[0]), to_pair(start[1])};
+  auto put_states = [&](float* to) {
+    const float2 v[2] = {of_pair(h[0]), of_pair(h[1])};
+    store_packed(to + mine, a.NP, 4 * lane.l, lane.on, v);
   };
-  load(sp.lo);
-  for (int64_t r0 = sp.lo; r0 < sp.hi; r0 += kSub) {
-    const bool edge = seq.lo == r0 || seq.hi <= r0 + kSub;
-    float x1[S::PER], z1[S::PER];
+  const float2 bias = t.pair_of(a.bias), skip = t.pair_of(a.Dk);
+  const bool whole = !LOCAL && t.template whole<T>(a.y, a.D);
+  T* out = (T*)a.y + (sp.lo + t.pr) * a.D + t.d0 + t.pc;
+  float* keep = a.saved + block_states(a, sp.b, sp.lo);
+  SelSides side(a, sp, 0);
+
+  int at = 0;
+  for (int r0 = 0; r0 < sp.rows; r0 += kSub, at ^= 1) {
+    const SelRaw<T, L, false>& raw = s.raw[at];
+    const bool edge = side.lo == r0 || side.hi <= r0 + kSub;
+    const int rows = sp.rows - r0;  // that are left
+    copies_done();
+    __syncthreads();
+    if (rows > kSub) request_copies(a, s, at ^ 1, rows - kSub, vec);
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) {
-      float d = dt[i] + bias;
-      if (a.softplus) d = softplus_f(d);
-      if (r0 + t.sr + L * i >= sp.hi) d = 0.f;  // rows behind the last leave the states as they are
-      s.dd[t.sr + L * i][t.sc] = make_float2(d, d * x[i]);
-      x1[i] = x[i];
-      z1[i] = z[i];
+      const int row = t.pr + i * S::STEP;
+      if (S::STEP > kSub && row >= kSub) break;
+      const int p = row * S::CH + t.pc;
+      float2 d = add2((a.dt_f32 ? pair_at(s.dt32.v[at] + p) : raw.dt(p)), bias);
+      if (a.softplus) d = softplus2(d);
+      if (row >= rows) d = f2(0.f);  // rows behind the last leave the states as they are
+      const float2 u = mul2(d, raw.x(p));
+      *reinterpret_cast<float4*>(&s.dd[row][t.pc]) = make_float4(d.x, u.x, d.y, u.y);
     }
-    t.put_vectors(s.b, vb);
-    if constexpr (!LOCAL) t.put_vectors(s.c, vc);
-    if (edge) mark_edges(a, s.edges, sp.b, r0, sp.hi);
-    __syncthreads();
-    if (r0 + kSub < sp.hi) load(r0 + kSub);
+    widen<T, L>(s.b, raw.vec);
+    if constexpr (!LOCAL) widen<T, L>(s.c, raw.vec + kSub * S::NL);
+    if (edge) mark_edges(a, s.edges, sp.b, sp.lo + r0, sp.lo + sp.rows);
     if constexpr (!LOCAL)
-      if (a.saved)
-        store_states4(a.saved + (((int64_t)sp.b * a.subs + (r0 - (int64_t)sp.b * a.T) / kSub) * a.D + t.d) * a.NP,
-                      a.NP, 4 * t.l, t.on, h);
-    if (edge) {
-      fwd_rows<T, L, LOCAL, true>(a, s, t, A2, h, dsum);
-      if (r0 + kSub < sp.hi) seq = seq_of(a, sp.b, r0 + kSub);
-    } else {
-      fwd_rows<T, L, LOCAL, false>(a, s, t, A2, h, dsum);
-    }
+      if (a.saved) {
+        put_states(keep);
+        keep += (int64_t)a.D * a.NP;
+      }
     __syncthreads();
+    if (edge) {
+      fwd_rows<LOCAL, true>(a, s, lane, A2, h, dsum);
+      if (rows > kSub) side = SelSides(a, sp, r0 + kSub);
+    } else {
+      fwd_rows<LOCAL, false>(a, s, lane, A2, h, dsum);
+    }
     if constexpr (!LOCAL) {
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < S::PER; ++i) {
-        const int64_t r = r0 + t.sr + L * i;
-        float y = fmaf(skip, x1[i], s.y[t.sr + L * i][t.sc]);
-        if (a.z) y *= z1[i] * sigmoid_of<T>(z1[i]);
-        if (r < sp.hi && t.sc < t.nch) ((T*)a.y)[r * a.D + t.d0 + t.sc] = from_f<T>(y);
+        const int row = t.pr + i * S::STEP;
+        if (S::STEP > kSub && row >= kSub) break;
+        const int p = row * S::CH + t.pc;
+        const float* share = s.y[row] + t.pc * L;
+        float2 y = fma2(skip, raw.x(p), make_float2(sum_shares<L>(share), sum_shares<L>(share + L)));
+        if (a.z) {
+          const float2 z = raw.z(p);
+          y = mul2(y, mul2(z, sigmoid2(z)));
+        }
+        if (row < rows) t.store_pair(out + (int64_t)i * S::STEP * a.D, whole, y);
       }
+      out += (int64_t)kSub * a.D;
     }
   }
   if constexpr (LOCAL) {
-    store_states4(a.carry + ((int64_t)bc * a.D + t.d) * a.NP, a.NP, 4 * t.l, t.on, h);
-    if (t.l == 0 && t.on) a.decay[(int64_t)bc * a.D + t.d] = dsum;
+    put_states(a.carry + (int64_t)bc * a.D * a.NP);
+    if (lane.l == 0 && lane.on) a.decay[(int64_t)bc * a.D + lane.d] = dsum;
   }
 }
 
@@ -365,23 +586,37 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_fwd(const SelArgs a) {
 // front of it (BACK: from the gradient in front of chunk c to the one behind it).
 // A sequence that begins in a chunk keeps what is in front of it out.
 template <bool BACK> __global__ void __launch_bounds__(256) k_sel_carry(const SelArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)a.D * a.NP;
-  if (i >= a.B * per) return;
-  const int b = (int)(i / per);
-  const int64_t at = i - b * per;
+  constexpr int U = 8;  // chunks whose values are on their way together
+  __shared__ bool begins[kMostChunks];
+  const int64_t per = (int64_t)a.D * a.NP, tiles = (per + 255) / 256;
+  const int b = (int)(blockIdx.x / tiles);
+  const int64_t at = (blockIdx.x - b * tiles) * 256 + threadIdx.x;
+  const int64_t base = (int64_t)b * a.chunks;
+  for (int c = threadIdx.x; c < a.chunks; c += 256) {
+    const SelSpan sp = sel_span(a, (int)(base + c));
+    begins[c] = seq_of(a, b, sp.lo + sp.rows - 1).lo >= sp.lo;
+  }
+  __syncthreads();
+  if (at >= per) return;
   const int d = (int)(at / a.NP), n = (int)(at - (int64_t)d * a.NP);
   const float A2 = n < a.N ? a.A[(int64_t)d * a.N + n] * kLog2e : 0.f;
   float run = 0.f;
-  const int64_t base = (int64_t)b * a.chunks;
-  for (int k = 0; k < a.chunks; ++k) {
-    const int c = BACK ? a.chunks - 1 - k : k;
-    const SelSpan sp = sel_span(a, (int)(base + c));
-    float* p = a.carry + (base + c) * per + at;
-    const bool last = k + 1 == a.chunks;
-    const float own = last ? 0.f : *p, dsum = last ? 0.f : a.decay[(base + c) * a.D + d];
-    *p = run;
-    const bool begins = seq_of(a, b, sp.hi - 1).lo >= sp.lo;
-    run = begins ? own : fmaf(fast_exp2(dsum * A2), run, own);
+  for (int k0 = 0; k0 < a.chunks; k0 += U) {
+    float own[U], dsum[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = BACK ? a.chunks - 1 - (k0 + i) : k0 + i;
+      const bool used = k0 + i + 1 < a.chunks;  // the last chunk's is not written
+      own[i] = used ? a.carry[(base + c) * per + at] : 0.f;
+      dsum[i] = used ? a.decay[(base + c) * a.D + d] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = BACK ? a.chunks - 1 - (k0 + i) : k0 + i;
+      if (k0 + i >= a.chunks) break;
+      a.carry[(base + c) * per + at] = run;
+      run = begins[c] ? own[i] : fmaf(fast_exp2(dsum[i] * A2), run, own[i]);
+    }
   }
 }
 
@@ -389,296 +624,428 @@ template <bool BACK> __global__ void __launch_bounds__(256) k_sel_carry(const Se
 // backward
 // ---------------------------------------------------------------------------
 template <typename T, int L> struct SelBwdShared {
-  using S = SelTile<T, L>;
+  using S = SelTile<L>;
+  static constexpr int G = 2 * L;           // lanes of a channel
+  SelRaw<T, L, true> raw[2];
   alignas(16) float b[kSub * S::NL];
   alignas(16) float c[kSub * S::NL];
-  float2 dd[kSub][S::CH];       // dt, dt x
-  float o[kSub][S::CH];         // dy silu(z)
-  float y[kSub][S::PAD], sb[kSub][S::PAD], sa[kSub][S::PAD];
-  alignas(16) float bc[kSelWarps][kSub][2 * S::NL];  // dB, dC of a warp's channels
-  float fold[2][kSelThreads];
+  alignas(16) float2 dd[kSub][S::CH];       // dt, dt x
+  alignas(16) float o[kSub][S::CH];         // dy silu(z)
+  // shares of three sums over the states of a pair of channels: B e, A2 a h' e, and
+  // C h, where neighbouring lanes have added theirs (one has the first channel's)
+  alignas(16) float2 share[2][kHalf][S::PAIRS * G];
+  alignas(16) float share_y[kHalf][S::PAIRS * G];
+  float bc[kSelWarps][kHalf][2][2][8];      // dB, dC of a warp's channels: state 0 and 1 of each lane
+  alignas(16) BlockSums sum_a, sum_d;        // dA; dD and ddt_bias of the staged pair
+  alignas(8) float2 par[2][S::PAIRS];       // dt_bias and D of the pairs
   SelEdges edges;
+  SelCopies<T, L, true> copies;
+  SelDt32<L> dt32;
+  static constexpr int without_dt32() { return (int)(sizeof(SelBwdShared) - sizeof(SelDt32<L>)); }
 };
 
-// Eight values of each lane, four of dB and four of dC, summed over the channels
-// of the warp (lanes L apart) into the warp's row of shared memory.
-template <int L> __device__ __forceinline__ void sum_channels(float (&v)[8], float* row, int lane) {
-  constexpr int CW = 32 / L, NL = 4 * L;       // channels of a warp
-  constexpr int W = CW < 8 ? CW : 8;           // lanes that end with different values
-  const int l = lane % L, w = lane / L;
-  int first = 0;                               // of the values that this lane still holds
-#pragma unroll
-  for (int o = W / 2, n = 4; o > 0; o /= 2, n /= 2) {
-    const bool up = w & o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) {
-        const float keep = up ? v[i + n] : v[i], send = up ? v[i] : v[i + n];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o * L);
-      }
-    first += up ? n : 0;
+// Where a lane stands in the backward: two neighbouring channels, two states of
+// each.  Lane 4 g + k of a warp has channels 2 k, 2 k + 1 of eight, as a tensor-core
+// operand of 16 states by 8 channels has them; its states are the group l = g of
+// eight groups, or of the warp's eight lanes-of-four several channel sets share
+// (fewer than 16 states) or several warps make up the groups (more).
+template <int L> struct BwdLane {
+  static constexpr int G = 2 * L, SETS = G < 8 ? 8 / G : 1, BLOCKS = G > 8 ? G / 8 : 1;
+  int l, mc, d, set;
+  bool on[2];
+  __device__ __forceinline__ BwdLane(const SelTile<L>& t) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+    set = G < 8 ? g / G : 0;
+    l = G < 8 ? g % G : (warp % BLOCKS) * 8 + g;
+    mc = ((warp / BLOCKS) * SETS + set) * 8 + 2 * (lane & 3);
+    d = t.d0 + mc;
+    on[0] = mc < t.nch;
+    on[1] = mc + 1 < t.nch;
   }
-  constexpr int left = 8 / W;
+  __device__ __forceinline__ void load(const float* p, int N, float2 (&v)[2]) const {
 #pragma unroll
-  for (int o = W; o < CW; o *= 2)
-#pragma unroll
-    for (int i = 0; i < left; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o * L);
-  if (w < W) {
-#pragma unroll
-    for (int i = 0; i < left; ++i) {
-      const int at = first + i;
-      row[(at >> 2) * NL + 4 * l + (at & 3)] = v[i];
+    for (int i = 0; i < 2; ++i) {
+      float2 x[1];
+      load_states<2>(p ? p + (int64_t)(d + i) * N : nullptr, N, 2 * l, on[i], x);
+      v[i] = x[0];
     }
+  }
+  __device__ __forceinline__ void store(float* p, int N, const float2 (&v)[2]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 x[1] = {v[i]};
+      store_states<2>(p + (int64_t)(d + i) * N, N, 2 * l, on[i], x);
+    }
+  }
+  __device__ __forceinline__ void load_packed(const float* p, int NP, float2 (&v)[2]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] = on[i] && 2 * l < NP ? *reinterpret_cast<const float2*>(p + (int64_t)(d + i) * NP + 2 * l) : f2(0.f);
+  }
+  __device__ __forceinline__ void store_packed(float* p, int NP, const float2 (&v)[2]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (on[i] && 2 * l < NP) *reinterpret_cast<float2*>(p + (int64_t)(d + i) * NP + 2 * l) = v[i];
+  }
+};
+
+// d = A B from a zero start (m16n8k8, TF32).
+__device__ __forceinline__ void mma_tf32_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// A value as a TF32 operand, of which the tensor core takes the upper 19 bits: half
+// a step is added where it is to be rounded to nearest.
+__device__ __forceinline__ uint32_t tf32_near(float x) { return __float_as_uint(x) + 0x1000u; }
+__device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x) & 0xffffe000u; }
+
+// Sums over a warp's eight channels (of each set) by the tensor core: A holds a
+// value for each state and channel as the lanes have them, B the channels' factors
+// in every column.  bf16 results: the operands are rounded to TF32's 11 bits, three
+// more than the result keeps, and the sums are fp32.  Others: an operand is the sum
+// of two TF32 values, which leaves 2^-21 of it, and three products are summed.
+template <typename T>
+__device__ __forceinline__ void sum_channels(float (&sum)[4], const float2 (&v)[2], float w0, float w1) {
+  const float x[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+  uint32_t hi[4];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = tf32_near(x[i]);
+    mma_tf32_new(sum, hi, tf32_near(w0), tf32_near(w1));
+  } else {
+    uint32_t lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = tf32_cut(x[i]);
+      lo[i] = tf32_near(x[i] - __uint_as_float(hi[i]));
+    }
+    const uint32_t h0 = tf32_cut(w0), h1 = tf32_cut(w1);
+    mma_tf32_new(sum, hi, h0, h1);
+    mma_tf32(sum, lo, h0, h1);
+    mma_tf32(sum, hi, tf32_near(w0 - __uint_as_float(h0)), tf32_near(w1 - __uint_as_float(h1)));
   }
 }
 
-// One row's states from those in front of it.
+// What a row has for a lane's two channels and two states.
+struct BwdRow {
+  float d[2], u[2];  // dt, dt x
+  template <typename T, int L>
+  __device__ __forceinline__ void load(const SelBwdShared<T, L>& s, const BwdLane<L>& t, int r) {
+    const float4 v = *reinterpret_cast<const float4*>(&s.dd[r][t.mc]);
+    d[0] = v.x; u[0] = v.y; d[1] = v.z; u[1] = v.w;
+  }
+};
+
+// One row's states from those in front of it; da and p: the decays, and the
+// decayed states.
 template <bool EDGE, typename T, int L>
-__device__ __forceinline__ void state_row(const SelArgs& a, const SelBwdShared<T, L>& s, const SelTile<T, L>& t,
-                                          int r, const float2 (&A2)[2], float2 (&h)[2], float2 (&da)[2],
-                                          float2 (&p)[2]) {
-  using S = SelTile<T, L>;
-  const float2 dd = s.dd[r][t.mc];
-  const float4 B = *reinterpret_cast<const float4*>(s.b + r * S::NL + 4 * t.l);
+__device__ __forceinline__ void state_row(const SelArgs& a, const SelBwdShared<T, L>& s, const BwdLane<L>& t,
+                                          int r, const BwdRow& x, const float2 (&A2)[2], float2 (&h)[2],
+                                          float2 (&da)[2], float2 (&p)[2]) {
   if constexpr (EDGE) {
     const int n = s.edges.begin[r];
-    if (n >= 0)
-      load_states(a.h0 ? a.h0 + ((int64_t)n * a.D + t.d) * a.N : nullptr, a.N, 4 * t.l, t.on, h);
+    if (n >= 0) t.load(a.h0 ? a.h0 + (int64_t)n * a.D * a.N : nullptr, a.N, h);
   }
-  da[0] = decay2(dd.x, A2[0]);
-  da[1] = decay2(dd.x, A2[1]);
-  p[0] = mul2(da[0], h[0]);
-  p[1] = mul2(da[1], h[1]);
-  h[0] = fma2(f2(dd.y), make_float2(B.x, B.y), p[0]);
-  h[1] = fma2(f2(dd.y), make_float2(B.z, B.w), p[1]);
-}
-
-template <bool EDGE, typename T, int L>
-__device__ __forceinline__ void bwd_half(const SelArgs& a, SelBwdShared<T, L>& s, const SelTile<T, L>& t, int q,
-                                         const float2 (&A2)[2], float2 (&h)[2], float2 (&e)[2],
-                                         float2 (&dA)[2]) {
-  using S = SelTile<T, L>;
-  constexpr int R = L < kHalf ? L : kHalf;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float2 da[kHalf][2], p[kHalf][2];
+  const float2 B = *reinterpret_cast<const float2*>(s.b + r * SelTile<L>::NL + 2 * t.l);
 #pragma unroll
-  for (int j = 0; j < kHalf; ++j) state_row<EDGE>(a, s, t, q + j, A2, h, da[j], p[j]);
-#pragma unroll
-  for (int k = kHalf - R; k >= 0; k -= R) {
-    float vy[R], vb[R], va[R];
-#pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      const int j = k + i, r = q + j;
-      const float2 dd = s.dd[r][t.mc];
-      const float o = s.o[r][t.mc];
-      const float4 B = *reinterpret_cast<const float4*>(s.b + r * S::NL + 4 * t.l);
-      const float4 C = *reinterpret_cast<const float4*>(s.c + r * S::NL + 4 * t.l);
-      const float2 B2[2] = {make_float2(B.x, B.y), make_float2(B.z, B.w)};
-      const float2 C2[2] = {make_float2(C.x, C.y), make_float2(C.z, C.w)};
-      if constexpr (EDGE) {
-        const int n = s.edges.end[r];
-        if (n >= 0)
-          load_states(a.dht ? a.dht + ((int64_t)n * a.D + t.d) * a.N : nullptr, a.N, 4 * t.l, t.on, e);
-      }
-      float v[8];
-      float2 sy, sb, sa;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float2 hh = fma2(f2(dd.y), B2[u], p[j][u]);
-        e[u] = fma2(f2(o), C2[u], e[u]);
-        const float2 dC = mul2(f2(o), hh), dB = mul2(f2(dd.y), e[u]);
-        v[2 * u] = dB.x; v[2 * u + 1] = dB.y;
-        v[4 + 2 * u] = dC.x; v[5 + 2 * u] = dC.y;
-        const float2 g = mul2(p[j][u], e[u]);
-        sy = u ? fma2(hh, C2[u], sy) : mul2(hh, C2[u]);
-        sb = u ? fma2(e[u], B2[u], sb) : mul2(e[u], B2[u]);
-        sa = u ? fma2(g, A2[u], sa) : mul2(g, A2[u]);
-        dA[u] = fma2(f2(dd.x), g, dA[u]);
-        e[u] = mul2(da[j][u], e[u]);
-      }
-      vy[i] = sy.x + sy.y;
-      vb[i] = sb.x + sb.y;
-      va[i] = sa.x + sa.y;
-      if constexpr (EDGE) {
-        const int n = s.edges.begin[r];
-        if (n >= 0) {
-          if (a.dh0) store_states(a.dh0 + ((int64_t)n * a.D + t.d) * a.N, a.N, 4 * t.l, t.on, e);
-          e[0] = e[1] = f2(0.f);
-        }
-      }
-      sum_channels<L>(v, s.bc[warp][r], lane);
-    }
-    const float ry = sum_transposed<L, R>(vy, t.l), rb = sum_transposed<L, R>(vb, t.l);
-    const float ra = sum_transposed<L, R>(va, t.l);
-    if (t.l < R) {
-      const int r = q + k + t.l;
-      s.y[r][t.mc] = ry;
-      s.sb[r][t.mc] = rb;
-      s.sa[r][t.mc] = ra;
-    }
+  for (int i = 0; i < 2; ++i) {
+    da[i] = exp2_2(scale2(x.d[i], A2[i]));
+    p[i] = mul2(da[i], h[i]);
+    h[i] = scale_add2(x.u[i], B, p[i]);
   }
 }
 
+// Four rows from q on: their states again, then back through them.
 template <bool EDGE, typename T, int L>
-__device__ __forceinline__ void bwd_rows(const SelArgs& a, SelBwdShared<T, L>& s, const SelTile<T, L>& t,
+__device__ __forceinline__ void bwd_rows(const SelArgs& a, SelBwdShared<T, L>& s, const BwdLane<L>& t, int q,
                                          const float2 (&A2)[2], const float2 (&h0)[2], float2 (&e)[2],
                                          float2 (&dA)[2]) {
-  float2 h[2] = {h0[0], h0[1]}, da[2], p[2];
-#pragma unroll 2
-  for (int r = 0; r < kHalf; ++r) state_row<EDGE>(a, s, t, r, A2, h, da, p);
-  bwd_half<EDGE>(a, s, t, kHalf, A2, h, e, dA);
-  h[0] = h0[0];
-  h[1] = h0[1];
-  bwd_half<EDGE>(a, s, t, 0, A2, h, e, dA);
+  using W = BwdLane<L>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = lane & 3;
+  // the columns 2 k, 2 k + 1 of a product belong to the set k / (4 / SETS); with one
+  // set all are equal, and two lanes write the same
+  const int which = k & 1;  // 0: dB, 1: dC
+  const bool writes = W::SETS == 1 || k / (4 / W::SETS) == t.set;
+  float* const to_bc = &s.bc[warp][0][which][0][lane >> 2];
+  float2 h[2] = {h0[0], h0[1]}, da[kHeld][2], p[kHeld][2];
+  BwdRow x[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) x[j].load(s, t, q + j);
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) state_row<EDGE>(a, s, t, q + j, x[j], A2, h, da[j], p[j]);
+#pragma unroll
+  for (int j = kHeld - 1; j >= 0; --j) {
+    const int r = q + j, at = r & (kHalf - 1);
+    const float2 B = *reinterpret_cast<const float2*>(s.b + r * SelTile<L>::NL + 2 * t.l), C = *reinterpret_cast<const float2*>(s.c + r * SelTile<L>::NL + 2 * t.l);
+    const float2 o = *reinterpret_cast<const float2*>(&s.o[r][t.mc]);
+    if constexpr (EDGE) {
+      const int n = s.edges.end[r];
+      if (n >= 0) t.load(a.dht ? a.dht + (int64_t)n * a.D * a.N : nullptr, a.N, e);
+    }
+    float2 hh[2], v[3];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      hh[i] = scale_add2(x[j].u[i], B, p[j][i]);
+      e[i] = scale_add2(i ? o.y : o.x, C, e[i]);
+    }
+    float sb[4], sc[4];
+    sum_channels<T>(sb, e, x[j].u[0], x[j].u[1]);
+    sum_channels<T>(sc, hh, o.x, o.y);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 g = mul2(p[j][i], e[i]);
+      (i ? v[0].y : v[0].x) = fmaf(hh[i].y, C.y, hh[i].x * C.x);
+      (i ? v[1].y : v[1].x) = fmaf(e[i].y, B.y, e[i].x * B.x);
+      (i ? v[2].y : v[2].x) = fmaf(g.y, A2[i].y, g.x * A2[i].x);
+      dA[i] = scale_add2(x[j].d[i], g, dA[i]);
+      e[i] = mul2(da[j][i], e[i]);
+    }
+    const int mine = (t.mc >> 1) * W::G + t.l;
+    s.share[0][at][mine] = v[1];
+    s.share[1][at][mine] = v[2];
+    const bool odd = t.l & 1;
+    s.share_y[at][mine] = (odd ? v[0].y : v[0].x) + __shfl_xor_sync(0xffffffffu, odd ? v[0].x : v[0].y, 4);
+    if (writes) {
+      to_bc[at * 32] = which ? sc[0] : sb[0];
+      to_bc[at * 32 + 8] = which ? sc[2] : sb[2];
+    }
+    if constexpr (EDGE) {
+      const int n = s.edges.begin[r];
+      if (n >= 0) {
+        if (a.dh0) t.store(a.dh0 + (int64_t)n * a.D * a.N, a.N, e);
+        e[0] = e[1] = f2(0.f);
+      }
+    }
+  }
 }
 
 // LOCAL: only e, from zero behind the chunk to what it is in front of it.
 template <bool EDGE, typename T, int L>
-__device__ __forceinline__ void bwd_rows_local(const SelArgs& a, SelBwdShared<T, L>& s, const SelTile<T, L>& t,
-                                               const float2 (&A2)[2], float2 (&e)[2], float& dsum) {
-  using S = SelTile<T, L>;
-#pragma unroll 4
+__device__ __forceinline__ void bwd_rows_local(const SelArgs& a, SelBwdShared<T, L>& s, const BwdLane<L>& t,
+                                               const float2 (&A2)[2], float2 (&e)[2], float2& dsum) {
+#pragma unroll 8
   for (int r = kSub - 1; r >= 0; --r) {
-    const float2 dd = s.dd[r][t.mc];
-    const float o = s.o[r][t.mc];
-    const float4 C = *reinterpret_cast<const float4*>(s.c + r * S::NL + 4 * t.l);
+    const float2 C = *reinterpret_cast<const float2*>(s.c + r * SelTile<L>::NL + 2 * t.l);
+    const float2 o = *reinterpret_cast<const float2*>(&s.o[r][t.mc]);
+    const float4 v = *reinterpret_cast<const float4*>(&s.dd[r][t.mc]);
     if constexpr (EDGE) {
       const int n = s.edges.end[r];
-      if (n >= 0)
-        load_states(a.dht ? a.dht + ((int64_t)n * a.D + t.d) * a.N : nullptr, a.N, 4 * t.l, t.on, e);
+      if (n >= 0) t.load(a.dht ? a.dht + (int64_t)n * a.D * a.N : nullptr, a.N, e);
     }
-    e[0] = mul2(decay2(dd.x, A2[0]), fma2(f2(o), make_float2(C.x, C.y), e[0]));
-    e[1] = mul2(decay2(dd.x, A2[1]), fma2(f2(o), make_float2(C.z, C.w), e[1]));
-    dsum += dd.x;
+    e[0] = mul2(exp2_2(scale2(v.x, A2[0])), scale_add2(o.x, C, e[0]));
+    e[1] = mul2(exp2_2(scale2(v.z, A2[1])), scale_add2(o.y, C, e[1]));
+    dsum = add2(dsum, make_float2(v.x, v.z));
     if constexpr (EDGE)
       if (s.edges.begin[r] >= 0) e[0] = e[1] = f2(0.f);
   }
 }
 
+// The sum of the G shares of a pair; neighbours start at different places, which
+// spreads them over the banks.
+template <int G> __device__ __forceinline__ float2 sum_pairs(const float2* p, int pair) {
+  float2 f = f2(0.f);
+#pragma unroll
+  for (int i = 0; i < G / 2; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(p + 2 * (i ^ ((pair >> 1) & (G / 2 - 1))));
+    f = add2(f, add2(lo2(v), hi2(v)));
+  }
+  return f;
+}
+
 template <typename T, int L, bool LOCAL>
-__global__ void __launch_bounds__(kSelThreads, LOCAL ? 4 : 3) k_sel_bwd(const SelArgs a) {
-  using S = SelTile<T, L>;
+__global__ void __launch_bounds__(kSelThreads, 4) k_sel_bwd(const SelArgs a) {
+  using S = SelTile<L>;
+  using W = BwdLane<L>;
   extern __shared__ __align__(16) char raw_shared[];
   SelBwdShared<T, L>& s = *reinterpret_cast<SelBwdShared<T, L>*>(raw_shared);
   const int bc = blockIdx.x / a.tiles;
   const S t(a, blockIdx.x - bc * a.tiles);
   const SelSpan sp = sel_span(a, bc);
   if (LOCAL && sp.c == 0) return;  // nothing is in front of the first
-  float2 A2[2], e[2];
-  t.load_rates(a, A2);
-  float dsum = 0.f;
-  if (LOCAL || sp.c + 1 == a.chunks) e[0] = e[1] = f2(0.f);
-  else load_states4(a.carry + ((int64_t)bc * a.D + t.d) * a.NP, a.NP, 4 * t.l, t.on, e);
-  const float bias = a.bias && t.sc < t.nch ? a.bias[t.d0 + t.sc] : 0.f;
-  const float skip = a.Dk && t.sc < t.nch ? a.Dk[t.d0 + t.sc] : 0.f;
-  LongSum sum_a[4], sum_d, sum_bias;
-  SelSeq seq = seq_of(a, sp.b, sp.hi - 1);
+  const int last = (sp.rows - 1) / kSub * kSub;  // the last 16 rows' first
+  const bool vec = start_copies<T, L, true>(a, t, s, sp.lo + last);
+  request_copies(a, s, 0, sp.rows - last, vec);
+  const W lane(t);
+  float2 A2[2], e[2] = {f2(0.f), f2(0.f)}, dsum = f2(0.f);
+  lane.load(a.A, a.N, A2);
+  A2[0] = mul2(A2[0], f2(kLog2e));
+  A2[1] = mul2(A2[1], f2(kLog2e));
+  const int64_t states = (int64_t)a.D * a.NP;
+  if (!LOCAL && sp.c + 1 < a.chunks) lane.load_packed(a.carry + bc * states, a.NP, e);
+  if (threadIdx.x < S::PAIRS) {
+    s.par[0][threadIdx.x] = t.pair_of(a.bias);
+    s.par[1][threadIdx.x] = t.pair_of(a.Dk);
+  }
+  s.sum_a.clear();
+  s.sum_d.clear();
+  SelSides side(a, sp, sp.rows - 1);
+  bool whole = false, whole_dt = false;
+  const float* keep = nullptr;
+  int64_t out = 0;       // of the pair in the block's results
+  float* to_part = nullptr;
+  float2 dA[2] = {f2(0.f), f2(0.f)}, dd = f2(0.f), db = f2(0.f);
+  int held = 0;          // blocks in these sums
+  // what this thread adds up of the warps' dB and dC
+  const int bc_v = threadIdx.x % (2 * S::NL), bc_row = threadIdx.x / (2 * S::NL);
+  const int bc_n = bc_v % S::NL, bc_l = bc_n >> 1;
+  const float* const from_bc =
+      &s.bc[W::BLOCKS > 1 ? bc_l >> 3 : 0][bc_row][bc_v / S::NL][bc_n & 1][W::G < 8 ? bc_l : bc_l & 7];
+  if constexpr (!LOCAL) {
+    keep = a.saved + block_states(a, sp.b, sp.lo + last);
+    out = (sp.lo + last + t.pr) * a.D + t.d0 + t.pc;
+    to_part = a.part_bc + (((int64_t)t.tile * a.B * a.T + sp.lo + last + bc_row) * 2 + bc_v / S::NL) * a.N + bc_n;
+    whole = t.template whole<T>(a.dx, a.D) && (!a.z || t.template whole<T>(a.dz, a.D));
+    whole_dt = a.dt_f32 ? t.template whole<float>(a.ddt, a.D) : t.template whole<T>(a.ddt, a.D);
+  }
 
-  const int64_t n_sub = (sp.hi - sp.lo + kSub - 1) / kSub;
-  for (int64_t k = n_sub - 1; k >= 0; --k) {
-    const int64_t r0 = sp.lo + k * kSub;
-    const bool edge = seq.lo >= r0 || seq.hi <= r0 + kSub;
-    float x[S::PER], pre[S::PER], dy[S::PER], z[S::PER];
-    {
-      float vb[S::VPT], vc[S::VPT];
-      t.load_tokens(a.x, false, a.ldx, r0, sp.hi, x);
-      t.load_tokens(a.dt, a.dt_f32, a.lddt, r0, sp.hi, pre);
-      t.load_tokens(a.dy, false, a.lddy, r0, sp.hi, dy);
-      if (a.z) t.load_tokens(a.z, false, a.ldz, r0, sp.hi, z);
-      if constexpr (!LOCAL) t.load_vectors(a, a.Bv, a.ldb, r0, sp.hi, vb);
-      t.load_vectors(a, a.Cv, a.ldc, r0, sp.hi, vc);
-      if constexpr (!LOCAL) t.put_vectors(s.b, vb);
-      t.put_vectors(s.c, vc);
+  int at = 0;
+  for (int r0 = last; r0 >= 0; r0 -= kSub, at ^= 1) {
+    const SelRaw<T, L, true>& raw = s.raw[at];
+    const bool edge = side.lo >= r0 || side.hi <= r0 + kSub;
+    const int rows = sp.rows - r0;  // from here on
+    copies_done();
+    __syncthreads();
+    if (r0 > 0) request_copies(a, s, at ^ 1, kSub, vec);
+    float2 hs[kSub / kHeld][2];
+    if constexpr (!LOCAL) {
+      lane.load_packed(keep, a.NP, hs[0]);
+      keep -= states;
     }
-    float2 h0[2];
-    if constexpr (!LOCAL)
-      load_states4(a.saved + (((int64_t)sp.b * a.subs + (r0 - (int64_t)sp.b * a.T) / kSub) * a.D + t.d) * a.NP,
-                   a.NP, 4 * t.l, t.on, h0);
-    float dt[S::PER], sig[S::PER];
+    const float2 bias = s.par[0][t.pc >> 1];
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) {
-      pre[i] += bias;
-      dt[i] = a.softplus ? softplus_f(pre[i]) : pre[i];
-      if (r0 + t.sr + L * i >= sp.hi) dt[i] = 0.f;
-      s.dd[t.sr + L * i][t.sc] = make_float2(dt[i], dt[i] * x[i]);
-      float o = dy[i];
+      const int row = t.pr + i * S::STEP;
+      if (S::STEP > kSub && row >= kSub) break;
+      const int p = row * S::CH + t.pc;
+      float2 d = add2((a.dt_f32 ? pair_at(s.dt32.v[at] + p) : raw.dt(p)), bias);
+      if (a.softplus) d = softplus2(d);
+      if (row >= rows) d = f2(0.f);
+      const float2 u = LOCAL ? d : mul2(d, raw.x(p));
+      *reinterpret_cast<float4*>(&s.dd[row][t.pc]) = make_float4(d.x, u.x, d.y, u.y);
+      float2 o = raw.dy(p);
       if (a.z) {
-        sig[i] = sigmoid_of<T>(z[i]);
-        o *= z[i] * sig[i];
+        const float2 z = raw.z(p);
+        o = mul2(o, mul2(z, sigmoid2(z)));
       }
-      s.o[t.sr + L * i][t.sc] = o;
+      *reinterpret_cast<float2*>(&s.o[row][t.pc]) = o;
     }
-    if (edge) mark_edges(a, s.edges, sp.b, r0, sp.hi);
+    if constexpr (!LOCAL) widen<T, L>(s.b, raw.vec);
+    widen<T, L>(s.c, raw.vec + kSub * S::NL);
+    if (edge) mark_edges(a, s.edges, sp.b, sp.lo + r0, sp.lo + sp.rows);
     __syncthreads();
     if constexpr (LOCAL) {
-      if (edge) bwd_rows_local<true>(a, s, t, A2, e, dsum);
-      else bwd_rows_local<false>(a, s, t, A2, e, dsum);
+      if (edge) bwd_rows_local<true>(a, s, lane, A2, e, dsum);
+      else bwd_rows_local<false>(a, s, lane, A2, e, dsum);
     } else {
-      float2 dA[2] = {f2(0.f), f2(0.f)};
-      if (edge) bwd_rows<true>(a, s, t, A2, h0, e, dA);
-      else bwd_rows<false>(a, s, t, A2, h0, e, dA);
-      sum_a[0].add(dA[0].x);
-      sum_a[1].add(dA[0].y);
-      sum_a[2].add(dA[1].x);
-      sum_a[3].add(dA[1].y);
-    }
-    if (edge && r0 > sp.lo) seq = seq_of(a, sp.b, r0 - 1);
-    __syncthreads();
-    if constexpr (!LOCAL) {
-      float dd = 0.f, db = 0.f;
+      // the states in front of every four rows
 #pragma unroll
-      for (int i = 0; i < S::PER; ++i) {
-        const int rr = t.sr + L * i;
-        const int64_t r = r0 + rr;
-        const float sb = s.sb[rr][t.sc], sa = s.sa[rr][t.sc] * kSelLn2, o = s.o[rr][t.sc];
-        float ddt = fmaf(x[i], sb, sa);
-        if (a.softplus) ddt *= sigmoid_of<float>(pre[i]);
-        if (r < sp.hi && t.sc < t.nch) {
-          const int64_t at = r * a.D + t.d0 + t.sc;
-          ((T*)a.dx)[at] = from_f<T>(fmaf(dt[i], sb, skip * o));
-          if (a.dt_f32) ((float*)a.ddt)[at] = ddt;
-          else ((T*)a.ddt)[at] = from_f<T>(ddt);
-          if (a.z) {
-            const float y = fmaf(skip, x[i], s.y[rr][t.sc]);
-            ((T*)a.dz)[at] = from_f<T>(dy[i] * y * sig[i] * fmaf(z[i], 1.f - sig[i], 1.f));
-          }
-          dd = fmaf(o, x[i], dd);
-          db += ddt;
+      for (int k = 1; k < kSub / kHeld; ++k) {
+        float2 da[2], p[2];
+        hs[k][0] = hs[k - 1][0];
+        hs[k][1] = hs[k - 1][1];
+#pragma unroll
+        for (int r = (k - 1) * kHeld; r < k * kHeld; ++r) {
+          BwdRow x;
+          x.load(s, lane, r);
+          if (edge) state_row<true>(a, s, lane, r, x, A2, hs[k], da, p);
+          else state_row<false>(a, s, lane, r, x, A2, hs[k], da, p);
         }
       }
-      sum_d.add(dd);
-      sum_bias.add(db);
-      // this CTA's share of dB and dC
-      for (int i = threadIdx.x; i < kSub * 2 * S::NL; i += kSelThreads) {
-        const int rr = i / (2 * S::NL), v = i % (2 * S::NL), n = v % S::NL;
-        if (r0 + rr >= sp.hi || n >= a.N) continue;
-        float f = s.bc[0][rr][v];
+#pragma unroll 1
+      for (int q = kHalf; q >= 0; q -= kHalf) {
 #pragma unroll
-        for (int w = 1; w < kSelWarps; ++w) f += s.bc[w][rr][v];
-        a.part_bc[(((int64_t)t.tile * a.B * a.T + r0 + rr) * 2 + v / S::NL) * a.N + n] = f;
+        for (int k = kHalf / kHeld - 1; k >= 0; --k) {
+          const float2 h[2] = {q ? hs[k + kHalf / kHeld][0] : hs[k][0], q ? hs[k + kHalf / kHeld][1] : hs[k][1]};
+          if (edge) bwd_rows<true>(a, s, lane, q + k * kHeld, A2, h, e, dA);
+          else bwd_rows<false>(a, s, lane, q + k * kHeld, A2, h, e, dA);
+        }
+        __syncthreads();
+        const float2 bias = s.par[0][t.pc >> 1], skip = s.par[1][t.pc >> 1];
+#pragma unroll
+        for (int m = 0; m < S::PER_HALF; ++m) {
+          const int j = t.pr + m * S::STEP;
+          if (S::STEP > kHalf && j >= kHalf) break;
+          const int row = q + j, p = row * S::CH + t.pc, pair = t.pc >> 1;
+          if (row >= rows) break;
+          const float2 sum[3] = {
+              sum_pairs<W::G / 2>(reinterpret_cast<const float2*>(s.share_y[j] + pair * W::G), pair),
+              sum_pairs<W::G>(s.share[0][j] + pair * W::G, pair),
+              sum_pairs<W::G>(s.share[1][j] + pair * W::G, pair)};
+          const float2 x = raw.x(p), pre = add2((a.dt_f32 ? pair_at(s.dt32.v[at] + p) : raw.dt(p)), bias);
+          const float4 du = *reinterpret_cast<const float4*>(&s.dd[row][t.pc]);
+          const float2 dt = make_float2(du.x, du.z);
+          const float2 o = *reinterpret_cast<const float2*>(&s.o[row][t.pc]);
+          float2 ddt = fma2(x, sum[1], mul2(sum[2], f2(kSelLn2)));
+          if (a.softplus) ddt = mul2(ddt, sigmoid2(pre));
+          const int64_t r = out + (q + m * S::STEP) * a.D;
+          t.store_pair((T*)a.dx + r, whole, fma2(dt, sum[1], mul2(skip, o)));
+          if (a.dt_f32) t.store_pair((float*)a.ddt + r, whole_dt, ddt);
+          else t.store_pair((T*)a.ddt + r, whole_dt, ddt);
+          if (a.z) {
+            const float2 z = raw.z(p), sig = sigmoid2(z), dy = raw.dy(p);
+            // silu'(z) = sig + z sig (1 - sig)
+            const float2 f = fma2(mul2(z, sig), add2(f2(1.f), neg2(sig)), sig);
+            t.store_pair((T*)a.dz + r, whole, mul2(mul2(dy, fma2(skip, x, sum[0])), f));
+          }
+          dd = fma2(o, x, dd);
+          db = add2(db, ddt);
+        }
+        // this CTA's share of dB and dC: a thread's state is the same for all rows
+#pragma unroll
+        for (int m = 0; m < S::BC_ROWS; ++m) {
+          if (q + bc_row + m * S::BC_STEP >= rows || bc_n >= a.N) break;
+          float f = 0.f;
+#pragma unroll
+          for (int w = 0; w < kSelWarps / W::BLOCKS; ++w)
+#pragma unroll
+            for (int k = 0; k < W::SETS; ++k)
+              f += from_bc[(w * W::BLOCKS * kHalf + m * S::BC_STEP) * 32 + k * W::G];
+          to_part[(q + m * S::BC_STEP) * 2 * a.N] = f;
+        }
+        if (q) __syncthreads();
+      }
+      out -= (int64_t)kSub * a.D;
+      to_part -= kSub * 2 * a.N;
+      if (++held == 16 || r0 == 0) {
+        s.sum_a.add(dA[0], dA[1]);
+        s.sum_d.add(dd, db);
+        dA[0] = dA[1] = dd = db = f2(0.f);
+        held = 0;
       }
     }
+    if (edge && r0 > 0) side = SelSides(a, sp, r0 - 1);
   }
   if constexpr (LOCAL) {
-    store_states4(a.carry + ((int64_t)bc * a.D + t.d) * a.NP, a.NP, 4 * t.l, t.on, e);
-    if (t.l == 0 && t.on) a.decay[(int64_t)bc * a.D + t.d] = dsum;
+    lane.store_packed(a.carry + bc * states, a.NP, e);
+    if (lane.l == 0) {
+      if (lane.on[0]) a.decay[(int64_t)bc * a.D + lane.d] = dsum.x;
+      if (lane.on[1]) a.decay[(int64_t)bc * a.D + lane.d + 1] = dsum.y;
+    }
   } else {
-    const float2 g[2] = {make_float2(sum_a[0].get(), sum_a[1].get()),
-                         make_float2(sum_a[2].get(), sum_a[3].get())};
-    store_states4(a.part_a + ((int64_t)bc * a.D + t.d) * a.NP, a.NP, 4 * t.l, t.on, g);
-    s.fold[0][threadIdx.x] = sum_d.get();
-    s.fold[1][threadIdx.x] = sum_bias.get();
+    const float4 f = s.sum_a.v[threadIdx.x];
+    const float2 g[2] = {lo2(f), hi2(f)};
+    lane.store_packed(a.part_a + bc * states, a.NP, g);
     __syncthreads();
-    if (threadIdx.x < t.nch) {
-      float x = 0.f, y = 0.f;
+    if (threadIdx.x < S::PAIRS) {  // threads PAIRS apart staged the same pair
+      float4 f = s.sum_d.v[threadIdx.x];
 #pragma unroll
-      for (int i = 0; i < L; ++i) {
-        x += s.fold[0][threadIdx.x + i * S::CH];
-        y += s.fold[1][threadIdx.x + i * S::CH];
+      for (int i = 1; i < S::STEP; ++i) {
+        const float4 v = s.sum_d.v[threadIdx.x + i * S::PAIRS];
+        f = make_float4(f.x + v.x, f.y + v.y, f.z + v.z, f.w + v.w);
       }
-      const int64_t n = (int64_t)a.B * a.chunks * a.D, at = (int64_t)bc * a.D + t.d0 + threadIdx.x;
-      a.part_d[at] = x;
-      a.part_d[n + at] = y;
+      const int64_t n = (int64_t)a.B * a.chunks * a.D, to = (int64_t)bc * a.D + t.d0 + t.pc;
+      if (t.pc < t.nch) {
+        a.part_d[to] = f.x;
+        a.part_d[n + to] = f.z;
+      }
+      if (t.pc + 1 < t.nch) {
+        a.part_d[to + 1] = f.y;
+        a.part_d[n + to + 1] = f.w;
+      }
     }
   }
 }
@@ -721,6 +1088,31 @@ __global__ void __launch_bounds__(256) k_sel_params(const SelArgs a, float* dA, 
 // ---------------------------------------------------------------------------
 // one token
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ void load_four(const float* p, int N, int n0, bool vec, float2 (&h)[2]) {
+  if (vec) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (n0 < N) v = *reinterpret_cast<const float4*>(p + n0);
+    h[0] = make_float2(v.x, v.y);
+    h[1] = make_float2(v.z, v.w);
+  } else {
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = n0 + i < N ? p[n0 + i] : 0.f;
+    h[0] = make_float2(f[0], f[1]);
+    h[1] = make_float2(f[2], f[3]);
+  }
+}
+__device__ __forceinline__ void store_four(float* p, int N, int n0, bool vec, const float2 (&h)[2]) {
+  if (vec) {
+    if (n0 < N) *reinterpret_cast<float4*>(p + n0) = make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
+  } else {
+    const float f[4] = {h[0].x, h[0].y, h[1].x, h[1].y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n0 + i < N) p[n0 + i] = f[i];
+  }
+}
+
 // Every lane has four states of a channel.
 template <typename T, int L>
 __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float* state, int64_t stride,
@@ -740,13 +1132,8 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float
                    (reinterpret_cast<uintptr_t>(a.A) & 15) == 0;
   float x = 0.f, dt = 0.f;
   if (on) {
-    if (vec) {
-      load_states4(p, a.N, 4 * l, true, h);
-      load_states4(a.A + (int64_t)d * a.N, a.N, 4 * l, true, A2);
-    } else {
-      load_states(p, a.N, 4 * l, true, h);
-      load_states(a.A + (int64_t)d * a.N, a.N, 4 * l, true, A2);
-    }
+    load_four(p, a.N, 4 * l, vec, h);
+    load_four(a.A + (int64_t)d * a.N, a.N, 4 * l, vec, A2);
     x = to_f<T>(((const T*)a.x)[n * a.ldx + d]);
     dt = a.dt_f32 ? ((const float*)a.dt)[n * a.lddt + d] : to_f<T>(((const T*)a.dt)[n * a.lddt + d]);
     if (a.bias) dt += a.bias[d];
@@ -767,21 +1154,18 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float
   for (int u = 0; u < 2; ++u) {
     B[u] = make_float2(b[2 * u], b[2 * u + 1]);
     C[u] = make_float2(c[2 * u], c[2 * u + 1]);
-    h[u] = fma2(decay2(dt, mul2(A2[u], f2(kLog2e))), h[u], mul2(f2(dt * x), B[u]));
+    h[u] = fma2(exp2_2(mul2(f2(dt), mul2(A2[u], f2(kLog2e)))), h[u], mul2(f2(dt * x), B[u]));
     const float2 o = mul2(h[u], C[u]);
     out += o.x + o.y;
   }
-  if (on) {
-    if (vec) store_states4(p, a.N, 4 * l, true, h);
-    else store_states(p, a.N, 4 * l, true, h);
-  }
+  if (on) store_four(p, a.N, 4 * l, vec, h);
 #pragma unroll
   for (int o = L / 2; o > 0; o /= 2) out += __shfl_xor_sync(0xffffffffu, out, o);
   if (on && l == 0) {
     if (a.Dk) out = fmaf(a.Dk[d], x, out);
     if (a.z) {
       const float z = to_f<T>(((const T*)a.z)[n * a.ldz + d]);
-      out *= z * sigmoid_of<T>(z);
+      out *= z * sigmoid_f(z);
     }
     ((T*)a.y)[(int64_t)n * a.D + d] = from_f<T>(out);
   }
@@ -873,10 +1257,23 @@ SelArgs sel_args(const gdn2_selective_problem* p, const SelPlan& q) {
   a.B = p->B; a.D = p->D; a.G = p->G; a.N = p->N; a.NP = (p->N + 3) / 4 * 4; a.n_seqs = p->n_seqs;
   a.T = p->T; a.cu = p->cu_seqlens;
   a.ldx = p->ld_x; a.lddt = p->ld_dt; a.ldz = p->ld_z; a.ldb = p->ld_b; a.ldc = p->ld_c; a.lddy = p->ld_dy;
-  a.dt_f32 = p->dt_dtype == GDN2_DTYPE_F32; a.softplus = p->dt_softplus != 0;
+  a.dt_f32 = p->dt_dtype == GDN2_DTYPE_F32 && p->dtype != GDN2_DTYPE_F32; a.softplus = p->dt_softplus != 0;
   a.chunk = q.chunk; a.subs = q.subs; a.chunks = q.chunks;
   a.tiles_per_group = q.tiles_per_group; a.tiles = q.tiles;
   return a;
+}
+
+// The tensors that come in by rows; dy NULL in the forward.
+void sel_sources(SelArgs& a, const void* x, const void* dy, const void* z, const void* dt, const void* Bv,
+                 const void* Cv) {
+  int k = 0;
+  a.tok[k++] = SelSource{x, a.ldx};
+  if (dy) a.tok[k++] = SelSource{dy, a.lddy};
+  a.tok[k++] = SelSource{z, a.ldz};
+  a.tok[k++] = SelSource{a.dt_f32 ? nullptr : dt, a.lddt};
+  a.dt32 = SelSource{a.dt_f32 ? dt : nullptr, a.lddt};
+  a.vec[0] = SelSource{Bv, a.ldb};
+  a.vec[1] = SelSource{Cv, a.ldc};
 }
 
 // f(T{}, integral_constant<L>)
@@ -899,6 +1296,15 @@ cudaError_t pass_states(const gdn2_selective_problem* p, const float* from, floa
   if (!to || !some || !bytes) return cudaSuccess;
   return from ? cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st)
               : cudaMemsetAsync(to, 0, bytes, st);
+}
+
+unsigned carry_grid(const SelArgs& a) {
+  return (unsigned)((int64_t)a.B * (((int64_t)a.D * a.NP + 255) / 256));
+}
+
+template <typename K> cudaError_t allow_shared(K local, K full, int bytes) {
+  const cudaError_t e = cudaFuncSetAttribute(full, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? cudaFuncSetAttribute(local, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : e;
 }
 
 bool too_many(int64_t ctas) { return ctas > 2147483647LL; }
@@ -944,7 +1350,8 @@ int gdn2_selective_fwd(const gdn2_selective_problem* p, const void* x, const voi
   if (e != cudaSuccess) return cuda_status(e, fn);
   if (!some) return GDN2_OK;
   SelArgs a = sel_args(p, q);
-  a.x = x; a.dt = dt; a.A = A; a.Bv = Bv; a.Cv = Cv; a.Dk = D; a.z = z; a.bias = dt_bias; a.h0 = h0;
+  sel_sources(a, x, nullptr, z, dt, Bv, Cv);
+  a.A = A; a.Dk = D; a.z = z; a.bias = dt_bias; a.h0 = h0;
   a.y = y; a.ht = ht; a.saved = saved;
   if (w.total) {
     a.carry = (float*)((char*)workspace + w.carry);
@@ -953,12 +1360,19 @@ int gdn2_selective_fwd(const gdn2_selective_problem* p, const void* x, const voi
   return cuda_status(with_lanes(p->dtype, p->N, [&](auto t, auto lanes) {
     using T = decltype(t);
     constexpr int L = decltype(lanes)::value;
+    constexpr int most = (int)sizeof(SelFwdShared<T, L>);
+    const int smem = a.dt_f32 ? most : SelFwdShared<T, L>::without_dt32();
+    auto local = k_sel_fwd<T, L, true>;
+    auto full = k_sel_fwd<T, L, false>;
+    cudaError_t e = allow_shared(local, full, most);
+    if (e != cudaSuccess) return e;
     if (q.chunks > 1) {
-      k_sel_fwd<T, L, true><<<(unsigned)ctas, kSelThreads, 0, st>>>(a);
-      const int64_t n = (int64_t)a.B * a.D * a.NP;
-      k_sel_carry<false><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+      SelArgs b = a;  // the states need no z and no C
+      b.tok[1].p = b.vec[1].p = nullptr;
+      local<<<(unsigned)ctas, kSelThreads, smem, st>>>(b);
+      k_sel_carry<false><<<carry_grid(a), 256, 0, st>>>(a);
     }
-    k_sel_fwd<T, L, false><<<(unsigned)ctas, kSelThreads, 0, st>>>(a);
+    full<<<(unsigned)ctas, kSelThreads, smem, st>>>(a);
     return cudaGetLastError();
   }), fn);
 }
@@ -994,8 +1408,9 @@ int gdn2_selective_bwd(const gdn2_selective_problem* p, const void* x, const voi
     return cuda_status(e, fn);
   }
   SelArgs a = sel_args(p, q);
-  a.x = x; a.dt = dt; a.A = A; a.Bv = Bv; a.Cv = Cv; a.Dk = D; a.z = z; a.bias = dt_bias; a.h0 = h0;
-  a.saved = const_cast<float*>(saved); a.dy = dy; a.dht = dht;
+  sel_sources(a, x, dy, z, dt, Bv, Cv);
+  a.A = A; a.Dk = D; a.z = z; a.bias = dt_bias; a.h0 = h0;
+  a.saved = const_cast<float*>(saved); a.dht = dht;
   a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dh0;
   char* ws = (char*)workspace;
   a.carry = (float*)(ws + w.carry); a.decay = (float*)(ws + w.decay);
@@ -1003,17 +1418,17 @@ int gdn2_selective_bwd(const gdn2_selective_problem* p, const void* x, const voi
   return cuda_status(with_lanes(p->dtype, p->N, [&](auto t, auto lanes) {
     using T = decltype(t);
     constexpr int L = decltype(lanes)::value;
-    constexpr int smem = (int)sizeof(SelBwdShared<T, L>);
+    constexpr int most = (int)sizeof(SelBwdShared<T, L>);
+    const int smem = a.dt_f32 ? most : SelBwdShared<T, L>::without_dt32();
     auto local = k_sel_bwd<T, L, true>;
     auto full = k_sel_bwd<T, L, false>;
-    cudaError_t e = cudaFuncSetAttribute(full, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(local, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_shared(local, full, most);
     if (e != cudaSuccess) return e;
     if (q.chunks > 1) {
-      local<<<(unsigned)ctas, kSelThreads, smem, st>>>(a);
-      const int64_t n = (int64_t)a.B * a.D * a.NP;
-      k_sel_carry<true><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+      SelArgs b = a;  // the states' gradients need no x and no B
+      b.tok[0].p = b.vec[0].p = nullptr;
+      local<<<(unsigned)ctas, kSelThreads, smem, st>>>(b);
+      k_sel_carry<true><<<carry_grid(a), 256, 0, st>>>(a);
     }
     full<<<(unsigned)ctas, kSelThreads, smem, st>>>(a);
     k_sel_vectors<T><<<(unsigned)((values + 255) / 256), 256, 0, st>>>(a, (T*)dB, (T*)dC);
