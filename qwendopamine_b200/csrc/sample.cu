@@ -9,21 +9,26 @@
 //
 // A token far down the vocabulary may hold a millionth of the sum, so whether
 // the running sum has passed the target is decided by digits that fp32 does not
-// have: weights and sums are fp64 (2^y from a table of 16 roots and the Taylor
+// have: weights and sums are fp64 (2^-y from a table of 16 roots and the Taylor
 // polynomial of 2^f, |f| <= 1/32, to f^5: 2e-13 relative).  Sums are formed in a
 // fixed order or as whole numbers: equal inputs give equal tokens.
 //
-// Top-k and top-p need no sort of the row.  A histogram over bins of equal width
-// in x (counts, and weights as whole numbers of 2^-44) gives the bin in which the
-// bound lies; what is in the bin, or all down to it where that is a short list,
-// is sorted in shared memory.  A bin with more values than the list holds is cut
-// by the digits of the values' ordered bits, 11 at a time, and among equal values
-// the lower indices are counted out.
+// Top-k, top-p and min-p rarely need more than a short list.  The k-th largest of
+// the threads' largest values bounds the k largest from below, so that a second
+// sweep, which skips most vectors by their largest value, hands a few more than k
+// values to the cluster's first CTA; it sorts them, applies the rules and takes the
+// token.  With min-p alone the list is what min-p keeps, with top-p alone it is
+// about the 512 largest, which have to reach the bound.
+// Where the list does not hold the set, a histogram of the row over bins of equal
+// width in x (counts, and weights as whole numbers of 2^-44) gives the bin in which
+// the bound lies, and what is in the bin is sorted.  A bin with more values than the
+// list holds is cut by the digits of the values' ordered bits, 11 at a time, and
+// among equal values the lower indices are counted out.
 //
 // Bound: by temperature alone the row is read once and the time is that of the
-// fp64 pipe, 11 operations for a value; with a bound the row is read again from
-// L2 for the histogram, the list and the sums.  Few rows are split over the CTAs
-// of a cluster, which exchange through distributed shared memory.
+// fp64 pipe, 12 operations for a value; with a short list the row is read once from
+// memory and once from L2.  Few rows are split over the CTAs of a cluster, which
+// exchange through distributed shared memory.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -40,10 +45,10 @@ namespace {
 
 constexpr int kSmThreads = 512;
 constexpr int kSmWarps = kSmThreads / 32;
-constexpr int kSmUnroll = 4;                   // vectors of a lane in flight
 constexpr int kBins = 2048;
 constexpr int kBinsPer = kBins / kSmThreads;   // bins of a thread
 constexpr int kList = 2048;                    // longest list that is sorted
+constexpr int kQuick = 512;                    // values that a list for top-p alone starts from
 constexpr float kBinsPerUnit = 46.f;           // bins of a logit: 44 units below the maximum
 
 struct SampleArgs {
@@ -76,24 +81,25 @@ struct SampleShared {
   uint32_t warp_count[kSmWarps];
   uint64_t warp_mass[kSmWarps];
   Decision d;
-  int n_list;
+  int n_list, first, reached;
   uint32_t count[kBins];
   uint64_t mass[kBins];
   uint64_t list[kList];
 };
 
-// 2^y for y <= 0 as fp64; 0 below 2^-1022, and for -inf
-__device__ __forceinline__ double pow2_of(const double* root, double y) {
+// 2^-y for y >= 0 as fp64; 0 beyond 1022, for infinity and NaN
+__device__ __forceinline__ double pow2_neg(const double* root, double y) {
   constexpr double magic = 6755399441055744.;  // 1.5 * 2^52: rounds to whole numbers
   constexpr double c1 = 0.69314718055994531, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
                    c5 = c4 * c1 / 5;
-  const double t = fma(y, 16., magic);
+  const double t = fma(y, -16., magic);
   const int k = __double2loint(t);
-  const double f = fma(t - magic, -.0625, y);
+  const double f = fma(t - magic, -.0625, -y);
   double p = fma(fma(fma(fma(fma(c5, f, c4), f, c3), f, c2), f, c1), f, 1.);
   p *= root[k & 15];
   const double w = __hiloint2double(__double2hiint(p) + ((k >> 4) << 20), __double2loint(p));
-  return y >= -1022. ? w : 0.;
+  // numbers that are not negative order as their bits do
+  return (uint32_t)__double2hiint(y) <= 0x408ff000u ? w : 0.;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(uint32_t w, float) { return w & 0x7fffffffu; }
@@ -119,33 +125,38 @@ template <typename T> __device__ __forceinline__ bool bits_are_nan(uint32_t m) {
   }
 }
 
-// Row r of a CTA of a cluster: the vectors [lo, hi) of its warp, in the order of
-// the row (parts, then warps).
+// A CTA's part of a row, in the order of the row: parts, then warps.
 template <typename T> struct RowShare {
   RowView<T> row;
-  int lo, hi, part, parts;
+  int plo, phi, wper, part, parts;
   static constexpr int VE = RowView<T>::VE;
   __device__ __forceinline__ RowShare(const T* p, int V, int part_, int parts_)
       : row(p, V), part(part_), parts(parts_) {
     const int per = (row.nvec + parts - 1) / parts;
-    const int plo = min(part * per, row.nvec), phi = min(plo + per, row.nvec);
-    const int wper = (phi - plo + kSmWarps - 1) / kSmWarps;
-    lo = min(plo + (int)(threadIdx.x >> 5) * wper, phi);
-    hi = min(lo + wper, phi);
+    plo = min(part * per, row.nvec);
+    phi = min(plo + per, row.nvec);
+    wper = (phi - plo + kSmWarps - 1) / kSmWarps;
   }
+  __device__ __forceinline__ int lo(int warp) const { return min(plo + warp * wper, phi); }
   __device__ __forceinline__ int64_t index(int j, int e) const { return (int64_t)j * VE + e - row.off; }
-  // f(vector, its place) for the lane's vectors of the warp's
-  template <typename F> __device__ __forceinline__ void sweep(F&& f) const {
-    const int lane = threadIdx.x & 31;
-    int j = lo + lane;
-    for (; j + (kSmUnroll - 1) * 32 < hi; j += kSmUnroll * 32) {
-      Raw<T, VE> v[kSmUnroll];
+  // f(vector, its place) for the lane's vectors of [lo, hi), U of them in flight
+  template <int U, typename F> __device__ __forceinline__ void sweep(int lo, int hi, F&& f) const {
+    int j = lo + (int)(threadIdx.x & 31);
+    if constexpr (U > 1) {
+      for (; j + (U - 1) * 32 < hi; j += U * 32) {
+        Raw<T, VE> v[U];
 #pragma unroll
-      for (int u = 0; u < kSmUnroll; ++u) v[u] = row.load(j + u * 32);
+        for (int u = 0; u < U; ++u) v[u] = row.load(j + u * 32);
 #pragma unroll
-      for (int u = 0; u < kSmUnroll; ++u) f(v[u], j + u * 32);
+        for (int u = 0; u < U; ++u) f(v[u], j + u * 32);
+      }
     }
+#pragma unroll 1
     for (; j < hi; j += 32) f(row.load(j), j);
+  }
+  template <int U, typename F> __device__ __forceinline__ void sweep(F&& f) const {
+    const int warp = threadIdx.x >> 5;
+    sweep<U>(lo(warp), lo(warp + 1), f);
   }
 };
 
@@ -158,18 +169,42 @@ __device__ __forceinline__ double warp_total(double x) {
 // The parameters of one row, and which values they keep.
 struct RowRule {
   float m;
-  double c, min_y;   // weights 2^((x - m) c); kept from y = min_y
+  double c, most_y;  // weights 2^-y, y = (m - x) c; kept up to y = most_y
   uint64_t bound;    // and from this key
   float tau;         // the bound's value
   bool all_y, all_keys;
   const double* root;
-  __device__ __forceinline__ double weight(float x) const { return pow2_of(root, ((double)x - m) * c); }
+  // falling values have rising bins; the same function wherever a bin is asked for
+  __device__ __forceinline__ int bin(float x) const {
+    return min((int)(__fmul_rn(__fsub_rn(m, x), kBinsPerUnit)), kBins - 1);
+  }
+  __device__ __forceinline__ double weight(float x) const { return pow2_neg(root, ((double)m - x) * c); }
   __device__ __forceinline__ bool keeps(float x, int64_t i) const {
     if (x == -INFINITY) return false;
     if (!all_keys && !(x > tau) && (x < tau || key_of(x, (int)i) < bound)) return false;
-    return all_y || ((double)x - m) * c >= min_y;
+    return all_y || ((double)m - x) * c <= most_y;
   }
 };
+
+// The first of kSmWarps sums with which the running sum, from `before` on, exceeds
+// goal; -1 and `some` the last that is not zero where rounding leaves none.
+__device__ __forceinline__ int which_warp(const double* sums, double goal, double& before, int& some) {
+  double run = before;
+  int who = -1;
+  some = 0;
+  for (int i = 0; i < kSmWarps; ++i) {
+    const double t = sums[i];
+    if (t > 0.) {
+      some = i;
+      if (who < 0 && run + t > goal) {
+        who = i;
+        before = run;
+      }
+    }
+    run += t;
+  }
+  return who;
+}
 
 // The index at which the running sum of f(x, index) >= 0 over the row, in fp64,
 // exceeds target(sum); where rounding leaves none, the last with f > 0.  The
@@ -180,13 +215,16 @@ __device__ __forceinline__ void locate(cg::cluster_group& cluster, SampleShared&
                                        bool have, F&& f, G&& target) {
   constexpr int VE = RowView<T>::VE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (!have) {
+  auto sum_of = [&](int lo, int hi) {
     double mine = 0.;
-    sh.sweep([&](const Raw<T, VE>& v, int j) {
+    sh.template sweep<1>(lo, hi, [&](const Raw<T, VE>& v, int j) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) mine += f(raw_get(v, e), sh.index(j, e));
     });
-    mine = warp_total(mine);
+    return warp_total(mine);
+  };
+  if (!have) {
+    const double mine = sum_of(sh.lo(warp), sh.lo(warp + 1));
     if (lane == 0) s.warp_sum[warp] = mine;
   }
   __syncthreads();
@@ -211,51 +249,56 @@ __device__ __forceinline__ void locate(cg::cluster_group& cluster, SampleShared&
   bool none = owner < 0;
   if (none) owner = last;
   if (owner == sh.part) {
-    // the warp with the target, by the same sums in the same order
-    int who = -1, some = 0;
-    double at = before;
-    if (!none) {
-      double r = before;
-      for (int i = 0; i < kSmWarps; ++i) {
-        const double t = s.warp_sum[i];
-        if (who < 0 && t > 0. && r + t > goal) { who = i; at = r; }
-        r += t;
-      }
-    }
-    for (int i = 0; i < kSmWarps; ++i)
-      if (s.warp_sum[i] > 0.) some = i;
+    // the warp whose vectors have the target, then a sixteenth of them, by the same
+    // sums in the same order
+    int some;
+    int who = which_warp(s.warp_sum, none ? INFINITY : goal, before, some);
     if (who < 0) {
       who = some;
       none = true;
     }
+    int lo = sh.lo(who), hi = sh.lo(who + 1);
+    const int per = (hi - lo + kSmWarps - 1) / kSmWarps;
+    const double mine = sum_of(min(lo + warp * per, hi), min(lo + (warp + 1) * per, hi));
+    __syncthreads();  // the first sums have been read
+    if (lane == 0) s.warp_sum[warp] = mine;
+    __syncthreads();
+    who = which_warp(s.warp_sum, none ? INFINITY : goal, before, some);
+    if (who < 0) {
+      who = some;
+      none = true;
+    }
+    hi = min(lo + (who + 1) * per, hi);
+    lo = min(lo + who * per, hi);
     if (warp == who) {
       int64_t found = -1, tail = -1;  // tail: the last index with a weight
-      for (int j0 = sh.lo; j0 < sh.hi && found < 0; j0 += 32) {
+      double at = before;
+      for (int j0 = lo; j0 < hi && found < 0; j0 += 32) {
         const int j = j0 + lane;
         Raw<T, VE> v;
-        double mine = 0.;
+        double own = 0.;
         int64_t mytail = -1;
-        if (j < sh.hi) {
+        if (j < hi) {
           v = sh.row.load(j);
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
             const double w = f(raw_get(v, e), sh.index(j, e));
             if (w > 0.) mytail = sh.index(j, e);
-            mine += w;
+            own += w;
           }
         }
-        double incl = mine;
+        double incl = own;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
           const double y = __shfl_up_sync(0xffffffffu, incl, o);
           if (lane >= o) incl += y;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, !none && mine > 0. && at + incl > goal);
+        const unsigned hit = __ballot_sync(0xffffffffu, !none && own > 0. && at + incl > goal);
         if (hit) {
           const int l = __ffs(hit) - 1;
           int64_t mineat = -1;
           if (lane == l) {
-            double r = at + (incl - mine);
+            double r = at + (incl - own);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
               const double w = f(raw_get(v, e), sh.index(j, e));
@@ -392,12 +435,13 @@ __device__ __forceinline__ int count_by_mass(SampleShared& s, int n, uint64_t ab
   if (lane == 31) s.warp_mass[warp] = before;
   __syncthreads();
   before += above - ws;
-  uint64_t own = 0u;
+  uint64_t own = above;
   for (int i = 0; i < kSmWarps; ++i) {
     if (i < warp) before += s.warp_mass[i];
     own += s.warp_mass[i];
   }
   const double goal = share * (double)(all ? all : own);
+  if (tid == 0) s.reached = (double)own >= goal;
   int kept = 0;
 #pragma unroll
   for (int i = 0; i < per; ++i) {
@@ -422,8 +466,6 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
   constexpr int VE = RowView<T>::VE;
   const int tid = threadIdx.x;
   SampleShared* lead = cluster.map_shared_rank(&s, 0);
-  // falling values have rising bins; the same function wherever a bin is asked for
-  auto bin_of = [&](float x) { return min((int)(__fmul_rn(__fsub_rn(rule.m, x), kBinsPerUnit)), kBins - 1); };
   int bin = -1, shift = 32;   // the bin that was cut, the bits of `prefix` are those above shift
   uint32_t prefix = 0u, above = 0u;
   uint64_t mass_above = 0u, mass_all = 0u;
@@ -434,12 +476,12 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
     for (int i = tid; i < kBins; i += kSmThreads) { s.count[i] = 0u; s.mass[i] = 0u; }
     if (tid == 0) s.n_list = 0;
     __syncthreads();
-    sh.sweep([&](const Raw<T, VE>& v, int j) {
+    sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         const float x = raw_get(v, e);
         if (!rule.keeps(x, sh.index(j, e))) continue;
-        int b = bin_of(x);
+        int b = rule.bin(x);
         if (round > 0) {
           if (b != bin) continue;
           const uint32_t o = order_of(x);
@@ -466,14 +508,14 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
     const uint32_t in = lead->d.in;
     const bool whole = round == 0 && above + in <= kList;  // all down to the bin as one list
     if (whole || in <= kList) {
-      sh.sweep([&](const Raw<T, VE>& v, int j) {
+      sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
         const float most = raw_max(v);
-        if (most == -INFINITY || (round == 0 ? bin_of(most) > b : bin_of(most) > bin)) return;
+        if (most == -INFINITY || (round == 0 ? rule.bin(most) > b : rule.bin(most) > bin)) return;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const float x = raw_get(v, e);
           if (!rule.keeps(x, sh.index(j, e))) continue;
-          const int c = bin_of(x);
+          const int c = rule.bin(x);
           if (round == 0) {
             if (c > b || (!whole && c < b)) continue;
           } else {
@@ -538,6 +580,109 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
   }
 }
 
+// What a list of at most kList values can decide: the values in bins up to that of
+// the k-th largest of the threads' largest values (k < 0: all that the rule keeps)
+// are sorted, top-k and top-p applied, and the token taken.  total: the weights'
+// sum where top-p follows no other rule, else 0.  Returns whether the list held
+// the set.  `mine` is the thread's largest value.
+template <typename T>
+__device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, SampleShared& s,
+                                               const RowShare<T>& sh, const SampleArgs& a, const RowRule& rule,
+                                               float mine, int k, int64_t top_k, double top_p, double total,
+                                               double u) {
+  constexpr int VE = RowView<T>::VE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  SampleShared* lead = cluster.map_shared_rank(&s, 0);
+  int most = kBins - 1;
+  if (tid == 0) s.n_list = 0;
+  if (k >= 0) {
+    for (int i = tid; i < kBins; i += kSmThreads) { s.count[i] = 0u; s.mass[i] = 0u; }
+    __syncthreads();
+    if (mine != -INFINITY) atomicAdd(&s.count[rule.bin(mine)], 1u);
+    __syncthreads();
+    find_bin<false>(cluster, s, sh.part, sh.parts, (uint32_t)k, 0., 0u, 0u, 0u);
+    most = lead->d.bin;
+  }
+  cluster.sync();
+  if (most < 0) return false;  // fewer threads than k have a value
+  sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
+    const float top = raw_max(v);
+    if (top == -INFINITY || rule.bin(top) > most) return;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float x = raw_get(v, e);
+      if (!rule.keeps(x, sh.index(j, e)) || rule.bin(x) > most) continue;
+      const int at = atomicAdd(&lead->n_list, 1);
+      if (at < kList) lead->list[at] = key_of(x, (int)sh.index(j, e));
+    }
+  });
+  cluster.sync();
+  if (sh.part == 0) {
+    const int n = s.n_list;
+    int kept = 0;
+    if (n <= kList) {
+      sort_list(s, n);
+      kept = top_k > 1 ? (int)min(top_k, (int64_t)n) : n;
+      if (top_p < 1.) {
+        const int all = kept;
+        const uint64_t whole = total > 0. ? (uint64_t)__double2ll_rn(total * (4503599627370496. / a.weight_unit)) : 0u;
+        kept = count_by_mass(s, all, 0u, top_p, whole, rule, a.weight_unit);
+        // the list ends before the bound: the set goes on
+        if (total > 0. && kept == all && s.reached == 0) kept = 0;
+      }
+    }
+    if (kept > 0) {
+      // by rising index, weights behind it
+      __syncthreads();
+      for (int i = tid; i < kept; i += kSmThreads) {
+        const uint64_t key = s.list[i];
+        s.list[i] = key << 32 | key >> 32;
+      }
+      __syncthreads();
+      sort_list(s, kept);
+      constexpr int per = kList / kSmThreads;
+      double w[per], ws = 0.;
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int at = tid * per + i;
+        w[i] = at < kept ? rule.weight(value_of((uint32_t)s.list[at])) : 0.;
+        ws += w[i];
+      }
+      double run = ws;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const double y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+      }
+      if (lane == 31) s.warp_sum[warp] = run;
+      if (tid == 0) s.first = kept - 1;
+      __syncthreads();
+      run -= ws;
+      double sum = 0.;
+      for (int i = 0; i < kSmWarps; ++i) {
+        if (i < warp) run += s.warp_sum[i];
+        sum += s.warp_sum[i];
+      }
+      const double goal = u * sum;
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        run += w[i];
+        if (w[i] > 0. && run > goal) {
+          atomicMin(&s.first, tid * per + i);
+          break;
+        }
+      }
+      __syncthreads();
+      if (tid == 0) s.d.at = (int64_t)(uint32_t)~(uint32_t)(s.list[s.first] >> 32);
+    }
+    if (tid == 0) s.d.bin = kept;
+  }
+  cluster.sync();
+  const bool done = lead->d.bin > 0;
+  cluster.sync();
+  return done;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, const int parts) {
   constexpr int VE = RowView<T>::VE;
@@ -562,26 +707,29 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
   // lane's in units of its own running maximum.
   // (a factor of at most 1e300 keeps the maximum's weight at 2^0)
   RowRule rule{0.f, fmin(1.4426950408889634 / temperature, 1e300), 0., 0u, -INFINITY, true, true, s.root};
-  const bool at_once = !greedy && !by_k && !by_p && !by_min;
+  const bool at_once = !greedy && !by_k && !by_min;  // sums with the maximum: temperature, top-p
   float mine = -INFINITY;
   double sum = 0.;
   uint32_t bits = 0u;
-  sh.sweep([&](const Raw<T, VE>& v, int) {
-    bits = largest_bits(v, bits);
-    const float top = raw_max(v);
-    if (at_once) {
+  if (at_once) {
+    sh.template sweep<2>([&](const Raw<T, VE>& v, int) {
+      bits = largest_bits(v, bits);
+      const float top = raw_max(v);
       if (top > mine) {
-        if (sum > 0.) sum *= pow2_of(s.root, ((double)mine - top) * rule.c);
+        if (sum > 0.) sum *= pow2_neg(s.root, ((double)top - mine) * rule.c);
         mine = top;
       }
-      if (mine != -INFINITY) {
+      if (mine == -INFINITY) return;
+      const double m = mine;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) sum += pow2_of(s.root, ((double)raw_get(v, e) - mine) * rule.c);
-      }
-    } else {
-      mine = fmaxf(mine, top);
-    }
-  });
+      for (int e = 0; e < VE; ++e) sum += pow2_neg(s.root, (m - (double)raw_get(v, e)) * rule.c);
+    });
+  } else {
+    sh.template sweep<4>([&](const Raw<T, VE>& v, int) {
+      bits = largest_bits(v, bits);
+      mine = fmaxf(mine, raw_max(v));
+    });
+  }
   // absent elements read as -inf, whose bits are those of infinity
   const bool nan = bits_are_nan<T>(bits);
   {
@@ -617,20 +765,40 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
   } else {
     if (by_min) {
       rule.all_y = false;
-      rule.min_y = min_p < 1. ? log2(min_p) : 0.;
+      rule.most_y = min_p < 1. ? -log2(min_p) : 0.;
     }
-    bool done = false;
-    if (by_k) done = narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1.);
-    if (by_p && !done) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
+    const double u = fmin(fmax((double)uniform, 0.), 1.);
     if (at_once) {
-      const double f = mine == -INFINITY ? 0. : pow2_of(s.root, ((double)mine - rule.m) * rule.c);
+      const double f = mine == -INFINITY ? 0. : pow2_neg(s.root, ((double)rule.m - mine) * rule.c);
       sum = warp_total(sum * f);
       if (lane == 0) s.warp_sum[warp] = sum;
     }
-    const double u = fmin(fmax((double)uniform, 0.), 1.);
-    locate<T>(cluster, s, sh, at_once,
-              [&](float x, int64_t i) { return rule.keeps(x, i) ? rule.weight(x) : 0.; },
-              [&](double w) { return u * w; });
+    bool done = false;
+    if (by_k || by_p || by_min) {
+      double total = 0.;
+      if (at_once) {  // top-p alone: of the whole row
+        __syncthreads();
+        if (tid == 0) {
+          double t = 0.;
+          for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
+          s.total = t;
+        }
+        cluster.sync();
+        for (int q = 0; q < parts; ++q) total += *cluster.map_shared_rank(&s.total, q);
+      }
+      const int k = a.V <= kList ? -1 : by_k ? (int)top_k : by_min ? -1 : kQuick;
+      if (k <= kList)
+        done = take_from_list<T>(cluster, s, sh, a, rule, mine, k, by_k ? top_k : 0, by_p ? top_p : 1., total, u);
+      if (!done) {
+        if (by_k) done = narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1.);
+        if (by_p && !done) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
+        done = false;
+      }
+    }
+    if (!done)
+      locate<T>(cluster, s, sh, at_once && !by_p,
+                [&](float x, int64_t i) { return rule.keeps(x, i) ? rule.weight(x) : 0.; },
+                [&](double w) { return u * w; });
   }
   if (part == 0 && tid == 0) a.ids[r] = s.d.at;
 }

@@ -228,14 +228,14 @@ template <typename E, int W, int K> struct RowCursor {
   static __device__ __forceinline__ int row_of(int i) {
     return (threadIdx.x % PIECES) / CPR + (i * kSelThreads % PIECES) / CPR;
   }
-  // Blocks from row r0 on, forward (way 1) or backward (-1).  Returns whether all
-  // rows start on 16-byte boundaries, as asynchronous copies need.
-  __device__ __forceinline__ bool start(const SelSource* src, int64_t r0, int64_t col, int ncols, int way) {
-    bool vec = true;
+  // Blocks from row r0 on, forward (way 1) or backward (-1).  Returns the bits of all
+  // rows' addresses, of which the lowest says how they are aligned.
+  __device__ __forceinline__ uint32_t start(const SelSource* src, int64_t r0, int64_t col, int ncols, int way) {
+    uint32_t bits = 0u;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      vec = vec && (!src[k].p || ((reinterpret_cast<uintptr_t>((const E*)src[k].p + col) |
-                                   (uint64_t)(src[k].ld * sizeof(E))) & 15) == 0);
+      if (src[k].p)
+        bits |= (uint32_t)reinterpret_cast<uintptr_t>((const E*)src[k].p + col) | (uint32_t)(src[k].ld * sizeof(E));
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int k = (threadIdx.x + i * kSelThreads) / PIECES;
@@ -249,20 +249,39 @@ template <typename E, int W, int K> struct RowCursor {
       }
       of[i][threadIdx.x] = x;
     }
-    return vec;
+    return bits;
   }
-  // the next block, of which `rows` rows exist
-  __device__ __forceinline__ void request(E* to, int rows, bool vec) {
+  // the next block, of which `rows` rows exist; `size`: of an asynchronous copy that
+  // the rows' alignment allows (16, 8 or 4 bytes, 0: none)
+  __device__ __forceinline__ void request(E* to, int rows, int size) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const Piece x = of[i][threadIdx.x];
       if (x.bytes < 0) continue;
       E* dst = to + (threadIdx.x + i * kSelThreads) * VE;
-      if (rows >= kSub && vec) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(x.p), "r"(x.bytes)
+      const int bytes = row_of(i) < rows ? x.bytes : 0;
+      if (rows >= kSub && size == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(x.p), "r"(bytes)
                      : "memory");
+      } else if (bytes == 0) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+      } else if (size == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(x.p), "r"(bytes)
+                     : "memory");
+      } else if (size == 8) {
+#pragma unroll
+        for (int b = 0; b < 16; b += 8)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst) + b),
+                       "l"(x.p + (b < bytes ? b : 0)), "r"(max(0, min(bytes - b, 8)))
+                       : "memory");
+      } else if (size == 4) {
+#pragma unroll
+        for (int b = 0; b < 16; b += 4)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst) + b),
+                       "l"(x.p + (b < bytes ? b : 0)), "r"(max(0, min(bytes - b, 4)))
+                       : "memory");
       } else {
-        const int n = row_of(i) < rows ? x.bytes / (int)sizeof(E) : 0;
+        const int n = bytes / (int)sizeof(E);
 #pragma unroll
         for (int e = 0; e < VE; ++e) dst[e] = e < n ? ((const E*)x.p)[e] : from_f<E>(0.f);
       }
@@ -334,18 +353,18 @@ template <typename T, int L, bool BWD> struct SelCopies {
   RowCursor<T, S::NL, 2> vec;
 };
 template <typename T, int L, bool BWD, typename Shared>
-__device__ __forceinline__ bool start_copies(const SelArgs& a, const SelTile<L>& t, Shared& s, int64_t r0) {
+__device__ __forceinline__ int start_copies(const SelArgs& a, const SelTile<L>& t, Shared& s, int64_t r0) {
   constexpr int way = BWD ? -1 : 1;
-  bool vec = s.copies.tok.start(a.tok, r0, t.d0, t.nch, way);
-  vec &= s.copies.vec.start(a.vec, r0, (int64_t)t.g * a.N, a.N, way);
-  if (a.dt_f32) vec &= s.dt32.cursor.start(&a.dt32, r0, t.d0, t.nch, way);
-  return vec;
+  uint32_t bits = s.copies.tok.start(a.tok, r0, t.d0, t.nch, way);
+  bits |= s.copies.vec.start(a.vec, r0, (int64_t)t.g * a.N, a.N, way);
+  if (a.dt_f32) bits |= s.dt32.cursor.start(&a.dt32, r0, t.d0, t.nch, way);
+  return (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : 0;
 }
 template <typename Shared>
-__device__ __forceinline__ void request_copies(const SelArgs& a, Shared& s, int at, int rows, bool vec) {
-  s.copies.tok.request(s.raw[at].tok, rows, vec);
-  s.copies.vec.request(s.raw[at].vec, rows, vec);
-  if (a.dt_f32) s.dt32.cursor.request(s.dt32.v[at], rows, vec);
+__device__ __forceinline__ void request_copies(const SelArgs& a, Shared& s, int at, int rows, int size) {
+  s.copies.tok.request(s.raw[at].tok, rows, size);
+  s.copies.vec.request(s.raw[at].vec, rows, size);
+  if (a.dt_f32) s.dt32.cursor.request(s.dt32.v[at], rows, size);
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 // dt as fp32, of both blocks: the end of shared memory, left out where dt is not.
@@ -502,8 +521,8 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_fwd(const SelArgs a) {
   const S t(a, blockIdx.x - bc * a.tiles);
   const SelSpan sp = sel_span(a, bc);
   if (LOCAL && sp.c + 1 == a.chunks) return;  // nothing follows the last
-  const bool vec = start_copies<T, L, false>(a, t, s, sp.lo);
-  request_copies(a, s, 0, sp.rows, vec);
+  const int size = start_copies<T, L, false>(a, t, s, sp.lo);
+  request_copies(a, s, 0, sp.rows, size);
   const int mc = threadIdx.x / L;
   const FwdLane lane{(int)threadIdx.x % L, mc, t.d0 + mc, mc < t.nch};
   float2 rate[2], start[2] = {f2(0.f), f2(0.f)};
@@ -531,7 +550,7 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_fwd(const SelArgs a) {
     const int rows = sp.rows - r0;  // that are left
     copies_done();
     __syncthreads();
-    if (rows > kSub) request_copies(a, s, at ^ 1, rows - kSub, vec);
+    if (rows > kSub) request_copies(a, s, at ^ 1, rows - kSub, size);
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) {
       const int row = t.pr + i * S::STEP;
@@ -867,8 +886,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) k_sel_bwd(const SelArgs a) {
   const SelSpan sp = sel_span(a, bc);
   if (LOCAL && sp.c == 0) return;  // nothing is in front of the first
   const int last = (sp.rows - 1) / kSub * kSub;  // the last 16 rows' first
-  const bool vec = start_copies<T, L, true>(a, t, s, sp.lo + last);
-  request_copies(a, s, 0, sp.rows - last, vec);
+  const int size = start_copies<T, L, true>(a, t, s, sp.lo + last);
+  request_copies(a, s, 0, sp.rows - last, size);
   const W lane(t);
   float2 A2[2], e[2] = {f2(0.f), f2(0.f)}, dsum = f2(0.f);
   lane.load(a.A, a.N, A2);
@@ -909,7 +928,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) k_sel_bwd(const SelArgs a) {
     const int rows = sp.rows - r0;  // from here on
     copies_done();
     __syncthreads();
-    if (r0 > 0) request_copies(a, s, at ^ 1, kSub, vec);
+    if (r0 > 0) request_copies(a, s, at ^ 1, kSub, size);
     float2 hs[kSub / kHeld][2];
     if constexpr (!LOCAL) {
       lane.load_packed(keep, a.NP, hs[0]);
