@@ -13,22 +13,26 @@
 // polynomial of 2^f, |f| <= 1/32, to f^5: 2e-13 relative).  Sums are formed in a
 // fixed order or as whole numbers: equal inputs give equal tokens.
 //
-// Top-k, top-p and min-p rarely need more than a short list.  The k-th largest of
-// the threads' largest values bounds the k largest from below, so that a second
-// sweep, which skips most vectors by their largest value, hands a few more than k
-// values to the cluster's first CTA; it sorts them, applies the rules and takes the
-// token.  With min-p alone the list is what min-p keeps, with top-p alone it is
-// about the 512 largest, which have to reach the bound.
-// Where the list does not hold the set, a histogram of the row over bins of equal
-// width in x (counts, and weights as whole numbers of 2^-44) gives the bin in which
-// the bound lies, and what is in the bin is sorted.  A bin with more values than the
-// list holds is cut by the digits of the values' ordered bits, 11 at a time, and
-// among equal values the lower indices are counted out.
+// Top-k, top-p and min-p need no sort of the row.  The k-th largest of the threads'
+// largest values bounds the k largest from below (min-p bounds what it keeps
+// itself), so that a second sweep, which skips most vectors by their largest value,
+// hands a short list to the cluster's first CTA; it sorts the list, applies the
+// rules and takes the token.  Top-p alone, and what the list does not hold, go by a
+// histogram over bins of equal width in x: counts, and the values' mean place in the
+// bin.  A bin's weight is close to its count times the weight at that place, which
+// puts top-p's bound within a bin; the next sweep forms the exact sum above a window of three bins and lists the window,
+// and if the bound is not in it the window moves.  Where the window and all above it
+// are short, the list decides as before.
+// A bin with more values than the list holds (equal logits, or logits within a
+// hundredth) is cut by the digits of the values' ordered bits, 11 at a time, with
+// weights as whole numbers of 2^-44, and among equal values the lower indices are
+// counted out.
 //
 // Bound: by temperature alone the row is read once and the time is that of the
 // fp64 pipe, 12 operations for a value; with a short list the row is read once from
 // memory and once from L2.  Few rows are split over the CTAs of a cluster, which
-// exchange through distributed shared memory.
+// exchange through distributed shared memory: what is counted is added to the first
+// CTA's histogram by remote atomics, which nobody waits for.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -48,7 +52,7 @@ constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kBinsPer = kBins / kSmThreads;   // bins of a thread
 constexpr int kList = 2048;                    // longest list that is sorted
-constexpr int kQuick = 512;                    // values that a list for top-p alone starts from
+constexpr int kPlaces = 4096;                  // of a bin: 2^20 values' places fit 32 bits
 constexpr float kBinsPerUnit = 46.f;           // bins of a logit: 44 units below the maximum
 
 struct SampleArgs {
@@ -83,7 +87,10 @@ struct SampleShared {
   Decision d;
   int n_list, first, reached;
   uint32_t count[kBins];
-  uint64_t mass[kBins];
+  union {
+    uint64_t mass[kBins];
+    uint32_t place[kBins];       // sums of the places in a bin, in parts of kPlaces
+  };
   uint64_t list[kList];
 };
 
@@ -177,6 +184,16 @@ struct RowRule {
   // falling values have rising bins; the same function wherever a bin is asked for
   __device__ __forceinline__ int bin(float x) const {
     return min((int)(__fmul_rn(__fsub_rn(m, x), kBinsPerUnit)), kBins - 1);
+  }
+  // the least value in bins up to b: bins fall as the ordered bits rise
+  __device__ __forceinline__ float least(int b) const {
+    if (b < 0) return INFINITY;
+    uint32_t lo = order_of(-FLT_MAX), hi = order_of(m);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (bin(value_of(mid)) <= b) hi = mid; else lo = mid + 1;
+    }
+    return value_of(lo);
   }
   __device__ __forceinline__ double weight(float x) const { return pow2_neg(root, ((double)m - x) * c); }
   __device__ __forceinline__ bool keeps(float x, int64_t i) const {
@@ -580,42 +597,163 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
   }
 }
 
-// What a list of at most kList values can decide: the values in bins up to that of
-// the k-th largest of the threads' largest values (k < 0: all that the rule keeps)
-// are sorted, top-k and top-p applied, and the token taken.  total: the weights'
-// sum where top-p follows no other rule, else 0.  Returns whether the list held
-// the set.  `mine` is the thread's largest value.
-template <typename T>
-__device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, SampleShared& s,
-                                               const RowShare<T>& sh, const SampleArgs& a, const RowRule& rule,
-                                               float mine, int k, int64_t top_k, double top_p, double total,
-                                               double u) {
-  constexpr int VE = RowView<T>::VE;
+// The token among the first `kept` of the sorted list (the leader's threads): into
+// s.d.at.
+__device__ __forceinline__ void pick_from_list(SampleShared& s, int kept, const RowRule& rule, double u) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  SampleShared* lead = cluster.map_shared_rank(&s, 0);
-  int most = kBins - 1;
-  if (tid == 0) s.n_list = 0;
-  if (k >= 0) {
-    for (int i = tid; i < kBins; i += kSmThreads) { s.count[i] = 0u; s.mass[i] = 0u; }
-    __syncthreads();
-    if (mine != -INFINITY) atomicAdd(&s.count[rule.bin(mine)], 1u);
-    __syncthreads();
-    find_bin<false>(cluster, s, sh.part, sh.parts, (uint32_t)k, 0., 0u, 0u, 0u);
-    most = lead->d.bin;
+  __syncthreads();
+  for (int i = tid; i < kept; i += kSmThreads) {  // by rising index, values behind it
+    const uint64_t key = s.list[i];
+    s.list[i] = key << 32 | key >> 32;
   }
-  cluster.sync();
-  if (most < 0) return false;  // fewer threads than k have a value
+  __syncthreads();
+  sort_list(s, kept);
+  constexpr int per = kList / kSmThreads;
+  double w[per], ws = 0.;
+#pragma unroll
+  for (int i = 0; i < per; ++i) {
+    const int at = tid * per + i;
+    w[i] = at < kept ? rule.weight(value_of((uint32_t)s.list[at])) : 0.;
+    ws += w[i];
+  }
+  double run = ws;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const double y = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += y;
+  }
+  if (lane == 31) s.warp_sum[warp] = run;
+  if (tid == 0) s.first = kept - 1;
+  __syncthreads();
+  run -= ws;
+  double sum = 0.;
+  for (int i = 0; i < kSmWarps; ++i) {
+    if (i < warp) run += s.warp_sum[i];
+    sum += s.warp_sum[i];
+  }
+  const double goal = u * sum;
+#pragma unroll
+  for (int i = 0; i < per; ++i) {
+    run += w[i];
+    if (w[i] > 0. && run > goal) {
+      atomicMin(&s.first, tid * per + i);
+      break;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) s.d.at = (int64_t)(uint32_t)~(uint32_t)(s.list[s.first] >> 32);
+}
+
+// Hands the values in [least, below) that the rule keeps to the leader's list.
+template <typename T>
+__device__ __forceinline__ void list_values(SampleShared* lead, const RowShare<T>& sh, const RowRule& rule,
+                                            float least, float below) {
+  constexpr int VE = RowView<T>::VE;
   sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
-    const float top = raw_max(v);
-    if (top == -INFINITY || rule.bin(top) > most) return;
+    if (!(raw_max(v) >= least)) return;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const float x = raw_get(v, e);
-      if (!rule.keeps(x, sh.index(j, e)) || rule.bin(x) > most) continue;
+      if (!(x >= least) || x >= below || !rule.keeps(x, sh.index(j, e))) continue;
       const int at = atomicAdd(&lead->n_list, 1);
       if (at < kList) lead->list[at] = key_of(x, (int)sh.index(j, e));
     }
   });
+}
+
+// The first of the leader's bins at which the running count reaches k, or (MASS)
+// the running weight, each bin's taken at its mean place, reaches goal; the last bin
+// with a value where rounding leaves none.  Into s.d.bin (-1: fewer than k), with the
+// counts above and in it and its neighbours'.  The leader's threads.
+template <bool MASS>
+__device__ __forceinline__ void scan_bins(SampleShared& s, uint32_t k, double goal, const RowRule& rule) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t c[kBinsPer], cs = 0u;
+  double w[kBinsPer], ws = 0.;
+#pragma unroll
+  for (int i = 0; i < kBinsPer; ++i) {
+    const int b = tid * kBinsPer + i;
+    c[i] = s.count[b];
+    cs += c[i];
+    const double place = MASS && c[i] ? b + (double)s.place[b] / (kPlaces * (double)c[i]) : 0.;
+    w[i] = MASS && c[i] ? c[i] * pow2_neg(rule.root, place * (1. / kBinsPerUnit) * rule.c) : 0.;
+    ws += w[i];
+  }
+  uint32_t ci = cs;
+  double wi = ws;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, ci, o);
+    const double b = __shfl_up_sync(0xffffffffu, wi, o);
+    if (lane >= o) { ci += a; wi += b; }
+  }
+  if (lane == 31) { s.warp_count[warp] = ci; s.warp_sum[warp] = wi; }
+  if (tid == 0) { s.d.bin = -1; s.first = -1; }
+  __syncthreads();
+  uint32_t cb = ci - cs;
+  double wb = wi - ws;
+  for (int i = 0; i < warp; ++i) { cb += s.warp_count[i]; wb += s.warp_sum[i]; }
+  int last = -1;
+#pragma unroll
+  for (int i = 0; i < kBinsPer; ++i) {
+    const int b = tid * kBinsPer + i;
+    if (c[i]) last = b;
+    const bool here = MASS ? c[i] && wb < goal && wb + w[i] >= goal : cb < k && cb + c[i] >= k;
+    if (here) s.d.bin = b;  // rounding may leave two neighbours: either will do
+    cb += c[i];
+    wb += w[i];
+  }
+  if constexpr (MASS) {
+    if (last >= 0) atomicMax(&s.first, last);
+    __syncthreads();
+    if (tid == 0 && s.d.bin < 0) s.d.bin = s.first;
+  }
+  __syncthreads();
+}
+
+// Values in bins up to b (the leader's threads, all get it).
+__device__ __forceinline__ uint32_t count_to(SampleShared& s, int b) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t c = 0u;
+#pragma unroll
+  for (int i = 0; i < kBinsPer; ++i)
+    if (tid * kBinsPer + i <= b) c += s.count[tid * kBinsPer + i];
+  c = __reduce_add_sync(0xffffffffu, c);
+  __syncthreads();
+  if (lane == 0) s.warp_count[warp] = c;
+  __syncthreads();
+  c = 0u;
+  for (int i = 0; i < kSmWarps; ++i) c += s.warp_count[i];
+  return c;
+}
+
+// What a list of at most kList values can decide: the values in bins up to that of
+// the k-th largest of the threads' largest values (k < 0: all that the rule keeps)
+// are sorted, top-k and top-p applied, and the token taken.  Returns whether the
+// list held the set.  `mine` is the thread's largest value.
+template <typename T>
+__device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, SampleShared& s,
+                                               const RowShare<T>& sh, const SampleArgs& a, const RowRule& rule,
+                                               float mine, int k, int64_t top_k, double top_p, double u) {
+  const int tid = threadIdx.x;
+  SampleShared* lead = cluster.map_shared_rank(&s, 0);
+  float least = -FLT_MAX;
+  if (sh.part == 0) {
+    for (int i = tid; i < kBins; i += kSmThreads) s.count[i] = 0u;
+    if (tid == 0) s.n_list = 0;
+  }
+  cluster.sync();
+  if (k >= 0) {
+    if (mine != -INFINITY) atomicAdd(&lead->count[rule.bin(mine)], 1u);
+    cluster.sync();
+    if (sh.part == 0) scan_bins<false>(s, (uint32_t)k, 0., rule);
+    cluster.sync();
+    const int most = lead->d.bin;
+    cluster.sync();
+    if (most < 0) return false;  // fewer threads than k have a value
+    least = rule.least(most);
+  }
+  list_values(lead, sh, rule, least, INFINITY);
   cluster.sync();
   if (sh.part == 0) {
     const int n = s.n_list;
@@ -623,57 +761,8 @@ __device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, Sampl
     if (n <= kList) {
       sort_list(s, n);
       kept = top_k > 1 ? (int)min(top_k, (int64_t)n) : n;
-      if (top_p < 1.) {
-        const int all = kept;
-        const uint64_t whole = total > 0. ? (uint64_t)__double2ll_rn(total * (4503599627370496. / a.weight_unit)) : 0u;
-        kept = count_by_mass(s, all, 0u, top_p, whole, rule, a.weight_unit);
-        // the list ends before the bound: the set goes on
-        if (total > 0. && kept == all && s.reached == 0) kept = 0;
-      }
-    }
-    if (kept > 0) {
-      // by rising index, weights behind it
-      __syncthreads();
-      for (int i = tid; i < kept; i += kSmThreads) {
-        const uint64_t key = s.list[i];
-        s.list[i] = key << 32 | key >> 32;
-      }
-      __syncthreads();
-      sort_list(s, kept);
-      constexpr int per = kList / kSmThreads;
-      double w[per], ws = 0.;
-#pragma unroll
-      for (int i = 0; i < per; ++i) {
-        const int at = tid * per + i;
-        w[i] = at < kept ? rule.weight(value_of((uint32_t)s.list[at])) : 0.;
-        ws += w[i];
-      }
-      double run = ws;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const double y = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += y;
-      }
-      if (lane == 31) s.warp_sum[warp] = run;
-      if (tid == 0) s.first = kept - 1;
-      __syncthreads();
-      run -= ws;
-      double sum = 0.;
-      for (int i = 0; i < kSmWarps; ++i) {
-        if (i < warp) run += s.warp_sum[i];
-        sum += s.warp_sum[i];
-      }
-      const double goal = u * sum;
-#pragma unroll
-      for (int i = 0; i < per; ++i) {
-        run += w[i];
-        if (w[i] > 0. && run > goal) {
-          atomicMin(&s.first, tid * per + i);
-          break;
-        }
-      }
-      __syncthreads();
-      if (tid == 0) s.d.at = (int64_t)(uint32_t)~(uint32_t)(s.list[s.first] >> 32);
+      if (top_p < 1.) kept = count_by_mass(s, kept, 0u, top_p, 0u, rule, a.weight_unit);
+      pick_from_list(s, kept, rule, u);
     }
     if (tid == 0) s.d.bin = kept;
   }
@@ -681,6 +770,154 @@ __device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, Sampl
   const bool done = lead->d.bin > 0;
   cluster.sync();
   return done;
+}
+
+enum { kNarrowed, kTaken, kCrowded };
+
+// The bound of top-k (MASS false: the k largest of what the rule keeps), or of top-p
+// with `goal` of the weights' sum, by a histogram.  kTaken: a list held all that is
+// kept, and the token is taken (with then_share < 1 after top-p of the k largest);
+// kNarrowed: the rule has the bound; kCrowded: a bin has more values than the list.
+template <typename T, bool MASS>
+__device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
+                                         const SampleArgs& a, RowRule& rule, int64_t k, double goal,
+                                         double then_share, double u) {
+  constexpr int VE = RowView<T>::VE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  SampleShared* lead = cluster.map_shared_rank(&s, 0);
+  for (int i = tid; i < kBins; i += kSmThreads) {
+    s.count[i] = 0u;
+    s.place[i] = 0u;
+  }
+  cluster.sync();
+  uint32_t far = 0u;  // in the last bin, where masks by low values all are
+  sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float x = raw_get(v, e);
+      if (!rule.keeps(x, sh.index(j, e))) continue;
+      const float at = __fmul_rn(__fsub_rn(rule.m, x), kBinsPerUnit);
+      const int b = min((int)at, kBins - 1);  // as rule.bin
+      if (b == kBins - 1) {
+        ++far;
+        continue;
+      }
+      atomicAdd(&s.count[b], 1u);
+      if constexpr (MASS) atomicAdd(&s.place[b], (uint32_t)((at - b) * kPlaces));
+    }
+  });
+  far = __reduce_add_sync(0xffffffffu, far);
+  if (lane == 0 && far) atomicAdd(&s.count[kBins - 1], far);
+  __syncthreads();
+  if (sh.part != 0)
+    for (int i = tid; i < kBins; i += kSmThreads)
+      if (s.count[i]) {
+        atomicAdd(&lead->count[i], s.count[i]);
+        if constexpr (MASS) atomicAdd(&lead->place[i], s.place[i]);
+      }
+  cluster.sync();
+  if (sh.part == 0) scan_bins<MASS>(s, (uint32_t)min(k, (int64_t)0x7fffffff), goal, rule);
+  cluster.sync();
+  int at = lead->d.bin;
+  if (at < 0) {
+    cluster.sync();
+    return kNarrowed;  // fewer values than k: all are kept
+  }
+  cluster.sync();  // the bin has been read
+  for (int way = 0;;) {
+    // the window: the bin, for weights with its neighbours where the list holds them
+    if (sh.part == 0) {
+      int b0 = MASS ? max(at - 1, 0) : at, b1 = MASS ? min(at + 1, kBins - 1) : at;
+      uint32_t to1 = count_to(s, b1);
+      uint32_t to0 = b0 ? count_to(s, b0 - 1) : 0u;
+      if (to1 - to0 > kList) {
+        b0 = b1 = at;
+        to1 = count_to(s, b1);
+        to0 = b0 ? count_to(s, b0 - 1) : 0u;
+      }
+      if (to1 <= kList) {
+        b0 = 0;
+        to0 = 0u;
+      }
+      if (tid == 0) {
+        s.d.bin = to1 - to0 > kList ? -1 : b0;
+        s.d.in = (uint32_t)b1;
+        s.d.above = to0;
+        s.n_list = 0;
+      }
+      const uint32_t all = MASS ? count_to(s, kBins - 1) : 0u;
+      if (tid == 0) s.d.mass = to1 == all;  // nothing is below the window
+    }
+    cluster.sync();
+    const int b0 = lead->d.bin, b1 = (int)lead->d.in;
+    if (b0 < 0) {
+      cluster.sync();
+      return kCrowded;
+    }
+    const float least = rule.least(b1), below = rule.least(b0 - 1);
+    double sum = 0.;
+    if (MASS && b0 > 0) {  // the exact sum above the window
+      sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
+        if (!(raw_max(v) >= below)) return;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float x = raw_get(v, e);
+          if (x >= below && rule.keeps(x, sh.index(j, e))) sum += rule.weight(x);
+        }
+      });
+      sum = warp_total(sum);
+    }
+    __syncthreads();
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      double t = 0.;
+      for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
+      s.total = t;
+    }
+    list_values(lead, sh, rule, least, below);
+    cluster.sync();
+    if (sh.part == 0) {
+      const int n = min(s.n_list, kList);
+      double above = 0.;
+      for (int q = 0; q < sh.parts; ++q) above += *cluster.map_shared_rank(&s.total, q);
+      sort_list(s, n);
+      int kept = MASS ? 0 : (int)min(k - (int64_t)s.d.above, (int64_t)n), miss = 0;
+      if constexpr (MASS) {
+        const double unit = 4503599627370496. / a.weight_unit;  // whole weights of the goal's part in the list
+        if (above < goal) {
+          const double rest = (goal - above) * unit;
+          kept = count_by_mass(s, n, 0u, 1., (uint64_t)__double2ll_ru(rest), rule, a.weight_unit);
+          if (!s.reached && !s.d.mass) miss = 1;        // the bound is below the window
+        } else {
+          miss = -1;                                    // or above it
+        }
+      } else if (b0 == 0 && then_share < 1.) {
+        kept = count_by_mass(s, kept, 0u, then_share, 0u, rule, a.weight_unit);
+      }
+      if (miss == 0 && kept < 1) miss = -1;
+      if (miss == 0) {
+        const uint64_t bound = s.list[kept - 1];
+        if (b0 == 0) pick_from_list(s, kept, rule, u);
+        if (tid == 0) s.d.bound = bound;
+      }
+      __syncthreads();
+      if (tid == 0) s.d.bin = miss;
+    }
+    cluster.sync();
+    const int miss = lead->d.bin;
+    rule.bound = lead->d.bound;
+    cluster.sync();
+    if (miss == 0) {
+      rule.tau = value_of((uint32_t)(rule.bound >> 32));
+      rule.all_keys = false;
+      return b0 == 0 ? kTaken : kNarrowed;
+    }
+    // the sums' roundings at a bin's edge may send it back and forth: once is enough
+    if (way && way != miss) return kCrowded;
+    way = miss;
+    at = miss > 0 ? min(b1 + 1, kBins - 1) : max(b0 - 1, 0);
+  }
 }
 
 template <typename T>
@@ -707,7 +944,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
   // lane's in units of its own running maximum.
   // (a factor of at most 1e300 keeps the maximum's weight at 2^0)
   RowRule rule{0.f, fmin(1.4426950408889634 / temperature, 1e300), 0., 0u, -INFINITY, true, true, s.root};
-  const bool at_once = !greedy && !by_k && !by_min;  // sums with the maximum: temperature, top-p
+  const bool at_once = !greedy && !by_k && !by_min;  // the sums with the maximum: temperature, top-p
   float mine = -INFINITY;
   double sum = 0.;
   uint32_t bits = 0u;
@@ -774,26 +1011,43 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
       if (lane == 0) s.warp_sum[warp] = sum;
     }
     bool done = false;
-    if (by_k || by_p || by_min) {
-      double total = 0.;
-      if (at_once) {  // top-p alone: of the whole row
-        __syncthreads();
-        if (tid == 0) {
-          double t = 0.;
-          for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
-          s.total = t;
-        }
-        cluster.sync();
-        for (int q = 0; q < parts; ++q) total += *cluster.map_shared_rank(&s.total, q);
-      }
-      const int k = a.V <= kList ? -1 : by_k ? (int)top_k : by_min ? -1 : kQuick;
+    if (by_k || by_min) {
+      const int k = a.V <= kList || !by_k ? -1 : (int)top_k;
       if (k <= kList)
-        done = take_from_list<T>(cluster, s, sh, a, rule, mine, k, by_k ? top_k : 0, by_p ? top_p : 1., total, u);
-      if (!done) {
-        if (by_k) done = narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1.);
-        if (by_p && !done) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
-        done = false;
+        done = take_from_list<T>(cluster, s, sh, a, rule, mine, k, by_k ? top_k : 0, by_p ? top_p : 1., u);
+    }
+    if (!done && by_k) {
+      const int how = by_window<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1., u);
+      if (how == kCrowded) narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., 1.);
+      done = how == kTaken;
+    }
+    if (!done && by_p) {
+      // the weights' sum: formed with the maximum, or of what the rule keeps
+      if (!at_once) {
+        double own = 0.;
+        sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float x = raw_get(v, e);
+            if (rule.keeps(x, sh.index(j, e))) own += rule.weight(x);
+          }
+        });
+        own = warp_total(own);
+        if (lane == 0) s.warp_sum[warp] = own;
       }
+      __syncthreads();
+      if (tid == 0) {
+        double t = 0.;
+        for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
+        s.total = t;
+      }
+      cluster.sync();
+      double total = 0.;
+      for (int q = 0; q < parts; ++q) total += *cluster.map_shared_rank(&s.total, q);
+      cluster.sync();
+      const int how = by_window<T, true>(cluster, s, sh, a, rule, 0, top_p * total, 1., u);
+      if (how == kCrowded) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
+      done = how == kTaken;
     }
     if (!done)
       locate<T>(cluster, s, sh, at_once && !by_p,
