@@ -20,9 +20,9 @@
 // rules and takes the token.  Top-p alone, and what the list does not hold, go by a
 // histogram over bins of equal width in x: counts, and the values' mean place in the
 // bin.  A bin's weight is close to its count times the weight at that place, which
-// puts top-p's bound within a bin; the next sweep forms the exact sum above a window of three bins and lists the window,
-// and if the bound is not in it the window moves.  Where the window and all above it
-// are short, the list decides as before.
+// puts top-p's bound within a bin; the next sweep forms the exact sum above it and lists the bin, and if the bound is not
+// in it the next bin is taken.  Where the bin and all above it are few, the list
+// decides as before.
 // A bin with more values than the list holds (equal logits, or logits within a
 // hundredth) is cut by the digits of the values' ordered bits, 11 at a time, with
 // weights as whole numbers of 2^-44, and among equal values the lower indices are
@@ -52,6 +52,7 @@ constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kBinsPer = kBins / kSmThreads;   // bins of a thread
 constexpr int kList = 2048;                    // longest list that is sorted
+constexpr int kShort = kSmThreads;             // of a list that is sorted by counting
 constexpr int kPlaces = 4096;                  // of a bin: 2^20 values' places fit 32 bits
 constexpr float kBinsPerUnit = 46.f;           // bins of a logit: 44 units below the maximum
 
@@ -145,6 +146,12 @@ template <typename T> struct RowShare {
     wper = (phi - plo + kSmWarps - 1) / kSmWarps;
   }
   __device__ __forceinline__ int lo(int warp) const { return min(plo + warp * wper, phi); }
+  // which warp of all parts has vector j
+  __device__ __forceinline__ int warp_of(int j) const {
+    const int per = (row.nvec + parts - 1) / parts, p = j / per;
+    const int n = min(per, row.nvec - p * per), w = (n + kSmWarps - 1) / kSmWarps;
+    return p * kSmWarps + (j - p * per) / w;
+  }
   __device__ __forceinline__ int64_t index(int j, int e) const { return (int64_t)j * VE + e - row.off; }
   // f(vector, its place) for the lane's vectors of [lo, hi), U of them in flight
   template <int U, typename F> __device__ __forceinline__ void sweep(int lo, int hi, F&& f) const {
@@ -185,15 +192,21 @@ struct RowRule {
   __device__ __forceinline__ int bin(float x) const {
     return min((int)(__fmul_rn(__fsub_rn(m, x), kBinsPerUnit)), kBins - 1);
   }
-  // the least value in bins up to b: bins fall as the ordered bits rise
+  // the least value in bins up to b: bins fall as the ordered bits rise.  By all lanes
+  // of a warp, a 32nd of the range at a time.
   __device__ __forceinline__ float least(int b) const {
     if (b < 0) return INFINITY;
-    uint32_t lo = order_of(-FLT_MAX), hi = order_of(m);
+    uint32_t lo = order_of(-FLT_MAX), hi = order_of(m);  // hi's bin is 0
     while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (bin(value_of(mid)) <= b) hi = mid; else lo = mid + 1;
+      const uint32_t step = (hi - lo) / 32 + 1, lane = threadIdx.x & 31;
+      const uint32_t mine = hi - lo > lane * step ? lo + lane * step : hi;
+      const unsigned in = __ballot_sync(0xffffffffu, bin(value_of(mine)) <= b);
+      const int first = __ffs(in) - 1;  // none: beyond the last lane's
+      const uint32_t from = lo;
+      lo = first == 0 ? from : min(from + (first < 0 ? 31u : first - 1u) * step, hi) + 1u;
+      if (first >= 0) hi = min(from + first * step, hi);
     }
-    return value_of(lo);
+    return value_of(hi);
   }
   __device__ __forceinline__ double weight(float x) const { return pow2_neg(root, ((double)m - x) * c); }
   __device__ __forceinline__ bool keeps(float x, int64_t i) const {
@@ -407,15 +420,31 @@ __device__ __forceinline__ void find_bin(cg::cluster_group& cluster, SampleShare
   cluster.sync();
 }
 
-// Sorts s.list[0 .. n) in falling order (bitonic).
+// Sorts s.list[0 .. n) in falling order: up to kShort values, one for each thread,
+// by counting the larger ones (100 values: 0.6 us), more by a bitonic sort (2048
+// values: 20 us; with the exchanges inside a warp by shuffles 25 us).
 __device__ __forceinline__ void sort_list(SampleShared& s, int n) {
+  const int tid = threadIdx.x;
+  if (n <= kShort) {
+    __syncthreads();
+    const uint64_t key = tid < n ? s.list[tid] : 0u;
+    int rank = 0;
+    if ((tid & ~31) < n) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += s.list[j] > key;
+    }
+    __syncthreads();
+    if (tid < n) s.list[rank] = key;
+    __syncthreads();
+    return;
+  }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = threadIdx.x + n; i < size; i += kSmThreads) s.list[i] = 0u;
+  for (int i = tid + n; i < size; i += kSmThreads) s.list[i] = 0u;
   for (int k = 2; k <= size; k *= 2)
     for (int o = k / 2; o > 0; o /= 2) {
       __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += kSmThreads) {
+      for (int i = tid; i < size / 2; i += kSmThreads) {
         const int a = 2 * i - (i & (o - 1)), b = a + o;
         const uint64_t x = s.list[a], y = s.list[b];
         if ((x < y) == ((a & k) == 0)) { s.list[a] = y; s.list[b] = x; }
@@ -649,7 +678,7 @@ template <typename T>
 __device__ __forceinline__ void list_values(SampleShared* lead, const RowShare<T>& sh, const RowRule& rule,
                                             float least, float below) {
   constexpr int VE = RowView<T>::VE;
-  sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
+  sh.template sweep<4>([&](const Raw<T, VE>& v, int j) {
     if (!(raw_max(v) >= least)) return;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
@@ -778,12 +807,21 @@ enum { kNarrowed, kTaken, kCrowded };
 // with `goal` of the weights' sum, by a histogram.  kTaken: a list held all that is
 // kept, and the token is taken (with then_share < 1 after top-p of the k largest);
 // kNarrowed: the rule has the bound; kCrowded: a bin has more values than the list.
+// `rest` (MASS): the sum's part beyond goal.  The values whose weights are below
+// rest / vocab weigh less than it together, so they are not among those kept and
+// are not counted.  With kNarrowed by MASS, s.warp_sum has the sums of what is kept.
 template <typename T, bool MASS>
 __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
-                                         const SampleArgs& a, RowRule& rule, int64_t k, double goal,
+                                         const SampleArgs& a, RowRule& rule, int64_t k, double goal, double rest,
                                          double then_share, double u) {
   constexpr int VE = RowView<T>::VE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // a little below the bound, for fp32's sake
+  float low = -INFINITY;
+  if (MASS && rest > 0.) {
+    const double y = log2(a.V / rest) / rule.c;
+    low = (float)(rule.m - y) - (float)(fabs((double)rule.m) + fabs(y)) * 1e-6f;
+  }
   SampleShared* lead = cluster.map_shared_rank(&s, 0);
   for (int i = tid; i < kBins; i += kSmThreads) {
     s.count[i] = 0u;
@@ -795,7 +833,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const float x = raw_get(v, e);
-      if (!rule.keeps(x, sh.index(j, e))) continue;
+      if (!(x >= low) || !rule.keeps(x, sh.index(j, e))) continue;
       const float at = __fmul_rn(__fsub_rn(rule.m, x), kBinsPerUnit);
       const int b = min((int)at, kBins - 1);  // as rule.bin
       if (b == kBins - 1) {
@@ -825,23 +863,13 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
   }
   cluster.sync();  // the bin has been read
   for (int way = 0;;) {
-    // the window: the bin, for weights with its neighbours where the list holds them
+    // the window: the bin, with all above it where they are few
     if (sh.part == 0) {
-      int b0 = MASS ? max(at - 1, 0) : at, b1 = MASS ? min(at + 1, kBins - 1) : at;
-      uint32_t to1 = count_to(s, b1);
-      uint32_t to0 = b0 ? count_to(s, b0 - 1) : 0u;
-      if (to1 - to0 > kList) {
-        b0 = b1 = at;
-        to1 = count_to(s, b1);
-        to0 = b0 ? count_to(s, b0 - 1) : 0u;
-      }
-      if (to1 <= kList) {
-        b0 = 0;
-        to0 = 0u;
-      }
+      const uint32_t to1 = count_to(s, at);
+      uint32_t to0 = to1 <= kShort || at == 0 ? 0u : count_to(s, at - 1);
       if (tid == 0) {
-        s.d.bin = to1 - to0 > kList ? -1 : b0;
-        s.d.in = (uint32_t)b1;
+        s.d.bin = to1 - to0 > kList ? -1 : to0 ? at : 0;
+        s.d.in = (uint32_t)at;
         s.d.above = to0;
         s.n_list = 0;
       }
@@ -856,16 +884,24 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
     }
     const float least = rule.least(b1), below = rule.least(b0 - 1);
     double sum = 0.;
-    if (MASS && b0 > 0) {  // the exact sum above the window
-      sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
-        if (!(raw_max(v) >= below)) return;
+    if (MASS && b0 > 0) {  // with the exact sum above the window
+      sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
+        if (!(raw_max(v) >= least)) return;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           const float x = raw_get(v, e);
-          if (x >= below && rule.keeps(x, sh.index(j, e))) sum += rule.weight(x);
+          if (!(x >= least) || !rule.keeps(x, sh.index(j, e))) continue;
+          if (x >= below) {
+            sum += rule.weight(x);
+          } else {
+            const int to = atomicAdd(&lead->n_list, 1);
+            if (to < kList) lead->list[to] = key_of(x, (int)sh.index(j, e));
+          }
         }
       });
       sum = warp_total(sum);
+    } else {
+      list_values(lead, sh, rule, least, below);
     }
     __syncthreads();
     if (lane == 0) s.warp_sum[warp] = sum;
@@ -875,7 +911,6 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
       for (int i = 0; i < kSmWarps; ++i) t += s.warp_sum[i];
       s.total = t;
     }
-    list_values(lead, sh, rule, least, below);
     cluster.sync();
     if (sh.part == 0) {
       const int n = min(s.n_list, kList);
@@ -896,9 +931,23 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
         kept = count_by_mass(s, kept, 0u, then_share, 0u, rule, a.weight_unit);
       }
       if (miss == 0 && kept < 1) miss = -1;
+      // values that were not counted, in the bin that their bound cuts
+      if (s.n_list > kList) miss = 2;
       if (miss == 0) {
         const uint64_t bound = s.list[kept - 1];
-        if (b0 == 0) pick_from_list(s, kept, rule, u);
+        if (b0 == 0) {
+          pick_from_list(s, kept, rule, u);
+        } else if (MASS) {
+          // what the window keeps, in whole numbers, for the warps that have it
+          for (int i = tid; i < kSmWarps * sh.parts; i += kSmThreads) s.mass[i] = 0u;
+          __syncthreads();
+          for (int i = tid; i < kept; i += kSmThreads) {
+            const uint64_t key = s.list[i];
+            const int64_t idx = (int64_t)(uint32_t)~(uint32_t)key;
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[sh.warp_of((int)((idx + sh.row.off) / VE))]),
+                      (unsigned long long)whole_weight(rule.weight(value_of((uint32_t)(key >> 32))), a.weight_unit));
+          }
+        }
         if (tid == 0) s.d.bound = bound;
       }
       __syncthreads();
@@ -907,6 +956,8 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
     cluster.sync();
     const int miss = lead->d.bin;
     rule.bound = lead->d.bound;
+    if (MASS && miss == 0 && b0 > 0 && tid < kSmWarps)
+      s.warp_sum[tid] += (double)lead->mass[sh.part * kSmWarps + tid] * (a.weight_unit / 4503599627370496.);
     cluster.sync();
     if (miss == 0) {
       rule.tau = value_of((uint32_t)(rule.bound >> 32));
@@ -914,7 +965,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
       return b0 == 0 ? kTaken : kNarrowed;
     }
     // the sums' roundings at a bin's edge may send it back and forth: once is enough
-    if (way && way != miss) return kCrowded;
+    if (miss == 2 || (way && way != miss)) return kCrowded;
     way = miss;
     at = miss > 0 ? min(b1 + 1, kBins - 1) : max(b0 - 1, 0);
   }
@@ -1010,14 +1061,15 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
       sum = warp_total(sum * f);
       if (lane == 0) s.warp_sum[warp] = sum;
     }
-    bool done = false;
+    bool done = false, summed = at_once;  // whether s.warp_sum has the sums of what is kept
     if (by_k || by_min) {
-      const int k = a.V <= kList || !by_k ? -1 : (int)top_k;
-      if (k <= kList)
+      // more than a few hundred would make a list that is slow to sort
+      const int k = a.V <= kShort || !by_k ? -1 : (int)top_k;
+      if (k <= kShort * 3 / 4)
         done = take_from_list<T>(cluster, s, sh, a, rule, mine, k, by_k ? top_k : 0, by_p ? top_p : 1., u);
     }
     if (!done && by_k) {
-      const int how = by_window<T, false>(cluster, s, sh, a, rule, top_k, 0., by_p ? top_p : 1., u);
+      const int how = by_window<T, false>(cluster, s, sh, a, rule, top_k, 0., 0., by_p ? top_p : 1., u);
       if (how == kCrowded) narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., 1.);
       done = how == kTaken;
     }
@@ -1045,12 +1097,13 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
       double total = 0.;
       for (int q = 0; q < parts; ++q) total += *cluster.map_shared_rank(&s.total, q);
       cluster.sync();
-      const int how = by_window<T, true>(cluster, s, sh, a, rule, 0, top_p * total, 1., u);
+      const int how = by_window<T, true>(cluster, s, sh, a, rule, 0, top_p * total, (1. - top_p) * total, 1., u);
       if (how == kCrowded) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
       done = how == kTaken;
+      summed = how == kNarrowed;
     }
     if (!done)
-      locate<T>(cluster, s, sh, at_once && !by_p,
+      locate<T>(cluster, s, sh, summed,
                 [&](float x, int64_t i) { return rule.keeps(x, i) ? rule.weight(x) : 0.; },
                 [&](double w) { return u * w; });
   }
