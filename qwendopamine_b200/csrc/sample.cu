@@ -1,6 +1,6 @@
 // sample.cu -- one token for each row of logits from one given random number.
 //
-// Mathematics, with m = max x and w_i = exp((x_i - m) / temperature) = 2^y_i:
+// Mathematics, with m = max x and w_i = exp((x_i - m) / temperature) = 2^-y_i:
 //   kept by min-p:  w_i >= min_p;   by top-k: the k largest of those;
 //   by top-p: of what is left, in falling order, up to the first running sum
 //   that reaches top_p of the sum;  equal logits rank by rising index
@@ -20,19 +20,21 @@
 // rules and takes the token.  Top-p alone, and what the list does not hold, go by a
 // histogram over bins of equal width in x: counts, and the values' mean place in the
 // bin.  A bin's weight is close to its count times the weight at that place, which
-// puts top-p's bound within a bin; the next sweep forms the exact sum above it and lists the bin, and if the bound is not
-// in it the next bin is taken.  Where the bin and all above it are few, the list
-// decides as before.
+// gives the bin that has top-p's bound; the next sweep forms the exact sum above it
+// and lists the bin, and if the bound is not in it the next bin is taken.  Where the
+// bin and all above it are few, the list decides as before.
 // A bin with more values than the list holds (equal logits, or logits within a
 // hundredth) is cut by the digits of the values' ordered bits, 11 at a time, with
-// weights as whole numbers of 2^-44, and among equal values the lower indices are
-// counted out.
+// weights as whole numbers of 2^-44 (larger units for vocabularies beyond 2^18), and
+// among equal values the lower indices are counted out.
 //
 // Bound: by temperature alone the row is read once and the time is that of the
-// fp64 pipe, 12 operations for a value; with a short list the row is read once from
-// memory and once from L2.  Few rows are split over the CTAs of a cluster, which
-// exchange through distributed shared memory: what is counted is added to the first
-// CTA's histogram by remote atomics, which nobody waits for.
+// fp64 pipe, 12 operations for a value (256 x 151936 bf16: 88 us a
+// call); with a short list the row is read once from memory and once from L2 (64 x
+// 151936 with top-k 50 31 us, 256 rows 51 us); with top-p 0.6 alone 98 and 272 us.
+// Few rows are split over the CTAs of a cluster, which exchange through distributed
+// shared memory: what is counted is added to the first CTA's histogram by remote
+// atomics, which nobody waits for.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -53,7 +55,7 @@ constexpr int kBins = 2048;
 constexpr int kBinsPer = kBins / kSmThreads;   // bins of a thread
 constexpr int kList = 2048;                    // longest list that is sorted
 constexpr int kShort = kSmThreads;             // of a list that is sorted by counting
-constexpr int kPlaces = 4096;                  // of a bin: 2^20 values' places fit 32 bits
+constexpr int kPlaces = 4096;                  // of a bin; 2^20 values' sum fits 32 bits
 constexpr float kBinsPerUnit = 46.f;           // bins of a logit: 44 units below the maximum
 
 struct SampleArgs {
@@ -503,12 +505,10 @@ __device__ __forceinline__ int count_by_mass(SampleShared& s, int n, uint64_t ab
 }
 
 // Narrows rule.bound to the k largest kept values (MASS false), or to those whose
-// weight before them is below share * (all).  With then_share < 1 the second
-// follows the first, if a list serves both; returns whether it did.
+// weight before them is below share * (all).
 template <typename T, bool MASS>
-__device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
-                                       const SampleArgs& a, RowRule& rule, int64_t k, double share,
-                                       double then_share) {
+__device__ __forceinline__ void narrow(cg::cluster_group& cluster, SampleShared& s, const RowShare<T>& sh,
+                                       const SampleArgs& a, RowRule& rule, int64_t k, double share) {
   constexpr int VE = RowView<T>::VE;
   const int tid = threadIdx.x;
   SampleShared* lead = cluster.map_shared_rank(&s, 0);
@@ -546,14 +546,13 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
     const int b = lead->d.bin;
     if (b < 0) {  // fewer values than k: all are kept
       cluster.sync();
-      return false;
+      return;
     }
     above = lead->d.above;
     mass_above = lead->d.mass_above;
     mass_all = lead->d.mass;
     const uint32_t in = lead->d.in;
-    const bool whole = round == 0 && above + in <= kList;  // all down to the bin as one list
-    if (whole || in <= kList) {
+    if (in <= kList) {
       sh.template sweep<1>([&](const Raw<T, VE>& v, int j) {
         const float most = raw_max(v);
         if (most == -INFINITY || (round == 0 ? rule.bin(most) > b : rule.bin(most) > bin)) return;
@@ -563,7 +562,7 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
           if (!rule.keeps(x, sh.index(j, e))) continue;
           const int c = rule.bin(x);
           if (round == 0) {
-            if (c > b || (!whole && c < b)) continue;
+            if (c != b) continue;
           } else {
             if (c != bin) continue;
             const uint32_t o = order_of(x);
@@ -578,15 +577,9 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
       if (sh.part == 0) {
         const int n = min(s.n_list, kList);
         sort_list(s, n);
-        if (whole) above = 0u;
         int kept;
-        if constexpr (MASS) {
-          kept = count_by_mass(s, n, whole ? 0u : mass_above, share, mass_all, rule, a.weight_unit);
-        } else {
-          kept = (int)min(k - above, (int64_t)n);
-          if (whole && then_share < 1.)
-            kept = count_by_mass(s, kept, 0u, then_share, 0u, rule, a.weight_unit);
-        }
+        if constexpr (MASS) kept = count_by_mass(s, n, mass_above, share, mass_all, rule, a.weight_unit);
+        else kept = (int)min(k - above, (int64_t)n);
         if (tid == 0) s.d.bound = s.list[kept - 1];
       }
       cluster.sync();
@@ -594,7 +587,7 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
       rule.tau = value_of((uint32_t)(rule.bound >> 32));
       rule.all_keys = false;
       cluster.sync();
-      return whole;
+      return;
     }
     if (round == 0) {
       bin = b;
@@ -621,7 +614,7 @@ __device__ __forceinline__ bool narrow(cg::cluster_group& cluster, SampleShared&
       rule.tau = x0;
       rule.all_keys = false;
       cluster.sync();
-      return false;
+      return;
     }
   }
 }
@@ -695,7 +688,8 @@ __device__ __forceinline__ void list_values(SampleShared* lead, const RowShare<T
 // with a value where rounding leaves none.  Into s.d.bin (-1: fewer than k), with the
 // counts above and in it and its neighbours'.  The leader's threads.
 template <bool MASS>
-__device__ __forceinline__ void scan_bins(SampleShared& s, uint32_t k, double goal, const RowRule& rule) {
+__device__ __forceinline__ void scan_bins(SampleShared& s, uint32_t k, double goal, int places,
+                                          const RowRule& rule) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t c[kBinsPer], cs = 0u;
   double w[kBinsPer], ws = 0.;
@@ -704,7 +698,7 @@ __device__ __forceinline__ void scan_bins(SampleShared& s, uint32_t k, double go
     const int b = tid * kBinsPer + i;
     c[i] = s.count[b];
     cs += c[i];
-    const double place = MASS && c[i] ? b + (double)s.place[b] / (kPlaces * (double)c[i]) : 0.;
+    const double place = MASS && c[i] ? b + (double)s.place[b] / (places * (double)c[i]) : 0.;
     w[i] = MASS && c[i] ? c[i] * pow2_neg(rule.root, place * (1. / kBinsPerUnit) * rule.c) : 0.;
     ws += w[i];
   }
@@ -775,7 +769,7 @@ __device__ __forceinline__ bool take_from_list(cg::cluster_group& cluster, Sampl
   if (k >= 0) {
     if (mine != -INFINITY) atomicAdd(&lead->count[rule.bin(mine)], 1u);
     cluster.sync();
-    if (sh.part == 0) scan_bins<false>(s, (uint32_t)k, 0., rule);
+    if (sh.part == 0) scan_bins<false>(s, (uint32_t)k, 0., 1, rule);
     cluster.sync();
     const int most = lead->d.bin;
     cluster.sync();
@@ -828,6 +822,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
     s.place[i] = 0u;
   }
   cluster.sync();
+  const int places = a.V <= 1 << 20 ? kPlaces : 1;  // beyond, the bin's start: more bins are tried
   uint32_t far = 0u;  // in the last bin, where masks by low values all are
   sh.template sweep<2>([&](const Raw<T, VE>& v, int j) {
 #pragma unroll
@@ -841,7 +836,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
         continue;
       }
       atomicAdd(&s.count[b], 1u);
-      if constexpr (MASS) atomicAdd(&s.place[b], (uint32_t)((at - b) * kPlaces));
+      if constexpr (MASS) atomicAdd(&s.place[b], (uint32_t)((at - b) * places));
     }
   });
   far = __reduce_add_sync(0xffffffffu, far);
@@ -854,7 +849,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
         if constexpr (MASS) atomicAdd(&lead->place[i], s.place[i]);
       }
   cluster.sync();
-  if (sh.part == 0) scan_bins<MASS>(s, (uint32_t)min(k, (int64_t)0x7fffffff), goal, rule);
+  if (sh.part == 0) scan_bins<MASS>(s, (uint32_t)min(k, (int64_t)0x7fffffff), goal, places, rule);
   cluster.sync();
   int at = lead->d.bin;
   if (at < 0) {
@@ -1070,7 +1065,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
     }
     if (!done && by_k) {
       const int how = by_window<T, false>(cluster, s, sh, a, rule, top_k, 0., 0., by_p ? top_p : 1., u);
-      if (how == kCrowded) narrow<T, false>(cluster, s, sh, a, rule, top_k, 0., 1.);
+      if (how == kCrowded) narrow<T, false>(cluster, s, sh, a, rule, top_k, 0.);
       done = how == kTaken;
     }
     if (!done && by_p) {
@@ -1098,7 +1093,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
       for (int q = 0; q < parts; ++q) total += *cluster.map_shared_rank(&s.total, q);
       cluster.sync();
       const int how = by_window<T, true>(cluster, s, sh, a, rule, 0, top_p * total, (1. - top_p) * total, 1., u);
-      if (how == kCrowded) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p, 1.);
+      if (how == kCrowded) narrow<T, true>(cluster, s, sh, a, rule, 0, top_p);
       done = how == kTaken;
       summed = how == kNarrowed;
     }

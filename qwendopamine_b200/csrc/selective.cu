@@ -10,20 +10,26 @@
 //   dx_t = dt_t sum_n B_t e_t + D o_t,  ddt_t = sum_n A a_t h_{t-1} e_t + x_t sum_n B_t e_t
 //   dA = sum_t dt_t a_t h_{t-1} e_t,  dD = sum_t o_t x_t,  dz_t = dy_t (sum_n C_t h_t + D x_t) silu'(z_t)
 //
-// A channel takes L lanes with four states each, in registers from row to row;
-// what a row needs of a channel (dt, dt x, o) and of a group (B, C) is formed
-// once, 16 rows at a time, in shared memory.  Sums over a channel's lanes, and
-// over a warp's channels for dB and dC, travel transposed: each step halves both
-// the lanes that are apart and the values that a lane still holds.
+// A channel's states stay in registers from row to row, four to a lane forward and
+// two of each of two channels backward.  Rows come in 16 at a time by asynchronous
+// copies, one block ahead; what a row needs of a channel (dt, dt x, o) is formed once
+// for all lanes, in shared memory, and there the lanes leave their shares of sums over
+// a channel's states.  The sums over channels, dB and dC, are products on the tensor
+// core (TF32 operands, fp32 sums): a lane has its operands' values as they are.
 //
 // The time axis is cut where channels and sequences alone leave SMs idle: each
 // chunk's end state is formed from a zero start, a second launch carries them from
 // chunk to chunk (a chunk's decay is exp(A sum dt)), and the third starts every
 // chunk from its state.  The backward does the same with e.  The forward keeps the
-// state in front of every 16 rows; the backward forms the 16 rows' states again,
-// eight at a time in registers.  dB and dC are summed over a CTA's channels in
-// shared memory and over the CTAs by a launch of their own: every sum has a fixed
-// order, equal inputs give equal bits.
+// state in front of every 16 rows; the backward forms the 16 rows' states again and
+// holds four rows' at a time.  The CTAs' shares of dB and dC are summed by a launch of
+// their own: every sum has a fixed order, equal inputs give equal bits.
+//
+// Bound: shared memory's bandwidth and the exponentials forward (8 x 4096 tokens x
+// 2048 channels x 16 states in bf16: 690 us, of which one exponential a state and
+// row takes 239), instructions issued backward (2.1 ms, three times the forward's
+// arithmetic); both were twice as long with rows read as they were needed and sums
+// exchanged between lanes.
 #include "mma16.cuh"
 #include "op_util.cuh"
 
@@ -38,6 +44,7 @@ constexpr int kSub = 16;   // rows of a block: one kept state for each
 constexpr int kHeld = 4;   // rows whose states the backward holds at a time
 constexpr int kHalf = 8;   // rows whose sums it hands on at a time
 constexpr int kMostChunks = 640;  // of the time axis
+constexpr float kNear = 1.f + .72f / 2048.f;  // of TF32's rounding
 constexpr float kSelLn2 = 0.6931471805599453f;
 
 struct SelSource {  // a token tensor's rows
@@ -398,14 +405,6 @@ __device__ __forceinline__ pair64 pfma(pair64 a, pair64 b, pair64 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-__device__ __forceinline__ pair64 pexp2(pair64 a) {  // as fast_exp2
-  pair64 d;
-  asm("{\n\t.reg .f32 x, y;\n\tmov.b64 {x, y}, %1;\n\tex2.approx.ftz.f32 x, x;\n\t"
-      "ex2.approx.ftz.f32 y, y;\n\tmov.b64 %0, {x, y};\n\t}"
-      : "=l"(d)
-      : "l"(a));
-  return d;
-}
 __device__ __forceinline__ pair64 to_pair(float2 v) {
   pair64 d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(v.x), "f"(v.y));
@@ -634,7 +633,8 @@ template <bool BACK> __global__ void __launch_bounds__(256) k_sel_carry(const Se
       const int c = BACK ? a.chunks - 1 - (k0 + i) : k0 + i;
       if (k0 + i >= a.chunks) break;
       a.carry[(base + c) * per + at] = run;
-      run = begins[c] ? own[i] : fmaf(fast_exp2(dsum[i] * A2), run, own[i]);
+      // nothing stays nothing, however large the factor
+      run = begins[c] || run == 0.f ? own[i] : fmaf(fast_exp2(dsum[i] * A2), run, own[i]);
     }
   }
 }
@@ -717,9 +717,10 @@ __device__ __forceinline__ void mma_tf32_new(float (&d)[4], const uint32_t (&a)[
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// A value as a TF32 operand, of which the tensor core takes the upper 19 bits: half
-// a step is added where it is to be rounded to nearest.
-__device__ __forceinline__ uint32_t tf32_near(float x) { return __float_as_uint(x) + 0x1000u; }
+// A value as a TF32 operand, of which the tensor core takes the upper 19 bits: a
+// factor of 1 + 0.72 * 2^-11 in front of that keeps values of 11 bits, infinities and
+// NaN, and leaves the others within 1.28 * 2^-11 with errors of mean zero.
+__device__ __forceinline__ uint32_t tf32_near(float x) { return __float_as_uint(x * kNear); }
 __device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x) & 0xffffe000u; }
 
 // Sums over a warp's eight channels (of each set) by the tensor core: A holds a
@@ -799,7 +800,8 @@ __device__ __forceinline__ void bwd_rows(const SelArgs& a, SelBwdShared<T, L>& s
 #pragma unroll
   for (int j = kHeld - 1; j >= 0; --j) {
     const int r = q + j, at = r & (kHalf - 1);
-    const float2 B = *reinterpret_cast<const float2*>(s.b + r * SelTile<L>::NL + 2 * t.l), C = *reinterpret_cast<const float2*>(s.c + r * SelTile<L>::NL + 2 * t.l);
+    const float2 B = *reinterpret_cast<const float2*>(s.b + r * SelTile<L>::NL + 2 * t.l);
+    const float2 C = *reinterpret_cast<const float2*>(s.c + r * SelTile<L>::NL + 2 * t.l);
     const float2 o = *reinterpret_cast<const float2*>(&s.o[r][t.mc]);
     if constexpr (EDGE) {
       const int n = s.edges.end[r];
@@ -1132,61 +1134,59 @@ __device__ __forceinline__ void store_four(float* p, int N, int n0, bool vec, co
   }
 }
 
-// Every lane has four states of a channel.
+// Every lane has four states of a channel.  What does not depend on the token's place
+// in the pool is read first.  The time is that of short chains of reads: 64 tokens of
+// 4096 channels of 16 states take 11 us (their states 5.5 us of traffic), 256 45 us at
+// three quarters of the issue rate.  Two channels to a lane (half the instructions),
+// four tokens to a CTA, and the next token's values on their way while one is worked
+// on were no faster (45, 47 and 103 us for the 256).
 template <typename T, int L>
 __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float* state, int64_t stride,
                                                           int pool, const int32_t* idx) {
-  constexpr int CH = kSelThreads / L;
-  const int tiles = (a.D + CH - 1) / CH;
-  const int n = blockIdx.x / tiles, d = (blockIdx.x - n * tiles) * CH + threadIdx.x / L, l = threadIdx.x % L;
-  const bool on = d < a.D;
-  const int slot = idx ? idx[n] : n;
+  const int64_t n = blockIdx.x;
+  const int d = (int)(blockIdx.y + gridDim.y * blockIdx.z) * (kSelThreads / L) + threadIdx.x / L, l = threadIdx.x % L;
+  const unsigned lanes = __ballot_sync(0xffffffffu, d < a.D);
+  if (d >= a.D) return;  // all of a channel's lanes
+  const int slot = idx ? idx[n] : (int)n;
+  const bool vec = (a.N & 3) == 0 && ((reinterpret_cast<uintptr_t>(state) | (stride * 4) |
+                                       reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+  const bool vec_bc = (a.N & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.Bv) | reinterpret_cast<uintptr_t>(a.Cv) |
+                                          ((a.ldb | a.ldc) * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
+  const int left = a.N - 4 * l, at = (a.G > 1 ? d / (a.D / a.G) * a.N : 0) + 4 * l;
+  const T* pb = (const T*)a.Bv + n * a.ldb + at;
+  const T* pc = (const T*)a.Cv + n * a.ldc + at;
+  const Raw<T, 4> B = vec_bc ? load_group<T, 4, true>(pb, left) : load_group<T, 4, false>(pb, left);
+  const Raw<T, 4> C = vec_bc ? load_group<T, 4, true>(pc, left) : load_group<T, 4, false>(pc, left);
+  const float x = to_f<T>(((const T*)a.x)[n * a.ldx + d]);
+  float dt = a.dt_f32 ? ((const float*)a.dt)[n * a.lddt + d] : to_f<T>(((const T*)a.dt)[n * a.lddt + d]);
+  const float z = a.z ? to_f<T>(((const T*)a.z)[n * a.ldz + d]) : 0.f;
+  float2 A2[2], h[2];
+  load_four(a.A + (int64_t)d * a.N, a.N, 4 * l, vec, A2);
+  T* y = (T*)a.y + n * a.D + d;
   if (slot < 0 || slot >= pool) {
-    if (on && l == 0) ((T*)a.y)[(int64_t)n * a.D + d] = from_f<T>(0.f);
+    if (l == 0) *y = from_f<T>(0.f);
     return;
   }
-  float2 h[2] = {f2(0.f), f2(0.f)}, A2[2], B[2], C[2];
   float* p = state + slot * stride + (int64_t)d * a.N;
-  const bool vec = (a.N & 3) == 0 && ((reinterpret_cast<uintptr_t>(state) | (stride * 4)) & 15) == 0 &&
-                   (reinterpret_cast<uintptr_t>(a.A) & 15) == 0;
-  float x = 0.f, dt = 0.f;
-  if (on) {
-    load_four(p, a.N, 4 * l, vec, h);
-    load_four(a.A + (int64_t)d * a.N, a.N, 4 * l, vec, A2);
-    x = to_f<T>(((const T*)a.x)[n * a.ldx + d]);
-    dt = a.dt_f32 ? ((const float*)a.dt)[n * a.lddt + d] : to_f<T>(((const T*)a.dt)[n * a.lddt + d]);
-    if (a.bias) dt += a.bias[d];
-    if (a.softplus) dt = softplus_f(dt);
-  } else {
-    A2[0] = A2[1] = f2(0.f);
-  }
-  const int g = on ? d / (a.D / a.G) : 0;
-  float b[4], c[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = on && 4 * l + i < a.N;
-    b[i] = in ? to_f<T>(((const T*)a.Bv)[n * a.ldb + g * a.N + 4 * l + i]) : 0.f;
-    c[i] = in ? to_f<T>(((const T*)a.Cv)[n * a.ldc + g * a.N + 4 * l + i]) : 0.f;
-  }
+  load_four(p, a.N, 4 * l, vec, h);
+  if (a.bias) dt += a.bias[d];
+  if (a.softplus) dt = softplus_f(dt);
   float out = 0.f;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    B[u] = make_float2(b[2 * u], b[2 * u + 1]);
-    C[u] = make_float2(c[2 * u], c[2 * u + 1]);
-    h[u] = fma2(exp2_2(mul2(f2(dt), mul2(A2[u], f2(kLog2e)))), h[u], mul2(f2(dt * x), B[u]));
-    const float2 o = mul2(h[u], C[u]);
+  for (int i = 0; i < 2; ++i) {
+    const float2 b = make_float2(raw_get(B, 2 * i), raw_get(B, 2 * i + 1));
+    const float2 c = make_float2(raw_get(C, 2 * i), raw_get(C, 2 * i + 1));
+    h[i] = fma2(exp2_2(mul2(f2(dt), mul2(A2[i], f2(kLog2e)))), h[i], mul2(f2(dt * x), b));
+    const float2 o = mul2(h[i], c);
     out += o.x + o.y;
   }
-  if (on) store_four(p, a.N, 4 * l, vec, h);
+  store_four(p, a.N, 4 * l, vec, h);
 #pragma unroll
-  for (int o = L / 2; o > 0; o /= 2) out += __shfl_xor_sync(0xffffffffu, out, o);
-  if (on && l == 0) {
+  for (int o = L / 2; o > 0; o /= 2) out += __shfl_xor_sync(lanes, out, o);
+  if (l == 0) {
     if (a.Dk) out = fmaf(a.Dk[d], x, out);
-    if (a.z) {
-      const float z = to_f<T>(((const T*)a.z)[n * a.ldz + d]);
-      out *= z * sigmoid_f(z);
-    }
-    ((T*)a.y)[(int64_t)n * a.D + d] = from_f<T>(out);
+    if (a.z) out *= z * sigmoid_f(z);
+    *y = from_f<T>(out);
   }
 }
 
@@ -1216,10 +1216,10 @@ int check_sel(const gdn2_selective_problem* p, const char* fn) {
       return fail(GDN2_ERR_INVALID, "%s: row strides must be D .. 2^22 elements (got %lld)", fn, (long long)ld);
   if (p->ld_b < least || p->ld_b > most || p->ld_c < least || p->ld_c > most)
     return fail(GDN2_ERR_INVALID, "%s: row strides of B and C must be G N .. 2^22 elements", fn);
-  if (p->T > (int64_t)1 << 40 || (p->B && p->T > ((int64_t)1 << 40) / p->B))
+  if (p->B && p->T > ((int64_t)1 << 40) / p->B)
     return fail(GDN2_ERR_UNSUPPORTED, "%s: too many rows", fn);
-  if (p->cu_seqlens && p->T > 2147483647LL)
-    return fail(GDN2_ERR_UNSUPPORTED, "%s: packed rows are up to 2^31 - 1", fn);
+  if (p->T > 2147483647LL)
+    return fail(GDN2_ERR_UNSUPPORTED, "%s: sequences are up to 2^31 - 1 rows", fn);
   if (p->T > 0 && p->B > 0 && p->n_seqs == 0)
     return fail(GDN2_ERR_INVALID, "%s: rows without a sequence in cu_seqlens", fn);
   return GDN2_OK;
@@ -1232,8 +1232,9 @@ struct SelPlan {
 
 // Cuts the time axis into chunks of whole 16 rows where the CTAs of the channels
 // and batch entries alone are fewer than two for each of 148 SMs (the extra
-// launches cost three quarters of the forward once more); then as many chunks as
-// give four for each, of 64 rows at least.
+// launches cost two thirds of the forward and a quarter of the backward once more:
+// 201 + 10 of 515 us and 226 + 9 of 1206 us at 65536 tokens x 512 channels); then as
+// many chunks as give four for each, of 64 rows at least.
 SelPlan sel_plan(const gdn2_selective_problem* p) {
   SelPlan q;
   const int ch = kSelThreads / lanes_of(p->N);
@@ -1473,15 +1474,15 @@ int gdn2_selective_step(const gdn2_selective_problem* p, const void* x, const vo
                 (long long)p->D * p->N, (long long)state_stride);
   if (pool < 0 || (!state_indices && pool < p->B))
     return fail(GDN2_ERR_INVALID, "%s: %d sequences need as many states (got %d)", fn, p->B, pool);
-  const int ch = kSelThreads / lanes_of(p->N);
-  const int64_t ctas = (int64_t)p->B * ((p->D + ch - 1) / ch);
-  if (too_many(ctas)) return fail(GDN2_ERR_UNSUPPORTED, "%s: too many sequences", fn);
+  const int ch = kSelThreads / lanes_of(p->N), tiles = (p->D + ch - 1) / ch;
+  const unsigned most = 65535u, deep = (tiles + most - 1) / most;
+  const dim3 grid((unsigned)p->B, (tiles + deep - 1) / deep, deep);
   SelArgs a = sel_args(p, sel_plan(p));
   a.x = x; a.dt = dt; a.A = A; a.Bv = Bv; a.Cv = Cv; a.Dk = D; a.z = z; a.bias = dt_bias; a.y = y;
   const cudaStream_t st = (cudaStream_t)stream;
   return cuda_status(with_lanes(p->dtype, p->N, [&](auto t, auto lanes) {
     k_sel_step<decltype(t), decltype(lanes)::value>
-        <<<(unsigned)ctas, kSelThreads, 0, st>>>(a, state, state_stride, pool, state_indices);
+        <<<grid, kSelThreads, 0, st>>>(a, state, state_stride, pool, state_indices);
     return cudaGetLastError();
   }), fn);
 }

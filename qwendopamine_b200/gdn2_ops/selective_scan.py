@@ -186,9 +186,9 @@ def selective_scan(
     otherwise.  Returns ``(y, final_state)``, y in x's dtype; states and sums are
     float32.  Differentiable (once, in reverse mode) in every tensor but
     ``cu_seqlens``; for that the forward keeps a state every 16 tokens, ``D N / 4``
-    bytes a token, and the backward takes as much scratch again.  States that grow
-    (``d A > 0``) must stay finite over a chunk of the time axis, also where they are
-    zero.  Rows may be strided (slices of a fused projection).
+    bytes a token, and the backward takes as much scratch again.  The factor
+    by which states grow (``d A > 0``) must stay finite over a chunk of the time axis.
+    Rows may be strided (slices of a fused projection).
     """
     fn = "selective_scan"
     _check(fn, x, dt, A, B, C, D, z, dt_bias, 2)

@@ -5,7 +5,9 @@ A log2(e), 2^-24 of the product, times an exponent below 4) and takes the
 hardware's base-2 exponential (2^-22), then two products and a sum: below 2^-20.5
 in all, over an effective window of at most 30 steps at these decays (0.1 and more
 in the exponent): 2e-5.  16-bit results: one rounding of a value that is right to
-fp32, at most 2^-9 (bf16) or 2^-12 (fp16) of each element; twice that.  States and
+fp32, at most 2^-8 (bf16) or 2^-11 (fp16) of each element and 0.58 of that in the
+mean over elements; the terms of dB and dC in bf16 have two factors rounded within
+1.28 * 2^-11, a third of 2^-8 together.  States and
 the gradients of fp32 inputs are fp32 results whatever the token type; so are dA,
 dD, ddt_bias, whose terms with 16-bit gates carry 2^-21 more.
 """
@@ -222,6 +224,26 @@ def test_a_sequence_does_not_see_its_neighbours_nan(cuda_device):
             assert torch.equal(c[:, :20], d[:, :20]) and torch.equal(c[:, 37:], d[:, 37:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF, FH])
+@pytest.mark.parametrize("n", [4, 16, 40])
+def test_nan_reaches_what_it_is_in(cuda_device, n, dtype):
+    """A NaN in x is in y, dC and dA from its row on, in dB in its row alone; one in
+    dy is in dB and dx up to its row."""
+    for name, row in (("x", 25), ("dy", 40)):
+        v = inputs(cuda_device, 1, 70, 12, n, dtype, dtype, 1, seed=24)
+        v[name][:, row] = torch.nan
+        leaves = [v[k].requires_grad_() for k in ("x", "A", "B", "C")]
+        y, _ = run(v)
+        dx, dA, dB, dC = torch.autograd.grad(y, leaves, v["dy"])
+        at = torch.arange(70, device=cuda_device)[None, :, None]
+        nan = lambda t, rows: torch.equal(t.isnan(), rows.expand(t.shape))
+        assert dA.isnan().all()
+        if name == "x":
+            assert nan(y, at >= row) and nan(dC, at >= row) and nan(dB, at == row) and not dx.isnan().any()
+        else:
+            assert not y.isnan().any() and nan(dC, at == row) and nan(dB, at <= row) and nan(dx, at <= row)
+
+
 def test_equal_inputs_give_equal_bits(cuda_device):
     v = inputs(cuda_device, 1, 3000, 100, 16, BF, BF, 1, seed=15)
     a, b = check(v), check(v)
@@ -241,7 +263,8 @@ def test_scan_in_pieces_equals_the_whole(cuda_device):
 
 @pytest.mark.parametrize("dtype,dtdtype", TYPES)
 @pytest.mark.parametrize("n,d,states,groups", [(1, 1, 1, None), (5, 70, 16, None), (64, 48, 16, 2), (3, 33, 8, 3),
-                                               (2, 20, 64, None), (4, 20, 13, 4)])
+                                               (2, 20, 64, None), (4, 20, 13, 4), (601, 260, 16, None), (7, 33, 16, None),
+                                               (299, 500, 6, 5)])
 def test_step(cuda_device, n, d, states, groups, dtype, dtdtype):
     v = inputs(cuda_device, n, 1, d, states, dtype, dtdtype, n, groups=groups, seed=17)
     pool = torch.randn(n + 3, d, states, device=cuda_device)
