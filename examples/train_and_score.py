@@ -28,7 +28,7 @@ from torch import nn
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 from qwendopamine_b200 import (  # noqa: E402
-    AdamW, GatedDeltaNet2, gated_scan, gated_scan_step, token_logprobs)
+    AdamW, GatedDeltaNet2, gated_scan, gated_scan_step, grad_norm, token_logprobs)
 
 VOCAB, HIDDEN, IGNORE = 97, 128, -100
 
@@ -115,8 +115,8 @@ def train(model, steps, device):
         kept = (targets != IGNORE).sum()
         loss = -(r.logprobs.sum() + 1e-3 * r.entropy.sum()) / kept
         loss.backward()
-        norm = torch.stack([p.grad.float().norm() for p in model.parameters()]).norm()
-        opt.step(grad_scale=(1.0 / norm.clamp(min=1.0)).reshape(()))  # clip at 1, on the device
+        r = grad_norm([p.grad for p in model.parameters()], max_norm=1.0)
+        opt.step(grad_scale=r.clip_coef, found_inf=r.found_inf)  # clipped on the device
         last = loss.detach()
         first = last if first is None else first
     return float(first), float(last)
