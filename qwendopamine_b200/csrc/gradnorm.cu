@@ -6,10 +6,10 @@
 // Each CTA sums a chunk of one tensor into a double; a second launch of one CTA
 // adds those in a fixed order, so equal inputs give equal bits.  A thread adds
 // the squares of up to 64 values in fp32 and those sums in fp64: an error of a few
-// 2^-24 that does not grow with the number of values.  Squares leave fp32's range for values above 2^64 or
-// below 2^-75, which 16-bit gradients can hold: where a thread's fp32 sum
-// is outside [2^-80, finite] it forms the same sum in fp64 from the values that
-// it still has.  The largest magnitude is found on the bit patterns, where NaN
+// 2^-24 that does not grow with the number of values.  Squares leave fp32's range
+// for values above 2^64 or below 2^-75, which 16-bit gradients can hold: where a
+// thread's fp32 sum is outside [2^-80, finite] it forms the same sum in fp64 from the
+// values that it still has.  The largest magnitude is found on the bit patterns, where NaN
 // is above infinity.
 //
 // Bound: HBM, one read of the gradients (and one more read and a write where
@@ -375,8 +375,9 @@ int gdn2_grad_norm(const gdn2_grad_problem* p, const gdn2_grad_tensor* tensors, 
   if (!workspace || workspace_bytes < gdn2_grad_norm_workspace_bytes(n))
     return fail(GDN2_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes", fn,
                 gdn2_grad_norm_workspace_bytes(n));
-  if (!aligned_to(workspace, 8))
-    return fail(GDN2_ERR_INVALID, "%s: the workspace must start on an 8-byte boundary", fn);
+  if (!aligned_to(workspace, 8) || !aligned_to(out, 4))
+    return fail(GDN2_ERR_INVALID, "%s: the workspace must start on an 8-byte boundary, the results on a 4-byte one",
+                fn);
   double* partial = (double*)workspace;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool most = p->norm_type == 0;
@@ -402,7 +403,8 @@ int gdn2_grad_scale(const gdn2_grad_tensor* tensors, int32_t n, const float* coe
   if (total == 0) return GDN2_OK;
   rc = check_apart(tensors, n, fn);
   if (rc) return rc;
-  if (!coef) return fail(GDN2_ERR_INVALID, "%s: null coefficient", fn);
+  if (!coef || !aligned_to(coef, 4))
+    return fail(GDN2_ERR_INVALID, "%s: the coefficient is null or not aligned to 4 bytes", fn);
   const cudaStream_t st = (cudaStream_t)stream;
   return cuda_status(for_tables(tensors, n, grad_chunk(total),
                                 [&](const GradTensors& ts, unsigned chunks, int64_t) {

@@ -42,6 +42,9 @@ inline bool aligned_to(const void* p, size_t n) {
   return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
 }
 
+// Whether all of the pointers (NULL among them) are on multiples of n bytes.
+template <typename... P> bool all_aligned(size_t n, P... p) { return (aligned_to(p, n) && ...); }
+
 // f(T{}) with the element type of `dtype`.
 template <typename F> cudaError_t with_dtype(int dtype, F&& f) {
   switch (dtype) {

@@ -29,9 +29,9 @@
 // among equal values the lower indices are counted out.
 //
 // Bound: by temperature alone the row is read once and the time is that of the
-// fp64 pipe, 12 operations for a value (256 x 151936 bf16: 88 us a
-// call); with a short list the row is read once from memory and once from L2 (64 x
-// 151936 with top-k 50 31 us, 256 rows 51 us); with top-p 0.6 alone 98 and 272 us.
+// fp64 pipe, 12 operations for a value (256 x 151936 bf16: 88 us a call); with a
+// short list the row is read once from memory and once from L2 (64 x 151936 with
+// top-k 50 31 us, 256 rows 51 us); with top-p 0.6 alone 98 and 272 us.
 // Few rows are split over the CTAs of a cluster, which exchange through distributed
 // shared memory: what is counted is added to the first CTA's histogram by remote
 // atomics, which nobody waits for.
@@ -1151,8 +1151,9 @@ int gdn2_sample(const gdn2_sample_problem* p, const void* logits, const float* u
   if (p->rows > 2147483647LL / 8) return fail(GDN2_ERR_UNSUPPORTED, "%s: too many rows", fn);
   if (p->rows == 0) return GDN2_OK;
   if (!logits || !uniform || !token_ids) return fail(GDN2_ERR_INVALID, "%s: null pointer", fn);
-  if (!aligned_to(logits, dtype_size(p->dtype)))
-    return fail(GDN2_ERR_INVALID, "%s: logits are not aligned to their elements", fn);
+  if (!aligned_to(logits, dtype_size(p->dtype)) || !aligned_to(token_ids, 8) ||
+      !all_aligned(4, uniform, temperature, top_k, top_p, min_p))
+    return fail(GDN2_ERR_INVALID, "%s: a pointer is not aligned to its elements", fn);
   const cudaError_t e = num_sms(&sms);
   if (e != cudaSuccess) return cuda_status(e, fn);
   const int64_t row_bytes = (int64_t)p->vocab * (int64_t)dtype_size(p->dtype);

@@ -1327,6 +1327,16 @@ template <typename K> cudaError_t allow_shared(K local, K full, int bytes) {
   return e == cudaSuccess ? cudaFuncSetAttribute(local, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : e;
 }
 
+// What the element accesses of a call need: token tensors, dt, fp32 arrays.
+template <typename... P>
+int check_elements(const gdn2_selective_problem* p, const char* fn, const void* dt, const void* ddt, P... tok) {
+  if (all_aligned(dtype_size(p->dtype), tok...) && all_aligned(dtype_size(p->dt_dtype), dt, ddt)) return GDN2_OK;
+  return fail(GDN2_ERR_INVALID, "%s: a tensor is not aligned to its elements", fn);
+}
+template <typename... P> int check_words(const char* fn, P... f32) {
+  return all_aligned(4, f32...) ? GDN2_OK : fail(GDN2_ERR_INVALID, "%s: an fp32 array is not aligned to 4 bytes", fn);
+}
+
 bool too_many(int64_t ctas) { return ctas > 2147483647LL; }
 
 }  // namespace
@@ -1366,6 +1376,8 @@ int gdn2_selective_fwd(const gdn2_selective_problem* p, const void* x, const voi
     return fail(GDN2_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes", fn, w.total);
   if (!aligned_to(workspace, 16) || !aligned_to(saved, 16))
     return fail(GDN2_ERR_INVALID, "%s: workspace and saved must start on 16-byte boundaries", fn);
+  if (check_elements(p, fn, dt, nullptr, x, Bv, Cv, z, y) || check_words(fn, A, D, dt_bias, h0, ht, p->cu_seqlens))
+    return GDN2_ERR_INVALID;
   cudaError_t e = pass_states(p, h0, ht, st);
   if (e != cudaSuccess) return cuda_status(e, fn);
   if (!some) return GDN2_OK;
@@ -1419,6 +1431,9 @@ int gdn2_selective_bwd(const gdn2_selective_problem* p, const void* x, const voi
     return fail(GDN2_ERR_WORKSPACE, "%s: needs a workspace of %zu bytes", fn, w.total);
   if (!aligned_to(workspace, 16) || !aligned_to(saved, 16))
     return fail(GDN2_ERR_INVALID, "%s: workspace and saved must start on 16-byte boundaries", fn);
+  if (check_elements(p, fn, dt, ddt, x, Bv, Cv, z, dy, dx, dB, dC, dz) ||
+      check_words(fn, A, D, dt_bias, h0, dht, dA, dD, ddt_bias, dh0, p->cu_seqlens))
+    return GDN2_ERR_INVALID;
   cudaError_t e = pass_states(p, dht, dh0, st);
   if (e != cudaSuccess) return cuda_status(e, fn);
   if (!some) {
@@ -1474,6 +1489,8 @@ int gdn2_selective_step(const gdn2_selective_problem* p, const void* x, const vo
                 (long long)p->D * p->N, (long long)state_stride);
   if (pool < 0 || (!state_indices && pool < p->B))
     return fail(GDN2_ERR_INVALID, "%s: %d sequences need as many states (got %d)", fn, p->B, pool);
+  if (check_elements(p, fn, dt, nullptr, x, Bv, Cv, z, y) || check_words(fn, A, D, dt_bias, state, state_indices))
+    return GDN2_ERR_INVALID;
   const int ch = kSelThreads / lanes_of(p->N), tiles = (p->D + ch - 1) / ch;
   const unsigned most = 65535u, deep = (tiles + most - 1) / most;
   const dim3 grid((unsigned)p->B, (tiles + deep - 1) / deep, deep);

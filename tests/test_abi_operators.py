@@ -73,6 +73,23 @@ def test_selective_step(lib):
     assert step(sel(T=1, B=0, n_seqs=0)) == N.OK
 
 
+def test_selective_pointers_off_their_elements(lib):
+    """Each pointer in turn one byte off: refused in front of any CUDA call."""
+    odd = ctypes.c_void_p(0x1001)
+    p = sel()
+    for i in range(12):  # x dt A B C D z dt_bias h0 y ht saved
+        args = [odd if k == i else F for k in range(12)]
+        assert lib.gdn2_selective_fwd(p, *args, F, 1 << 40, None) == N.ERR_INVALID, i
+    for i in range(21):  # the inputs to h0, saved, dy, dht, then the gradients
+        args = [odd if k == i else F for k in range(21)]
+        assert lib.gdn2_selective_bwd(p, *args, F, 1 << 40, None) == N.ERR_INVALID, i
+    one = sel(T=1)
+    for i in (0, 1, 2, 3, 4, 5, 6, 7, 8, 11, 12):
+        args = [odd if k == i else F for k in range(13)]
+        args[9], args[10] = 1024, 2
+        assert lib.gdn2_selective_step(one, *args, None) == N.ERR_INVALID, i
+
+
 def sample(**kw):
     base = dict(rows=4, ld=1000, vocab=1000, dtype=1, top_k=0, temperature=1.0, top_p=1.0, min_p=0.0)
     return N.SampleProblem(**{**base, **kw})
@@ -91,6 +108,10 @@ def test_sample_pointers_and_sizes(lib):
     for bad in (dict(x=None), dict(u=None), dict(ids=None), dict(x=ctypes.c_void_p(0x1001))):
         assert call(sample(), **bad) == N.ERR_INVALID
     assert call(sample(rows=1 << 30)) == N.ERR_UNSUPPORTED
+    odd = ctypes.c_void_p(0x1002)
+    for i in range(6):  # uniform temperature top_k top_p min_p token_ids
+        args = [odd if k == i else F for k in range(6)]
+        assert lib.gdn2_sample(sample(), F, *args, None) == N.ERR_INVALID, i
 
 
 def table(*rows):
@@ -106,6 +127,8 @@ def test_gradient_norm(lib):
     assert norm(good, 1, out=None) == N.ERR_INVALID
     assert norm(good, 1, ws=None) == N.ERR_WORKSPACE and norm(good, 1, size=100) == N.ERR_WORKSPACE
     assert norm(good, 1, ws=ctypes.c_void_p(0x1004)) == N.ERR_INVALID
+    assert norm(good, 1, out=ctypes.c_void_p(0x1002)) == N.ERR_INVALID
+    assert lib.gdn2_grad_scale(good, 1, ctypes.c_void_p(0x1002), None) == N.ERR_INVALID
     for bad, status in ((( 0x1000, -1, 0), N.ERR_INVALID), ((0, 10, 0), N.ERR_INVALID), ((0x1000, 10, 3), N.ERR_INVALID),
                         ((0x1002, 10, 0), N.ERR_INVALID), ((0x1001, 10, 1), N.ERR_INVALID),
                         ((0x1000, 1 << 50, 0), N.ERR_UNSUPPORTED)):
