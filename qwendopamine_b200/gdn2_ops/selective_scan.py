@@ -30,6 +30,13 @@ __all__ = ["SelectiveScanFunction", "selective_scan", "selective_scan_step"]
 MAX_STATES = 64
 
 
+def _f32(p):
+    """A parameter as the kernels read it (its address is all that is used)."""
+    if p is None or p.dtype is torch.float32 and p.is_contiguous():
+        return p
+    return p.detach().float().contiguous()
+
+
 class _Call:
     """Sizes, packing, row strides and parameters of one call."""
 
@@ -45,8 +52,7 @@ class _Call:
         self.z, self.ldz = (None, d) if z is None else _rows(z, b, t, d)
         self.B, self.ldb = _rows(B, b, t, g * n)
         self.C, self.ldc = _rows(C, b, t, g * n)
-        f32 = lambda p: None if p is None else p.detach().float().contiguous()
-        self.A, self.D, self.bias = f32(A), f32(D), f32(dt_bias)
+        self.A, self.D, self.bias = _f32(A), _f32(D), _f32(dt_bias)
 
     def problem(self, lddy=None):
         return N.SelectiveProblem(self.b, self.d, self.g, self.states, self.t, N.dtype_code(self.x.dtype),
@@ -117,8 +123,8 @@ class SelectiveScanFunction(torch.autograd.Function):
 
 
 def _check(fn, x, dt, A, B, C, D, z, dt_bias, lead):
-    given = {"x": x, "dt": dt, "A": A, "B": B, "C": C, "D": D, "z": z, "dt_bias": dt_bias}
-    for t in given.values():
+    device, dtype = x.device, x.dtype
+    for t in (x, dt, A, B, C, D, z, dt_bias):
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{fn}: inputs must be CUDA tensors -- the B200 build has no CPU path")
     if x.ndim != lead + 1 or x.shape[-1] == 0:
@@ -129,8 +135,7 @@ def _check(fn, x, dt, A, B, C, D, z, dt_bias, lead):
     n = A.shape[1]
     if n > MAX_STATES:
         raise NotImplementedError(f"{fn}: up to {MAX_STATES} states are supported; got {n}")
-    for name in ("dt", "z"):
-        t = given[name]
+    for name, t in (("dt", dt), ("z", z)):
         if t is not None and t.shape != x.shape:
             raise ValueError(f"{fn}: {name} must have x's shape {tuple(x.shape)}; got {tuple(t.shape)}")
     if B.shape != C.shape or B.ndim not in (lead + 1, lead + 2) or B.shape[:lead] != x.shape[:lead] \
@@ -139,19 +144,20 @@ def _check(fn, x, dt, A, B, C, D, z, dt_bias, lead):
                          f"{tuple(B.shape)} and {tuple(C.shape)}")
     if B.ndim == lead + 2 and (B.shape[lead] == 0 or d % B.shape[lead]):
         raise ValueError(f"{fn}: {d} channels do not divide into {B.shape[lead]} groups")
-    for name in ("D", "dt_bias"):
-        t = given[name]
+    for name, t in (("D", D), ("dt_bias", dt_bias)):
         if t is not None and t.shape != (d,):
             raise ValueError(f"{fn}: {name} must be [{d}]; got {tuple(t.shape)}")
-    for name, t in given.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{fn}: {name} is on {t.device}, x on {x.device}")
-        if t is not None:
+    for name, t in (("dt", dt), ("A", A), ("B", B), ("C", C), ("D", D), ("z", z), ("dt_bias", dt_bias)):
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{fn}: {name} is on {t.device}, x on {device}")
+        if t.dtype is not torch.float32:
             N.dtype_code(t.dtype)
-    for name in ("B", "C", "z"):
-        t = given[name]
-        if t is not None and t.dtype != x.dtype:
-            raise NotImplementedError(f"{fn}: x ({x.dtype}) and {name} ({t.dtype}) must share a dtype")
+    N.dtype_code(dtype)
+    for name, t in (("B", B), ("C", C), ("z", z)):
+        if t is not None and t.dtype is not dtype:
+            raise NotImplementedError(f"{fn}: x ({dtype}) and {name} ({t.dtype}) must share a dtype")
     if dt.dtype != x.dtype and dt.dtype != torch.float32:
         raise NotImplementedError(f"{fn}: dt ({dt.dtype}) must be float32 or x's dtype ({x.dtype})")
 
@@ -269,7 +275,8 @@ def selective_scan_step(
         idx = state_indices
         if idx.dtype is not torch.int32:  # outside the pool stays outside in 32 bits
             idx = idx.to(torch.int64).clamp(-1, state.shape[0]).to(torch.int32)
-        idx = idx.to(x.device).contiguous()
+        if idx.device != x.device or not idx.is_contiguous():
+            idx = idx.to(x.device).contiguous()
     elif state.shape[0] < n:
         raise ValueError(f"{n} sequences need as many states; got {state.shape[0]}")
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
