@@ -472,7 +472,8 @@ int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensor
  * values in a row [G][N] of B and C.  N <= 64.  Row r = b*T + t of a tensor starts at
  * element r * ld_* (up to 2^22); y and the gradients are contiguous.  cu_seqlens
  * (int32 [n_seqs+1], device) starts at 0, ends at T and does not decrease; n_seqs =
- * B without it.  A sequence without tokens passes its state on.
+ * B without it.  A sequence without tokens passes its state on.  T < 2^31; every
+ * pointer is aligned to its elements.
  * Where the time axis is cut (few channels and sequences), a chunk's decays are
  * composed before they are applied: with d A > 0 their product over a chunk has
  * to stay finite in fp32.
