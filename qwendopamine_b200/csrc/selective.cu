@@ -34,6 +34,7 @@
 #include "op_util.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace gdn2 {
 namespace {
@@ -725,25 +726,36 @@ __device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x
 
 // Sums over a warp's eight channels (of each set) by the tensor core: A holds a
 // value for each state and channel as the lanes have them, B the channels' factors
-// in every column.  bf16 results: the operands are rounded to TF32's 11 bits, three
-// more than the result keeps, and the sums are fp32.  Others: an operand is the sum
-// of two TF32 values, which leaves 2^-21 of it, and three products are summed.
+// in every column.  An operand is the sum of two TF32 values and three products are
+// summed in fp32, whatever the results' type: shares that cancel leave digits that
+// one TF32 operand (11 bits) does not have.  (One product, 8 x 4096 x 2048 x 16 in
+// bf16: forward and backward 2.81 ms, three 3.23 ms.)
 template <typename T>
 __device__ __forceinline__ void sum_channels(float (&sum)[4], const float2 (&v)[2], float w0, float w1) {
   const float x[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
-  uint32_t hi[4];
+  uint32_t hi[4], lo[4];
+  const uint32_t h0 = tf32_cut(w0), h1 = tf32_cut(w1);
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    // what the cuts leave (below 2^-20 of a value, and of a product's second order)
+    // counts where the first product is finite: infinity minus itself is NaN
 #pragma unroll
-    for (int i = 0; i < 4; ++i) hi[i] = tf32_near(x[i]);
-    mma_tf32_new(sum, hi, tf32_near(w0), tf32_near(w1));
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = tf32_cut(x[i]);
+      lo[i] = tf32_cut(x[i] - __uint_as_float(hi[i]));
+    }
+    float more[4];
+    mma_tf32_new(sum, hi, h0, h1);
+    mma_tf32_new(more, lo, h0, h1);
+    mma_tf32(more, hi, tf32_cut(w0 - __uint_as_float(h0)), tf32_cut(w1 - __uint_as_float(h1)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (fabsf(sum[i]) <= FLT_MAX) sum[i] += more[i];
   } else {
-    uint32_t lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       hi[i] = tf32_cut(x[i]);
       lo[i] = tf32_near(x[i] - __uint_as_float(hi[i]));
     }
-    const uint32_t h0 = tf32_cut(w0), h1 = tf32_cut(w1);
     mma_tf32_new(sum, hi, h0, h1);
     mma_tf32(sum, lo, h0, h1);
     mma_tf32(sum, hi, tf32_near(w0 - __uint_as_float(h0)), tf32_near(w1 - __uint_as_float(h1)));

@@ -1,0 +1,49 @@
+"""Values at which the selective scan's arithmetic is easily lost, against the float64
+oracle."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import op_oracle as O
+from qwendopamine_b200 import selective_scan
+
+pytestmark = pytest.mark.gpu
+F32, BF, FH = torch.float32, torch.bfloat16, torch.float16
+HALF_STEP = {F32: 2.0 ** -24, BF: 2.0 ** -8, FH: 2.0 ** -11}  # of a result's rounding
+
+
+def np64(t):
+    return t.detach().double().cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, FH])
+@pytest.mark.parametrize("n", [4, 16, 40])
+@pytest.mark.parametrize("pairs", [1, 20])
+def test_sums_over_channels_that_cancel(cuda_device, pairs, n, dtype):
+    """dB and dC where each channel's neighbour takes back all but a 2^-9th of its
+    share: what is left is made of digits that operands of 11 bits do not have.
+
+    Of the shares' sum of magnitudes: 4 rows' states and gradients, all of one sign, are
+    within 4 * 2^-20.5 (a decay and two products a row) and the products of operands cut
+    into two TF32 values within 2^-18, together below 2^-17; and the result's rounding."""
+    gen = torch.Generator().manual_seed(30 + pairs)
+    B, T, d = 2, 4, 2 * pairs
+    two = lambda t, sign=1: torch.stack([t, sign * t], -1).flatten(-2)
+    some = lambda *s: torch.rand(*s, generator=gen) + 0.5
+    dt = some(B, T, pairs)
+    dt = torch.stack([dt, dt * (1 + 2.0 ** -9 * some(B, T, pairs))], -1).flatten(-2)
+    A = -two(some(n, pairs)).t().contiguous()
+    x, dy = two(some(B, T, pairs)).to(dtype), two(some(B, T, pairs), -1).to(dtype)
+    vec = [some(B, T, n).to(dtype) for _ in range(2)]
+    ops = [t.to(cuda_device) for t in (x, dt, A, *vec)]
+    leaves = [t.requires_grad_() for t in ops[3:]]
+    y, _ = selective_scan(*ops)
+    got = torch.autograd.grad(y, leaves, dy.to(cuda_device))
+    # each channel its own group: the shares
+    wide = [np.repeat(np64(v)[:, :, None], d, 2) for v in vec]
+    g = O.selective_bwd(*(np64(t) for t in (x, dt, A)), *wide, None, None, None, False, None, np64(dy))
+    for v, k in zip(got, "BC"):
+        want, size = g[k].sum(2), np.abs(g[k]).sum(2)
+        assert (np.abs(want) < size * 2.0 ** -6).all()
+        assert (np.abs(np64(v) - want) <= HALF_STEP[dtype] * np.abs(want) + 2.0 ** -17 * size).all()
