@@ -250,8 +250,9 @@ template <typename E, int W, int K> struct RowCursor {
       Piece x{nullptr, 0, -1};
       if ((K * PIECES % kSelThreads == 0 || k < K) && src[k].p) {
         const int c = threadIdx.x % CPR * VE, n = max(0, min(ncols - c, VE));
-        // a piece without a value reads nothing, from an address that exists
-        x.p = (const char*)((const E*)src[k].p + (n ? (r0 + row_of(i)) * src[k].ld + col + c : 0));
+        // a piece without a value reads nothing, from an address that exists and has the
+        // alignment that was looked at (a group's first column may have another than column 0)
+        x.p = (const char*)((const E*)src[k].p + col + (n ? (r0 + row_of(i)) * src[k].ld + c : 0));
         x.step = n ? (int)(way * kSub * src[k].ld * (int)sizeof(E)) : 0;
         x.bytes = n * (int)sizeof(E);
       }

@@ -47,3 +47,33 @@ def test_sums_over_channels_that_cancel(cuda_device, pairs, n, dtype):
         want, size = g[k].sum(2), np.abs(g[k]).sum(2)
         assert (np.abs(want) < size * 2.0 ** -6).all()
         assert (np.abs(np64(v) - want) <= HALF_STEP[dtype] * np.abs(want) + 2.0 ** -17 * size).all()
+
+
+@pytest.mark.parametrize("dtype,dtdtype", [(F32, F32), (BF, F32), (BF, BF), (FH, FH)])
+@pytest.mark.parametrize("off", [1, 2, 3, 4, 6, 8, 12])
+@pytest.mark.parametrize("d,n", [(24, 20), (20, 10)])
+def test_groups_in_rows_off_every_alignment(cuda_device, d, n, off, dtype, dtdtype):
+    """Two groups of 12 or 10 channels and 20 or 10 states: their first columns are
+    aligned otherwise than the rows, and their last pieces are empty.  Equal bits."""
+    gen = torch.Generator().manual_seed(32)
+    B, T, g = 2, 50, 2
+    rn = lambda *s, dtype=dtype: torch.randn(*s, generator=gen).to(cuda_device, dtype)
+    A = -(torch.rand(d, n, generator=gen) + 0.5).to(cuda_device)
+    ops = [rn(B, T, d), rn(B, T, d, dtype=dtdtype), A, rn(B, T, g, n), rn(B, T, g, n), rn(d, dtype=F32), rn(B, T, d)]
+    dy = rn(B, T, d)
+
+    def moved(o):
+        if o.ndim < 3:
+            return o
+        flat = o.flatten(2)
+        wide = torch.full((B, T, 64), torch.nan, dtype=o.dtype, device=cuda_device)
+        wide[..., off:off + flat.shape[2]] = flat
+        return wide[..., off:off + flat.shape[2]].unflatten(2, o.shape[2:])
+
+    def both(ops, dy):
+        leaves = [o.detach().requires_grad_() for o in ops]
+        y, ht = selective_scan(*leaves, dt_softplus=True, output_final_state=True)
+        return [y.detach(), ht.detach(), *torch.autograd.grad((y, ht), leaves, (dy, torch.ones_like(ht)))]
+
+    want, got = both(ops, dy), both([moved(o) for o in ops], moved(dy))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
