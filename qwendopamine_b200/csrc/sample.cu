@@ -950,7 +950,7 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
     }
     cluster.sync();
     const int miss = lead->d.bin;
-    rule.bound = lead->d.bound;
+    if (miss == 0) rule.bound = lead->d.bound;  // a window that missed has none: the rule's own stays
     if (MASS && miss == 0 && b0 > 0 && tid < kSmWarps)
       s.warp_sum[tid] += (double)lead->mass[sh.part * kSmWarps + tid] * (a.weight_unit / 4503599627370496.);
     cluster.sync();

@@ -1,0 +1,42 @@
+"""Rows for which the token sampling's short ways do not suffice, against the float64
+oracle."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import op_oracle as O
+from qwendopamine_b200 import sample_tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def near_miss(gap, many):
+    """A row of 10 large values, then ``many`` equal ones ``gap`` below, and the top-p
+    that 1000 of these make the ten fall short of by a millionth.
+
+    Nine of the ten lie a 4096th of a bin (of 46 to a logit), less a tenth, further down
+    than the histogram's whole 4096ths say: their weight is taken for 4.8e-6 more than
+    it is, and half of that is what top-p asks beyond it."""
+    m = np.float32(6.0)
+    x1 = np.float32(m - np.float32((20 + (2048 + 0.9) / 4096) / 46))
+    w1, w0 = np.exp(float(x1) - 6.0), np.exp(-float(gap))
+    place = np.float32(m - x1) * np.float32(46.0)
+    over = (float(place) * 4096 % 1) / 4096 / 46
+    assert 4e-6 < over < 5.3e-6
+    row = np.full(6000, -np.inf, dtype=np.float32)
+    row[3:12], row[20] = x1, m
+    row[40:40 + many] = m - np.float32(gap)
+    return row, (1 + 9 * w1 * (1 + over / 2)) / (1 + 9 * w1 + 1000 * w0)
+
+
+def test_top_p_behind_equal_values_at_top_k(cuda_device):
+    """3000 equal logits at the top-k bound (more than a list holds: the first 1000 are
+    kept), and a top-p whose first window misses: the bound that top-k left stands."""
+    row, top_p = near_miss(6.0, 3000)
+    u = np.array([0.0, 0.3, 0.9, 0.999, 0.9999, 0.99999, 1 - 2.0 ** -24], dtype=np.float32)
+    want = [O.sample_token(row, float(v), 1.0, 1010, top_p) for v in u]
+    assert want[-1] == 40 and want[3] < 40  # ten large values and one of the others
+    x = torch.from_numpy(np.stack([row] * len(u))).to(cuda_device)
+    got = sample_tokens(x, torch.from_numpy(u).to(cuda_device), top_k=1010, top_p=top_p)
+    assert got.tolist() == want
