@@ -946,10 +946,23 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
         if (tid == 0) s.d.bound = bound;
       }
       __syncthreads();
-      if (tid == 0) s.d.bin = miss;
+      // a window that missed: the next bin that has values, below it or above
+      if (tid == 0) {
+        s.d.bin = miss;
+        s.first = miss > 0 ? kBins - 1 : 0;
+      }
+      __syncthreads();
+      if (MASS && (miss == 1 || miss == -1))
+#pragma unroll
+        for (int i = 0; i < kBinsPer; ++i) {
+          const int b = tid * kBinsPer + i;
+          if (!s.count[b]) continue;
+          if (miss > 0 && b > b1) atomicMin(&s.first, b);
+          if (miss < 0 && b < b0) atomicMax(&s.first, b);
+        }
     }
     cluster.sync();
-    const int miss = lead->d.bin;
+    const int miss = lead->d.bin, next = lead->first;
     if (miss == 0) rule.bound = lead->d.bound;  // a window that missed has none: the rule's own stays
     if (MASS && miss == 0 && b0 > 0 && tid < kSmWarps)
       s.warp_sum[tid] += (double)lead->mass[sh.part * kSmWarps + tid] * (a.weight_unit / 4503599627370496.);
@@ -960,9 +973,9 @@ __device__ __forceinline__ int by_window(cg::cluster_group& cluster, SampleShare
       return b0 == 0 ? kTaken : kNarrowed;
     }
     // the sums' roundings at a bin's edge may send it back and forth: once is enough
-    if (miss == 2 || (way && way != miss)) return kCrowded;
+    if (!MASS || miss == 2 || (way && way != miss)) return kCrowded;
     way = miss;
-    at = miss > 0 ? min(b1 + 1, kBins - 1) : max(b0 - 1, 0);
+    at = next;
   }
 }
 

@@ -40,3 +40,13 @@ def test_top_p_behind_equal_values_at_top_k(cuda_device):
     x = torch.from_numpy(np.stack([row] * len(u))).to(cuda_device)
     got = sample_tokens(x, torch.from_numpy(u).to(cuda_device), top_k=1010, top_p=top_p)
     assert got.tolist() == want
+
+
+@pytest.mark.parametrize("gap,many", [(6.0, 1000), (16.0, 1000), (6.0, 1990)])
+def test_a_gap_behind_a_window_that_misses(cuda_device, gap, many):
+    row, top_p = near_miss(gap, many)
+    u = np.concatenate([[0.0, 0.5, 0.99], 1 - 2.0 ** -np.arange(10, 25.0)]).astype(np.float32)
+    want = [O.sample_token(row, float(v), 1.0, 0, top_p) for v in u]
+    assert want[-1] >= 40
+    x = torch.from_numpy(np.stack([row] * len(u))).to(cuda_device)
+    assert sample_tokens(x, torch.from_numpy(u).to(cuda_device), top_p=top_p).tolist() == want
