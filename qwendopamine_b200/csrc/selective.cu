@@ -45,7 +45,6 @@ constexpr int kSub = 16;   // rows of a block: one kept state for each
 constexpr int kHeld = 4;   // rows whose states the backward holds at a time
 constexpr int kHalf = 8;   // rows whose sums it hands on at a time
 constexpr int kMostChunks = 640;  // of the time axis
-constexpr float kNear = 1.f + .72f / 2048.f;  // of TF32's rounding
 constexpr float kSelLn2 = 0.6931471805599453f;
 
 struct SelSource {  // a token tensor's rows
@@ -719,10 +718,8 @@ __device__ __forceinline__ void mma_tf32_new(float (&d)[4], const uint32_t (&a)[
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// A value as a TF32 operand, of which the tensor core takes the upper 19 bits: a
-// factor of 1 + 0.72 * 2^-11 in front of that keeps values of 11 bits, infinities and
-// NaN, and leaves the others within 1.28 * 2^-11 with errors of mean zero.
-__device__ __forceinline__ uint32_t tf32_near(float x) { return __float_as_uint(x * kNear); }
+// A value's upper 19 bits, a TF32 operand as it stands; of NaN those of the one that
+// arithmetic gives stay NaN.
 __device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x) & 0xffffe000u; }
 
 // Sums over a warp's eight channels (of each set) by the tensor core: A holds a
@@ -730,37 +727,25 @@ __device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x
 // in every column.  An operand is the sum of two TF32 values and three products are
 // summed in fp32, whatever the results' type: shares that cancel leave digits that
 // one TF32 operand (11 bits) does not have.  (One product, 8 x 4096 x 2048 x 16 in
-// bf16: forward and backward 2.81 ms, three 3.23 ms.)
-template <typename T>
+// bf16: forward and backward 2.81 ms, three 3.23 ms.)  What the cuts leave (below 2^-20
+// of a value, and of a product's second order) counts where the first product is
+// finite: infinity minus itself is NaN.
 __device__ __forceinline__ void sum_channels(float (&sum)[4], const float2 (&v)[2], float w0, float w1) {
   const float x[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
   uint32_t hi[4], lo[4];
-  const uint32_t h0 = tf32_cut(w0), h1 = tf32_cut(w1);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    // what the cuts leave (below 2^-20 of a value, and of a product's second order)
-    // counts where the first product is finite: infinity minus itself is NaN
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      hi[i] = tf32_cut(x[i]);
-      lo[i] = tf32_cut(x[i] - __uint_as_float(hi[i]));
-    }
-    float more[4];
-    mma_tf32_new(sum, hi, h0, h1);
-    mma_tf32_new(more, lo, h0, h1);
-    mma_tf32(more, hi, tf32_cut(w0 - __uint_as_float(h0)), tf32_cut(w1 - __uint_as_float(h1)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (fabsf(sum[i]) <= FLT_MAX) sum[i] += more[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      hi[i] = tf32_cut(x[i]);
-      lo[i] = tf32_near(x[i] - __uint_as_float(hi[i]));
-    }
-    mma_tf32_new(sum, hi, h0, h1);
-    mma_tf32(sum, lo, h0, h1);
-    mma_tf32(sum, hi, tf32_near(w0 - __uint_as_float(h0)), tf32_near(w1 - __uint_as_float(h1)));
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = tf32_cut(x[i]);
+    lo[i] = tf32_cut(x[i] - __uint_as_float(hi[i]));
   }
+  const uint32_t h0 = tf32_cut(w0), h1 = tf32_cut(w1);
+  float more[4];
+  mma_tf32_new(sum, hi, h0, h1);
+  mma_tf32_new(more, lo, h0, h1);
+  mma_tf32(more, hi, tf32_cut(w0 - __uint_as_float(h0)), tf32_cut(w1 - __uint_as_float(h1)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (fabsf(sum[i]) <= FLT_MAX) sum[i] += more[i];
 }
 
 // What a row has for a lane's two channels and two states.
@@ -827,8 +812,8 @@ __device__ __forceinline__ void bwd_rows(const SelArgs& a, SelBwdShared<T, L>& s
       e[i] = scale_add2(i ? o.y : o.x, C, e[i]);
     }
     float sb[4], sc[4];
-    sum_channels<T>(sb, e, x[j].u[0], x[j].u[1]);
-    sum_channels<T>(sc, hh, o.x, o.y);
+    sum_channels(sb, e, x[j].u[0], x[j].u[1]);
+    sum_channels(sc, hh, o.x, o.y);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float2 g = mul2(p[j][i], e[i]);
@@ -964,6 +949,9 @@ __global__ void __launch_bounds__(kSelThreads, 4) k_sel_bwd(const SelArgs a) {
       if (a.z) {
         const float2 z = raw.z(p);
         o = mul2(o, mul2(z, sigmoid2(z)));
+      } else if constexpr (sizeof(T) == 4) {  // the one NaN that tf32_cut keeps
+        if (o.x != o.x) o.x = __uint_as_float(0x7fffffffu);
+        if (o.y != o.y) o.y = __uint_as_float(0x7fffffffu);
       }
       *reinterpret_cast<float2*>(&s.o[row][t.pc]) = o;
     }

@@ -77,3 +77,45 @@ def test_groups_in_rows_off_every_alignment(cuda_device, d, n, off, dtype, dtdty
 
     want, got = both(ops, dy), both([moved(o) for o in ops], moved(dy))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, FH])
+@pytest.mark.parametrize("n", [4, 16, 40])
+def test_infinity_reaches_the_vectors_gradients(cuda_device, n, dtype):
+    """One infinite x or dy: dB and dC are infinite where their sums are, not NaN."""
+    gen = torch.Generator().manual_seed(31)
+    T, d, at = 70, 12, 30
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    for name in ("x", "dy"):
+        # decays of 0.8 and more: 40 steps keep an infinite state infinite, and finite ones finite
+        v = dict(x=rn(1, T, d).to(dtype), dt=(torch.rand(1, T, d, generator=gen) + 0.5).to(dtype),
+                 A=-0.1 * torch.rand(d, n, generator=gen), B=rn(1, T, n).to(dtype), C=rn(1, T, n).to(dtype),
+                 dy=rn(1, T, d).to(dtype))
+        v[name][0, at, 5] = torch.inf
+        ops = [v[k].to(cuda_device) for k in ("x", "dt", "A", "B", "C")]
+        leaves = [t.requires_grad_() for t in ops[3:]]
+        y, _ = selective_scan(*ops)
+        got = torch.autograd.grad(y, leaves, v["dy"].to(cuda_device))
+        with np.errstate(invalid="ignore"):
+            g = O.selective_bwd(*(np64(v[k]) for k in ("x", "dt", "A", "B", "C")), None, None, None, False, None,
+                                np64(v["dy"]))
+        for u, k in zip(got, "BC"):
+            a, want = np64(u), g[k]
+            assert np.isinf(want).any() and not np.isnan(want).any()
+            assert np.array_equal(np.isinf(a), np.isinf(want)) and not np.isnan(a).any()
+            assert np.array_equal(a[np.isinf(want)], want[np.isinf(want)])
+
+
+def test_every_nan_reaches_the_vectors_gradients(cuda_device):
+    """NaN of a gradient whose bits are all in the lower half of the word."""
+    gen = torch.Generator().manual_seed(33)
+    T, d, n, at = 40, 10, 16, 21
+    rn = lambda *s: torch.randn(*s, generator=gen).to(cuda_device)
+    ops = [rn(1, T, d), torch.rand(1, T, d, generator=gen).to(cuda_device), -rn(d, n).abs(), rn(1, T, n), rn(1, T, n)]
+    leaves = [t.requires_grad_() for t in ops[3:]]
+    dy = rn(1, T, d)
+    dy.view(torch.int32)[0, at, 3] = 0x7F800001
+    y, _ = selective_scan(*ops)
+    dB, dC = torch.autograd.grad(y, leaves, dy)
+    row = torch.arange(T, device=cuda_device)[None, :, None].expand(1, T, n)
+    assert torch.equal(dB.isnan(), row <= at) and torch.equal(dC.isnan(), row == at)
