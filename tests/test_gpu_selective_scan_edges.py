@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import op_oracle as O
-from qwendopamine_b200 import selective_scan
+from qwendopamine_b200 import selective_scan, selective_scan_step
 
 pytestmark = pytest.mark.gpu
 F32, BF, FH = torch.float32, torch.bfloat16, torch.float16
@@ -119,3 +119,50 @@ def test_every_nan_reaches_the_vectors_gradients(cuda_device):
     dB, dC = torch.autograd.grad(y, leaves, dy)
     row = torch.arange(T, device=cuda_device)[None, :, None].expand(1, T, n)
     assert torch.equal(dB.isnan(), row <= at) and torch.equal(dC.isnan(), row == at)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("n", [1, 3, 6, 12, 20, 33])
+@pytest.mark.parametrize("skip", [False, True])
+def test_infinity_in_states_that_do_not_fill_their_lanes(cuda_device, skip, n, dtype):
+    """One infinite x, dt or dy, everything else positive: sums that are infinite are
+    not NaN for the states that the lanes hold beyond the last, nor for a D that is not
+    there (with a positive one the same sums are infinite)."""
+    gen = torch.Generator().manual_seed(34)
+    T, d, at = 150, 10, 70
+    some = lambda *s: torch.rand(*s, generator=gen) + 0.5
+    for name in ("x", "dt", "dy"):
+        # decays of 0.97 and more: 150 steps keep what is infinite, and what is not
+        v = dict(x=some(1, T, d).to(dtype), dt=some(1, T, d).to(dtype), A=-0.02 * some(d, n), B=some(1, T, n).to(dtype),
+                 C=some(1, T, n).to(dtype), h0=some(1, d, n), D=some(d), dy=some(1, T, d).to(dtype))
+        v[name][0, at, 5] = torch.inf
+        ops = [v[k].to(cuda_device).requires_grad_(name != "dt") for k in ("x", "dt", "A", "B", "C", "h0")]
+        y, ht = selective_scan(*ops[:5], v["D"].to(cuda_device) if skip else None, initial_state=ops[5],
+                               output_final_state=True)
+        args = [*(np64(v[k]) for k in ("x", "dt", "A", "B", "C", "D")), None, None, False, np64(v["h0"])]
+        ry, _, rh = O.selective_fwd(*args)
+        pairs = [(y, ry), (ht, rh)]
+        if name != "dt":
+            got = torch.autograd.grad(y, ops, v["dy"].to(cuda_device))
+            with np.errstate(invalid="ignore"):
+                want = O.selective_bwd(*args, np64(v["dy"]))
+            pairs += [(g, want[k]) for g, k in zip(got, ("x", "dt", "A", "B", "C", "h0"))]
+        assert any(np.isinf(w).any() for _, w in pairs)
+        for a, w in pairs:
+            a = np64(a)
+            assert np.array_equal(np.isnan(a), np.isnan(w))
+            assert np.array_equal(np.isinf(a), np.isinf(w)) and (a[np.isinf(w)] == w[np.isinf(w)]).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 16, 20])
+def test_infinity_in_a_step(cuda_device, n):
+    one = lambda *s: torch.ones(*s, device=cuda_device)
+    for k in (0, 1):  # x, dt
+        ops = [one(2, 7), one(2, 7), -one(7, n), one(2, n), one(2, n)]
+        ops[k][0, 3] = torch.inf
+        pool = one(2, 7, n)
+        y = selective_scan_step(*ops, state=pool)
+        far = torch.zeros(2, 7, dtype=torch.bool, device=cuda_device)
+        far[0, 3] = True
+        assert torch.equal(y == torch.inf, far) and not y.isnan().any()
+        assert torch.equal(pool == torch.inf, far[..., None].expand_as(pool)) and not pool.isnan().any()
