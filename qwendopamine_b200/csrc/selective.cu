@@ -46,6 +46,7 @@ constexpr int kHeld = 4;   // rows whose states the backward holds at a time
 constexpr int kHalf = 8;   // rows whose sums it hands on at a time
 constexpr int kMostChunks = 640;  // of the time axis
 constexpr float kSelLn2 = 0.6931471805599453f;
+constexpr float kLog2eRest = 1.92596303e-8f;  // log2(e) - kLog2e
 
 struct SelSource {  // a token tensor's rows
   const void* p;
@@ -92,9 +93,15 @@ __device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_fast(x
 
 // ln(1 + e^v) = max(v, 0) + ln(1 + t), t = e^-|v|, without loss for very negative
 // v: with s = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh s = 2 (s + s^3/3 + s^5/5 ...),
-// whose terms from s^17 on are below 1e-9 of it.  Errors of about 2^-22.
+// whose terms from s^17 on are below 1e-9 of it.  t = 2^e (1 + r ln 2), where r is what
+// the exponent e = -|v| log2(e) loses to its rounding (up to |v| 2^-24) and log2(e) to
+// its own.  Within 3 * 2^-22 for v from -87 on; below, t is flushed to zero.
 __device__ __forceinline__ float2 softplus2(float2 v) {
-  const float2 t = exp2_2(mul2(make_float2(fabsf(v.x), fabsf(v.y)), f2(-kLog2e)));
+  // beyond 128 t is zero; the difference of two infinities would be NaN
+  const float2 w = make_float2(fminf(fabsf(v.x), 128.f), fminf(fabsf(v.y), 128.f));
+  const float2 e = mul2(w, f2(-kLog2e));
+  const float2 r = fma2(w, f2(-kLog2eRest), fma2(w, f2(-kLog2e), neg2(e)));
+  const float2 t0 = exp2_2(e), t = fma2(t0, mul2(r, f2(kSelLn2)), t0);
   const float2 s = mul2(t, rcp2(add2(t, f2(2.f)))), q = mul2(s, s);
   float2 p = fma2(q, f2(1.f / 15.f), f2(1.f / 13.f));
   p = fma2(q, p, f2(1.f / 11.f));
@@ -102,11 +109,12 @@ __device__ __forceinline__ float2 softplus2(float2 v) {
   p = fma2(q, p, f2(1.f / 7.f));
   p = fma2(q, p, f2(1.f / 5.f));
   p = fma2(q, p, f2(1.f / 3.f));
-  return fma2(f2(2.f), fma2(mul2(s, q), p, s), make_float2(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f)));
+  // NaN is not below zero
+  return fma2(f2(2.f), fma2(mul2(s, q), p, s), make_float2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y));
 }
 __device__ __forceinline__ float softplus_f(float v) { return softplus2(f2(v)).x; }
 
-// 1 / (1 + e^-v), errors of about 2^-21 (the exponent's rounding)
+// 1 / (1 + e^-v), within 2^-21; for v < 0 the exponent's rounding adds up to |v| 2^-23
 __device__ __forceinline__ float2 sigmoid2(float2 v) {
   return rcp2(add2(exp2_2(mul2(v, f2(-kLog2e))), f2(1.f)));
 }

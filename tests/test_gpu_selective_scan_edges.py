@@ -166,3 +166,27 @@ def test_infinity_in_a_step(cuda_device, n):
         far[0, 3] = True
         assert torch.equal(y == torch.inf, far) and not y.isnan().any()
         assert torch.equal(pool == torch.inf, far[..., None].expand_as(pool)) and not pool.isnan().any()
+
+
+def test_softplus_of_all_steps(cuda_device):
+    """One token whose y is softplus(dt): the hardware's base-2 exponential is within
+    2^-22, its reciprocal within 2^-23, and about four roundings add 2^-22: 3 * 2^-22."""
+    v = torch.linspace(-80.0, 20.0, 4096, device=cuda_device)
+    one = torch.ones(1, 1, 1, device=cuda_device)
+    A = -torch.ones(4096, 1, device=cuda_device)
+    y, _ = selective_scan(torch.ones(1, 1, 4096, device=cuda_device), v[None, None], A, one, one, dt_softplus=True)
+    x = np64(v)
+    want = np.maximum(x, 0) + np.log1p(np.exp(-np.abs(x)))
+    assert np.max(np.abs(np64(y)[0, 0] / want - 1)) <= 3 * 2.0 ** -22
+
+
+def test_softplus_of_no_numbers(cuda_device):
+    """Infinite steps and NaN, in a scan and in a step."""
+    v = torch.tensor([torch.inf, -torch.inf, torch.nan, -200.0, 3e38, -3e38], device=cuda_device)
+    one, A = torch.ones(1, 1, 1, device=cuda_device), -torch.ones(6, 1, device=cuda_device)
+    want = torch.tensor([torch.inf, 0.0, torch.nan, 0.0, 3e38, 0.0], device=cuda_device)
+    y, _ = selective_scan(torch.ones(1, 1, 6, device=cuda_device), v[None, None], A, one, one, dt_softplus=True)
+    y1 = selective_scan_step(torch.ones(1, 6, device=cuda_device), v[None], A, one[0], one[0], dt_softplus=True,
+                             state=torch.zeros(1, 6, 1, device=cuda_device))
+    for a in (y.flatten(), y1.flatten()):
+        assert torch.equal(a.nan_to_num(7.0, torch.inf), want.nan_to_num(7.0, torch.inf))
