@@ -46,7 +46,7 @@ constexpr int kHeld = 4;   // rows whose states the backward holds at a time
 constexpr int kHalf = 8;   // rows whose sums it hands on at a time
 constexpr int kMostChunks = 640;  // of the time axis
 constexpr float kSelLn2 = 0.6931471805599453f;
-constexpr float kLog2eRest = 1.92596303e-8f;  // log2(e) - kLog2e
+constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) - kLog2e
 
 struct SelSource {  // a token tensor's rows
   const void* p;

@@ -123,14 +123,21 @@ def clip_grad_norm_(
 ) -> GradNorm:
     r"""As :func:`grad_norm`, and ``grads`` multiplied in place by ``clip_coef``.
 
-    Each value is multiplied in float32 and rounded once to its tensor's dtype.
-    Gradients whose norm is within ``max_norm``, or not finite, stay as they are.
+    What is scaled is what is given, ``[p.grad for p in model.parameters()]``: unlike
+    the function of this name in ``torch.nn.utils`` it takes gradients, and refuses
+    ``nn.Parameter``.  Each value is multiplied in float32 and rounded once to its
+    tensor's dtype.  Gradients whose norm is 1e-6 and more within ``max_norm``, or not
+    finite, stay as they are.
     The tensors must fill their memory without gaps and must not overlap one
     another.  What is scaled counts as changed in place for autograd, also where
     the coefficient turns out to be 1 (nothing is read on the host).
     """
     fn = "clip_grad_norm_"
     kind, max_norm = _norm_code(fn, norm_type), _limit(fn, max_norm)
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if any(isinstance(g, torch.nn.Parameter) for g in grads):
+        raise TypeError(f"{fn}: takes gradients, and scales what it is given; got parameters "
+                        "(pass [p.grad for p in model.parameters()])")
     grads, device = _one_list(fn, grads)
     for g in grads:  # the order of the elements does not matter, gaps do
         if not g.is_contiguous() and not torch.ops.aten.is_non_overlapping_and_dense(g):
