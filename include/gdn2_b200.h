@@ -482,7 +482,9 @@ int gdn2_adamw_step(const gdn2_adamw_problem* p, const gdn2_adamw_tensor* tensor
  * others have their tensor's dtype.  `saved` (gdn2_selective_saved_bytes, 16-byte
  * aligned) is what the forward of the same inputs wrote, one state in front of
  * every 16 rows; a forward with saved NULL keeps nothing.  The workspace
- * (gdn2_selective_workspace_bytes, 16-byte aligned) belongs to one call at a time.
+ * (gdn2_selective_workspace_bytes, 16-byte aligned) belongs to one call at a time;
+ * in the backward it is 8 N bytes a row for each tile of 64, 32, 16 or 8 channels (N
+ * up to 8, 16, 32 or 64; every group has tiles of its own) and some for each chunk.
  * The order of all sums is fixed: equal inputs give equal bits. */
 typedef struct gdn2_selective_problem {
     int32_t B, D, G, N;

@@ -5,7 +5,8 @@ Per channel d and state n, ``h_t = exp(dt_t A) h_{t-1} + dt_t x_t B_t`` and ``y_
 (sum_n h_t C_t + D x_t) silu(z_t)``: decays and inputs depend on the token, and
 the vectors B and C are shared by a group of channels.  In front of it stands the
 block's short causal convolution (``short_conv``, for prompts and, with its prefix
-and state, for single tokens).
+and state, for single tokens; it knows no ``cu_seqlens``: packed sequences are
+convolved one by one, or as the rows of a padded batch).
 
 * :func:`selective_scan` -- whole sequences: fixed length ``[B, T, ...]`` or packed
   ``[1, T, ...]`` with ``cu_seqlens``, fp32 states in and out, differentiable.
@@ -192,7 +193,10 @@ def selective_scan(
     otherwise.  Returns ``(y, final_state)``, y in x's dtype; states and sums are
     float32.  Differentiable (once, in reverse mode) in every tensor but
     ``cu_seqlens``; for that the forward keeps a state every 16 tokens, ``D N / 4``
-    bytes a token, and the backward takes as much scratch again.  The factor
+    bytes a token (N rounded up to 4), and the backward takes ``8 N`` bytes of scratch a
+    token for each tile of 64, 32, 16 or 8 channels (up to 8, 16, 32 or 64 states): half
+    of what is kept, as much, twice or four times as much, and more where groups do not
+    fill their tiles, since each group has tiles of its own.  The factor
     by which states grow (``d A > 0``) must stay finite over a chunk of the time axis.
     Rows may be strided (slices of a fused projection).
     """
