@@ -556,8 +556,9 @@ int gdn2_sample(const gdn2_sample_problem* p, const void* logits, const float* u
  *   coef = min(1, max_norm / (norm + 1e-6))
  * out (fp32 [3], device): norm; coef, 1 for max_norm < 0 (none) and where norm is
  * not finite; 1 where norm is not finite, else 0.  Tensors are contiguous, their
- * dtypes may differ, a tensor may be listed twice and counts twice.  Sums are
- * fp64 and their order is fixed: equal inputs give equal bits.  The workspace
+ * dtypes may differ, a tensor may be listed twice and counts twice.  Squares are
+ * added in fp32 up to 64 at a time (in fp64 where fp32 does not hold their sum) and
+ * those sums in fp64, in a fixed order: equal inputs give equal bits.  The workspace
  * (gdn2_grad_norm_workspace_bytes, 8-byte aligned) belongs to one call at a time.
  * gdn2_grad_scale multiplies the tensors in place by a device scalar, rounded
  * once; a coefficient of 1 writes nothing.  Tensors that share memory are refused.

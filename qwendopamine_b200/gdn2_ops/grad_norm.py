@@ -101,8 +101,9 @@ def grad_norm(
     1e-6))`` (1 without ``max_norm``, and where the norm is not finite); and
     ``found_inf``, 1 where the norm is not finite, else 0.  ``AdamW.step`` takes
     the last two as ``grad_scale`` and ``found_inf``.  A tensor that is listed
-    twice counts twice; the norm of nothing but empty tensors is 0.  Squares that
-    float32 cannot hold are summed in float64.  Equal inputs give equal bits.
+    twice counts twice; the norm of nothing but empty tensors is 0.  Squares are added
+    in float32 up to 64 at a time (in float64 where float32 does not hold their sum)
+    and those sums in float64.  Equal inputs give equal bits.
     """
     kind = _norm_code("grad_norm", norm_type)
     if max_norm is not None:
