@@ -684,8 +684,9 @@ template <bool BACK> __global__ void __launch_bounds__(256) k_sel_carry(const Se
       const int c = BACK ? a.chunks - 1 - (k0 + i) : k0 + i;
       if (k0 + i >= a.chunks) break;
       a.carry[(base + c) * per + at] = run;
-      // nothing stays nothing, however large the factor
-      run = begins[c] || run == 0.f ? own[i] : fmaf(fast_exp2(dsum[i] * A2), run, own[i]);
+      // nothing stays nothing, however large the factor, and infinity infinite, however small
+      run = begins[c] || run == 0.f ? own[i]
+            : fabsf(run) == INFINITY ? run + own[i] : fmaf(fast_exp2(dsum[i] * A2), run, own[i]);
     }
   }
 }

@@ -190,3 +190,26 @@ def test_softplus_of_no_numbers(cuda_device):
                              state=torch.zeros(1, 6, 1, device=cuda_device))
     for a in (y.flatten(), y1.flatten()):
         assert torch.equal(a.nan_to_num(7.0, torch.inf), want.nan_to_num(7.0, torch.inf))
+
+
+@pytest.mark.parametrize("n", [3, 16])
+def test_infinity_in_a_chunk_stays_infinite_behind_it(cuda_device, n):
+    """Decays that are not zero, and whose product over a chunk of the time axis is."""
+    gen = torch.Generator().manual_seed(35)
+    T, d, at = 400, 10, 200
+    some = lambda *s: torch.rand(*s, generator=gen) + 0.5
+    for name in ("x", "dy"):
+        v = dict(x=some(1, T, d), dt=some(1, T, d), A=-3.0 * some(d, n), B=some(1, T, n), C=some(1, T, n), dy=some(1, T, d))
+        v[name][0, at, 5] = torch.inf
+        ops = [v[k].to(cuda_device).requires_grad_() for k in ("x", "dt", "A", "B", "C")]
+        y, ht = selective_scan(*ops, output_final_state=True)
+        dx, = torch.autograd.grad(y, ops[:1], v["dy"].to(cuda_device))
+        far = torch.zeros(1, T, d, dtype=torch.bool, device=cuda_device)
+        far[0, at:, 5] = name == "x"
+        assert torch.equal(y == torch.inf, far) and not y.isnan().any()
+        assert torch.equal(ht == torch.inf, far[:, -1, :, None].expand_as(ht)) and not ht.isnan().any()
+        far[0, :at + 1, 5] = name == "dy"
+        far[0, at + 1:] = False
+        if name == "x":
+            far[:] = False
+        assert torch.equal(dx == torch.inf, far) and not dx.isnan().any()
