@@ -112,7 +112,19 @@ __device__ __forceinline__ float2 softplus2(float2 v) {
   // NaN is not below zero
   return fma2(f2(2.f), fma2(mul2(s, q), p, s), make_float2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y));
 }
-__device__ __forceinline__ float softplus_f(float v) { return softplus2(f2(v)).x; }
+// The same of one value (one of a pair in its place: single tokens 15.5 us for 13.7).
+__device__ __forceinline__ float softplus_f(float v) {
+  const float w = fminf(fabsf(v), 128.f), e = w * -kLog2e, t0 = fast_exp2(e);
+  const float r = fmaf(w, -kLog2eRest, fmaf(w, -kLog2e, -e)), t = fmaf(t0, r * kSelLn2, t0);
+  const float s = t * rcp_fast(t + 2.f), q = s * s;
+  float p = fmaf(q, 1.f / 15.f, 1.f / 13.f);
+  p = fmaf(q, p, 1.f / 11.f);
+  p = fmaf(q, p, 1.f / 9.f);
+  p = fmaf(q, p, 1.f / 7.f);
+  p = fmaf(q, p, 1.f / 5.f);
+  p = fmaf(q, p, 1.f / 3.f);
+  return fmaf(2.f, fmaf(s * q, p, s), v < 0.f ? 0.f : v);
+}
 
 // 1 / (1 + e^-v), within 2^-21; for v < 0 the exponent's rounding adds up to |v| 2^-23
 __device__ __forceinline__ float2 sigmoid2(float2 v) {
@@ -1252,8 +1264,10 @@ __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float
     const float2 b = make_float2(raw_get(B, 2 * i), raw_get(B, 2 * i + 1));
     const float2 c = make_float2(raw_get(C, 2 * i), raw_get(C, 2 * i + 1));
     h[i] = fma2(exp2_2(mul2(f2(dt), mul2(A2[i], f2(kLog2e)))), h[i], mul2(f2(dt * x), b));
-    if (2 * i >= left) h[i].x = 0.f;  // beyond the last: infinity times zero is NaN
-    if (2 * i + 1 >= left) h[i].y = 0.f;
+    if (left < 4) {  // beyond the last: infinity times zero is NaN
+      if (2 * i >= left) h[i].x = 0.f;
+      if (2 * i + 1 >= left) h[i].y = 0.f;
+    }
     const float2 o = mul2(h[i], c);
     out += o.x + o.y;
   }
