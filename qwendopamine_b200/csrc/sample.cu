@@ -28,10 +28,11 @@
 // weights as whole numbers of 2^-44 (larger units for vocabularies beyond 2^18), and
 // among equal values the lower indices are counted out.
 //
-// Bound: by temperature alone the row is read once and the time is that of the
-// fp64 pipe, 12 operations for a value (256 x 151936 bf16: 88 us a call); with a
-// short list the row is read once from memory and once from L2 (64 x 151936 with
-// top-k 50 31 us, 256 rows 51 us); with top-p 0.6 alone 98 and 272 us.
+// Bound: by temperature alone the row is read once, with 44 instructions for a value,
+// 12 of them fp64 (256 x 151936 bf16: 88 us a call, of which the fp64 pipe is busy for
+// 42 % and the issue of instructions for 59 %; 40 of 148 SMs have one row, the others
+// two); with a short list the row is read once from memory and once from L2 (64 x
+// 151936 with top-k 50 31 us, 256 rows 51 us); with top-p 0.6 alone 98 and 272 us.
 // Few rows are split over the CTAs of a cluster, which exchange through distributed
 // shared memory: what is counted is added to the first CTA's histogram by remote
 // atomics, which nobody waits for.

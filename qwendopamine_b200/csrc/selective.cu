@@ -15,7 +15,8 @@
 // copies, one block ahead; what a row needs of a channel (dt, dt x, o) is formed once
 // for all lanes, in shared memory, and there the lanes leave their shares of sums over
 // a channel's states.  The sums over channels, dB and dC, are products on the tensor
-// core (TF32 operands, fp32 sums): a lane has its operands' values as they are.
+// core (operands of two TF32 values, fp32 sums): a lane has its operands' values as
+// they are.
 //
 // The time axis is cut where channels and sequences alone leave SMs idle: each
 // chunk's end state is formed from a zero start, a second launch carries them from
@@ -26,10 +27,11 @@
 // their own: every sum has a fixed order, equal inputs give equal bits.
 //
 // Bound: shared memory's bandwidth and the exponentials forward (8 x 4096 tokens x
-// 2048 channels x 16 states in bf16: 690 us, of which one exponential a state and
-// row takes 239), instructions issued backward (2.1 ms, three times the forward's
-// arithmetic); both were twice as long with rows read as they were needed and sums
-// exchanged between lanes.
+// 2048 channels x 16 states in bf16: 699 us, of which one exponential a state and
+// row takes 239); backward (2.5 ms, 3.8 times the forward's instructions) the issue of
+// instructions, 57 % busy, and waits for shared memory and the tensor core with 14
+// warps an SM.  Rows read as they were needed and sums exchanged between lanes took
+// 1523 us and 4.6 ms.
 #include "mma16.cuh"
 #include "op_util.cuh"
 
@@ -1223,10 +1225,10 @@ __device__ __forceinline__ void store_four(float* p, int N, int n0, bool vec, co
 
 // Every lane has four states of a channel.  What does not depend on the token's place
 // in the pool is read first.  The time is that of short chains of reads: 64 tokens of
-// 4096 channels of 16 states take 11 us (their states 5.5 us of traffic), 256 45 us at
-// three quarters of the issue rate.  Two channels to a lane (half the instructions),
+// 4096 channels of 16 states take 13.7 us (their states 5.5 us of traffic), 256 41.5 us
+// at three quarters of the issue rate.  Two channels to a lane (half the instructions),
 // four tokens to a CTA, and the next token's values on their way while one is worked
-// on were no faster (45, 47 and 103 us for the 256).
+// on were no faster (45, 47 and 103 us for the 256, where this took 43).
 template <typename T, int L>
 __global__ void __launch_bounds__(kSelThreads) k_sel_step(const SelArgs a, float* state, int64_t stride,
                                                           int pool, const int32_t* idx) {
@@ -1323,9 +1325,11 @@ struct SelPlan {
 
 // Cuts the time axis into chunks of whole 16 rows where the CTAs of the channels
 // and batch entries alone are fewer than two for each of 148 SMs (the extra
-// launches cost two thirds of the forward and a quarter of the backward once more:
-// 201 + 10 of 515 us and 226 + 9 of 1206 us at 65536 tokens x 512 channels); then as
-// many chunks as give four for each, of 64 rows at least.
+// launches cost two thirds of the forward and a fifth of the backward once more:
+// 207 + 10 of 525 us and 228 + 10 of 1384 us at 65536 tokens x 512 channels); then as
+// many chunks as give four for each, of 64 rows at least.  Both sides of the border, n x
+// 8192 tokens x 2048 channels x 16 states, forward and backward: 256 CTAs 4.09 ms cut
+// and 4.50 whole, 320 CTAs 5.50 and 5.31 (forward alone 1.00 and 0.96, 1.26 and 1.13).
 SelPlan sel_plan(const gdn2_selective_problem* p) {
   SelPlan q;
   const int ch = kSelThreads / lanes_of(p->N);
