@@ -529,7 +529,8 @@ int gdn2_selective_step(const gdn2_selective_problem* p, const void* x, const vo
  *      reaches top_p of their sum; equal logits rank by rising index;
  *   4. token_ids[r] is the lowest index whose running sum of kept weights, by
  *      rising index, exceeds uniform[r] * (their sum).
- * Weights and sums are fp64, equal inputs give equal tokens.  temperature,
+ * Weights and sums are fp64 (weights below 2^-1022 are zero), -0 and 0 are equal, and
+ * equal inputs give equal tokens.  temperature,
  * top_k, top_p, min_p: device arrays [rows] (fp32, int32), or NULL for the
  * problem's value.  Temperature or top_p <= 0, or top_k = 1, take the first
  * maximum; top_k <= 0, top_p >= 1 and min_p <= 0 keep everything.  -inf logits are

@@ -98,7 +98,7 @@ struct SampleShared {
   uint64_t list[kList];
 };
 
-// 2^-y for y >= 0 as fp64; 0 beyond 1022, for infinity and NaN
+// 2^-y for y >= +0 as fp64; 0 beyond 1022, for infinity and NaN
 __device__ __forceinline__ double pow2_neg(const double* root, double y) {
   constexpr double magic = 6755399441055744.;  // 1.5 * 2^52: rounds to whole numbers
   constexpr double c1 = 0.69314718055994531, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
@@ -1014,7 +1014,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SampleArgs a, co
       const float top = raw_max(v);
       if (top > mine) {
         if (sum > 0.) sum *= pow2_neg(s.root, ((double)top - mine) * rule.c);
-        mine = top;
+        mine = top + 0.f;  // not -0, from which +0 would be a negative zero away
       }
       if (mine == -INFINITY) return;
       const double m = mine;

@@ -61,7 +61,7 @@ def sample_tokens(
     order, up to the first whose running sum reaches ``top_p`` of their sum
     (equal logits rank by rising id).  The token is the lowest id whose running
     sum of kept weights, by rising id, exceeds ``uniform`` times their sum.
-    Weights and sums are float64.
+    Weights and sums are float64 (weights below 2^-1022 are zero); -0 and 0 are equal.
 
     ``temperature`` 0, ``top_k`` 1 and ``top_p`` 0 take the first maximum;
     ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 keep everything.  In tensors, which

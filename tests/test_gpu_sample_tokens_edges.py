@@ -50,3 +50,16 @@ def test_a_gap_behind_a_window_that_misses(cuda_device, gap, many):
     assert want[-1] >= 40
     x = torch.from_numpy(np.stack([row] * len(u))).to(cuda_device)
     assert sample_tokens(x, torch.from_numpy(u).to(cuda_device), top_p=top_p).tolist() == want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("options", [dict(), dict(top_p=0.7), dict(top_k=600), dict(min_p=0.5), dict(temperature=0.0)])
+def test_zeros_of_both_signs_are_equal(cuda_device, options, dtype):
+    """The largest logits are zeros, some of them negative ones."""
+    gen = torch.Generator().manual_seed(4)
+    x = torch.where(torch.rand(40, 5000, generator=gen) < 0.5, 0.0, -0.0)
+    x[20:, ::3] = -1.0
+    u = torch.rand(40, generator=gen)
+    want = [O.sample_token(r, float(v), **options) for r, v in zip(x.numpy(), u.numpy())]
+    got = sample_tokens(x.to(cuda_device, dtype), u.to(cuda_device), **options)
+    assert got.tolist() == want
